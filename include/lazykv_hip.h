@@ -17,7 +17,8 @@
  *    any launch. lkv_last_error() returns a message for the calling thread's last failure.
  *  - Dtype codes: LKV_F16, LKV_BF16, LKV_F32 for model-dtype tensors; LKV_INT8_RECORD for the
  *    int8 warm/cold records of lazykv/quant.py:46-105 (kq | vq | k scale | k zero | v scale |
- *    v zero, float16 scales).
+ *    v zero, float16 scales); LKV_MXFP8 for rows held as 8-bit codes with shared scales
+ *    (lkv_kv_rows).
  */
 #ifndef LAZYKV_HIP_H
 #define LAZYKV_HIP_H
@@ -36,7 +37,7 @@ enum {
   LKV_ERR_UNSUPPORTED = -3
 };
 
-enum { LKV_F16 = 0, LKV_BF16 = 1, LKV_F32 = 2, LKV_INT8_RECORD = 3 };
+enum { LKV_F16 = 0, LKV_BF16 = 1, LKV_F32 = 2, LKV_INT8_RECORD = 3, LKV_MXFP8 = 4 };
 
 /* lkv_bound_topk flags */
 enum { LKV_SORTED = 1 };
@@ -280,6 +281,72 @@ int lkv_unpack_int8(uintptr_t stream, const void* records, int64_t m, int block_
                     void* pairs);
 /* packed_pair_bytes (lazykv/quant.py:46-49) */
 int64_t lkv_packed_pair_bytes(int block_size, int head_dim);
+
+/* ---- rows of dense caches: a cache in 8 bits, written as tokens arrive, and a batch over a shared
+ * prefix. No counterpart in the reference, whose dense store (lazykv/cache.py:20-115) holds the model
+ * dtype and one sequence.
+ *
+ * Where the keys and values of `seqs` sequences live, one row of head_dim values a token: token t of KV
+ * head h of sequence b at k (v) + b * seq_stride + h * head_stride + t * head_dim elements. dtype
+ * LKV_F16 / LKV_BF16: the model's values. LKV_MXFP8: one E4M3 byte a value, and for every 32 channels of
+ * a row a scale byte X that stands for 2^(X - 127), at k_scale (v_scale) + the element offset / 32;
+ * `deq_dtype` is the model dtype. Rows start on 16 bytes, strides are multiples of 32 elements, scales
+ * on head_dim / 32 bytes. Tokens 0 .. tokens-1 are addressable: nothing outside is read or written. */
+typedef struct lkv_kv_rows {
+  const void* k;
+  const void* v;
+  const uint8_t* k_scale;
+  const uint8_t* v_scale;
+  int64_t seq_stride;
+  int64_t head_stride;
+  int64_t tokens;
+  int32_t seqs;
+  int32_t dtype;
+  int32_t deq_dtype;
+} lkv_kv_rows;
+
+/* New rows into dst (whose buffers are written): token t of sequence b, of `tokens` each, becomes row
+ * start + starts[b] + t (starts, int32 on the device, may be NULL: 0); rows outside 0 .. dst->tokens-1
+ * are dropped. k / v: keys and values in the model dtype, element (b, h, t, c) at
+ * b * seq_stride + h * head_stride + t * token_stride + c, 16-byte aligned, strides multiples of 8.
+ * LKV_MXFP8: X is the least exponent (0 at the least) with max |x| <= 448 * 2^(X - 127) over the
+ * group's finite values; the code is x * 2^(127 - X) rounded to the nearest E4M3 value, ties to even,
+ * after x is limited to the largest four-bit significand of the model dtype (61440 in float16), so that
+ * every finite row reads back finite; what is not finite becomes the NaN code. A model-dtype dst takes
+ * the values as they are. */
+int lkv_append_rows(uintptr_t stream, const lkv_kv_rows* dst, const void* k, const void* v, int dtype, int64_t seq_stride,
+                    int64_t head_stride, int64_t token_stride, int n_seqs, int n_kv, int head_dim, int tokens,
+                    const int32_t* starts, int start);
+
+/* Rows first .. first + tokens - 1 of an LKV_MXFP8 src, each code times its scale, in the model dtype
+ * (exact there, but for bfloat16 values below its normal range, which are rounded) to k / v, laid out
+ * as in lkv_append_rows. */
+int lkv_read_rows(uintptr_t stream, const lkv_kv_rows* src, int n_seqs, int n_kv, int head_dim, int first, int tokens, void* k,
+                  void* v, int dtype, int64_t seq_stride, int64_t head_stride, int64_t token_stride);
+
+/* One decode token of each of n_seqs sequences: query head j of sequence b attends rows
+ * 0 .. prefix_tokens-1 of `prefix` (one sequence's rows, which all of the batch share and which are read
+ * once for it), then rows 0 .. len-1 of its own in `own`, len = own_tokens + lengths[b] (lengths, int32
+ * on the device, may be NULL: 0) limited to 0 .. max_own. prefix and own may be NULL where they have no
+ * tokens; each in the query's dtype or LKV_MXFP8 with that deq_dtype. q [n_seqs, n_q, head_dim]; writes
+ * out [n_seqs, n_q, head_dim] (out_dtype) and lse [n_seqs, n_q] (float32, natural log); a sequence
+ * without any rows gets zeros and -inf. `ws` as in the other calls. The launch depends on max_own, not
+ * on the lengths, so that a captured call follows lengths that change. */
+typedef struct lkv_shared_desc {
+  int32_t n_seqs;
+  int32_t n_q;
+  int32_t n_kv;
+  int32_t head_dim; /* 64 or 128 */
+  float scale;      /* positive */
+  int32_t prefix_tokens;
+  int32_t own_tokens;
+  int32_t max_own;
+} lkv_shared_desc;
+
+size_t lkv_shared_decode_workspace_bytes(const lkv_shared_desc* desc);
+int lkv_shared_decode(uintptr_t stream, const lkv_shared_desc* desc, const void* q, int q_dtype, const lkv_kv_rows* prefix,
+                      const lkv_kv_rows* own, const int32_t* lengths, void* out, int out_dtype, float* lse, void* ws,
+                      size_t ws_bytes);
 
 /* ---- measurement: a streaming read of `bytes` at `src` (HBM or mapped host memory), the
  * device-side probe of the link asymptote that the byte roofline uses; no reference

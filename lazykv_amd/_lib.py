@@ -16,7 +16,7 @@ import torch
 SO_PATH = Path(__file__).resolve().parent / "liblazykv_hip.so"
 
 LKV_OK, LKV_ERR_INVALID, LKV_ERR_HIP, LKV_ERR_UNSUPPORTED = 0, -1, -2, -3
-F16, BF16, F32, INT8_RECORD = 0, 1, 2, 3
+F16, BF16, F32, INT8_RECORD, MXFP8 = 0, 1, 2, 3, 4
 SORTED = 1
 RANK_F32, RANK_MODEL = 0, 1
 HOST_COHERENT = 1
@@ -116,6 +116,38 @@ class RowCopy(ctypes.Structure):
     ]
 
 
+class KVRows(ctypes.Structure):
+    """lkv_kv_rows: where the rows of a dense cache live (see include/lazykv_hip.h)."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("seq_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("tokens", ctypes.c_int64),
+        ("seqs", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("deq_dtype", ctypes.c_int32),
+    ]
+
+
+class SharedDesc(ctypes.Structure):
+    """lkv_shared_desc: shape and extent of a batch's decode over a shared prefix."""
+
+    _fields_ = [
+        ("n_seqs", ctypes.c_int32),
+        ("n_q", ctypes.c_int32),
+        ("n_kv", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("prefix_tokens", ctypes.c_int32),
+        ("own_tokens", ctypes.c_int32),
+        ("max_own", ctypes.c_int32),
+    ]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _I64 = ctypes.c_int64
@@ -167,6 +199,13 @@ SIGNATURES: dict[str, tuple] = {
     "lkv_pack_int8": (_I, [_U, _P, _I, _I64, _I, _I, _P]),
     "lkv_unpack_int8": (_I, [_U, _P, _I64, _I, _I, _I, _P]),
     "lkv_packed_pair_bytes": (_I64, [_I, _I]),
+    "lkv_append_rows": (_I, [_U, ctypes.POINTER(KVRows), _P, _P, _I, _I64, _I64, _I64, _I, _I, _I, _I, _P, _I]),
+    "lkv_read_rows": (_I, [_U, ctypes.POINTER(KVRows), _I, _I, _I, _I, _I, _P, _P, _I, _I64, _I64, _I64]),
+    "lkv_shared_decode_workspace_bytes": (_SZ, [ctypes.POINTER(SharedDesc)]),
+    "lkv_shared_decode": (
+        _I,
+        [_U, ctypes.POINTER(SharedDesc), _P, _I, ctypes.POINTER(KVRows), ctypes.POINTER(KVRows), _P, _P, _I, _P, _P, _SZ],
+    ),
     "lkv_stream_read": (_I, [_U, _P, _SZ, _I, _P]),
 }
 

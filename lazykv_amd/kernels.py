@@ -624,6 +624,238 @@ def _forward_level() -> int:
     return getattr(torch.autograd.forward_ad, "_current_level", 0)
 
 
+# -- rows of dense caches: 8 bits as tokens arrive, and a batch over a shared prefix ---------------------
+
+
+MX_GROUP = 32  # channels of a row that share a scale (LKV_MXFP8)
+
+
+@dataclass
+class Rows:
+    """A `lkv_kv_rows`: the keys' and values' rows of `seqs` sequences, one per token, in the model dtype or in 8 bits."""
+
+    k: int
+    v: int
+    k_scale: int | None
+    v_scale: int | None
+    seq_stride: int
+    head_stride: int
+    tokens: int
+    seqs: int
+    n_kv: int
+    head_dim: int
+    dtype: int  # _lib.F16, _lib.BF16 or _lib.MXFP8
+    model_dtype: torch.dtype
+    device: torch.device
+    owners: tuple = ()
+
+    def c(self) -> _lib.KVRows:
+        return _lib.KVRows(self.k, self.v, self.k_scale, self.v_scale, self.seq_stride, self.head_stride, self.tokens, self.seqs, self.dtype,
+                           _ROW_DTYPES[self.model_dtype])
+
+
+_ROW_DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+_CODE_DTYPES = (torch.float8_e4m3fn, torch.uint8)
+
+
+def _row_dtype(dtype: torch.dtype) -> int:
+    code = _ROW_DTYPES.get(dtype)
+    if code is None:
+        raise ValueError(f"rows are float16 or bfloat16, got {dtype}")
+    return code
+
+
+def dense_rows(keys: torch.Tensor, values: torch.Tensor) -> Rows:
+    """Rows in the model dtype: keys and values `[seqs, h, T, d]`, contiguous rows d elements apart, any strides above
+    that are multiples of 32 elements and the same for both."""
+    _lib.require_cuda(keys, values)
+    shape = tuple(keys.shape)
+    ks = keys.stride()
+    if len(shape) != 4 or tuple(values.shape) != shape or keys.dtype != values.dtype or keys.device != values.device:
+        raise ValueError(f"expected matching [seqs, h, T, d] keys/values, got {shape} {keys.dtype} / {tuple(values.shape)} {values.dtype}")
+    if ks[3] != 1 or ks[2] != shape[3] or values.stride() != ks:
+        raise ValueError("rows must be contiguous with a token stride of head_dim, keys and values with the same strides")
+    return Rows(keys.data_ptr(), values.data_ptr(), None, None, ks[0], ks[1], shape[2], shape[0], shape[1], shape[3], _row_dtype(keys.dtype),
+                keys.dtype, keys.device, (keys, values))
+
+
+def mx_rows(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> Rows:
+    """Rows in 8 bits: codes `[2, seqs, h, T, d]` (keys, values; float8_e4m3fn or uint8) and scales `[2, seqs, h, T, d / 32]`
+    (uint8), for a model of `dtype`. Views are fine whose scales are cut like their codes."""
+    _lib.require_cuda(codes, scales)
+    _row_dtype(dtype)
+    shape, cs, ss = tuple(codes.shape), codes.stride(), scales.stride()
+    if len(shape) != 5 or shape[0] != 2 or codes.dtype not in _CODE_DTYPES or scales.dtype != torch.uint8 or codes.device != scales.device:
+        raise ValueError(f"expected codes [2, seqs, h, T, d] and uint8 scales, got {shape} {codes.dtype} / {tuple(scales.shape)} {scales.dtype}")
+    d = shape[4]
+    if d % MX_GROUP or tuple(scales.shape) != shape[:4] + (d // MX_GROUP,):
+        raise ValueError(f"codes {shape} take scales {shape[:4] + (d // MX_GROUP,)}, got {tuple(scales.shape)}")
+    if cs[4] != 1 or cs[3] != d or ss[4] != 1 or ss[3] * MX_GROUP != d or ss[1] * MX_GROUP != cs[1] or ss[2] * MX_GROUP != cs[2]:
+        raise ValueError("codes' and scales' rows must be contiguous, and their strides alike")
+    k, k_scale = codes.data_ptr(), scales.data_ptr()
+    return Rows(k, k + cs[0], k_scale, k_scale + ss[0], cs[1], cs[2], shape[3], shape[1], shape[2], d, _lib.MXFP8, dtype, codes.device, (codes, scales))
+
+
+def mx_empty(seqs: int, n_kv: int, tokens: int, head_dim: int, device: torch.device | str) -> tuple[torch.Tensor, torch.Tensor]:
+    """Codes and scales of a cache in 8 bits (`mx_rows`), zero-filled: every row stands for zeros."""
+    codes = torch.zeros((2, seqs, n_kv, tokens, head_dim), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+    return codes, torch.zeros((2, seqs, n_kv, tokens, head_dim // MX_GROUP), dtype=torch.uint8, device=device)
+
+
+def _on(device: torch.device):  # noqa: ANN202
+    """The device a launch needs as the current one, where it is another."""
+    return torch.cuda.device(device) if device.index not in (None, torch.cuda.current_device()) else _NO_SWITCH
+
+
+class _NoSwitch:
+    def __enter__(self) -> None:
+        return None
+
+    def __exit__(self, *exc: object) -> None:
+        return None
+
+
+_NO_SWITCH = _NoSwitch()
+
+
+def _placed(x: torch.Tensor) -> torch.Tensor:
+    """`x` as the row kernels read it: contiguous channels, rows on 16 bytes. A copy where it lies otherwise."""
+    st = x.stride()
+    if st[3] != 1 or (st[0] | st[1] | st[2]) % 8 or x.data_ptr() % 16:
+        return x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def _starts(starts: torch.Tensor | None, seqs: int, device: torch.device, name: str) -> int | None:
+    if starts is None:
+        return None
+    if starts.device != device or starts.dtype != torch.int32 or tuple(starts.shape) != (seqs,) or not starts.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32 [{seqs}] on {device}, got {starts.dtype} {tuple(starts.shape)} on {starts.device}")
+    return starts.data_ptr()
+
+
+def append_rows(dst: Rows, keys: torch.Tensor, values: torch.Tensor, *, start: int = 0, starts: torch.Tensor | None = None) -> None:
+    """New tokens' keys and values `[seqs, h, T, d]` into a cache's rows (lkv_append_rows): token t of sequence b becomes row
+    `start + starts[b] + t`. Without `starts` the rows must exist (ValueError); with it, rows outside the cache are dropped. An
+    8-bit cache takes them as E4M3 codes with a power-of-two scale for every 32 channels, another one as they are."""
+    shape = tuple(keys.shape)
+    if shape != tuple(values.shape) or len(shape) != 4 or keys.dtype != dst.model_dtype or values.dtype != dst.model_dtype:
+        raise ValueError(f"expected matching {dst.model_dtype} keys/values [seqs, h, T, d], got {shape} {keys.dtype} / {tuple(values.shape)} {values.dtype}")
+    if (shape[0], shape[1], shape[3]) != (dst.seqs, dst.n_kv, dst.head_dim):
+        raise ValueError(f"keys/values {shape} do not match rows of {dst.seqs} sequences, {dst.n_kv} heads and head_dim {dst.head_dim}")
+    if keys.device != dst.device or values.device != dst.device:
+        raise ValueError(f"keys/values on {keys.device} / {values.device}, the cache on {dst.device}")
+    at = _starts(starts, dst.seqs, dst.device, "starts")
+    if 0 in shape:
+        return
+    x, y = _placed(keys), _placed(values)
+    if x.stride() != y.stride():
+        x, y = x.contiguous(), y.contiguous()
+        if x.stride() != y.stride():  # sizes of one leave strides free
+            x, y = torch.stack([x, y]).unbind(0)
+    st = x.stride()
+    with _on(dst.device):
+        rc = _lib.lib().lkv_append_rows(_lib.stream_of(x), ctypes.byref(dst.c()), x.data_ptr(), y.data_ptr(), _ROW_DTYPES[dst.model_dtype], st[0], st[1], st[2],
+                                        dst.seqs, dst.n_kv, dst.head_dim, shape[2], at, start)
+    _lib.check(rc, "append_rows")
+
+
+def read_rows(src: Rows, first: int, n: int, out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Rows first .. first + n - 1 of an 8-bit cache as keys and values `[seqs, h, n, d]` in the model dtype (lkv_read_rows),
+    each code times its scale; into `out` where given."""
+    if src.dtype != _lib.MXFP8:
+        raise ValueError("read_rows takes 8-bit rows; others are read where they are")
+    if first < 0 or n < 0 or first + n > src.tokens:
+        raise ValueError(f"rows {first}..{first + n} exceed the {src.tokens} there are")
+    shape = (src.seqs, src.n_kv, n, src.head_dim)
+    if out is None:
+        out = (torch.empty(shape, dtype=src.model_dtype, device=src.device), torch.empty(shape, dtype=src.model_dtype, device=src.device))
+    k, v = out
+    st = k.stride()
+    for x in out:
+        if tuple(x.shape) != shape or x.dtype != src.model_dtype or x.device != src.device:
+            raise ValueError(f"out must be {src.model_dtype} {shape} on {src.device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
+    if v.stride() != st or st[3] != 1 or (st[0] | st[1] | st[2]) % 8 or (k.data_ptr() | v.data_ptr()) % 16:
+        raise ValueError("out's rows must be contiguous and start on 16 bytes, both with the same strides")
+    if 0 in shape:
+        return out
+    with _on(src.device):
+        rc = _lib.lib().lkv_read_rows(_lib.stream_of(k), ctypes.byref(src.c()), src.seqs, src.n_kv, src.head_dim, first, n, k.data_ptr(), v.data_ptr(),
+                                      _ROW_DTYPES[src.model_dtype], st[0], st[1], st[2])
+    _lib.check(rc, "read_rows")
+    return out
+
+
+def shared_decode(
+    q: torch.Tensor,
+    *,
+    scale: float,
+    prefix: Rows | None = None,
+    prefix_tokens: int = 0,
+    own: Rows | None = None,
+    own_tokens: int = 0,
+    lengths: torch.Tensor | None = None,
+    max_own: int | None = None,
+    out: torch.Tensor | None = None,
+    out_dtype: torch.dtype | None = None,
+    lse: torch.Tensor | None = None,
+    ws: Workspace | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """One decode token of each of B sequences, q `[B, n_q, d]` or `[B, n_q, 1, d]` (lkv_shared_decode): sequence b attends rows
+    0 .. prefix_tokens-1 of `prefix`, one sequence's rows that are read once for the whole batch, and rows
+    0 .. own_tokens + lengths[b] - 1 of its own in `own`, at most `max_own` of them (default: own_tokens without
+    `lengths`, else all that `own` holds; a bound near the lengths divides the work better). Either may be left out: B = 1 over `own` alone is plain decode over an
+    8-bit cache. Returns (out [B, n_q, d], lse [B, n_q] float32, natural log); a sequence without any rows gets zeros and -inf.
+    Without `ws` the scratch is torch's, so calls on several streams and in several graphs do not meet."""
+    rows = own if own is not None else prefix
+    if rows is None:
+        raise ValueError("shared_decode needs a prefix's rows or the sequences' own")
+    _lib.require_cuda(q)
+    shape = tuple(q.shape)
+    if len(shape) == 4 and shape[2] == 1:
+        shape = (shape[0], shape[1], shape[3])
+    if len(shape) != 3 or q.dtype != rows.model_dtype or shape[2] != rows.head_dim or shape[1] == 0 or shape[1] % rows.n_kv:
+        raise ValueError(f"query {tuple(q.shape)} {q.dtype} does not match {rows.model_dtype} rows of {rows.n_kv} heads and head_dim {rows.head_dim}")
+    b, n_q, d = shape
+    if max_own is None:
+        max_own = own_tokens if lengths is None else (own.tokens if own is not None else 0)
+    for r, seqs, what in ((prefix, 1, "prefix"), (own, b, "own")):
+        if r is not None and (r.n_kv, r.head_dim, r.model_dtype, r.device, r.seqs) != (rows.n_kv, d, q.dtype, q.device, seqs):
+            raise ValueError(f"{what} rows of {r.seqs} sequences, {r.n_kv} heads, head_dim {r.head_dim}, {r.model_dtype} on {r.device} do not match "
+                             f"{seqs} of {rows.n_kv}, {d}, {q.dtype} on {q.device}")
+    if own is None and (lengths is not None or own_tokens or max_own):
+        raise ValueError("own_tokens, lengths and max_own describe `own`, which is not given")
+    at = _starts(lengths, b, q.device, "lengths")
+    if lengths is None and own_tokens > max_own:
+        raise ValueError(f"own_tokens={own_tokens} exceed max_own={max_own}")
+    qq = q.reshape(shape).contiguous()
+    if qq.data_ptr() % 16:
+        qq = qq.clone()
+    if out is None:
+        out = torch.empty(shape, dtype=out_dtype or q.dtype, device=q.device)
+    if lse is None:
+        lse = torch.empty((b, n_q), dtype=torch.float32, device=q.device)
+    if (not out.is_contiguous() or out.numel() != b * n_q * d or out.device != q.device or (out_dtype is not None and out.dtype != out_dtype)
+            or not lse.is_contiguous() or lse.numel() != b * n_q or lse.dtype != torch.float32 or lse.device != q.device):
+        raise ValueError(f"out must be contiguous [{b}, {n_q}, {d}] and lse contiguous float32 [{b}, {n_q}] on {q.device}")
+    if b == 0:
+        return out, lse
+    desc = _lib.SharedDesc(b, n_q, rows.n_kv, d, scale, prefix_tokens, own_tokens, max_own)
+    need = _lib.lib().lkv_shared_decode_workspace_bytes(ctypes.byref(desc))
+    if ws is None:
+        buf = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
+        ws_ptr, ws_n = buf.data_ptr(), buf.numel()
+    else:
+        ws_ptr, ws_n = ws.get(need)
+    with _on(q.device):
+        rc = _lib.lib().lkv_shared_decode(
+            _lib.stream_of(qq), ctypes.byref(desc), qq.data_ptr(), _ROW_DTYPES[q.dtype], ctypes.byref(prefix.c()) if prefix is not None else None,
+            ctypes.byref(own.c()) if own is not None else None, at, out.data_ptr(), _lib.dtype_code(out.dtype), lse.data_ptr(), ws_ptr, ws_n,
+        )
+    _lib.check(rc, "shared_decode")
+    return out, lse
+
+
 def packed_pair_bytes(block_size: int, head_dim: int) -> int:
     return int(_lib.lib().lkv_packed_pair_bytes(block_size, head_dim))
 

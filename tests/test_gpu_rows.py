@@ -1,0 +1,271 @@
+"""Rows of dense caches on the GPU: new tokens into a cache in 8 bits (or as they are) and back, against the 64-bit oracle.
+Codes, scales and rows that are read back are compared for equality: the only rounding on the way is that of the code, and it
+is to nearest even on both sides."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import rows as O
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def _kv(seed: int, shape: tuple, model: str) -> tuple[torch.Tensor, torch.Tensor]:
+    gen = torch.Generator().manual_seed(seed)
+    loud = torch.exp2(4 * torch.randn(shape[:-1] + (1,), generator=gen)) * torch.where(torch.rand(shape[-1:], generator=gen) < 0.1, 8.0, 1.0)
+    return tuple((torch.randn(shape, generator=gen) * loud).clamp(-6e4, 6e4).to(TYPES[model]) for _ in range(2))
+
+
+def _cache(seqs: int, h: int, cap: int, d: int, model: str):  # noqa: ANN202
+    from lazykv_amd import kernels
+
+    codes, scales = kernels.mx_empty(seqs, h, cap, d, "cuda")
+    codes.view(torch.uint8).fill_(0x55)
+    scales.fill_(0x66)
+    return codes, scales, kernels.mx_rows(codes, scales, TYPES[model])
+
+
+def _check(codes: torch.Tensor, scales: torch.Tensor, which: int, b: int, row: int, want: tuple) -> None:
+    """Rows row.. of cache `which` of sequence b hold the oracle's codes and scales [h, n, ...]."""
+    n = want[0].shape[1]
+    got = codes[which, b, :, row : row + n].double().cpu().numpy()
+    assert np.array_equal(got, want[0], equal_nan=True)
+    assert np.array_equal(scales[which, b, :, row : row + n].cpu().numpy(), want[1])
+
+
+@pytest.mark.parametrize("model", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize(("seqs", "h", "n", "cap", "start"), [(1, 1, 1, 1, 0), (1, 8, 1, 7, 6), (1, 2, 33, 40, 5), (3, 5, 17, 64, 0), (2, 8, 300, 301, 1), (7, 1, 2, 9, 3)])
+def test_rows_are_written_as_the_oracle_codes_them_and_read_back(model: str, d: int, seqs: int, h: int, n: int, cap: int, start: int) -> None:
+    from lazykv_amd import kernels
+
+    kv = _kv(seqs * 100 + n, (seqs, h, n, d), model)
+    codes, scales, rows = _cache(seqs, h, cap, d, model)
+    kernels.append_rows(rows, *(x.cuda() for x in kv), start=start)
+    back = kernels.read_rows(rows, start, n)
+    torch.cuda.synchronize()
+    for which, x in enumerate(kv):
+        c, s = O.mx_encode(x.double().numpy(), model)
+        for b in range(seqs):
+            _check(codes, scales, which, b, start, (c[b], s[b]))
+        assert np.array_equal(back[which].double().cpu().numpy(), O.mx_decode(c, s))
+    # Rows around are as they were.
+    raw = codes.view(torch.uint8)
+    for x, fill in ((raw, 0x55), (scales, 0x66)):
+        assert bool((x[:, :, :, :start] == fill).all()) and bool((x[:, :, :, start + n :] == fill).all())
+
+
+@pytest.mark.parametrize("model", ["f16", "bf16"])
+@pytest.mark.parametrize("lead", [0.0, 2.0**-24, 3e-5, 0.7, 1.75, 1.7578125, 448.0, 450.0, 61440.0, 61441.0, 65504.0, 3e38, float("inf"), float("nan")])
+def test_every_value_of_the_model_dtype_is_coded(model: str, lead: float) -> None:
+    """Every bit pattern of at most the lead's size, 31 to a group under a lead that sets the group's scale; a lead of 0 leaves
+    the patterns to set it, and so do infinity and NaN, which are held as NaN."""
+    from lazykv_amd import kernels
+
+    t = TYPES[model]
+    lead = float(torch.tensor(lead).to(t))
+    if model == "f16" and lead > 65504 and lead < float("inf"):
+        lead = 65504.0
+    x = torch.arange(65536, dtype=torch.int32).to(torch.uint16).view(t)
+    if 0 < lead < float("inf"):
+        x = x[~(x.float().abs() > lead)]
+    x = x[torch.randperm(len(x), generator=torch.Generator().manual_seed(1))]
+    n = len(x) // (31 * 4) * (31 * 4)
+    groups = torch.cat([torch.full((n // 31, 1), lead, dtype=t), x[:n].view(-1, 31)], 1)
+    kv = groups.view(1, 1, -1, 128)
+    codes, scales, rows = _cache(1, 1, kv.shape[2], 128, model)
+    kernels.append_rows(rows, kv.cuda(), kv.flip(2).cuda())
+    back = kernels.read_rows(rows, 0, kv.shape[2])
+    torch.cuda.synchronize()
+    for which, y in enumerate((kv, kv.flip(2))):
+        c, s = O.mx_encode(y[0].double().numpy(), model)
+        _check(codes, scales, which, 0, 0, (c, s))
+        want = O.mx_decode(c, s)
+        got = back[which][0].cpu()
+        # Exact in the model dtype; bfloat16 values below its normal range are rounded to it.
+        assert np.array_equal(got.double().numpy(), torch.from_numpy(want).to(t).double().numpy(), equal_nan=True)
+        assert np.array_equal(np.isnan(want), ~np.isfinite(y[0].double().numpy()))
+
+
+def test_sequences_write_at_places_of_their_own_and_drop_rows_outside() -> None:
+    from lazykv_amd import kernels
+
+    seqs, h, n, d, cap = 5, 3, 9, 64, 40
+    kv = _kv(3, (seqs, h, n, d), "bf16")
+    codes, scales, rows = _cache(seqs, h, cap, d, "bf16")
+    starts = torch.tensor([0, 31, 35, -4, 2147483647], dtype=torch.int32, device="cuda")
+    kernels.append_rows(rows, *(x.cuda() for x in kv), start=1, starts=starts)
+    torch.cuda.synchronize()
+    for which, x in enumerate(kv):
+        c, s = O.mx_encode(x.double().numpy(), "bf16")
+        _check(codes, scales, which, 0, 1, (c[0], s[0]))
+        _check(codes, scales, which, 1, 32, (c[1][:, :8], s[1][:, :8]))
+        _check(codes, scales, which, 2, 36, (c[2][:, :4], s[2][:, :4]))
+        _check(codes, scales, which, 3, 0, (c[3][:, 3:], s[3][:, 3:]))
+        assert bool((codes.view(torch.uint8)[which, 4] == 0x55).all()) and bool((scales[which, 4] == 0x66).all())
+        assert bool((codes.view(torch.uint8)[which, 0, :, 10:] == 0x55).all())
+
+
+@pytest.mark.parametrize("model", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_model_dtype_rows_are_written_as_they_are(model: str, d: int) -> None:
+    """A cache in the model dtype, every bit pattern among the rows (NaNs and their payloads too), at ragged places."""
+    from lazykv_amd import kernels
+
+    seqs, h, n, cap = 4, 2, 65536 // (4 * 2 * 64), 200
+    bits = torch.arange(seqs * h * n * d, dtype=torch.int32).to(torch.uint16).view(seqs, h, n, d).view(TYPES[model]).cuda()
+    store = torch.full((2, seqs, h, cap, d), 7.0, dtype=TYPES[model], device="cuda")
+    starts = torch.tensor([0, 3, 72, 1], dtype=torch.int32, device="cuda")
+    kernels.append_rows(kernels.dense_rows(store[0], store[1]), bits, bits.flip(3), starts=starts)
+    torch.cuda.synchronize()
+    for b, a in enumerate(starts.tolist()):
+        for which, x in enumerate((bits, bits.flip(3))):
+            got = store[which, b].view(torch.int16)
+            m = min(n, cap - a)
+            assert torch.equal(got[:, a : a + m], x[b, :, :m].contiguous().view(torch.int16))
+            assert bool((store[which, b, :, :a] == 7).all()) and bool((store[which, b, :, a + m :] == 7).all())
+
+
+@pytest.mark.parametrize("lay", ["tokens_first", "odd_start", "odd_strides", "reversed_heads", "expanded", "other_strides", "channels_apart"])
+def test_inputs_of_any_layout(lay: str) -> None:
+    from lazykv_amd import kernels
+
+    seqs, h, n, d = 2, 4, 11, 64
+    k, v = (x.cuda() for x in _kv(9, (seqs, h, n, d), "f16"))
+    if lay == "tokens_first":  # as a projection's view gives them
+        k, v = (x.transpose(1, 2).contiguous().transpose(1, 2) for x in (k, v))
+    elif lay == "odd_start":
+        k, v = (torch.cat([x.new_zeros(3), x.flatten()])[3:].view(x.shape) for x in (k, v))
+    elif lay == "odd_strides":
+        k, v = (torch.nn.functional.pad(x, (0, 3))[..., :d] for x in (k, v))
+    elif lay == "reversed_heads":
+        k, v = (x[:, [3, 1, 0, 2]][:, :, 1:] for x in (k, v))
+    elif lay == "expanded":
+        k, v = (x[:1].expand(seqs, h, n, d) for x in (k, v))
+    elif lay == "other_strides":
+        v = v.transpose(1, 2).contiguous().transpose(1, 2)
+    else:
+        k, v = (x.transpose(2, 3).contiguous().transpose(2, 3) for x in (k, v))
+    codes, scales, rows = _cache(seqs, h, 16, d, "f16")
+    kernels.append_rows(rows, k, v, start=2)
+    torch.cuda.synchronize()
+    for which, x in enumerate((k, v)):
+        c, s = O.mx_encode(x.double().cpu().numpy(), "f16")
+        for b in range(seqs):
+            _check(codes, scales, which, b, 2, (c[b], s[b]))
+
+
+def test_views_of_a_cache_and_an_output_of_the_callers() -> None:
+    """Heads and tokens of a larger cache (an odd first row: the scales start on 2 bytes), read into the middle of another buffer."""
+    from lazykv_amd import kernels
+
+    seqs, h, cap, d = 3, 6, 50, 64
+    codes, scales, _ = _cache(seqs, h, cap, d, "bf16")
+    part = kernels.mx_rows(codes[:, 1:, 2:5, 7:41], scales[:, 1:, 2:5, 7:41], torch.bfloat16)
+    kv = _kv(4, (seqs - 1, 3, 34, d), "bf16")
+    kernels.append_rows(part, *(x.cuda() for x in kv))
+    buf = torch.full((2, seqs - 1, 3, 60, d), 5.0, dtype=torch.bfloat16, device="cuda")
+    got = kernels.read_rows(part, 1, 30, out=(buf[0, :, :, 9:39], buf[1, :, :, 9:39]))
+    torch.cuda.synchronize()
+    for which, x in enumerate(kv):
+        c, s = O.mx_encode(x.double().numpy(), "bf16")
+        for b in range(seqs - 1):
+            got_c = codes[which, b + 1, 2:5, 7:41].double().cpu().numpy()
+            assert np.array_equal(got_c, c[b]) and np.array_equal(scales[which, b + 1, 2:5, 7:41].cpu().numpy(), s[b])
+        assert np.array_equal(got[which].double().cpu().numpy(), O.mx_decode(c, s)[:, :, 1:31])
+        assert bool((buf[which, :, :, :9] == 5).all()) and bool((buf[which, :, :, 39:] == 5).all())
+    raw = codes.view(torch.uint8)
+    assert bool((raw[:, 0] == 0x55).all()) and bool((raw[:, :, :2] == 0x55).all()) and bool((raw[:, :, 5] == 0x55).all())
+    assert bool((raw[:, :, :, :7] == 0x55).all()) and bool((raw[:, :, :, 41:] == 0x55).all())
+
+
+def test_nothing_to_write_or_read() -> None:
+    from lazykv_amd import kernels
+
+    codes, scales, rows = _cache(2, 2, 8, 64, "f16")
+    none = torch.zeros((2, 2, 0, 64), dtype=torch.float16, device="cuda")
+    kernels.append_rows(rows, none, none, start=8)
+    k, v = kernels.read_rows(rows, 8, 0)
+    assert k.shape == v.shape == (2, 2, 0, 64)
+    assert bool((codes.view(torch.uint8) == 0x55).all())
+
+
+def test_a_captured_write_follows_its_inputs() -> None:
+    from lazykv_amd import kernels
+
+    codes, scales, rows = _cache(3, 2, 20, 128, "f16")
+    x = torch.zeros((2, 3, 2, 1, 128), dtype=torch.float16, device="cuda")
+    starts = torch.zeros(3, dtype=torch.int32, device="cuda")
+    kernels.append_rows(rows, x[0], x[1], starts=starts)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kernels.append_rows(rows, x[0], x[1], starts=starts)
+        back = kernels.read_rows(rows, 0, 20)
+    for step in range(4):
+        kv = _kv(step, (3, 2, 1, 128), "f16")
+        x.copy_(torch.stack(kv))
+        starts.copy_(torch.tensor([step, 2 * step, 19 - step], dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        for which, y in enumerate(kv):
+            c, s = O.mx_encode(y.double().numpy(), "f16")
+            for b, a in enumerate(starts.tolist()):
+                _check(codes, scales, which, b, a, (c[b], s[b]))
+                assert np.array_equal(back[which][b, :, a].double().cpu().numpy(), O.mx_decode(c, s)[b, :, 0])
+
+
+def test_rows_past_32_bits_of_elements() -> None:
+    """A cache whose last rows lie beyond 2^32 codes: written and read where they belong."""
+    from lazykv_amd import kernels
+
+    h, cap, d = 2, (1 << 24) + 77, 128
+    codes = torch.zeros((2, 1, h, cap, d), dtype=torch.uint8, device="cuda")
+    scales = torch.zeros((2, 1, h, cap, d // 32), dtype=torch.uint8, device="cuda")
+    rows = kernels.mx_rows(codes, scales, torch.bfloat16)
+    kv = _kv(8, (1, h, 70, d), "bf16")
+    kernels.append_rows(rows, *(x.cuda() for x in kv), start=cap - 70)
+    back = kernels.read_rows(rows, cap - 70, 70)
+    torch.cuda.synchronize()
+    for which, x in enumerate(kv):
+        c, s = O.mx_encode(x.double().numpy(), "bf16")
+        assert np.array_equal(back[which].double().cpu().numpy(), O.mx_decode(c, s))
+        assert int((scales[which, 0, :, : cap - 70] != 0).sum()) == 0
+
+
+@pytest.mark.parametrize("bad", ["dtype", "heads", "head_dim", "past", "negative", "starts_dtype", "starts_shape", "strides", "scales", "read_past", "out"])
+def test_python_refusals(bad: str) -> None:
+    from lazykv_amd import kernels
+
+    codes, scales, rows = _cache(2, 2, 8, 64, "f16")
+    x = torch.zeros((2, 2, 3, 64), dtype=torch.float16, device="cuda")
+    starts = torch.zeros(2, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError):
+        if bad == "dtype":
+            kernels.append_rows(rows, x.bfloat16(), x.bfloat16())
+        elif bad == "heads":
+            kernels.append_rows(rows, x[:, :1], x[:, :1])
+        elif bad == "head_dim":
+            kernels.append_rows(rows, x[..., :32], x[..., :32])
+        elif bad == "past":
+            kernels.append_rows(rows, x, x, start=6)
+        elif bad == "negative":
+            kernels.append_rows(rows, x, x, start=-1)
+        elif bad == "starts_dtype":
+            kernels.append_rows(rows, x, x, starts=starts.long())
+        elif bad == "starts_shape":
+            kernels.append_rows(rows, x, x, starts=starts[:1])
+        elif bad == "strides":
+            kernels.mx_rows(codes.transpose(2, 3), scales.transpose(2, 3), torch.float16)
+        elif bad == "scales":
+            kernels.mx_rows(codes, scales[..., :1], torch.float16)
+        elif bad == "read_past":
+            kernels.read_rows(rows, 6, 3)
+        else:
+            kernels.read_rows(rows, 0, 3, out=(x.bfloat16(), x.bfloat16()))
+    assert bool((codes.view(torch.uint8) == 0x55).all())
