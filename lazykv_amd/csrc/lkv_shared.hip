@@ -21,6 +21,7 @@ namespace {
 
 constexpr int kWaves = 4;      // of a workgroup; each takes every fourth tile of the workgroup's tokens
 constexpr int kTile = 32;      // tokens
+constexpr float kSlack = 6.0f; // a weight is at most 2^kSlack: nothing to a 16-bit weight's precision or a float32 sum's
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -93,21 +94,35 @@ __device__ __forceinline__ Stream stream_of(const lkv_kv_rows& r, int64_t seq, i
           MX ? r.v_scale + e / kMxGroup : nullptr};
 }
 
+// Where a lane's rows of a tile lie, in bytes from the tile's first: fixed but for a tile that the end cuts, whose
+// tokens behind the end read the last one instead.
+template <int D, bool MX> struct LaneOffsets {
+  static constexpr int ROW = MX ? D : 2 * D;  // bytes
+  uint32_t key[2];
+  uint32_t value[8];
+  bool cut;
+  __device__ __forceinline__ void set(int last) {  // last: the last token of the tile that there is, 31 or less
+    const int lane = threadIdx.x & 63, quarter = lane >> 4;
+    cut = last < kTile - 1;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) key[u] = (uint32_t)(min(16 * u + (lane & 15), last) * ROW + quarter * (MX ? D / 4 : 16));
+#pragma unroll
+    for (int j = 0; j < 8; ++j) value[j] = (uint32_t)(min((j < 4 ? 0 : 16) + 4 * quarter + (j & 3), last) * ROW + (lane & 15) * (ROW / 16));
+  }
+};
+
 // Keys of a tile: two halves of 16 tokens, a lane token lane % 16 of each. Raw as loaded.
 // Model dtype: channels 32 i + 8 q .. + 8 for the i-th product. 8 bits: channels (d/4) q .. + d/4, so that a
 // lane's codes lie together under one scale; the i-th product takes the i-th eight of them.
 template <int D, bool MX> struct KeyRegs;
 template <int D> struct KeyRegs<D, false> {
   uint4 w[2][D / 32];
-  __device__ __forceinline__ void load(const Stream& s, int t0, int last) {
-    const int lane = threadIdx.x & 63;
+  __device__ __forceinline__ void load(const Stream& s, int64_t t, const LaneOffsets<D, false>& at) {
+    const uint8_t* base = s.k + t * (2 * D);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int t = min(t0 + 16 * u + (lane & 15), last);
-      const uint4* p = (const uint4*)(s.k + (int64_t)t * (2 * D) + (lane >> 4) * 16);
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) w[u][i] = p[i * 4];
-    }
+      for (int i = 0; i < D / 32; ++i) w[u][i] = *(const uint4*)(base + at.key[u] + i * 64);
   }
   template <int DT> __device__ __forceinline__ uint4 operand(int u, int i) const { return w[u][i]; }
   static __device__ __forceinline__ int channel(int q, int i) { return 32 * i + 8 * q; }
@@ -115,21 +130,19 @@ template <int D> struct KeyRegs<D, false> {
 template <int D> struct KeyRegs<D, true> {
   uint4 w[2][D / 64];
   uint32_t scale[2];
-  __device__ __forceinline__ void load(const Stream& s, int t0, int last) {
-    const int lane = threadIdx.x & 63;
+  __device__ __forceinline__ void load(const Stream& s, int64_t t, const LaneOffsets<D, true>& at) {
+    const uint8_t *base = s.k + t * D, *scales = s.ks + t * (D / kMxGroup);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int t = min(t0 + 16 * u + (lane & 15), last);
-      const int64_t at = (int64_t)t * D + (lane >> 4) * (D / 4);
 #pragma unroll
-      for (int i = 0; i < D / 64; ++i) w[u][i] = ((const uint4*)(s.k + at))[i];
-      scale[u] = s.ks[at / kMxGroup];
+      for (int i = 0; i < D / 64; ++i) w[u][i] = *(const uint4*)(base + at.key[u] + i * 16);
+      scale[u] = scales[at.key[u] / kMxGroup];
     }
   }
   template <int DT> __device__ __forceinline__ uint4 operand(int u, int i) const {
     const uint4& x = w[u][i / 2];
     const uint32_t lo = i & 1 ? x.z : x.x, hi = i & 1 ? x.w : x.y;
-    const float f = lkv::mx_scale(scale[u]);
+    const float f = lkv::bits_to_float(scale[u] << 23);  // the conversion takes a scale's exponent field alone
     return make_uint4(Mat<DT>::template widen<false>(lo, f), Mat<DT>::template widen<true>(lo, f), Mat<DT>::template widen<false>(hi, f),
                       Mat<DT>::template widen<true>(hi, f));
   }
@@ -140,17 +153,15 @@ template <int D> struct KeyRegs<D, true> {
 template <int D, bool MX> struct ValueRegs;
 template <int D> struct ValueRegs<D, false> {
   uint32_t w[8][D / 32];
-  __device__ __forceinline__ void load(const Stream& s, int t0, int last) {
-    const int lane = threadIdx.x & 63;
+  __device__ __forceinline__ void load(const Stream& s, int64_t t, const LaneOffsets<D, false>& at) {
+    const uint8_t* base = s.v + t * (2 * D);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int t = min(t0 + (j < 4 ? 0 : 16) + 4 * (lane >> 4) + (j & 3), last);
-      const uint8_t* p = s.v + (int64_t)t * (2 * D) + (lane & 15) * (D / 8);
       if constexpr (D == 128) {
-        const uint4 x = *(const uint4*)p;
+        const uint4 x = *(const uint4*)(base + at.value[j]);
         w[j][0] = x.x, w[j][1] = x.y, w[j][2] = x.z, w[j][3] = x.w;
       } else {
-        const uint2 x = *(const uint2*)p;
+        const uint2 x = *(const uint2*)(base + at.value[j]);
         w[j][0] = x.x, w[j][1] = x.y;
       }
     }
@@ -159,34 +170,59 @@ template <int D> struct ValueRegs<D, false> {
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) w[j][c] = 0;
   }
-  template <int DT> __device__ __forceinline__ uint32_t pair(int j, int c) const { return w[j][c]; }
+  template <int DT> __device__ __forceinline__ void widen(int c, uint32_t (&x)[8]) const {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = w[j][c];
+  }
 };
+// 8 bits: the scales of four tokens in a row come with one load.
 template <int D> struct ValueRegs<D, true> {
-  uint32_t w[8][D / 64];
-  uint32_t scale[8];
-  __device__ __forceinline__ void load(const Stream& s, int t0, int last) {
-    const int lane = threadIdx.x & 63;
+  static constexpr int WORDS = D / 64;  // a token's scales: 4 or 2 bytes
+  uint32_t w[8][WORDS];
+  uint32_t scale[2][2 * WORDS];  // of tokens 4q.. and 16+4q..
+  __device__ __forceinline__ void load(const Stream& s, int64_t t, const LaneOffsets<D, true>& at) {
+    const uint8_t *base = s.v + t * D, *scales = s.vs + t * (D / kMxGroup);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int t = min(t0 + (j < 4 ? 0 : 16) + 4 * (lane >> 4) + (j & 3), last);
-      const int64_t at = (int64_t)t * D + (lane & 15) * (D / 16);
       if constexpr (D == 128) {
-        const uint2 x = *(const uint2*)(s.v + at);
+        const uint2 x = *(const uint2*)(base + at.value[j]);
         w[j][0] = x.x, w[j][1] = x.y;
       } else {
-        w[j][0] = *(const uint32_t*)(s.v + at);
+        w[j][0] = *(const uint32_t*)(base + at.value[j]);
       }
-      scale[j] = s.vs[at / kMxGroup];
+    }
+    if (!at.cut) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        __builtin_memcpy(scale[u], scales + (uint32_t)(((threadIdx.x & 48) / 4 + 16 * u) * (D / kMxGroup)), sizeof(scale[u]));
+    } else {  // token by token: the four may not all be there
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t row = at.value[4 * u + j] / D * (D / kMxGroup);
+          if constexpr (D == 128) {
+            __builtin_memcpy(&scale[u][j], scales + row, 4);
+          } else {
+            uint16_t x;
+            __builtin_memcpy(&x, scales + row, 2);
+            scale[u][j / 2] = j & 1 ? scale[u][j / 2] | (uint32_t)x << 16 : x;
+          }
+        }
     }
   }
-  __device__ __forceinline__ void clear(int j) {
+  __device__ __forceinline__ void clear(int j) {  // a code of zero: nothing under any scale but 0xff, which NaN would be
 #pragma unroll
-    for (int c = 0; c < D / 64; ++c) w[j][c] = 0;
-    scale[j] = 127;
+    for (int c = 0; c < WORDS; ++c) w[j][c] = 0;
   }
-  template <int DT> __device__ __forceinline__ uint32_t pair(int j, int c) const {
-    const float f = lkv::mx_scale(scale[j]);
-    return c & 1 ? Mat<DT>::template widen<true>(w[j][c / 2], f) : Mat<DT>::template widen<false>(w[j][c / 2], f);
+  template <int DT> __device__ __forceinline__ void widen(int c, uint32_t (&x)[8]) const {
+    const int mine = (threadIdx.x & 15) * (D / 16) / kMxGroup * 8;  // this lane's scale in a token's
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t word = D == 128 ? scale[j / 4][j & 3] : scale[j / 4][(j & 3) / 2] >> (16 * (j & 1));
+      const float f = lkv::bits_to_float((word >> mine) << 23 & 0x7f800000u);
+      x[j] = c & 1 ? Mat<DT>::template widen<true>(w[j][c / 2], f) : Mat<DT>::template widen<false>(w[j][c / 2], f);
+    }
   }
 };
 
@@ -194,9 +230,44 @@ template <int D> struct ValueRegs<D, true> {
 // channel (d/4) q + (d/16) i + e in o[n][e][i].
 template <int D, int NR> struct Result {
   f32x4 o[NR][D / 16];
-  float m[NR];  // the maximum so far, in base 2
+  float m[NR];  // the rows' reference, in base 2: the maximum of some tile so far, at most kSlack below any score
   float l[NR];  // this lane's tokens' part of the sum
 };
+
+// A tile's scores of one row tile to weights, the second product's operand; m, l and o follow. `left`: tokens that the
+// tile has, if fewer than 32.
+template <int DT, int D>
+__device__ __forceinline__ uint4 weigh(f32x4 (&sc)[2], int left, float scale2, float& m, float& l, f32x4 (&o)[D / 16]) {
+  // Scaled before they are compared: as s * scale2 - m in one step, large scores' rounding in m alone would leave
+  // the largest weight far from 1.
+  sc[0] *= scale2;
+  sc[1] *= scale2;
+  if (left < kTile) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if ((j < 4 ? 0 : 16) + (int)(threadIdx.x & 48) / 4 + (j & 3) >= left) sc[j / 4][j & 3] = -INFINITY;
+  }
+  const float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])), fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+  // The reference of a row's weights need not be its maximum, only near it: it moves when a score is
+  // more than kSlack above it, so that most tiles pass without a look at the other lanes.
+  if (__any(top > m + kSlack)) {
+    const float up = fmaxf(lkv::pair_max<32>(lkv::pair_max<16>(top)), m);
+    const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - up);
+    m = up;
+    l *= keep;
+#pragma unroll
+    for (int e = 0; e < D / 16; ++e) o[e] *= keep;
+  }
+  const float base = m == -INFINITY ? 0.0f : m;
+  float w[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) w[j] = __builtin_amdgcn_exp2f(sc[j / 4][j & 3] - base);
+  l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+  return make_uint4(Mat<DT>::pack(w[0], w[1]), Mat<DT>::pack(w[2], w[3]), Mat<DT>::pack(w[4], w[5]), Mat<DT>::pack(w[6], w[7]));
+}
+
+// Loads stay on their side: moved down to where the next tile uses them, they would be waited for.
+__device__ __forceinline__ void load_fence() { asm volatile("" ::: "memory"); }
 
 // Tokens first, first + step, ... (tiles of 32) below end, for rows q[n].
 template <int DT, int D, bool MX, int NR>
@@ -219,8 +290,11 @@ __device__ __forceinline__ void attend_range(const Stream& s, const uint16_t* co
       qf[n][i] = q[n] ? *(const uint4*)(q[n] + KeyRegs<D, MX>::channel(quarter, i)) : make_uint4(0, 0, 0, 0);
   KeyRegs<D, MX> k;
   ValueRegs<D, MX> v;
-  k.load(s, first, end - 1);
-  v.load(s, first, end - 1);
+  LaneOffsets<D, MX> at;
+  at.set(min(kTile, end - first) - 1);
+  k.load(s, first, at);
+  v.load(s, first, at);
+  load_fence();
   for (int t = first; t < end; t += step) {
     f32x4 sc[NR][2];
 #pragma unroll
@@ -233,46 +307,24 @@ __device__ __forceinline__ void attend_range(const Stream& s, const uint16_t* co
 #pragma unroll
         for (int n = 0; n < NR; ++n) sc[n][u] = Mat<DT>::mma(a, qf[n][i], sc[n][u]);
       }
-    k.load(s, t + step, end - 1);
-    if (t + kTile > end) {  // tokens behind the end: no weight, and no value that a weight of 0 could turn to NaN
+    // The next tile's keys are under way while this one's weights are computed, its values from the end of
+    // this tile's products on. Behind the last tile that tile's own rows are read again.
+    const int next = t + step < end ? t + step : t;
+    if (next + kTile > end) at.set(end - next - 1);
+    k.load(s, next, at);
+    load_fence();
+    if (t + kTile > end) {  // tokens behind the end: no value that a weight of 0 could turn to NaN
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const bool live = t + (j < 4 ? 0 : 16) + 4 * quarter + (j & 3) < end;
-        if (!live) v.clear(j);
-#pragma unroll
-        for (int n = 0; n < NR; ++n) sc[n][j / 4][j & 3] = live ? sc[n][j / 4][j & 3] : -INFINITY;
-      }
+      for (int j = 0; j < 8; ++j)
+        if (t + (j < 4 ? 0 : 16) + 4 * quarter + (j & 3) >= end) v.clear(j);
     }
     uint4 p[NR];
 #pragma unroll
-    for (int n = 0; n < NR; ++n) {
-      // Scaled before they are compared: as s * scale2 - m in one step, large scores' rounding in m alone would leave
-      // the largest weight far from 1.
-      sc[n][0] *= scale2;
-      sc[n][1] *= scale2;
-      float top = fmaxf(fmaxf(fmaxf(sc[n][0][0], sc[n][0][1]), fmaxf(sc[n][0][2], sc[n][0][3])),
-                        fmaxf(fmaxf(sc[n][1][0], sc[n][1][1]), fmaxf(sc[n][1][2], sc[n][1][3])));
-      top = lkv::pair_max<32>(lkv::pair_max<16>(top));
-      if (__any(top > r.m[n])) {
-        const float next = fmaxf(top, r.m[n]);
-        const float keep = r.m[n] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(r.m[n] - next);
-        r.m[n] = next;
-        r.l[n] *= keep;
-#pragma unroll
-        for (int e = 0; e < D / 16; ++e) r.o[n][e] *= keep;
-      }
-      const float base = r.m[n] == -INFINITY ? 0.0f : r.m[n];
-      float w[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = __builtin_amdgcn_exp2f(sc[n][j / 4][j & 3] - base);
-      r.l[n] += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-      p[n] = make_uint4(Mat<DT>::pack(w[0], w[1]), Mat<DT>::pack(w[2], w[3]), Mat<DT>::pack(w[4], w[5]), Mat<DT>::pack(w[6], w[7]));
-    }
+    for (int n = 0; n < NR; ++n) p[n] = weigh<DT, D>(sc[n], end - t, scale2, r.m[n], r.l[n], r.o[n]);
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
       uint32_t x[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = v.template pair<DT>(j, c);
+      v.template widen<DT>(c, x);
       uint4 even, odd;
       even = make_uint4(__builtin_amdgcn_perm(x[1], x[0], 0x05040100u), __builtin_amdgcn_perm(x[3], x[2], 0x05040100u),
                         __builtin_amdgcn_perm(x[5], x[4], 0x05040100u), __builtin_amdgcn_perm(x[7], x[6], 0x05040100u));
@@ -284,7 +336,8 @@ __device__ __forceinline__ void attend_range(const Stream& s, const uint16_t* co
         r.o[n][2 * c + 1] = Mat<DT>::mma(odd, p[n], r.o[n][2 * c + 1]);
       }
     }
-    v.load(s, t + step, end - 1);
+    v.load(s, next, at);
+    load_fence();
   }
 #pragma unroll
   for (int n = 0; n < NR; ++n) r.l[n] = lkv::pair_sum<32>(lkv::pair_sum<16>(r.l[n]));
@@ -294,94 +347,93 @@ __device__ __forceinline__ float join_factor(float m, float l, float top) {
   return m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(m - top);
 }
 
-// The waves' results into wave 0's: waves 2 and 3 to 0 and 1, then 1 to 0, lane by lane.
-template <int D, int NR>
-__device__ __forceinline__ void join_waves(Result<D, NR>& r, f32x4* so, float2* sml) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// The results of wave groups 0 .. GROUPS - 1 into group 0's, lane by lane: the upper half's into the lower's,
+// and so on. `slot`: the wave's place in its group of `width`.
+template <int D, int NR, int GROUPS>
+__device__ __forceinline__ void join_waves(Result<D, NR>& r, int group, int slot, int width, f32x4* lds) {
+  const int lane = threadIdx.x & 63;
   constexpr int PER = NR * (D / 16);
+  float2* const sml = (float2*)(lds + (GROUPS / 2) * width * PER * 64);
 #pragma unroll
-  for (int half = kWaves / 2; half > 0; half /= 2) {
+  for (int half = GROUPS / 2; half > 0; half /= 2) {
     __syncthreads();
-    if (wave >= half && wave < 2 * half) {
+    if (group >= half && group < 2 * half) {
+      const int to = (group - half) * width + slot;
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
-        sml[((wave - half) * NR + n) * 64 + lane] = make_float2(r.m[n], r.l[n]);
+        sml[(to * NR + n) * 64 + lane] = make_float2(r.m[n], r.l[n]);
 #pragma unroll
-        for (int e = 0; e < D / 16; ++e) so[((wave - half) * PER + n * (D / 16) + e) * 64 + lane] = r.o[n][e];
+        for (int e = 0; e < D / 16; ++e) lds[(to * PER + n * (D / 16) + e) * 64 + lane] = r.o[n][e];
       }
     }
     __syncthreads();
-    if (wave < half) {
+    if (group < half) {
+      const int from = group * width + slot;
 #pragma unroll
       for (int n = 0; n < NR; ++n) {
-        const float2 other = sml[(wave * NR + n) * 64 + lane];
+        const float2 other = sml[(from * NR + n) * 64 + lane];
         const float top = fmaxf(r.m[n], other.x);
         const float f = join_factor(r.m[n], r.l[n], top), fo = join_factor(other.x, other.y, top);
         r.m[n] = top;
         r.l[n] = r.l[n] * f + other.y * fo;
 #pragma unroll
-        for (int e = 0; e < D / 16; ++e) r.o[n][e] = r.o[n][e] * f + so[(wave * PER + n * (D / 16) + e) * 64 + lane] * fo;
+        for (int e = 0; e < D / 16; ++e) r.o[n][e] = r.o[n][e] * f + lds[(from * PER + n * (D / 16) + e) * 64 + lane] * fo;
       }
     }
   }
 }
+constexpr int join_bytes(int d, int nr, int groups, int width) { return (groups / 2) * width * nr * 64 * (d / 16 * 16 + 8); }
 
-// A row's result: the output itself where this is its only part.
-template <int D>
+// A row's result: the output itself where this is its only part. TILED: channels 16 e + 4 q + i in o[e][i], else
+// (d/4) q + (d/16) i + e.
+template <int D, bool TILED>
 __device__ __forceinline__ void store_row(const SharedArgs& a, int64_t row, int part, float m, float l, const f32x4 (&o)[D / 16]) {
   const int parts = a.p_parts + a.o_parts, quarter = (threadIdx.x & 63) >> 4;
-  if (parts == 1) {
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int64_t at = row * D + quarter * (D / 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int e = 0; e < D / 16; ++e) lkv::store_any(a.out, at + (D / 16) * i + e, a.out_dtype, l == 0.0f ? 0.0f : o[e][i] * inv);
-    if (quarter == 0) a.lse[row] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * lkv::kLn2;
-    return;
+  const bool last = parts == 1;
+  const int64_t slot = last ? row : row * parts + part;
+  const float inv = !last ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
+  if (quarter == 0) {
+    if (last) {
+      a.lse[row] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * lkv::kLn2;
+    } else {
+      a.part_ml[slot] = make_float2(m, l);
+    }
   }
-  const int64_t slot = row * parts + part;
-  if (quarter == 0) a.part_ml[slot] = make_float2(m, l);
-  float* to = a.part_o + slot * D + quarter * (D / 4);
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int k = 0; k < D / 16; ++k) {
+    f32x4 x;
+    int c;
+    if constexpr (TILED) {
+      x = o[k];
+      c = 16 * k + 4 * quarter;
+    } else {
+      constexpr int E = D / 64;  // groups of four e for an i
+      const int i = k / E, e = k % E * 4;
+      x = f32x4{o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]};
+      c = (D / 4) * quarter + (D / 16) * i + e;
+    }
+    if (last) {
 #pragma unroll
-    for (int e = 0; e < D / 16; e += 4) *(f32x4*)(to + (D / 16) * i + e) = f32x4{o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]};
+      for (int i = 0; i < 4; ++i) lkv::store_any(a.out, slot * D + c + i, a.out_dtype, l == 0.0f ? 0.0f : x[i] * inv);
+    } else {
+      *(f32x4*)(a.part_o + slot * D + c) = x;
+    }
+  }
 }
 
-template <int DT, int D, bool PMX, bool OMX, int NR>
-__global__ __launch_bounds__(256, NR == 4 ? 1 : 2) void shared_decode_kernel(SharedArgs a) {
-  __shared__ f32x4 so[(kWaves / 2) * NR * (D / 16) * 64];
-  __shared__ float2 sml[(kWaves / 2) * NR * 64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int id = blockIdx.x;
-  const int p_blocks = a.p_groups * 8 * a.row_tiles;
-  if (id < p_blocks) {
-    // Workgroups go round the 8 XCDs by their number: the row tiles of one head and token range sit on
-    // one of them, one after the other, and find its keys and values in that L2.
-    const int unit = (id / (8 * a.row_tiles)) * 8 + id % 8, tile = id / 8 % a.row_tiles;
-    if (unit >= a.p_parts * a.n_kv) return;
-    const int part = unit / a.n_kv, h = unit % a.n_kv;
-    const uint16_t* q[NR];
-    int64_t row[NR];
-#pragma unroll
-    for (int n = 0; n < NR; ++n) {
-      const int x = (tile * NR + n) * 16 + (lane & 15), b = x / a.g;
-      row[n] = b < a.n_seqs ? (int64_t)b * a.n_q + h * a.g + (x - b * a.g) : -1;
-      q[n] = row[n] >= 0 ? a.q + row[n] * D : nullptr;
-    }
-    const int t0 = part * a.p_chunk, end = min(t0 + a.p_chunk, a.prefix_tokens);
-    Result<D, NR> r;
-    attend_range<DT, D, PMX, NR>(stream_of<D, PMX>(a.prefix, 0, h), q, t0 + wave * kTile, kWaves * kTile, end, a.scale2, r);
-    join_waves<D, NR>(r, so, sml);
-    if (wave == 0) {
-#pragma unroll
-      for (int n = 0; n < NR; ++n)
-        if (row[n] >= 0) store_row<D>(a, row[n], part, r.m[n], r.l[n], r.o[n]);
-    }
-    return;
-  }
-  id -= p_blocks;
+// A KV head's query row x of the prefix's: row x of all sequences', g a sequence; -1 behind the last.
+__device__ __forceinline__ int64_t prefix_row(const SharedArgs& a, int h, int x) {
+  const int b = x / a.g;
+  return b < a.n_seqs ? (int64_t)b * a.n_q + h * a.g + (x - b * a.g) : -1;
+}
+
+// The `item`-th piece of own rows, by four waves; `join`: the item's place in its workgroup's LDS. Every wave of the
+// workgroup takes part in the joins' barriers.
+template <int DT, int D, bool OMX>
+__device__ __forceinline__ void own_item(const SharedArgs& a, int64_t item, int wave, f32x4* join) {
+  const int lane = threadIdx.x & 63;
+  const bool live = item < (int64_t)a.n_seqs * a.n_kv * a.g_tiles * a.o_parts;
+  int id = live ? (int)item : 0;
   const int part = id % a.o_parts;
   id /= a.o_parts;
   const int tile = id % a.g_tiles;
@@ -389,38 +441,251 @@ __global__ __launch_bounds__(256, NR == 4 ? 1 : 2) void shared_decode_kernel(Sha
   const int h = id % a.n_kv, b = id / a.n_kv;
   const int j = tile * 16 + (lane & 15);
   const int64_t row = (int64_t)b * a.n_q + h * a.g + j;
-  const int t0 = part * a.o_chunk, end = min(t0 + a.o_chunk, own_length(a, b));
+  const int t0 = part * a.o_chunk, end = live ? min(t0 + a.o_chunk, own_length(a, b)) : 0;
   const uint16_t* q[1] = {j < a.g ? a.q + row * D : nullptr};
   Result<D, 1> r;
   attend_range<DT, D, OMX, 1>(stream_of<D, OMX>(a.own, b, h), q, t0 + wave * kTile, kWaves * kTile, end, a.scale2, r);
-  join_waves<D, 1>(r, so, sml);
-  if (wave == 0 && j < a.g) store_row<D>(a, row, a.p_parts + part, r.m[0], r.l[0], r.o[0]);
+  join_waves<D, 1, kWaves>(r, wave, 0, 1, join);
+  if (live && wave == 0 && j < a.g) store_row<D, false>(a, row, a.p_parts + part, r.m[0], r.l[0], r.o[0]);
 }
 
-// A wave a query row: its parts' results into one.
+template <int DT, int D, bool PMX, bool OMX, int NR>
+__global__ __launch_bounds__(256, 2) void shared_decode_kernel(SharedArgs a) {
+  __shared__ f32x4 join[join_bytes(D, NR, kWaves, 1) / 16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int id = blockIdx.x, p_blocks = a.p_groups * 8 * a.row_tiles;
+  if (id >= p_blocks) return own_item<DT, D, OMX>(a, id - p_blocks, wave, join);
+  // Workgroups go round the 8 XCDs by their number: the row tiles of one head and token range sit on
+  // one of them, one after the other, and find its keys and values in that L2.
+  const int unit = (id / (8 * a.row_tiles)) * 8 + id % 8, tile = id / 8 % a.row_tiles;
+  if (unit >= a.p_parts * a.n_kv) return;
+  const int part = unit / a.n_kv, h = unit % a.n_kv;
+  const uint16_t* q[NR];
+  int64_t row[NR];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    row[n] = prefix_row(a, h, (tile * NR + n) * 16 + (lane & 15));
+    q[n] = row[n] >= 0 ? a.q + row[n] * D : nullptr;
+  }
+  const int t0 = part * a.p_chunk, end = min(t0 + a.p_chunk, a.prefix_tokens);
+  Result<D, NR> r;
+  attend_range<DT, D, PMX, NR>(stream_of<D, PMX>(a.prefix, 0, h), q, t0 + wave * kTile, kWaves * kTile, end, a.scale2, r);
+  join_waves<D, NR, kWaves>(r, wave, 0, 1, join);
+  if (wave == 0) {
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+      if (row[n] >= 0) store_row<D, false>(a, row[n], part, r.m[n], r.l[n], r.o[n]);
+  }
+}
+
+// ---- many rows: the prefix through LDS --------------------------------------------------------------
+// Each wave on its own stream of tokens reads all keys and values for its 32 rows alone: with many rows of
+// a head, the reads from L2 bound that (10 TB/s over all row tiles). Here a workgroup of eight waves, WR across 32 rows each and
+// WT = 8 / WR across tokens, stages its tokens' keys and values in LDS once, in the model dtype (8-bit
+// rows are widened on the way, once for all rows). 16-byte pieces are swizzled by the row, so that the 16
+// tokens of an operand lie in different banks; the values' operands are read transposed.
+template <int D, int WR> struct Stage {
+  static constexpr int WT = 8 / WR;
+  static constexpr int TOKENS = WR == 2 ? 128 : 64;
+  static constexpr int TILES = TOKENS / (kTile * WT);      // of a wave in a stage
+  static constexpr int PIECES = D / 8;                     // 16-byte pieces of a row
+  static constexpr int LOADS = TOKENS * PIECES / 512;      // of a thread, for keys and for values
+  static constexpr int BYTES = TOKENS * 2 * D;             // of keys, and of values
+  static __device__ __forceinline__ int swizzle(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
+};
+
+template <int DT, int D, bool MX, int WR> struct StageRegs {
+  using S = Stage<D, WR>;
+  uint4 k[S::LOADS], v[S::LOADS];  // 8 bits: codes in x and y, the scale in z
+  // Tokens t0 .. of the stream; behind `end`, its last token.
+  __device__ __forceinline__ void load(const Stream& s, int t0, int end) {
+    const int last = min(S::TOKENS, end - t0) - 1;
+#pragma unroll
+    for (int i = 0; i < S::LOADS; ++i) {
+      const int x = i * 512 + threadIdx.x, row = min(x / S::PIECES, last), piece = x % S::PIECES;
+      if constexpr (MX) {
+        const uint32_t at = (uint32_t)(row * D + piece * 8);
+        const uint8_t *kb = s.k + (int64_t)t0 * D, *vb = s.v + (int64_t)t0 * D;
+        const uint8_t *ks = s.ks + (int64_t)t0 * (D / kMxGroup), *vs = s.vs + (int64_t)t0 * (D / kMxGroup);
+        const uint2 a = *(const uint2*)(kb + at), b = *(const uint2*)(vb + at);
+        k[i] = make_uint4(a.x, a.y, ks[at / kMxGroup], 0);
+        v[i] = make_uint4(b.x, b.y, vs[at / kMxGroup], 0);
+      } else {
+        const uint32_t at = (uint32_t)(row * (2 * D) + piece * 16);
+        k[i] = *(const uint4*)(s.k + (int64_t)t0 * (2 * D) + at);
+        v[i] = *(const uint4*)(s.v + (int64_t)t0 * (2 * D) + at);
+      }
+    }
+  }
+  static __device__ __forceinline__ uint4 widen(uint4 x) {
+    if constexpr (MX) {
+      const float f = lkv::bits_to_float(x.z << 23);
+      return make_uint4(Mat<DT>::template widen<false>(x.x, f), Mat<DT>::template widen<true>(x.x, f), Mat<DT>::template widen<false>(x.y, f),
+                        Mat<DT>::template widen<true>(x.y, f));
+    }
+    return x;
+  }
+  // Into LDS; values of tokens behind the end as zeros, which a weight of 0 leaves.
+  __device__ __forceinline__ void store(uint8_t* lds, int live) const {
+#pragma unroll
+    for (int i = 0; i < S::LOADS; ++i) {
+      const int x = i * 512 + threadIdx.x, row = x / S::PIECES, piece = (x % S::PIECES) ^ S::swizzle(row);
+      uint8_t* to = lds + row * (2 * D) + piece * 16;
+      *(uint4*)to = widen(k[i]);
+      *(uint4*)(to + S::BYTES) = row < live ? widen(v[i]) : make_uint4(0, 0, 0, 0);
+    }
+  }
+};
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+// Four tokens of one channel a lane, of a 4 x 16 piece whose rows the 16 lanes name eight bytes of.
+__device__ __forceinline__ uint2 read_transposed(const uint8_t* p) {
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+}
+
+template <int DT, int D, bool MX, int WR>
+__device__ __forceinline__ void attend_wide(const Stream& s, const uint16_t* const (&q)[2], int t0, int end, int wt, float scale2, Result<D, 2>& r,
+                                            uint8_t* lds) {
+  using S = Stage<D, WR>;
+  const int lane = threadIdx.x & 63, quarter = lane >> 4;
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    r.m[n] = -INFINITY;
+    r.l[n] = 0.0f;
+#pragma unroll
+    for (int e = 0; e < D / 16; ++e) r.o[n][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  uint4 qf[2][D / 32];
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) qf[n][i] = q[n] ? *(const uint4*)(q[n] + 32 * i + 8 * quarter) : make_uint4(0, 0, 0, 0);
+  // A lane's places in a tile of 32 tokens: keys of token lane % 16 (and 16 on), values of token 4 q + (lane % 16) / 4.
+  uint32_t key_at[D / 32], value_at[D / 16];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) key_at[i] = (lane & 15) * (2 * D) + ((4 * i + quarter) ^ S::swizzle(lane & 15)) * 16;
+#pragma unroll
+  for (int e = 0; e < D / 16; ++e) {
+    const int row = 4 * quarter + ((lane & 15) >> 2);
+    value_at[e] = S::BYTES + row * (2 * D) + ((2 * e + ((lane & 2) >> 1)) ^ S::swizzle(row)) * 16 + (lane & 1) * 8;
+  }
+  StageRegs<DT, D, MX, WR> regs;
+  regs.load(s, t0, end);
+  int buffer = 0;
+  for (int t = t0; t < end; t += S::TOKENS) {
+    uint8_t* const now = lds + buffer * (2 * S::BYTES);
+    regs.store(now, end - t);
+    __syncthreads();  // and the other buffer is read no more: its readers have passed this one's barrier before
+    if (t + S::TOKENS < end) regs.load(s, t + S::TOKENS, end);
+    load_fence();
+    buffer ^= 1;
+#pragma unroll
+    for (int tile = 0; tile < S::TILES; ++tile) {
+      const int first = (tile * S::WT + wt) * kTile;  // of the stage's tokens
+      const uint8_t* const base = now + first * (2 * D);
+      if (t + first >= end) break;
+      f32x4 sc[2][2];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) sc[n][0] = sc[n][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          const uint4 k = *(const uint4*)(base + key_at[i] + u * 16 * (2 * D));
+#pragma unroll
+          for (int n = 0; n < 2; ++n) sc[n][u] = Mat<DT>::mma(k, qf[n][i], sc[n][u]);
+        }
+      const int left = end - t - first;
+      uint4 p[2];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) p[n] = weigh<DT, D>(sc[n], left, scale2, r.m[n], r.l[n], r.o[n]);
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) {
+        const uint2 lo = read_transposed(base + value_at[e]), hi = read_transposed(base + value_at[e] + 16 * (2 * D));
+        const uint4 v = make_uint4(lo.x, lo.y, hi.x, hi.y);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) r.o[n][e] = Mat<DT>::mma(v, p[n], r.o[n][e]);
+      }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < 2; ++n) r.l[n] = lkv::pair_sum<32>(lkv::pair_sum<16>(r.l[n]));
+}
+
+template <int DT, int D, bool PMX, bool OMX, int WR>
+__global__ __launch_bounds__(512, 2) void shared_wide_kernel(SharedArgs a) {
+  using S = Stage<D, WR>;
+  constexpr int STAGES = 2 * 2 * S::BYTES, JOIN = join_bytes(D, 2, S::WT, WR), OWN = join_bytes(D, 1, kWaves, 1);
+  constexpr int BYTES = STAGES > JOIN ? (STAGES > 2 * OWN ? STAGES : 2 * OWN) : (JOIN > 2 * OWN ? JOIN : 2 * OWN);
+  __shared__ f32x4 lds[BYTES / 16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int id = blockIdx.x, p_blocks = a.p_groups * 8 * a.row_tiles;
+  if (id >= p_blocks) return own_item<DT, D, OMX>(a, (int64_t)(id - p_blocks) * 2 + wave / kWaves, wave % kWaves, lds + wave / kWaves * (OWN / 16));
+  const int unit = (id / (8 * a.row_tiles)) * 8 + id % 8, tile = id / 8 % a.row_tiles;
+  if (unit >= a.p_parts * a.n_kv) return;
+  const int part = unit / a.n_kv, h = unit % a.n_kv, wr = wave % WR, wt = wave / WR;
+  const uint16_t* q[2];
+  int64_t row[2];
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    row[n] = prefix_row(a, h, ((tile * WR + wr) * 2 + n) * 16 + (lane & 15));
+    q[n] = row[n] >= 0 ? a.q + row[n] * D : nullptr;
+  }
+  const int t0 = part * a.p_chunk, end = min(t0 + a.p_chunk, a.prefix_tokens);
+  Result<D, 2> r;
+  attend_wide<DT, D, PMX, WR>(stream_of<D, PMX>(a.prefix, 0, h), q, t0, end, wt, a.scale2, r, (uint8_t*)lds);
+  join_waves<D, 2, S::WT>(r, wt, wr, WR, lds);
+  if (wt == 0) {
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+      if (row[n] >= 0) store_row<D, true>(a, row[n], part, r.m[n], r.l[n], r.o[n]);
+  }
+}
+
+// A workgroup a query row: its parts' results into one. d/4 threads take a part's channels, four each, and
+// the threads' groups the parts in turn, so that all loads of 64 parts are in flight together.
 template <int D>
 __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= (int64_t)a.n_seqs * a.n_q) return;
-  const int lane = threadIdx.x & 63, parts = a.p_parts + a.o_parts;
+  constexpr int C = D / 4, GROUPS = 256 / C;
+  __shared__ f32x4 red[GROUPS][C];
+  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x & 63, parts = a.p_parts + a.o_parts, group = threadIdx.x / C, c = threadIdx.x % C;
   const float2* ml = a.part_ml + row * parts;
   float top = -INFINITY;
   for (int p = lane; p < parts; p += 64) top = fmaxf(top, ml[p].x);
   top = lkv::wave_max_f32(top);
-  float total = 0.0f, o[D / 64] = {};
-  const float* from = a.part_o + row * parts * D + lane * (D / 64);
-  for (int p = 0; p < parts; ++p) {
-    const float2 x = ml[p];
-    if (x.y == 0.0f) continue;
-    const float f = join_factor(x.x, x.y, top);
-    total += f * x.y;
+  float total = 0.0f;
+  f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  const float* from = a.part_o + row * parts * D + c * 4;
+  for (int p0 = 0; p0 < parts; p0 += 64) {
+    float f = 0.0f;
+    if (p0 + lane < parts) {
+      const float2 x = ml[p0 + lane];
+      f = join_factor(x.x, x.y, top);
+      total += x.y == 0.0f ? 0.0f : f * x.y;
+    }
+    f32x4 x[64 / GROUPS];
+    float w[64 / GROUPS];
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) o[i] += f * from[(int64_t)p * D + i];
+    for (int i = 0; i < 64 / GROUPS; ++i) {
+      const int p = p0 + i * GROUPS + group;
+      w[i] = __shfl(f, i * GROUPS + group);
+      // A part without weight is not read: an empty one holds zeros, and another's f is 0 from 150 powers of two below.
+      x[i] = p < parts && w[i] != 0.0f ? *(const f32x4*)(from + (int64_t)p * D) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+#pragma unroll
+    for (int i = 0; i < 64 / GROUPS; ++i) o += x[i] * w[i];
   }
+  red[group][c] = o;
+  total = lkv::wave_sum_f32(total);
+  __syncthreads();
+  if (threadIdx.x >= C) return;
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i)
-    lkv::store_any(a.out, row * D + lane * (D / 64) + i, a.out_dtype, total == 0.0f ? 0.0f : o[i] / total);
-  if (lane == 0) a.lse[row] = total == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * lkv::kLn2;
+  for (int i = 1; i < GROUPS; ++i) o += red[i][c];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) lkv::store_any(a.out, row * D + c * 4 + i, a.out_dtype, total == 0.0f ? 0.0f : o[i] / total);
+  if (threadIdx.x == 0) a.lse[row] = total == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * lkv::kLn2;
 }
 
 int check_desc(const lkv_shared_desc* d) {
@@ -441,24 +706,28 @@ int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 // How a call is divided: see SharedArgs.
 struct Plan {
-  int nr, row_tiles, p_parts, p_chunk, p_groups, g_tiles, o_parts, o_chunk;
+  int nr;  // tiles of 16 rows of a wave, on its own stream; 0: through LDS
+  int wr;  // there, waves across rows
+  int row_tiles, p_parts, p_chunk, p_groups, g_tiles, o_parts, o_chunk;
 };
 
 Plan plan_of(const lkv_shared_desc* d) {
   Plan p = {};
   const int g = d->n_q / d->n_kv;
   const int64_t rows = (int64_t)d->n_seqs * g;
-  p.nr = d->prefix_tokens == 0 || rows <= 16 ? 1 : (rows <= 32 ? 2 : 4);
-  p.row_tiles = ceil_div(rows, 16 * p.nr);
+  p.nr = d->prefix_tokens == 0 || rows <= 16 ? 1 : (rows <= 32 ? 2 : 0);
+  p.wr = rows <= 64 ? 2 : 4;
+  p.row_tiles = ceil_div(rows, p.nr ? 16 * p.nr : 32 * p.wr);
   p.g_tiles = ceil_div(g, 16);
   // Tokens that a workgroup takes: as many workgroups as the card holds at once, and no fewer than one tile
   // a wave.
-  const int64_t room = p.nr == 4 ? 256 : 512;
-  const int64_t tokens = (int64_t)p.row_tiles * d->n_kv * d->prefix_tokens + (int64_t)d->n_seqs * d->n_kv * p.g_tiles * d->max_own;
+  const int64_t room = p.nr == 1 ? 768 : (p.nr == 2 ? 512 : 256);
+  const int64_t tokens = (int64_t)p.row_tiles * d->n_kv * d->prefix_tokens + (p.nr ? (int64_t)d->n_seqs * d->n_kv * p.g_tiles * d->max_own : 0);
   const int64_t least = kWaves * kTile;
   int64_t chunk = (tokens / room + least - 1) / least * least;
   if (chunk < least) chunk = least;
   p.p_chunk = p.o_chunk = (int)(chunk > (1 << 30) ? (1 << 30) : chunk);
+  if (!p.nr) p.o_chunk = 1024;
   p.p_parts = ceil_div(d->prefix_tokens, p.p_chunk);
   p.o_parts = ceil_div(d->max_own, p.o_chunk);
   p.p_groups = ceil_div((int64_t)p.p_parts * d->n_kv, 8);
@@ -466,17 +735,18 @@ Plan plan_of(const lkv_shared_desc* d) {
 }
 
 template <int DT, int D, bool PMX, bool OMX>
-void launch(int nr, dim3 grid, hipStream_t s, const SharedArgs& a) {
-  auto kernel = nr == 1 ? shared_decode_kernel<DT, D, PMX, OMX, 1> : nr == 2 ? shared_decode_kernel<DT, D, PMX, OMX, 2> : shared_decode_kernel<DT, D, PMX, OMX, 4>;
-  hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a);
+void launch(const Plan& p, dim3 grid, hipStream_t s, const SharedArgs& a) {
+  auto kernel = p.nr == 1 ? shared_decode_kernel<DT, D, PMX, OMX, 1> : p.nr == 2 ? shared_decode_kernel<DT, D, PMX, OMX, 2>
+              : p.wr == 2 ? shared_wide_kernel<DT, D, PMX, OMX, 2> : p.wr == 4 ? shared_wide_kernel<DT, D, PMX, OMX, 4> : shared_wide_kernel<DT, D, PMX, OMX, 8>;
+  hipLaunchKernelGGL(kernel, grid, dim3(p.nr ? 256 : 512), 0, s, a);
 }
 
 template <int DT, int D>
-void launch(bool pmx, bool omx, int nr, dim3 grid, hipStream_t s, const SharedArgs& a) {
+void launch(bool pmx, bool omx, const Plan& p, dim3 grid, hipStream_t s, const SharedArgs& a) {
   if (pmx) {
-    omx ? launch<DT, D, true, true>(nr, grid, s, a) : launch<DT, D, true, false>(nr, grid, s, a);
+    omx ? launch<DT, D, true, true>(p, grid, s, a) : launch<DT, D, true, false>(p, grid, s, a);
   } else {
-    omx ? launch<DT, D, false, true>(nr, grid, s, a) : launch<DT, D, false, false>(nr, grid, s, a);
+    omx ? launch<DT, D, false, true>(p, grid, s, a) : launch<DT, D, false, false>(p, grid, s, a);
   }
 }
 
@@ -516,8 +786,9 @@ extern "C" int lkv_shared_decode(uintptr_t stream, const lkv_shared_desc* desc, 
   if (desc->n_seqs == 0) return LKV_OK;
   const Plan p = plan_of(desc);
   const int64_t rows = (int64_t)desc->n_seqs * desc->n_q, parts = p.p_parts + p.o_parts;
-  const int64_t blocks = (int64_t)p.p_groups * 8 * p.row_tiles + (int64_t)desc->n_seqs * desc->n_kv * p.g_tiles * p.o_parts;
-  LKV_CHECK_ARG(blocks < (1LL << 31) && rows * parts < (1LL << 31), "%lld workgroups in one call", (long long)blocks);
+  const int64_t items = (int64_t)desc->n_seqs * desc->n_kv * p.g_tiles * p.o_parts;
+  const int64_t blocks = (int64_t)p.p_groups * 8 * p.row_tiles + (p.nr ? items : (items + 1) / 2);
+  LKV_CHECK_ARG(blocks < (1LL << 31) && items < (1LL << 31) && rows * parts < (1LL << 31), "%lld workgroups in one call", (long long)blocks);
   a.q = (const uint16_t*)q;
   a.lengths = lengths;
   a.out = out;
@@ -546,15 +817,15 @@ extern "C" int lkv_shared_decode(uintptr_t stream, const lkv_shared_desc* desc, 
     const bool omx = p.o_parts ? own->dtype == LKV_MXFP8 : prefix->dtype == LKV_MXFP8, pmx = p.p_parts ? prefix->dtype == LKV_MXFP8 : omx;
     const dim3 grid((unsigned)blocks);
     if (half) {
-      wide ? launch<LKV_F16, 128>(pmx, omx, p.nr, grid, s, a) : launch<LKV_F16, 64>(pmx, omx, p.nr, grid, s, a);
+      wide ? launch<LKV_F16, 128>(pmx, omx, p, grid, s, a) : launch<LKV_F16, 64>(pmx, omx, p, grid, s, a);
     } else {
-      wide ? launch<LKV_BF16, 128>(pmx, omx, p.nr, grid, s, a) : launch<LKV_BF16, 64>(pmx, omx, p.nr, grid, s, a);
+      wide ? launch<LKV_BF16, 128>(pmx, omx, p, grid, s, a) : launch<LKV_BF16, 64>(pmx, omx, p, grid, s, a);
     }
     LKV_CHECK_LAUNCH("shared_decode");
   }
   if (parts != 1) {
     auto join = wide ? shared_join_kernel<128> : shared_join_kernel<64>;
-    hipLaunchKernelGGL(join, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(join, dim3((unsigned)rows), dim3(256), 0, s, a);
     LKV_CHECK_LAUNCH("shared_decode (join)");
   }
   return LKV_OK;
