@@ -94,6 +94,9 @@ __device__ __forceinline__ Stream stream_of(const lkv_kv_rows& r, int64_t seq, i
           MX ? r.v_scale + e / kMxGroup : nullptr};
 }
 
+// Keeps what a rarely taken branch computes in the branch: as selects it would be in every tile's way.
+template <class T> __device__ __forceinline__ void keep_here(T& x) { asm volatile("" : "+v"(x)); }
+
 // Where a lane's rows of a tile lie, in bytes from the tile's first: fixed but for a tile that the end cuts, whose
 // tokens behind the end read the last one instead.
 template <int D, bool MX> struct LaneOffsets {
@@ -166,9 +169,12 @@ template <int D> struct ValueRegs<D, false> {
       }
     }
   }
-  __device__ __forceinline__ void clear(int j) {
+  __device__ __forceinline__ void keep(int j, bool live) {
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c) w[j][c] = 0;
+    for (int c = 0; c < D / 32; ++c) {
+      w[j][c] = live ? w[j][c] : 0;
+      keep_here(w[j][c]);
+    }
   }
   template <int DT> __device__ __forceinline__ void widen(int c, uint32_t (&x)[8]) const {
 #pragma unroll
@@ -211,9 +217,12 @@ template <int D> struct ValueRegs<D, true> {
         }
     }
   }
-  __device__ __forceinline__ void clear(int j) {  // a code of zero: nothing under any scale but 0xff, which NaN would be
+  __device__ __forceinline__ void keep(int j, bool live) {  // the scales are the last token's there
 #pragma unroll
-    for (int c = 0; c < WORDS; ++c) w[j][c] = 0;
+    for (int c = 0; c < WORDS; ++c) {
+      w[j][c] = live ? w[j][c] : 0;
+      keep_here(w[j][c]);
+    }
   }
   template <int DT> __device__ __forceinline__ void widen(int c, uint32_t (&x)[8]) const {
     const int mine = (threadIdx.x & 15) * (D / 16) / kMxGroup * 8;  // this lane's scale in a token's
@@ -230,38 +239,54 @@ template <int D> struct ValueRegs<D, true> {
 // channel (d/4) q + (d/16) i + e in o[n][e][i].
 template <int D, int NR> struct Result {
   f32x4 o[NR][D / 16];
-  float m[NR];  // the rows' reference, in base 2: the maximum of some tile so far, at most kSlack below any score
+  float m[NR];  // the rows' reference, in base 2: the maximum of some tile, at most kSlack below any score
   float l[NR];  // this lane's tokens' part of the sum
 };
 
-// A tile's scores of one row tile to weights, the second product's operand; m, l and o follow. `left`: tokens that the
-// tile has, if fewer than 32.
+// Rows' reference: what their scores are taken from before the exponential. It need not be a row's maximum, only
+// near it: it moves when a score is more than kSlack (in base 2) above it, so that most tiles pass without a
+// look at the other lanes. The products start from its negative, so that scores come out relative to it.
+struct Reference {
+  f32x4 negative;  // four times -reference, the products' first addend; 0 at first
+  float limit;     // kSlack in scores; -inf until there is a reference
+  __device__ __forceinline__ void reset() {
+    negative = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    limit = -INFINITY;
+  }
+  // The reference in base 2, as partial results carry it.
+  __device__ __forceinline__ float level(float scale2) const { return limit == -INFINITY ? -INFINITY : -negative[0] * scale2; }
+};
+
+// A tile's scores of one row tile, relative to the reference, to weights, the second product's operand; the
+// reference, l and o follow. `left`: tokens that the tile has, if fewer than 32.
 template <int DT, int D>
-__device__ __forceinline__ uint4 weigh(f32x4 (&sc)[2], int left, float scale2, float& m, float& l, f32x4 (&o)[D / 16]) {
-  // Scaled before they are compared: as s * scale2 - m in one step, large scores' rounding in m alone would leave
-  // the largest weight far from 1.
-  sc[0] *= scale2;
-  sc[1] *= scale2;
+__device__ __forceinline__ uint4 weigh(f32x4 (&sc)[2], int left, float scale2, Reference& ref, float& l, f32x4 (&o)[D / 16]) {
   if (left < kTile) {
+    int mine = left - (int)(threadIdx.x & 48) / 4;
+    keep_here(mine);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if ((j < 4 ? 0 : 16) + (int)(threadIdx.x & 48) / 4 + (j & 3) >= left) sc[j / 4][j & 3] = -INFINITY;
+    for (int j = 0; j < 8; ++j) {
+      float x = (j < 4 ? 0 : 16) + (j & 3) < mine ? sc[j / 4][j & 3] : -INFINITY;
+      keep_here(x);
+      sc[j / 4][j & 3] = x;
+    }
   }
   const float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])), fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
-  // The reference of a row's weights need not be its maximum, only near it: it moves when a score is
-  // more than kSlack above it, so that most tiles pass without a look at the other lanes.
-  if (__any(top > m + kSlack)) {
-    const float up = fmaxf(lkv::pair_max<32>(lkv::pair_max<16>(top)), m);
-    const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - up);
-    m = up;
+  if (__any(top > ref.limit)) {
+    const float up = lkv::pair_max<32>(lkv::pair_max<16>(top));
+    const bool move = up > ref.limit && up < INFINITY;
+    const float by = move ? up : 0.0f, keep = ref.limit == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-by * scale2);
+    ref.negative -= by;
+    ref.limit = move ? kSlack / scale2 : ref.limit;
     l *= keep;
 #pragma unroll
     for (int e = 0; e < D / 16; ++e) o[e] *= keep;
+    sc[0] -= by;
+    sc[1] -= by;
   }
-  const float base = m == -INFINITY ? 0.0f : m;
   float w[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) w[j] = __builtin_amdgcn_exp2f(sc[j / 4][j & 3] - base);
+  for (int j = 0; j < 8; ++j) w[j] = __builtin_amdgcn_exp2f(sc[j / 4][j & 3] * scale2);
   l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
   return make_uint4(Mat<DT>::pack(w[0], w[1]), Mat<DT>::pack(w[2], w[3]), Mat<DT>::pack(w[4], w[5]), Mat<DT>::pack(w[6], w[7]));
 }
@@ -282,12 +307,15 @@ __device__ __forceinline__ void attend_range(const Stream& s, const uint16_t* co
     for (int e = 0; e < D / 16; ++e) r.o[n][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
   if (first >= end) return;
+  Reference ref[NR];
   uint4 qf[NR][D / 32];
 #pragma unroll
   for (int n = 0; n < NR; ++n)
 #pragma unroll
     for (int i = 0; i < D / 32; ++i)
       qf[n][i] = q[n] ? *(const uint4*)(q[n] + KeyRegs<D, MX>::channel(quarter, i)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int n = 0; n < NR; ++n) ref[n].reset();
   KeyRegs<D, MX> k;
   ValueRegs<D, MX> v;
   LaneOffsets<D, MX> at;
@@ -298,7 +326,7 @@ __device__ __forceinline__ void attend_range(const Stream& s, const uint16_t* co
   for (int t = first; t < end; t += step) {
     f32x4 sc[NR][2];
 #pragma unroll
-    for (int n = 0; n < NR; ++n) sc[n][0] = sc[n][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int n = 0; n < NR; ++n) sc[n][0] = sc[n][1] = ref[n].negative;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -316,11 +344,11 @@ __device__ __forceinline__ void attend_range(const Stream& s, const uint16_t* co
     if (t + kTile > end) {  // tokens behind the end: no value that a weight of 0 could turn to NaN
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        if (t + (j < 4 ? 0 : 16) + 4 * quarter + (j & 3) >= end) v.clear(j);
+        v.keep(j, t + (j < 4 ? 0 : 16) + 4 * quarter + (j & 3) < end);
     }
     uint4 p[NR];
 #pragma unroll
-    for (int n = 0; n < NR; ++n) p[n] = weigh<DT, D>(sc[n], end - t, scale2, r.m[n], r.l[n], r.o[n]);
+    for (int n = 0; n < NR; ++n) p[n] = weigh<DT, D>(sc[n], end - t, scale2, ref[n], r.l[n], r.o[n]);
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
       uint32_t x[8];
@@ -340,7 +368,10 @@ __device__ __forceinline__ void attend_range(const Stream& s, const uint16_t* co
     load_fence();
   }
 #pragma unroll
-  for (int n = 0; n < NR; ++n) r.l[n] = lkv::pair_sum<32>(lkv::pair_sum<16>(r.l[n]));
+  for (int n = 0; n < NR; ++n) {
+    r.l[n] = lkv::pair_sum<32>(lkv::pair_sum<16>(r.l[n]));
+    r.m[n] = ref[n].level(scale2);
+  }
 }
 
 __device__ __forceinline__ float join_factor(float m, float l, float top) {
@@ -384,40 +415,65 @@ __device__ __forceinline__ void join_waves(Result<D, NR>& r, int group, int slot
 }
 constexpr int join_bytes(int d, int nr, int groups, int width) { return (groups / 2) * width * nr * 64 * (d / 16 * 16 + 8); }
 
-// A row's result: the output itself where this is its only part. TILED: channels 16 e + 4 q + i in o[e][i], else
+// Four neighbouring outputs.
+template <int ODT>
+__device__ __forceinline__ void store_four(void* out, int64_t at, f32x4 x) {
+  if constexpr (ODT == LKV_F32) {
+    *(f32x4*)((float*)out + at) = x;
+  } else {
+    *(uint2*)((uint16_t*)out + at) = make_uint2(Mat<ODT>::pack(x[0], x[1]), Mat<ODT>::pack(x[2], x[3]));
+  }
+}
+
+// The k-th four channels of a lane's, and where they belong. TILED: channels 16 e + 4 q + i in o[e][i], else
 // (d/4) q + (d/16) i + e.
+template <int D, bool TILED>
+__device__ __forceinline__ f32x4 four_of(const f32x4 (&o)[D / 16], int k, int& channel) {
+  const int quarter = (threadIdx.x & 63) >> 4;
+  if constexpr (TILED) {
+    channel = 16 * k + 4 * quarter;
+    return o[k];
+  } else {
+    constexpr int E = D / 64;  // fours of e for an i
+    const int i = k / E, e = k % E * 4;
+    channel = (D / 4) * quarter + (D / 16) * i + e;
+    return f32x4{o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]};
+  }
+}
+
+template <int ODT, int D, bool TILED>
+__device__ __forceinline__ void store_output(void* out, int64_t row, float l, const f32x4 (&o)[D / 16]) {
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int k = 0; k < D / 16; ++k) {
+    int c;
+    f32x4 x = four_of<D, TILED>(o, k, c) * inv;
+    store_four<ODT>(out, row * D + c, x);
+  }
+}
+
+// A row's result: the output itself where this is its only part.
 template <int D, bool TILED>
 __device__ __forceinline__ void store_row(const SharedArgs& a, int64_t row, int part, float m, float l, const f32x4 (&o)[D / 16]) {
   const int parts = a.p_parts + a.o_parts, quarter = (threadIdx.x & 63) >> 4;
-  const bool last = parts == 1;
-  const int64_t slot = last ? row : row * parts + part;
-  const float inv = !last ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
-  if (quarter == 0) {
-    if (last) {
-      a.lse[row] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * lkv::kLn2;
-    } else {
-      a.part_ml[slot] = make_float2(m, l);
-    }
-  }
+  if (parts > 1) {
+    const int64_t slot = row * parts + part;
+    if (quarter == 0) a.part_ml[slot] = make_float2(m, l);
 #pragma unroll
-  for (int k = 0; k < D / 16; ++k) {
-    f32x4 x;
-    int c;
-    if constexpr (TILED) {
-      x = o[k];
-      c = 16 * k + 4 * quarter;
-    } else {
-      constexpr int E = D / 64;  // groups of four e for an i
-      const int i = k / E, e = k % E * 4;
-      x = f32x4{o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]};
-      c = (D / 4) * quarter + (D / 16) * i + e;
-    }
-    if (last) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) lkv::store_any(a.out, slot * D + c + i, a.out_dtype, l == 0.0f ? 0.0f : x[i] * inv);
-    } else {
+    for (int k = 0; k < D / 16; ++k) {
+      int c;
+      const f32x4 x = four_of<D, TILED>(o, k, c);
       *(f32x4*)(a.part_o + slot * D + c) = x;
     }
+    return;
+  }
+  if (quarter == 0) a.lse[row] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * lkv::kLn2;
+  if (a.out_dtype == LKV_F32) {
+    store_output<LKV_F32, D, TILED>(a.out, row, l, o);
+  } else if (a.out_dtype == LKV_BF16) {
+    store_output<LKV_BF16, D, TILED>(a.out, row, l, o);
+  } else {
+    store_output<LKV_F16, D, TILED>(a.out, row, l, o);
   }
 }
 
@@ -539,9 +595,50 @@ template <int DT, int D, bool MX, int WR> struct StageRegs {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
+typedef __attribute__((address_space(3))) const uint8_t* LdsPointer;
+
 // Four tokens of one channel a lane, of a 4 x 16 piece whose rows the 16 lanes name eight bytes of.
-__device__ __forceinline__ uint2 read_transposed(const uint8_t* p) {
+__device__ __forceinline__ uint2 read_transposed(LdsPointer p) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+}
+__device__ __forceinline__ uint4 read_piece(LdsPointer p) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  const u32x4 x = *(__attribute__((address_space(3))) const u32x4*)p;
+  return make_uint4(x.x, x.y, x.z, x.w);
+}
+
+// One tile of 32 tokens of a staged buffer, at compile-time offset AT in LDS from the lane's places.
+template <int DT, int D, int WR, int AT>
+__device__ __forceinline__ void wide_tile(const LdsPointer (&key_at)[D / 32], const LdsPointer (&value_at)[D / 16], const uint4 (&qf)[2][D / 32],
+                                          int left, float scale2, Reference (&ref)[2], Result<D, 2>& r) {
+  // All of the tile's reads first: one by one before their products, each would be waited for.
+  uint4 k[2][D / 32];
+  uint2 v[D / 16][2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) k[u][i] = read_piece(key_at[i] + AT + u * 16 * (2 * D));
+#pragma unroll
+  for (int e = 0; e < D / 16; ++e)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) v[e][u] = read_transposed(value_at[e] + AT + u * 16 * (2 * D));
+  __builtin_amdgcn_sched_barrier(0);
+  f32x4 sc[2][2];
+#pragma unroll
+  for (int n = 0; n < 2; ++n) sc[n][0] = sc[n][1] = ref[n].negative;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int n = 0; n < 2; ++n) sc[n][u] = Mat<DT>::mma(k[u][i], qf[n][i], sc[n][u]);
+  uint4 p[2];
+#pragma unroll
+  for (int n = 0; n < 2; ++n) p[n] = weigh<DT, D>(sc[n], left, scale2, ref[n], r.l[n], r.o[n]);
+#pragma unroll
+  for (int e = 0; e < D / 16; ++e)
+#pragma unroll
+    for (int n = 0; n < 2; ++n) r.o[n][e] = Mat<DT>::mma(make_uint4(v[e][0].x, v[e][0].y, v[e][1].x, v[e][1].y), p[n], r.o[n][e]);
 }
 
 template <int DT, int D, bool MX, int WR>
@@ -549,9 +646,10 @@ __device__ __forceinline__ void attend_wide(const Stream& s, const uint16_t* con
                                             uint8_t* lds) {
   using S = Stage<D, WR>;
   const int lane = threadIdx.x & 63, quarter = lane >> 4;
+  Reference ref[2];
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
-    r.m[n] = -INFINITY;
+    ref[n].reset();
     r.l[n] = 0.0f;
 #pragma unroll
     for (int e = 0; e < D / 16; ++e) r.o[n][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -561,56 +659,49 @@ __device__ __forceinline__ void attend_wide(const Stream& s, const uint16_t* con
   for (int n = 0; n < 2; ++n)
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) qf[n][i] = q[n] ? *(const uint4*)(q[n] + 32 * i + 8 * quarter) : make_uint4(0, 0, 0, 0);
-  // A lane's places in a tile of 32 tokens: keys of token lane % 16 (and 16 on), values of token 4 q + (lane % 16) / 4.
-  uint32_t key_at[D / 32], value_at[D / 16];
+  // A lane's places in its wave's first tile: keys of token lane % 16 (and 16 on), values of token 4 q + (lane % 16) / 4.
+  LdsPointer key_at[D / 32], value_at[D / 16];
+  const int tile0 = wt * S::TILES * kTile;  // a wave's tiles of a stage lie together
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) key_at[i] = (lane & 15) * (2 * D) + ((4 * i + quarter) ^ S::swizzle(lane & 15)) * 16;
+  for (int i = 0; i < D / 32; ++i) key_at[i] = (LdsPointer)lds + (tile0 + (lane & 15)) * (2 * D) + ((4 * i + quarter) ^ S::swizzle(lane & 15)) * 16;
 #pragma unroll
   for (int e = 0; e < D / 16; ++e) {
     const int row = 4 * quarter + ((lane & 15) >> 2);
-    value_at[e] = S::BYTES + row * (2 * D) + ((2 * e + ((lane & 2) >> 1)) ^ S::swizzle(row)) * 16 + (lane & 1) * 8;
+    value_at[e] = (LdsPointer)lds + S::BYTES + (tile0 + row) * (2 * D) + ((2 * e + ((lane & 2) >> 1)) ^ S::swizzle(row)) * 16 + (lane & 1) * 8;
   }
+  // As they stand: worked out anew for each tile, from what they have in common, they would cost more than registers.
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) keep_here(key_at[i]);
+#pragma unroll
+  for (int e = 0; e < D / 16; ++e) keep_here(value_at[e]);
   StageRegs<DT, D, MX, WR> regs;
   regs.load(s, t0, end);
-  int buffer = 0;
-  for (int t = t0; t < end; t += S::TOKENS) {
-    uint8_t* const now = lds + buffer * (2 * S::BYTES);
-    regs.store(now, end - t);
-    __syncthreads();  // and the other buffer is read no more: its readers have passed this one's barrier before
+  // Two stages a round, one in each buffer. A stage's barrier also ends the reads of the other buffer: its readers
+  // came to this one after them.
+  for (int t = t0; t < end; t += 2 * S::TOKENS) {
+    regs.store(lds, end - t);
+    __syncthreads();
     if (t + S::TOKENS < end) regs.load(s, t + S::TOKENS, end);
     load_fence();
-    buffer ^= 1;
-#pragma unroll
-    for (int tile = 0; tile < S::TILES; ++tile) {
-      const int first = (tile * S::WT + wt) * kTile;  // of the stage's tokens
-      const uint8_t* const base = now + first * (2 * D);
-      if (t + first >= end) break;
-      f32x4 sc[2][2];
-#pragma unroll
-      for (int n = 0; n < 2; ++n) sc[n][0] = sc[n][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-          const uint4 k = *(const uint4*)(base + key_at[i] + u * 16 * (2 * D));
-#pragma unroll
-          for (int n = 0; n < 2; ++n) sc[n][u] = Mat<DT>::mma(k, qf[n][i], sc[n][u]);
-        }
-      const int left = end - t - first;
-      uint4 p[2];
-#pragma unroll
-      for (int n = 0; n < 2; ++n) p[n] = weigh<DT, D>(sc[n], left, scale2, r.m[n], r.l[n], r.o[n]);
-#pragma unroll
-      for (int e = 0; e < D / 16; ++e) {
-        const uint2 lo = read_transposed(base + value_at[e]), hi = read_transposed(base + value_at[e] + 16 * (2 * D));
-        const uint4 v = make_uint4(lo.x, lo.y, hi.x, hi.y);
-#pragma unroll
-        for (int n = 0; n < 2; ++n) r.o[n][e] = Mat<DT>::mma(v, p[n], r.o[n][e]);
-      }
-    }
+    int left = end - t - tile0;
+    if (left > 0) wide_tile<DT, D, WR, 0>(key_at, value_at, qf, left, scale2, ref, r);
+    if constexpr (S::TILES > 1)
+      if (left > kTile) wide_tile<DT, D, WR, kTile * 2 * D>(key_at, value_at, qf, left - kTile, scale2, ref, r);
+    if (t + S::TOKENS >= end) break;
+    regs.store(lds + 2 * S::BYTES, end - t - S::TOKENS);
+    __syncthreads();
+    if (t + 2 * S::TOKENS < end) regs.load(s, t + 2 * S::TOKENS, end);
+    load_fence();
+    left -= S::TOKENS;
+    if (left > 0) wide_tile<DT, D, WR, 2 * S::BYTES>(key_at, value_at, qf, left, scale2, ref, r);
+    if constexpr (S::TILES > 1)
+      if (left > kTile) wide_tile<DT, D, WR, 2 * S::BYTES + kTile * 2 * D>(key_at, value_at, qf, left - kTile, scale2, ref, r);
   }
 #pragma unroll
-  for (int n = 0; n < 2; ++n) r.l[n] = lkv::pair_sum<32>(lkv::pair_sum<16>(r.l[n]));
+  for (int n = 0; n < 2; ++n) {
+    r.l[n] = lkv::pair_sum<32>(lkv::pair_sum<16>(r.l[n]));
+    r.m[n] = ref[n].level(scale2);
+  }
 }
 
 template <int DT, int D, bool PMX, bool OMX, int WR>
@@ -683,8 +774,14 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
   if (threadIdx.x >= C) return;
 #pragma unroll
   for (int i = 1; i < GROUPS; ++i) o += red[i][c];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) lkv::store_any(a.out, row * D + c * 4 + i, a.out_dtype, total == 0.0f ? 0.0f : o[i] / total);
+  o *= total == 0.0f ? 0.0f : 1.0f / total;
+  if (a.out_dtype == LKV_F32) {
+    store_four<LKV_F32>(a.out, row * D + c * 4, o);
+  } else if (a.out_dtype == LKV_BF16) {
+    store_four<LKV_BF16>(a.out, row * D + c * 4, o);
+  } else {
+    store_four<LKV_F16>(a.out, row * D + c * 4, o);
+  }
   if (threadIdx.x == 0) a.lse[row] = total == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * lkv::kLn2;
 }
 
