@@ -863,7 +863,7 @@ extern "C" int lkv_shared_decode(uintptr_t stream, const lkv_shared_desc* desc, 
   LKV_CHECK_ARG(q && out && lse, "NULL pointer");
   LKV_CHECK_ARG(q_dtype == LKV_F16 || q_dtype == LKV_BF16, "queries are float16 or bfloat16, got dtype %d", q_dtype);
   LKV_CHECK_ARG(lkv_is_model_dtype(out_dtype), "unsupported output dtype %d", out_dtype);
-  LKV_CHECK_ARG(((uintptr_t)q & 15) == 0, "queries must start on 16 bytes");
+  LKV_CHECK_ARG((((uintptr_t)q | (uintptr_t)out) & 15) == 0, "queries and outputs must start on 16 bytes");
   LKV_CHECK_ARG(ws && ws_bytes >= lkv_shared_decode_workspace_bytes(desc), "workspace of %zu bytes: %zu are needed", ws_bytes,
                 lkv_shared_decode_workspace_bytes(desc));
   LKV_CHECK_ARG(((uintptr_t)ws & 15) == 0, "the workspace must start on 16 bytes");

@@ -630,28 +630,25 @@ def _forward_level() -> int:
 MX_GROUP = 32  # channels of a row that share a scale (LKV_MXFP8)
 
 
-@dataclass
 class Rows:
-    """A `lkv_kv_rows`: the keys' and values' rows of `seqs` sequences, one per token, in the model dtype or in 8 bits."""
+    """A `lkv_kv_rows`: the keys' and values' rows of `seqs` sequences, one per token, in the model dtype or in 8 bits
+    (`dense_rows`, `mx_rows`). It describes the tensors it was made of and keeps them; a program may keep it."""
 
-    k: int
-    v: int
-    k_scale: int | None
-    v_scale: int | None
-    seq_stride: int
-    head_stride: int
-    tokens: int
-    seqs: int
-    n_kv: int
-    head_dim: int
-    dtype: int  # _lib.F16, _lib.BF16 or _lib.MXFP8
-    model_dtype: torch.dtype
-    device: torch.device
-    owners: tuple = ()
+    __slots__ = ("seqs", "n_kv", "tokens", "head_dim", "dtype", "model_dtype", "model_code", "device_index", "owners", "struct", "ref")
 
-    def c(self) -> _lib.KVRows:
-        return _lib.KVRows(self.k, self.v, self.k_scale, self.v_scale, self.seq_stride, self.head_stride, self.tokens, self.seqs, self.dtype,
-                           _ROW_DTYPES[self.model_dtype])
+    def __init__(self, k: int, v: int, k_scale: int | None, v_scale: int | None, seq_stride: int, head_stride: int, shape: tuple, dtype: int,
+                 model_dtype: torch.dtype, device_index: int, owners: tuple) -> None:
+        self.seqs, self.n_kv, self.tokens, self.head_dim = shape
+        self.dtype = dtype  # _lib.F16, _lib.BF16 or _lib.MXFP8
+        self.model_dtype, self.model_code = model_dtype, _ROW_DTYPES[model_dtype]
+        self.device_index = device_index
+        self.owners = owners
+        self.struct = _lib.KVRows(k, v, k_scale, v_scale, seq_stride, head_stride, self.tokens, self.seqs, dtype, self.model_code)
+        self.ref = ctypes.byref(self.struct)
+
+    @property
+    def device(self) -> torch.device:
+        return self.owners[0].device
 
 
 _ROW_DTYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
@@ -669,14 +666,12 @@ def dense_rows(keys: torch.Tensor, values: torch.Tensor) -> Rows:
     """Rows in the model dtype: keys and values `[seqs, h, T, d]`, contiguous rows d elements apart, any strides above
     that are multiples of 32 elements and the same for both."""
     _lib.require_cuda(keys, values)
-    shape = tuple(keys.shape)
-    ks = keys.stride()
-    if len(shape) != 4 or tuple(values.shape) != shape or keys.dtype != values.dtype or keys.device != values.device:
-        raise ValueError(f"expected matching [seqs, h, T, d] keys/values, got {shape} {keys.dtype} / {tuple(values.shape)} {values.dtype}")
+    shape, ks, device, dtype = keys.shape, keys.stride(), keys.get_device(), keys.dtype
+    if len(shape) != 4 or values.shape != shape or values.dtype != dtype or values.get_device() != device:
+        raise ValueError(f"expected matching [seqs, h, T, d] keys/values, got {tuple(shape)} {dtype} / {tuple(values.shape)} {values.dtype}")
     if ks[3] != 1 or ks[2] != shape[3] or values.stride() != ks:
         raise ValueError("rows must be contiguous with a token stride of head_dim, keys and values with the same strides")
-    return Rows(keys.data_ptr(), values.data_ptr(), None, None, ks[0], ks[1], shape[2], shape[0], shape[1], shape[3], _row_dtype(keys.dtype),
-                keys.dtype, keys.device, (keys, values))
+    return Rows(keys.data_ptr(), values.data_ptr(), None, None, ks[0], ks[1], shape, _row_dtype(dtype), dtype, device, (keys, values))
 
 
 def mx_rows(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> Rows:
@@ -684,16 +679,16 @@ def mx_rows(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> Ro
     (uint8), for a model of `dtype`. Views are fine whose scales are cut like their codes."""
     _lib.require_cuda(codes, scales)
     _row_dtype(dtype)
-    shape, cs, ss = tuple(codes.shape), codes.stride(), scales.stride()
-    if len(shape) != 5 or shape[0] != 2 or codes.dtype not in _CODE_DTYPES or scales.dtype != torch.uint8 or codes.device != scales.device:
-        raise ValueError(f"expected codes [2, seqs, h, T, d] and uint8 scales, got {shape} {codes.dtype} / {tuple(scales.shape)} {scales.dtype}")
+    shape, cs, ss, device = codes.shape, codes.stride(), scales.stride(), codes.get_device()
+    if len(shape) != 5 or shape[0] != 2 or codes.dtype not in _CODE_DTYPES or scales.dtype != torch.uint8 or scales.get_device() != device:
+        raise ValueError(f"expected codes [2, seqs, h, T, d] and uint8 scales, got {tuple(shape)} {codes.dtype} / {tuple(scales.shape)} {scales.dtype}")
     d = shape[4]
-    if d % MX_GROUP or tuple(scales.shape) != shape[:4] + (d // MX_GROUP,):
-        raise ValueError(f"codes {shape} take scales {shape[:4] + (d // MX_GROUP,)}, got {tuple(scales.shape)}")
+    if d % MX_GROUP or scales.shape != shape[:4] + (d // MX_GROUP,):
+        raise ValueError(f"codes {tuple(shape)} take scales {tuple(shape[:4]) + (d // MX_GROUP,)}, got {tuple(scales.shape)}")
     if cs[4] != 1 or cs[3] != d or ss[4] != 1 or ss[3] * MX_GROUP != d or ss[1] * MX_GROUP != cs[1] or ss[2] * MX_GROUP != cs[2]:
         raise ValueError("codes' and scales' rows must be contiguous, and their strides alike")
     k, k_scale = codes.data_ptr(), scales.data_ptr()
-    return Rows(k, k + cs[0], k_scale, k_scale + ss[0], cs[1], cs[2], shape[3], shape[1], shape[2], d, _lib.MXFP8, dtype, codes.device, (codes, scales))
+    return Rows(k, k + cs[0], k_scale, k_scale + ss[0], cs[1], cs[2], shape[1:], _lib.MXFP8, dtype, device, (codes, scales))
 
 
 def mx_empty(seqs: int, n_kv: int, tokens: int, head_dim: int, device: torch.device | str) -> tuple[torch.Tensor, torch.Tensor]:
@@ -702,12 +697,7 @@ def mx_empty(seqs: int, n_kv: int, tokens: int, head_dim: int, device: torch.dev
     return codes, torch.zeros((2, seqs, n_kv, tokens, head_dim // MX_GROUP), dtype=torch.uint8, device=device)
 
 
-def _on(device: torch.device):  # noqa: ANN202
-    """The device a launch needs as the current one, where it is another."""
-    return torch.cuda.device(device) if device.index not in (None, torch.cuda.current_device()) else _NO_SWITCH
-
-
-class _NoSwitch:
+class _Nothing:
     def __enter__(self) -> None:
         return None
 
@@ -715,7 +705,20 @@ class _NoSwitch:
         return None
 
 
-_NO_SWITCH = _NoSwitch()
+_NOTHING = _Nothing()
+
+
+def _on(index: int):  # noqa: ANN202
+    """The device a launch needs as the current one, where it is another."""
+    return _NOTHING if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+def _raw_stream(index: int) -> int:
+    """The current stream of a device as an integer, without an object for it where torch offers that."""
+    return _GET_RAW_STREAM(index) if _GET_RAW_STREAM is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+_GET_RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _placed(x: torch.Tensor) -> torch.Tensor:
@@ -726,38 +729,39 @@ def _placed(x: torch.Tensor) -> torch.Tensor:
     return x
 
 
-def _starts(starts: torch.Tensor | None, seqs: int, device: torch.device, name: str) -> int | None:
-    if starts is None:
+def _counts(x: torch.Tensor | None, seqs: int, device: int, name: str) -> int | None:
+    """The address of a count for each sequence, int32 on the device."""
+    if x is None:
         return None
-    if starts.device != device or starts.dtype != torch.int32 or tuple(starts.shape) != (seqs,) or not starts.is_contiguous():
-        raise ValueError(f"{name} must be contiguous int32 [{seqs}] on {device}, got {starts.dtype} {tuple(starts.shape)} on {starts.device}")
-    return starts.data_ptr()
+    if x.get_device() != device or x.dtype != torch.int32 or x.shape != (seqs,) or not x.is_contiguous():
+        raise ValueError(f"{name} must be contiguous int32 [{seqs}] on cuda:{device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
+    return x.data_ptr()
 
 
 def append_rows(dst: Rows, keys: torch.Tensor, values: torch.Tensor, *, start: int = 0, starts: torch.Tensor | None = None) -> None:
     """New tokens' keys and values `[seqs, h, T, d]` into a cache's rows (lkv_append_rows): token t of sequence b becomes row
     `start + starts[b] + t`. Without `starts` the rows must exist (ValueError); with it, rows outside the cache are dropped. An
     8-bit cache takes them as E4M3 codes with a power-of-two scale for every 32 channels, another one as they are."""
-    shape = tuple(keys.shape)
-    if shape != tuple(values.shape) or len(shape) != 4 or keys.dtype != dst.model_dtype or values.dtype != dst.model_dtype:
-        raise ValueError(f"expected matching {dst.model_dtype} keys/values [seqs, h, T, d], got {shape} {keys.dtype} / {tuple(values.shape)} {values.dtype}")
-    if (shape[0], shape[1], shape[3]) != (dst.seqs, dst.n_kv, dst.head_dim):
-        raise ValueError(f"keys/values {shape} do not match rows of {dst.seqs} sequences, {dst.n_kv} heads and head_dim {dst.head_dim}")
-    if keys.device != dst.device or values.device != dst.device:
+    shape, dtype, index = keys.shape, dst.model_dtype, dst.device_index
+    if len(shape) != 4 or values.shape != shape or keys.dtype != dtype or values.dtype != dtype:
+        raise ValueError(f"expected matching {dtype} keys/values [seqs, h, T, d], got {tuple(shape)} {keys.dtype} / {tuple(values.shape)} {values.dtype}")
+    seqs, n_kv, n, d = shape
+    if seqs != dst.seqs or n_kv != dst.n_kv or d != dst.head_dim:
+        raise ValueError(f"keys/values {tuple(shape)} do not match rows of {dst.seqs} sequences, {dst.n_kv} heads and head_dim {dst.head_dim}")
+    if keys.get_device() != index or values.get_device() != index:
         raise ValueError(f"keys/values on {keys.device} / {values.device}, the cache on {dst.device}")
-    at = _starts(starts, dst.seqs, dst.device, "starts")
+    at = _counts(starts, seqs, index, "starts")
     if 0 in shape:
         return
     x, y = _placed(keys), _placed(values)
-    if x.stride() != y.stride():
-        x, y = x.contiguous(), y.contiguous()
-        if x.stride() != y.stride():  # sizes of one leave strides free
-            x, y = torch.stack([x, y]).unbind(0)
     st = x.stride()
-    with _on(dst.device):
-        rc = _lib.lib().lkv_append_rows(_lib.stream_of(x), ctypes.byref(dst.c()), x.data_ptr(), y.data_ptr(), _ROW_DTYPES[dst.model_dtype], st[0], st[1], st[2],
-                                        dst.seqs, dst.n_kv, dst.head_dim, shape[2], at, start)
-    _lib.check(rc, "append_rows")
+    if y.stride() != st:
+        x, y = torch.stack([x, y]).unbind(0)
+        st = x.stride()
+    with _on(index):
+        rc = _lib.lib().lkv_append_rows(_raw_stream(index), dst.ref, x.data_ptr(), y.data_ptr(), dst.model_code, st[0], st[1], st[2], seqs, n_kv, d, n, at, start)
+    if rc:
+        _lib.check(rc, "append_rows")
 
 
 def read_rows(src: Rows, first: int, n: int, out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -767,22 +771,23 @@ def read_rows(src: Rows, first: int, n: int, out: tuple[torch.Tensor, torch.Tens
         raise ValueError("read_rows takes 8-bit rows; others are read where they are")
     if first < 0 or n < 0 or first + n > src.tokens:
         raise ValueError(f"rows {first}..{first + n} exceed the {src.tokens} there are")
-    shape = (src.seqs, src.n_kv, n, src.head_dim)
+    shape, index = (src.seqs, src.n_kv, n, src.head_dim), src.device_index
     if out is None:
         out = (torch.empty(shape, dtype=src.model_dtype, device=src.device), torch.empty(shape, dtype=src.model_dtype, device=src.device))
     k, v = out
     st = k.stride()
     for x in out:
-        if tuple(x.shape) != shape or x.dtype != src.model_dtype or x.device != src.device:
+        if x.shape != shape or x.dtype != src.model_dtype or x.get_device() != index:
             raise ValueError(f"out must be {src.model_dtype} {shape} on {src.device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
     if v.stride() != st or st[3] != 1 or (st[0] | st[1] | st[2]) % 8 or (k.data_ptr() | v.data_ptr()) % 16:
         raise ValueError("out's rows must be contiguous and start on 16 bytes, both with the same strides")
     if 0 in shape:
         return out
-    with _on(src.device):
-        rc = _lib.lib().lkv_read_rows(_lib.stream_of(k), ctypes.byref(src.c()), src.seqs, src.n_kv, src.head_dim, first, n, k.data_ptr(), v.data_ptr(),
-                                      _ROW_DTYPES[src.model_dtype], st[0], st[1], st[2])
-    _lib.check(rc, "read_rows")
+    with _on(index):
+        rc = _lib.lib().lkv_read_rows(_raw_stream(index), src.ref, src.seqs, src.n_kv, src.head_dim, first, n, k.data_ptr(), v.data_ptr(), src.model_code,
+                                      st[0], st[1], st[2])
+    if rc:
+        _lib.check(rc, "read_rows")
     return out
 
 
@@ -804,55 +809,60 @@ def shared_decode(
     """One decode token of each of B sequences, q `[B, n_q, d]` or `[B, n_q, 1, d]` (lkv_shared_decode): sequence b attends rows
     0 .. prefix_tokens-1 of `prefix`, one sequence's rows that are read once for the whole batch, and rows
     0 .. own_tokens + lengths[b] - 1 of its own in `own`, at most `max_own` of them (default: own_tokens without
-    `lengths`, else all that `own` holds; a bound near the lengths divides the work better). Either may be left out: B = 1 over `own` alone is plain decode over an
-    8-bit cache. Returns (out [B, n_q, d], lse [B, n_q] float32, natural log); a sequence without any rows gets zeros and -inf.
-    Without `ws` the scratch is torch's, so calls on several streams and in several graphs do not meet."""
+    `lengths`, else all that `own` holds; a bound near the lengths divides the work better). Either may be left out: B = 1 over
+    `own` alone is plain decode over an 8-bit cache. Returns (out [B, n_q, d], lse [B, n_q] float32, natural log); a sequence
+    without any rows gets zeros and -inf. Without `ws` the scratch is torch's, so calls on several streams and in several graphs
+    do not meet."""
     rows = own if own is not None else prefix
     if rows is None:
         raise ValueError("shared_decode needs a prefix's rows or the sequences' own")
     _lib.require_cuda(q)
-    shape = tuple(q.shape)
+    shape, index, dtype = q.shape, rows.device_index, rows.model_dtype
     if len(shape) == 4 and shape[2] == 1:
         shape = (shape[0], shape[1], shape[3])
-    if len(shape) != 3 or q.dtype != rows.model_dtype or shape[2] != rows.head_dim or shape[1] == 0 or shape[1] % rows.n_kv:
-        raise ValueError(f"query {tuple(q.shape)} {q.dtype} does not match {rows.model_dtype} rows of {rows.n_kv} heads and head_dim {rows.head_dim}")
+    if len(shape) != 3 or q.dtype != dtype or shape[2] != rows.head_dim or shape[1] == 0 or shape[1] % rows.n_kv or q.get_device() != index:
+        raise ValueError(f"query {tuple(q.shape)} {q.dtype} on {q.device} does not match {dtype} rows of {rows.n_kv} heads and head_dim {rows.head_dim} on "
+                         f"{rows.device}")
     b, n_q, d = shape
-    if max_own is None:
-        max_own = own_tokens if lengths is None else (own.tokens if own is not None else 0)
-    for r, seqs, what in ((prefix, 1, "prefix"), (own, b, "own")):
-        if r is not None and (r.n_kv, r.head_dim, r.model_dtype, r.device, r.seqs) != (rows.n_kv, d, q.dtype, q.device, seqs):
-            raise ValueError(f"{what} rows of {r.seqs} sequences, {r.n_kv} heads, head_dim {r.head_dim}, {r.model_dtype} on {r.device} do not match "
-                             f"{seqs} of {rows.n_kv}, {d}, {q.dtype} on {q.device}")
-    if own is None and (lengths is not None or own_tokens or max_own):
-        raise ValueError("own_tokens, lengths and max_own describe `own`, which is not given")
-    at = _starts(lengths, b, q.device, "lengths")
+    if own is None:
+        if lengths is not None or own_tokens or max_own:
+            raise ValueError("own_tokens, lengths and max_own describe `own`, which is not given")
+        max_own = 0
+    elif own.seqs != b:
+        raise ValueError(f"own rows of {own.seqs} sequences, queries of {b}")
+    elif max_own is None:
+        max_own = own_tokens if lengths is None else own.tokens
+    if prefix is not None and (prefix.seqs != 1 or prefix.n_kv != rows.n_kv or prefix.head_dim != d or prefix.model_dtype != dtype or prefix.device_index != index):
+        raise ValueError(f"a prefix of {prefix.seqs} sequences, {prefix.n_kv} heads, head_dim {prefix.head_dim}, {prefix.model_dtype} on {prefix.device} "
+                         f"does not match one of {rows.n_kv}, {d}, {dtype} on {rows.device}")
+    at = _counts(lengths, b, index, "lengths")
     if lengths is None and own_tokens > max_own:
         raise ValueError(f"own_tokens={own_tokens} exceed max_own={max_own}")
-    qq = q.reshape(shape).contiguous()
-    if qq.data_ptr() % 16:
-        qq = qq.clone()
+    if not q.is_contiguous() or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
     if out is None:
-        out = torch.empty(shape, dtype=out_dtype or q.dtype, device=q.device)
+        out = torch.empty(shape, dtype=out_dtype or dtype, device=q.device)
+    elif not out.is_contiguous() or out.numel() != b * n_q * d or out.get_device() != index or (out_dtype is not None and out.dtype != out_dtype) or out.data_ptr() % 16:
+        raise ValueError(f"out must be contiguous [{b}, {n_q}, {d}] on {rows.device}, on 16 bytes")
     if lse is None:
         lse = torch.empty((b, n_q), dtype=torch.float32, device=q.device)
-    if (not out.is_contiguous() or out.numel() != b * n_q * d or out.device != q.device or (out_dtype is not None and out.dtype != out_dtype)
-            or not lse.is_contiguous() or lse.numel() != b * n_q or lse.dtype != torch.float32 or lse.device != q.device):
-        raise ValueError(f"out must be contiguous [{b}, {n_q}, {d}] and lse contiguous float32 [{b}, {n_q}] on {q.device}")
+    elif not lse.is_contiguous() or lse.numel() != b * n_q or lse.dtype != torch.float32 or lse.get_device() != index:
+        raise ValueError(f"lse must be contiguous float32 [{b}, {n_q}] on {rows.device}")
     if b == 0:
         return out, lse
-    desc = _lib.SharedDesc(b, n_q, rows.n_kv, d, scale, prefix_tokens, own_tokens, max_own)
-    need = _lib.lib().lkv_shared_decode_workspace_bytes(ctypes.byref(desc))
+    lib = _lib.lib()
+    desc = ctypes.byref(_lib.SharedDesc(b, n_q, rows.n_kv, d, scale, prefix_tokens, own_tokens, max_own))
+    need = lib.lkv_shared_decode_workspace_bytes(desc)
     if ws is None:
         buf = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
-        ws_ptr, ws_n = buf.data_ptr(), buf.numel()
+        ws_ptr, ws_n = buf.data_ptr(), need if need > 16 else 16
     else:
         ws_ptr, ws_n = ws.get(need)
-    with _on(q.device):
-        rc = _lib.lib().lkv_shared_decode(
-            _lib.stream_of(qq), ctypes.byref(desc), qq.data_ptr(), _ROW_DTYPES[q.dtype], ctypes.byref(prefix.c()) if prefix is not None else None,
-            ctypes.byref(own.c()) if own is not None else None, at, out.data_ptr(), _lib.dtype_code(out.dtype), lse.data_ptr(), ws_ptr, ws_n,
-        )
-    _lib.check(rc, "shared_decode")
+    with _on(index):
+        rc = lib.lkv_shared_decode(_raw_stream(index), desc, q.data_ptr(), rows.model_code, prefix.ref if prefix is not None else None,
+                                   own.ref if own is not None else None, at, out.data_ptr(), _lib.dtype_code(out.dtype), lse.data_ptr(), ws_ptr, ws_n)
+    if rc:
+        _lib.check(rc, "shared_decode")
     return out, lse
 
 
