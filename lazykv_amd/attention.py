@@ -4,7 +4,9 @@ Mirrors lazykv/attention.py:139-182 (`lazykv_attention_forward`, registered as "
 transformers' AttentionInterface, :269-290). For a decode token of a selecting layer, the
 selector (`TieredCache.select`) returns the finished attention of the step -- bound, top-K,
 sparse attention and, for the exact tier, the LSE merge, all on the device -- which short-circuits
-`attend`. Dense decode (`select` returns None) runs the same kernel over the whole cache.
+`attend`. Dense decode (`select` returns None) runs the same kernel over the whole cache, or the
+batch decode's over an 8-bit one. A batch is taken from a selector that says it is `batched`
+(`cache.SharedPrefixCache`).
 
 `attend` keeps the reference's signature (:97-136). Its decode case (q_len == 1) is the HIP
 kernel. Chunked prefill (q_len > 1) is not on this path: it is handed to torch's
@@ -42,7 +44,8 @@ def attend(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, scaling:
     """Exact attention of `query` [1, n_q, q_len, d] over all of `key`/`value` [1, kv, L, d].
 
     Decode (q_len 1) runs the HIP decode kernel over the L tokens (whole blocks from the cache
-    plus a partial last block). `mask`, if given, must be the current-block mask of
+    plus a partial last block); over an 8-bit layer's codes (`cache.MXFP8Layer`) it runs
+    `kernels.shared_decode`. `mask`, if given, must be the current-block mask of
     lazykv/selection.py:65-69; the kernel needs only its count of live positions. Every name in
     STRATEGIES selects this path; another name is a ValueError, as in the reference (:113). `bucket`
     is accepted for the reference's signature: the kernel reads exactly the live prefix, so there is
@@ -52,13 +55,19 @@ def attend(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, scaling:
     del bucket
     q_len, kv_len, d = query.shape[-2], key.shape[-2], query.shape[-1]
     scale = scaling if scaling is not None else d**-0.5
+    rows = getattr(key, "lazykv_rows", None)  # keys of an 8-bit layer's decode token: codes, read where they are
     if q_len > 1:
+        if rows is not None:
+            raise ValueError("8-bit keys are attended by one token; a forward of several takes them read back (MXFP8Layer.dense)")
         from torch.nn.attention.bias import causal_lower_right
 
         return torch.nn.functional.scaled_dot_product_attention(query, key, value, attn_mask=causal_lower_right(q_len, kv_len), scale=scale, enable_gqa=True)
     live = kv_len
     if mask is not None:
         live = int((mask.reshape(-1) == 0).sum().item())  # host sync: the seam's fallback only
+    if rows is not None:
+        out, _ = kernels.shared_decode(query, scale=scale, own=rows, own_tokens=live)
+        return out.view(query.shape)
     out, _ = dense_decode(query, key[:, :, :live], value[:, :, :live], scale)
     return out
 
@@ -90,9 +99,9 @@ def lazykv_attention_forward(
     """transformers attention function (lazykv/attention.py:139-182). Returns ([1, q_len, n_q, d], None)."""
     if attention_mask is not None:
         raise RuntimeError("lazykv attention owns causality; a mask should never be passed")
-    if query.shape[0] != 1:
-        raise RuntimeError("batch size 1 only")
     selector = kwargs.get("lazykv_selector")
+    if query.shape[0] != 1 and not getattr(selector, "batched", False):
+        raise RuntimeError("batch size 1 only (a batch over one prefix: cache.SharedPrefixCache)")
     out = None
     if selector is not None:
         decoded = selector.select(int(getattr(module, "layer_idx")), query, key, value, scaling)

@@ -13,7 +13,10 @@ The transformers `Cache` surface of the reference's dense store (`FullGPUCache`,
 * The slab is zero-filled once. The HIP kernels never read rows past the live length, but a
   consumer that masks unused rows by adding -inf would turn uninitialised NaN into NaN.
 
-Batch size 1, as in the reference.
+Batch size 1, as in the reference. Two stores go beyond it: `MXFP8Cache` holds every layer in 8 bits
+(E4M3 codes, a power-of-two scale for every 32 channels of a row), written as tokens arrive and read in
+place by the decode, and `SharedPrefixCache` is a batch of sequences over one prefilled cache, each with
+rows of its own behind it.
 """
 
 from __future__ import annotations
@@ -22,6 +25,8 @@ from dataclasses import dataclass
 
 import torch
 from transformers.cache_utils import Cache, CacheLayerMixin
+
+from lazykv_amd import kernels
 
 
 @dataclass
@@ -72,16 +77,31 @@ class DenseLayer(CacheLayerMixin):
         self.is_initialized = True
 
     def update(self, key_states: torch.Tensor, value_states: torch.Tensor, *args: object, **kwargs: object) -> tuple[torch.Tensor, torch.Tensor]:
+        self.store(key_states, value_states)
+        return self.dense()
+
+    def store(self, key_states: torch.Tensor, value_states: torch.Tensor) -> None:
+        """Append the tokens' keys and values [1, h, T, d]."""
         if not self.is_initialized:
             self.lazy_initialization(key_states, value_states)
         a = self.length
         b = a + key_states.shape[-2]
         if b > self.max_len:
             raise RuntimeError(f"dense layer full: appending {b - a} tokens to {a} exceeds its {self.max_len}-token capacity")
+        self._write(key_states, value_states, a, b)
+        self.length = b
+
+    def _write(self, key_states: torch.Tensor, value_states: torch.Tensor, a: int, b: int) -> None:
         self.keys[:, :, a:b].copy_(key_states)
         self.values[:, :, a:b].copy_(value_states)
-        self.length = b
-        return self.keys[:, :, :b], self.values[:, :, :b]
+
+    def dense(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """The live tokens' keys and values [1, h, n, d] in the model dtype."""
+        return self.keys[:, :, : self.length], self.values[:, :, : self.length]
+
+    def rows(self) -> kernels.Rows:
+        """The layer's rows as the batch decode reads them."""
+        return kernels.dense_rows(self.keys, self.values)
 
     def _set_length(self, n: int) -> None:
         if n < 0 or n > self.length:
@@ -126,11 +146,57 @@ class DenseLayer(CacheLayerMixin):
 PreallocatedLayer = DenseLayer  # the reference's name for the per-layer store (lazykv/cache.py:20)
 
 
+class MXFP8Layer(DenseLayer):
+    """A dense layer in 8 bits: E4M3 codes under a power-of-two scale for every 32 channels of a row (`kernels.mx_rows`), 33/64 of
+    the model dtype's bytes. Tokens are quantised as they are stored, each on its own, so what the layer holds does not depend on
+    how they came. Every query attends what the layer holds: a forward of several tokens gets all rows read back in the model
+    dtype (exact, but for the code's own rounding), a decode token's attention reads the codes in place (`attention.attend`
+    finds them by the `lazykv_rows` that the returned keys carry)."""
+
+    def lazy_initialization(self, key_states: torch.Tensor, value_states: torch.Tensor) -> None:
+        if key_states.shape[0] != 1 or key_states.shape != value_states.shape:
+            raise ValueError(f"dense layers hold batch-1 KV with matching key/value shapes, got {tuple(key_states.shape)} / {tuple(value_states.shape)}")
+        _, h, _, d = key_states.shape
+        if d not in (64, 128):
+            raise ValueError(f"8-bit layers take head_dim 64 or 128, got {d}")
+        self.codes, self.scales = kernels.mx_empty(1, h, self.max_len, d, key_states.device)
+        self._rows = kernels.mx_rows(self.codes, self.scales, key_states.dtype)
+        self.slab = self.codes
+        self.keys, self.values = self.codes[0], self.codes[1]
+        self.dtype, self.device = key_states.dtype, key_states.device
+        self.is_initialized = True
+
+    def update(self, key_states: torch.Tensor, value_states: torch.Tensor, *args: object, **kwargs: object) -> tuple[torch.Tensor, torch.Tensor]:
+        self.store(key_states, value_states)
+        if key_states.shape[-2] != 1:
+            return self.dense()
+        k, v = self.keys[:, :, : self.length], self.values[:, :, : self.length]
+        k.lazykv_rows = self._rows
+        return k, v
+
+    def _write(self, key_states: torch.Tensor, value_states: torch.Tensor, a: int, b: int) -> None:
+        kernels.append_rows(self._rows, key_states, value_states, start=a)
+
+    def dense(self) -> tuple[torch.Tensor, torch.Tensor]:
+        return kernels.read_rows(self._rows, 0, self.length)
+
+    def rows(self) -> kernels.Rows:
+        return self._rows
+
+    def _token_bytes(self) -> int:
+        if self.slab is None:
+            return 0
+        _, _, h, _, d = self.slab.shape
+        return 2 * h * (d + d // kernels.MX_GROUP)
+
+
 class FullGPUCache(Cache):
     """Every layer's KV held densely in VRAM (the reference's rung 1, lazykv/cache.py:80-102)."""
 
+    layer_type: type[DenseLayer] = DenseLayer
+
     def __init__(self, num_layers: int, max_len: int) -> None:
-        super().__init__(layers=[DenseLayer(max_len) for _ in range(num_layers)])
+        super().__init__(layers=[self.layer_type(max_len) for _ in range(num_layers)])
         self.max_len = max_len
 
     def truncate(self, length: int) -> None:
@@ -151,5 +217,230 @@ class FullGPUCache(Cache):
         """A cache holding copies of per-layer prompt KV [1, h, L, d]."""
         cache = cls(len(layers), max_len)
         for dense, (k, v) in zip(cache.layers, layers):
-            dense.update(k, v)
+            dense.store(k, v)
         return cache
+
+
+class MXFP8Cache(FullGPUCache):
+    """Every layer's KV held in VRAM in 8 bits (`MXFP8Layer`). It takes a FullGPUCache's place: as a model's cache, under a
+    TieredCache (whose dense layers then stay in 8 bits), as a SharedPrefixCache's prefix."""
+
+    layer_type = MXFP8Layer
+
+
+QUANTS = (None, "mxfp8")
+
+
+class SharedLayer(CacheLayerMixin):
+    """One layer of a SharedPrefixCache: the prefix's layer, read only, and the sequences' own rows behind it."""
+
+    def __init__(self, prefix: DenseLayer, n_seqs: int, max_new: int, quant: str | None) -> None:
+        super().__init__()
+        self.prefix = prefix
+        self.prefix_tokens = prefix.get_seq_length()
+        self.prefix_rows = prefix.rows()
+        self.n_seqs, self.max_new, self.quant = n_seqs, max_new, quant
+        self.base = 0  # the longest sequence's own tokens when lengths were last set
+        self.added = 0  # tokens of every sequence since then
+        self.own: tuple[torch.Tensor, ...] = ()  # keys, values, or codes and scales
+        self.own_rows: kernels.Rows | None = None
+
+    def lazy_initialization(self, key_states: torch.Tensor, value_states: torch.Tensor) -> None:
+        p = self.prefix_rows
+        h, d, dtype = p.n_kv, p.head_dim, p.model_dtype
+        if tuple(key_states.shape[:2]) != (self.n_seqs, h) or key_states.shape[3] != d or key_states.dtype != dtype or key_states.device != p.device:
+            raise ValueError(f"expected {dtype} KV of {self.n_seqs} sequences [{self.n_seqs}, {h}, T, {d}] on {p.device}, got {key_states.dtype} "
+                             f"{tuple(key_states.shape)} on {key_states.device}")
+        if self.quant is None:
+            self._hold(torch.zeros((2, self.n_seqs, h, self.max_new, d), dtype=dtype, device=p.device))
+        else:
+            self._hold(*kernels.mx_empty(self.n_seqs, h, self.max_new, d, p.device))
+        self.dtype, self.device = dtype, key_states.device
+        self.is_initialized = True
+
+    def _hold(self, *own: torch.Tensor) -> None:
+        self.own = own
+        self.keys, self.values = own[0][0], own[0][1]
+        self.own_rows = kernels.dense_rows(self.keys, self.values) if self.quant is None else kernels.mx_rows(*own, self.prefix_rows.model_dtype)
+
+    def update(self, key_states: torch.Tensor, value_states: torch.Tensor, *args: object, **kwargs: object) -> tuple[torch.Tensor, torch.Tensor]:
+        raise RuntimeError("a shared layer is written through its SharedPrefixCache")
+
+    def own_dense(self, b: int, n: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """Sequence b's first n own rows [1, h, n, d] in the model dtype."""
+        if self.quant is None:
+            return self.keys[b : b + 1, :, :n], self.values[b : b + 1, :, :n]
+        codes, scales = self.own
+        return kernels.read_rows(kernels.mx_rows(codes[:, b : b + 1], scales[:, b : b + 1], self.prefix_rows.model_dtype), 0, n)
+
+    def keep(self, indices: torch.Tensor) -> None:
+        self.n_seqs = indices.numel()
+        if self.is_initialized:
+            self._hold(*(x.index_select(1, indices) for x in self.own))
+
+    def get_mask_sizes(self, query_length: int) -> tuple[int, int]:
+        return self.get_seq_length() + query_length, 0
+
+    def get_seq_length(self) -> int:
+        return self.prefix_tokens + self.base + self.added
+
+    def get_max_length(self) -> int:
+        return self.prefix_tokens + self.max_new
+
+    def own_bytes(self) -> int:
+        """VRAM of the sequences' own rows."""
+        return sum(x.numel() * x.element_size() for x in self.own)
+
+
+class SharedPrefixCache(Cache):
+    """A batch of `n_seqs` sequences that continue one prefilled cache, the prefix: samples of one prompt, questions about one
+    document. The prefix is held once, however many sequences there are, and is not written to; each sequence has up to `max_new`
+    rows of its own behind it, in the model dtype or, with `quant="mxfp8"`, in 8 bits (what the prefix is held in is its own
+    matter: a FullGPUCache or an MXFP8Cache). It must not be cut below the length it had here while the batch lives.
+
+    A decode forward (input_ids [n_seqs, 1], `**cache.model_kwargs()`) writes each sequence's token and attends in one call, the
+    prefix's keys and values read once for all sequences (`kernels.shared_decode`). A forward of several tokens gives every
+    sequence that many; its attention goes sequence by sequence, over the prefix and the sequence's rows, with the causal attention
+    of `attention.attend`. Sequences of different lengths: write them padded on the right and `truncate` to the lengths they have;
+    later tokens are written and attended behind each one's own end (the model needs position_ids then, [n_seqs, T] from
+    `positions`)."""
+
+    batched = True  # the attention function takes a batch from this selector
+    policy_name = "shared_prefix"
+
+    def __init__(self, prefix: FullGPUCache, n_seqs: int, max_new: int, quant: str | None = None) -> None:
+        if quant not in QUANTS:
+            raise ValueError(f"unknown precision {quant!r}; expected one of {QUANTS}")
+        if n_seqs <= 0 or max_new <= 0:
+            raise ValueError(f"a batch needs sequences and room for their tokens, got n_seqs={n_seqs}, max_new={max_new}")
+        lengths = {layer.get_seq_length() if layer.is_initialized else 0 for layer in prefix.layers}
+        if len(lengths) != 1 or 0 in lengths:
+            raise ValueError(f"the prefix must be prefilled, every layer with as many tokens; they hold {sorted(lengths)}")
+        super().__init__(layers=[SharedLayer(layer, n_seqs, max_new, quant) for layer in prefix.layers])
+        self.full = prefix
+        self.n_seqs, self.max_new, self.quant = n_seqs, max_new, quant
+        self.prefix_tokens = lengths.pop()
+        self._base = [0] * n_seqs  # own lengths as last set; a layer has `added` more
+        self._starts: torch.Tensor | None = None  # those on the device, where they differ
+        self._scratch: tuple[torch.Tensor, torch.Tensor] | None = None
+
+    # -- lengths ----------------------------------------------------------------------------------
+
+    def _room(self, layer: SharedLayer) -> tuple[int, int]:
+        """(what a call adds to `_starts`, tokens of its own that a sequence has at the most) in a layer."""
+        most = layer.base + layer.added
+        return (most if self._starts is None else layer.added), most
+
+    def lengths(self, layer_idx: int = 0) -> list[int]:
+        """Own tokens of each sequence."""
+        return [n + self.layers[layer_idx].added for n in self._base]
+
+    def positions(self, n_new: int = 1) -> torch.Tensor:
+        """position_ids [n_seqs, n_new] of each sequence's next tokens."""
+        start = torch.tensor(self.lengths(), device=self.layers[0].prefix_rows.device) + self.prefix_tokens
+        return start[:, None] + torch.arange(n_new, device=start.device)
+
+    def truncate(self, lengths: int | list[int]) -> None:
+        """Forget each sequence's own tokens past its length (one for all, or one each), between forwards."""
+        new = [lengths] * self.n_seqs if isinstance(lengths, int) else [int(n) for n in lengths]
+        now = self._whole()
+        if len(new) != self.n_seqs or any(n < 0 or n > m for n, m in zip(new, now)):
+            raise ValueError(f"sequences of {now} own tokens cannot be cut to {new}")
+        self._set(new)
+
+    def keep(self, indices: list[int] | torch.Tensor) -> None:
+        """Go on with these sequences, in this order: finished ones left out, one more than once (a beam's branches, each with a
+        copy of its rows)."""
+        chosen = [int(i) for i in indices]
+        if not chosen or any(i < 0 or i >= self.n_seqs for i in chosen):
+            raise ValueError(f"sequences {chosen} of {self.n_seqs}")
+        now = self._whole()
+        at = torch.tensor(chosen, dtype=torch.int64, device=self.layers[0].prefix_rows.device)
+        for layer in self.layers:
+            layer.keep(at)
+        self.n_seqs = len(chosen)
+        self._set([now[i] for i in chosen])
+
+    def _whole(self) -> list[int]:
+        if len({layer.added for layer in self.layers}) != 1:
+            raise RuntimeError("lengths are set between forwards: the layers hold different numbers of tokens")
+        return self.lengths()
+
+    def _set(self, lengths: list[int]) -> None:
+        self._base = lengths
+        for layer in self.layers:
+            layer.base, layer.added = max(lengths), 0
+        same = len(set(lengths)) == 1
+        self._starts = None if same else torch.tensor(lengths, dtype=torch.int32, device=self.layers[0].prefix_rows.device)
+
+    # -- transformers plumbing --------------------------------------------------------------------
+
+    def update(self, key_states: torch.Tensor, value_states: torch.Tensor, layer_idx: int, *args: object, **kwargs: object) -> tuple[torch.Tensor, torch.Tensor]:
+        """The tokens' keys and values [n_seqs, h, T, d] behind each sequence's own. What is returned is the new tokens' alone:
+        the attention is `select`'s."""
+        layer = self.layers[layer_idx]
+        if not layer.is_initialized:
+            layer.lazy_initialization(key_states, value_states)
+        n_new = key_states.shape[-2]
+        start, most = self._room(layer)
+        if most + n_new > self.max_new:
+            raise RuntimeError(f"sequences full: appending {n_new} tokens to {most} exceeds their {self.max_new}-token capacity")
+        kernels.append_rows(layer.own_rows, key_states, value_states, start=start, starts=self._starts)
+        layer.added += n_new
+        return key_states, value_states
+
+    def get_seq_length(self, layer_idx: int = 0) -> int:
+        """The longest sequence's tokens, the prefix's among them."""
+        return self.prefix_tokens + self._room(self.layers[layer_idx])[1]
+
+    def model_kwargs(self) -> dict[str, object]:
+        """The forward's extra keyword: this cache, as the attention function's selector."""
+        return {"lazykv_selector": self}
+
+    def select(self, layer_idx: int, query: torch.Tensor, key: torch.Tensor | None = None, value: torch.Tensor | None = None,
+               scaling: float | None = None) -> Decoded:
+        """The attention of the forward's tokens, whose keys and values `update` has taken: query [n_seqs, n_q, T, d]. The lse is that
+        of a decode step; of a forward of several tokens it is empty."""
+        layer = self.layers[layer_idx]
+        if query.shape[0] != self.n_seqs:
+            raise ValueError(f"queries of {query.shape[0]} sequences, the cache holds {self.n_seqs}")
+        _, n_q, n_new, d = query.shape
+        scale = scaling if scaling is not None else d**-0.5
+        if n_new > 1:
+            return self._select_many(layer, query, scale)
+        start, most = self._room(layer)
+        out, lse = kernels.shared_decode(query, scale=scale, prefix=layer.prefix_rows, prefix_tokens=self.prefix_tokens, own=layer.own_rows,
+                                         own_tokens=start, lengths=self._starts, max_own=most)
+        return Decoded(out.view(self.n_seqs, n_q, 1, d), lse)
+
+    def _select_many(self, layer: SharedLayer, query: torch.Tensor, scale: float) -> Decoded:
+        """Several tokens of each sequence: the prefix into one dense buffer, then each sequence's rows behind it in turn."""
+        from lazykv_amd.attention import attend
+
+        p, r = self.prefix_tokens, layer.prefix_rows
+        lengths = [n + layer.added for n in self._base]
+        total = p + max(lengths)
+        if self._scratch is None or self._scratch[0].shape[1] != r.n_kv or self._scratch[0].shape[2] < total:
+            shape = (1, r.n_kv, -(-total // 256) * 256, r.head_dim)
+            self._scratch = (torch.empty(shape, dtype=r.model_dtype, device=r.device), torch.empty(shape, dtype=r.model_dtype, device=r.device))
+        k, v = self._scratch
+        if isinstance(layer.prefix, MXFP8Layer):
+            kernels.read_rows(r, 0, p, out=(k[:, :, :p], v[:, :, :p]))
+        else:
+            k[:, :, :p].copy_(layer.prefix.keys[:, :, :p])
+            v[:, :, :p].copy_(layer.prefix.values[:, :, :p])
+        outs = []
+        for b, n in enumerate(lengths):
+            own_k, own_v = layer.own_dense(b, n)
+            k[:, :, p : p + n].copy_(own_k)
+            v[:, :, p : p + n].copy_(own_v)
+            outs.append(attend(query[b : b + 1], k[:, :, : p + n], v[:, :, : p + n], scale))
+        return Decoded(torch.cat(outs), torch.empty(0, device=r.device))
+
+    def stats(self) -> CacheStats:
+        """The prefix's bytes, once, and the sequences' own."""
+        p = self.full.stats()
+        own = sum(layer.own_bytes() for layer in self.layers)
+        used = own * sum(self.lengths()) // (self.n_seqs * self.max_new)
+        return CacheStats(seq_len=self.get_seq_length(), gpu_resident_kv_bytes=p.gpu_resident_kv_bytes + used, host_kv_bytes=0,
+                          gpu_allocated_kv_bytes=p.gpu_allocated_kv_bytes + own)

@@ -21,7 +21,7 @@ import torch
 from transformers.cache_utils import Cache
 
 from lazykv_amd import _lib, kernels
-from lazykv_amd.cache import CacheStats, Decoded, FullGPUCache
+from lazykv_amd.cache import CacheStats, Decoded, FullGPUCache, MXFP8Layer
 
 QUEST_DENSE_LAYERS = 2  # lazykv/selection.py:35 -- Quest's first two layers stay dense
 
@@ -120,6 +120,8 @@ class QuestView(Cache):
 
     def __init__(self, full: FullGPUCache, k_blocks: int, block_size: int, dense_layers: int = QUEST_DENSE_LAYERS,
                  bound_dtype: torch.dtype | None = None) -> None:
+        if any(isinstance(layer, MXFP8Layer) for layer in full.layers[dense_layers:]):
+            raise ValueError("the selecting layers' rows are read in the model dtype; an 8-bit cache has none")
         super().__init__(layers=full.layers)
         self.full = full  # decode writes into the full cache's own layers; this view holds no KV
         self.k_blocks = k_blocks

@@ -32,7 +32,7 @@ from typing import Any
 
 import torch
 
-from lazykv_amd.cache import FullGPUCache
+from lazykv_amd.cache import FullGPUCache, MXFP8Cache
 from lazykv_amd.pinned import pinned_empty
 from lazykv_amd.tiered import TieredCache, TieredLayer
 
@@ -89,6 +89,8 @@ def save(cache: TieredCache, next_logits: torch.Tensor, path: Path) -> SaveStats
     (lazykv/snapshot.py:67-114). The int8 tier is refused, as in the reference."""
     if cache.quant is not None:
         raise ValueError("snapshots hold model-dtype pairs; the int8 tier is not supported")
+    if isinstance(cache.full, MXFP8Cache):
+        raise ValueError("snapshots hold model-dtype rows; 8-bit dense layers are not supported")
     t0 = time.perf_counter()
     torch.cuda.synchronize()
     tiers = cache.tiers

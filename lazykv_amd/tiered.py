@@ -614,7 +614,7 @@ class TieredCache(Cache):
 
     `full` is the exactly prefilled cache (a FullGPUCache, or a list of per-layer (keys, values)
     [1, h, L, d] on the GPU, which is copied into one). Its first `dense_layers` layers stay in it
-    and keep growing during decode; every other layer becomes a TieredLayer, unless `tiers` brings
+    and keep growing during decode (in 8 bits where it is an MXFP8Cache); every other layer becomes a TieredLayer, unless `tiers` brings
     them prebuilt (the layer-major prefill, which never holds them in `full`). `select` returns a
     `Decoded` (the finished attention of the step), or None to attend densely.
 
@@ -709,10 +709,9 @@ class TieredCache(Cache):
             return tiers
         built: dict[int, TieredLayer] = {}
         for j, layer_idx in enumerate(selecting):
-            dense = self.full.layers[layer_idx]
-            length = dense.get_seq_length()
+            keys, values = self.full.layers[layer_idx].dense()
             pool = host_pools[j] if host_pools is not None else None
-            built[layer_idx] = TieredLayer(dense.keys[:, :, :length], dense.values[:, :, :length], self.k_blocks, self.block_size, capacity_tokens,
+            built[layer_idx] = TieredLayer(keys, values, self.k_blocks, self.block_size, capacity_tokens,
                                            pool, n_slots, quant=self.quant, fetch=self.fetch, exact=self.exact_split, rank_dtype=rank_dtype)
         return built
 

@@ -28,7 +28,7 @@ from typing import Any
 import torch
 from transformers.cache_utils import Cache
 
-from lazykv_amd.cache import DenseLayer, FullGPUCache
+from lazykv_amd.cache import QUANTS, DenseLayer, FullGPUCache, MXFP8Cache
 from lazykv_amd.selection import QUEST_DENSE_LAYERS
 from lazykv_amd.tiered import TieredCache, TieredLayer
 
@@ -122,11 +122,13 @@ def tiered_prefill(
     host_pools: list[torch.Tensor] | None = None,
     n_slots: int | None = None,
     quant: str | None = None,
+    dense_quant: str | None = None,
     **cache_kwargs: Any,
 ) -> TieredPrefillResult:
     """Prefill `input_ids` layer by layer into a decode-ready TieredCache (the reference's
     signature, lazykv/tiered_prefill.py:70-82). `cache_kwargs` (fetch, exact, rank_dtype, ...) go
-    to the cache, and the ones that shape a tier to each layer's tier as well."""
+    to the cache, and the ones that shape a tier to each layer's tier as well. `dense_quant="mxfp8"` (this
+    library's own) holds the layers below `dense_layers` in 8 bits, from the prompt on."""
     backbone = model.model
     device = next(model.parameters()).device
     prompt = input_ids.to(device).reshape(1, -1)
@@ -135,6 +137,8 @@ def tiered_prefill(
         raise ValueError(f"prompt of {n} tokens exceeds capacity {capacity_tokens}")
     if chunk_size <= 0:
         raise ValueError(f"chunk_size must be positive, got {chunk_size}")
+    if dense_quant not in QUANTS:
+        raise ValueError(f"unknown dense precision {dense_quant!r}; expected one of {QUANTS}")
     tier_kw = {key: value for key, value in cache_kwargs.items() if key in _TIER_KW}
     tier_kw.setdefault("fetch", "runs")  # the layers are read the way the cache will read them: its default
     torch.cuda.synchronize(device)
@@ -149,7 +153,7 @@ def tiered_prefill(
     states = [embedded[:, a:b] for a, b in spans]  # per-chunk hidden states, replaced layer by layer
     chunk_rope = [((positions[:, a:b]), (cos[:, a:b], sin[:, a:b])) for a, b in spans]
 
-    full = FullGPUCache(len(backbone.layers), capacity_tokens)
+    full = (FullGPUCache if dense_quant is None else MXFP8Cache)(len(backbone.layers), capacity_tokens)
     scratch = DenseLayer(n)
     tier_stream = torch.cuda.Stream(device)
     router = _StreamingTierCache(full, dense_layers, tier_stream)
