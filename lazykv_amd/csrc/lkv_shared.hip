@@ -19,11 +19,12 @@
 
 namespace {
 
-constexpr int kWaves = 4;      // of a workgroup; each takes every fourth tile of the workgroup's tokens
+constexpr int kWaves = 4;      // of a workgroup on streams
 constexpr int kTile = 32;      // tokens
 constexpr float kSlack = 6.0f; // a weight is at most 2^kSlack: nothing to a 16-bit weight's precision or a float32 sum's
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -378,43 +379,6 @@ __device__ __forceinline__ float join_factor(float m, float l, float top) {
   return m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(m - top);
 }
 
-// The results of wave groups 0 .. GROUPS - 1 into group 0's, lane by lane: the upper half's into the lower's,
-// and so on. `slot`: the wave's place in its group of `width`.
-template <int D, int NR, int GROUPS>
-__device__ __forceinline__ void join_waves(Result<D, NR>& r, int group, int slot, int width, f32x4* lds) {
-  const int lane = threadIdx.x & 63;
-  constexpr int PER = NR * (D / 16);
-  float2* const sml = (float2*)(lds + (GROUPS / 2) * width * PER * 64);
-#pragma unroll
-  for (int half = GROUPS / 2; half > 0; half /= 2) {
-    __syncthreads();
-    if (group >= half && group < 2 * half) {
-      const int to = (group - half) * width + slot;
-#pragma unroll
-      for (int n = 0; n < NR; ++n) {
-        sml[(to * NR + n) * 64 + lane] = make_float2(r.m[n], r.l[n]);
-#pragma unroll
-        for (int e = 0; e < D / 16; ++e) lds[(to * PER + n * (D / 16) + e) * 64 + lane] = r.o[n][e];
-      }
-    }
-    __syncthreads();
-    if (group < half) {
-      const int from = group * width + slot;
-#pragma unroll
-      for (int n = 0; n < NR; ++n) {
-        const float2 other = sml[(from * NR + n) * 64 + lane];
-        const float top = fmaxf(r.m[n], other.x);
-        const float f = join_factor(r.m[n], r.l[n], top), fo = join_factor(other.x, other.y, top);
-        r.m[n] = top;
-        r.l[n] = r.l[n] * f + other.y * fo;
-#pragma unroll
-        for (int e = 0; e < D / 16; ++e) r.o[n][e] = r.o[n][e] * f + lds[(from * PER + n * (D / 16) + e) * 64 + lane] * fo;
-      }
-    }
-  }
-}
-constexpr int join_bytes(int d, int nr, int groups, int width) { return (groups / 2) * width * nr * 64 * (d / 16 * 16 + 8); }
-
 // Four neighbouring outputs.
 template <int ODT>
 __device__ __forceinline__ void store_four(void* out, int64_t at, f32x4 x) {
@@ -425,57 +389,112 @@ __device__ __forceinline__ void store_four(void* out, int64_t at, f32x4 x) {
   }
 }
 
-// The k-th four channels of a lane's, and where they belong. TILED: channels 16 e + 4 q + i in o[e][i], else
-// (d/4) q + (d/16) i + e.
+// Where the k-th four channels of a lane's lie. TILED: channels 16 e + 4 q + i in o[e][i], else (d/4) q + (d/16) i + e.
+template <int D, bool TILED>
+__device__ __forceinline__ int channel_of(int k) {
+  const int quarter = (threadIdx.x & 63) >> 4;
+  return TILED ? 16 * k + 4 * quarter : (D / 4) * quarter + (D / 16) * (k / (D / 64)) + k % (D / 64) * 4;
+}
 template <int D, bool TILED>
 __device__ __forceinline__ f32x4 four_of(const f32x4 (&o)[D / 16], int k, int& channel) {
-  const int quarter = (threadIdx.x & 63) >> 4;
+  channel = channel_of<D, TILED>(k);
   if constexpr (TILED) {
-    channel = 16 * k + 4 * quarter;
     return o[k];
   } else {
-    constexpr int E = D / 64;  // fours of e for an i
-    const int i = k / E, e = k % E * 4;
-    channel = (D / 4) * quarter + (D / 16) * i + e;
+    const int i = k / (D / 64), e = k % (D / 64) * 4;
     return f32x4{o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]};
   }
 }
 
-template <int ODT, int D, bool TILED>
-__device__ __forceinline__ void store_output(void* out, int64_t row, float l, const f32x4 (&o)[D / 16]) {
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-  for (int k = 0; k < D / 16; ++k) {
-    int c;
-    f32x4 x = four_of<D, TILED>(o, k, c) * inv;
-    store_four<ODT>(out, row * D + c, x);
+// Four channels of a row: a part's, or, where it is the only part, the output's.
+template <int D>
+__device__ __forceinline__ void store_part(const SharedArgs& a, int64_t row, int part, int channel, float l, f32x4 x) {
+  const int parts = a.p_parts + a.o_parts;
+  if (parts > 1) {
+    *(f32x4*)(a.part_o + (row * parts + part) * D + channel) = x;
+    return;
+  }
+  x *= l == 0.0f ? 0.0f : 1.0f / l;
+  if (a.out_dtype == LKV_F32) {
+    store_four<LKV_F32>(a.out, row * D + channel, x);
+  } else if (a.out_dtype == LKV_BF16) {
+    store_four<LKV_BF16>(a.out, row * D + channel, x);
+  } else {
+    store_four<LKV_F16>(a.out, row * D + channel, x);
+  }
+}
+__device__ __forceinline__ void store_sums(const SharedArgs& a, int64_t row, int part, float m, float l) {
+  const int parts = a.p_parts + a.o_parts;
+  if (parts > 1) {
+    a.part_ml[row * parts + part] = make_float2(m, l);
+  } else {
+    a.lse[row] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * lkv::kLn2;
   }
 }
 
-// A row's result: the output itself where this is its only part.
-template <int D, bool TILED>
-__device__ __forceinline__ void store_row(const SharedArgs& a, int64_t row, int part, float m, float l, const f32x4 (&o)[D / 16]) {
-  const int parts = a.p_parts + a.o_parts, quarter = (threadIdx.x & 63) >> 4;
-  if (parts > 1) {
-    const int64_t slot = row * parts + part;
-    if (quarter == 0) a.part_ml[slot] = make_float2(m, l);
+// The end of a part: the results that GROUPS waves have for the same rows, each from its own tokens, joined and
+// stored. All waves write theirs to LDS, then each takes its share of the channels. `group` and `slot`: which of
+// the waves this is, and whose rows of `width` sets it has. row[n]: this lane's rows, -1 for none.
+template <int D, int NR, int GROUPS, bool TILED>
+__device__ __forceinline__ void finish(const SharedArgs& a, const Result<D, NR>& r, const int64_t (&row)[NR], int part, int group, int slot, int width,
+                                       f32x4* lds) {
+  constexpr int FOURS = D / 16;
+  const int lane = threadIdx.x & 63, quarter = lane >> 4;
+  if constexpr (GROUPS == 1) {
 #pragma unroll
-    for (int k = 0; k < D / 16; ++k) {
-      int c;
-      const f32x4 x = four_of<D, TILED>(o, k, c);
-      *(f32x4*)(a.part_o + slot * D + c) = x;
+    for (int n = 0; n < NR; ++n) {
+      if (row[n] < 0) continue;
+      if (quarter == 0) store_sums(a, row[n], part, r.m[n], r.l[n]);
+#pragma unroll
+      for (int k = 0; k < FOURS; ++k) {
+        int c;
+        const f32x4 x = four_of<D, TILED>(r.o[n], k, c);
+        store_part<D>(a, row[n], part, c, r.l[n], x);
+      }
     }
     return;
-  }
-  if (quarter == 0) a.lse[row] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * lkv::kLn2;
-  if (a.out_dtype == LKV_F32) {
-    store_output<LKV_F32, D, TILED>(a.out, row, l, o);
-  } else if (a.out_dtype == LKV_BF16) {
-    store_output<LKV_BF16, D, TILED>(a.out, row, l, o);
   } else {
-    store_output<LKV_F16, D, TILED>(a.out, row, l, o);
+    float2* const ml = (float2*)(lds + GROUPS * width * NR * FOURS * 64);
+    __syncthreads();  // what LDS held before is read no more
+    const int mine = (group * width + slot) * NR;
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      ml[(mine + n) * 64 + lane] = make_float2(r.m[n], r.l[n]);
+#pragma unroll
+      for (int k = 0; k < FOURS; ++k) {
+        int c;
+        lds[((mine + n) * FOURS + k) * 64 + lane] = four_of<D, TILED>(r.o[n], k, c);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      float2 x[GROUPS];
+      float top = -INFINITY, total = 0.0f;
+#pragma unroll
+      for (int i = 0; i < GROUPS; ++i) {
+        x[i] = ml[((i * width + slot) * NR + n) * 64 + lane];
+        top = fmaxf(top, x[i].x);
+      }
+#pragma unroll
+      for (int i = 0; i < GROUPS; ++i) {
+        x[i].x = join_factor(x[i].x, x[i].y, top);
+        total += x[i].x * x[i].y;
+      }
+      if (group == 0 && quarter == 0 && row[n] >= 0) store_sums(a, row[n], part, top, total);
+#pragma unroll
+      for (int j = 0; j < (FOURS + GROUPS - 1) / GROUPS; ++j) {
+        const int k = j * GROUPS + group;
+        if (FOURS % GROUPS != 0 && k >= FOURS) break;
+        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < GROUPS; ++i) o += lds[(((i * width + slot) * NR + n) * FOURS + k) * 64 + lane] * x[i].x;
+        if (row[n] >= 0) store_part<D>(a, row[n], part, channel_of<D, TILED>(k), total, o);
+      }
+    }
   }
 }
+constexpr int finish_bytes(int d, int nr, int groups, int width) { return groups == 1 ? 0 : groups * width * nr * 64 * (d + 8); }
 
 // A KV head's query row x of the prefix's: row x of all sequences', g a sequence; -1 behind the last.
 __device__ __forceinline__ int64_t prefix_row(const SharedArgs& a, int h, int x) {
@@ -483,11 +502,10 @@ __device__ __forceinline__ int64_t prefix_row(const SharedArgs& a, int h, int x)
   return b < a.n_seqs ? (int64_t)b * a.n_q + h * a.g + (x - b * a.g) : -1;
 }
 
-// The `item`-th piece of own rows, by four waves; `join`: the item's place in its workgroup's LDS. Every wave of the
-// workgroup takes part in the joins' barriers.
-template <int DT, int D, bool OMX>
-__device__ __forceinline__ void own_item(const SharedArgs& a, int64_t item, int wave, f32x4* join) {
-  const int lane = threadIdx.x & 63;
+// The `item`-th piece of own rows, by W waves; `lds`: the item's own. Every wave of the workgroup takes part in the
+// barriers at the end.
+template <int DT, int D, bool OMX, int W>
+__device__ __forceinline__ void own_item(const SharedArgs& a, int64_t item, int wave, f32x4* lds) {
   const bool live = item < (int64_t)a.n_seqs * a.n_kv * a.g_tiles * a.o_parts;
   int id = live ? (int)item : 0;
   const int part = id % a.o_parts;
@@ -495,22 +513,22 @@ __device__ __forceinline__ void own_item(const SharedArgs& a, int64_t item, int 
   const int tile = id % a.g_tiles;
   id /= a.g_tiles;
   const int h = id % a.n_kv, b = id / a.n_kv;
-  const int j = tile * 16 + (lane & 15);
-  const int64_t row = (int64_t)b * a.n_q + h * a.g + j;
+  const int j = tile * 16 + (threadIdx.x & 15);
+  const int64_t row[1] = {live && j < a.g ? (int64_t)b * a.n_q + h * a.g + j : -1};
   const int t0 = part * a.o_chunk, end = live ? min(t0 + a.o_chunk, own_length(a, b)) : 0;
-  const uint16_t* q[1] = {j < a.g ? a.q + row * D : nullptr};
+  const uint16_t* q[1] = {row[0] >= 0 ? a.q + row[0] * D : nullptr};
   Result<D, 1> r;
-  attend_range<DT, D, OMX, 1>(stream_of<D, OMX>(a.own, b, h), q, t0 + wave * kTile, kWaves * kTile, end, a.scale2, r);
-  join_waves<D, 1, kWaves>(r, wave, 0, 1, join);
-  if (live && wave == 0 && j < a.g) store_row<D, false>(a, row, a.p_parts + part, r.m[0], r.l[0], r.o[0]);
+  attend_range<DT, D, OMX, 1>(stream_of<D, OMX>(a.own, b, h), q, t0 + wave * kTile, W * kTile, end, a.scale2, r);
+  finish<D, 1, W, false>(a, r, row, a.p_parts + part, wave, 0, 1, lds);
 }
 
+// Few rows: every wave on its own stream of tokens, straight from memory to registers.
 template <int DT, int D, bool PMX, bool OMX, int NR>
-__global__ __launch_bounds__(256, 2) void shared_decode_kernel(SharedArgs a) {
-  __shared__ f32x4 join[join_bytes(D, NR, kWaves, 1) / 16];
+__global__ __launch_bounds__(64 * kWaves, 2) void shared_decode_kernel(SharedArgs a) {
+  __shared__ f32x4 lds[finish_bytes(D, NR, kWaves, 1) / 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int id = blockIdx.x, p_blocks = a.p_groups * 8 * a.row_tiles;
-  if (id >= p_blocks) return own_item<DT, D, OMX>(a, id - p_blocks, wave, join);
+  if (id >= p_blocks) return own_item<DT, D, OMX, kWaves>(a, id - p_blocks, wave, lds);
   // Workgroups go round the 8 XCDs by their number: the row tiles of one head and token range sit on
   // one of them, one after the other, and find its keys and values in that L2.
   const int unit = (id / (8 * a.row_tiles)) * 8 + id % 8, tile = id / 8 % a.row_tiles;
@@ -526,12 +544,7 @@ __global__ __launch_bounds__(256, 2) void shared_decode_kernel(SharedArgs a) {
   const int t0 = part * a.p_chunk, end = min(t0 + a.p_chunk, a.prefix_tokens);
   Result<D, NR> r;
   attend_range<DT, D, PMX, NR>(stream_of<D, PMX>(a.prefix, 0, h), q, t0 + wave * kTile, kWaves * kTile, end, a.scale2, r);
-  join_waves<D, NR, kWaves>(r, wave, 0, 1, join);
-  if (wave == 0) {
-#pragma unroll
-    for (int n = 0; n < NR; ++n)
-      if (row[n] >= 0) store_row<D, false>(a, row[n], part, r.m[n], r.l[n], r.o[n]);
-  }
+  finish<D, NR, kWaves, false>(a, r, row, part, wave, 0, 1, lds);
 }
 
 // ---- many rows: the prefix through LDS --------------------------------------------------------------
@@ -542,53 +555,82 @@ __global__ __launch_bounds__(256, 2) void shared_decode_kernel(SharedArgs a) {
 // tokens of an operand lie in different banks; the values' operands are read transposed.
 template <int D, int WR> struct Stage {
   static constexpr int WT = 8 / WR;
-  static constexpr int TOKENS = WR == 2 ? 128 : 64;
+  static constexpr int TOKENS = WR == 8 ? 64 : 128;
   static constexpr int TILES = TOKENS / (kTile * WT);      // of a wave in a stage
   static constexpr int PIECES = D / 8;                     // 16-byte pieces of a row
-  static constexpr int LOADS = TOKENS * PIECES / 512;      // of a thread, for keys and for values
   static constexpr int BYTES = TOKENS * 2 * D;             // of keys, and of values
   static __device__ __forceinline__ int swizzle(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
 };
 
-template <int DT, int D, bool MX, int WR> struct StageRegs {
+// What a thread holds of a stage on its way to LDS.
+template <int DT, int D, bool MX, int WR> struct StageRegs;
+template <int DT, int D, int WR> struct StageRegs<DT, D, false, WR> {
   using S = Stage<D, WR>;
-  uint4 k[S::LOADS], v[S::LOADS];  // 8 bits: codes in x and y, the scale in z
+  static constexpr int LOADS = S::TOKENS * S::PIECES / 512;  // 16-byte pieces of keys, and of values
+  u32x4 k[LOADS], v[LOADS];
   // Tokens t0 .. of the stream; behind `end`, its last token.
   __device__ __forceinline__ void load(const Stream& s, int t0, int end) {
     const int last = min(S::TOKENS, end - t0) - 1;
+    const uint8_t *kb = s.k + (int64_t)t0 * (2 * D), *vb = s.v + (int64_t)t0 * (2 * D);
 #pragma unroll
-    for (int i = 0; i < S::LOADS; ++i) {
-      const int x = i * 512 + threadIdx.x, row = min(x / S::PIECES, last), piece = x % S::PIECES;
-      if constexpr (MX) {
-        const uint32_t at = (uint32_t)(row * D + piece * 8);
-        const uint8_t *kb = s.k + (int64_t)t0 * D, *vb = s.v + (int64_t)t0 * D;
-        const uint8_t *ks = s.ks + (int64_t)t0 * (D / kMxGroup), *vs = s.vs + (int64_t)t0 * (D / kMxGroup);
-        const uint2 a = *(const uint2*)(kb + at), b = *(const uint2*)(vb + at);
-        k[i] = make_uint4(a.x, a.y, ks[at / kMxGroup], 0);
-        v[i] = make_uint4(b.x, b.y, vs[at / kMxGroup], 0);
-      } else {
-        const uint32_t at = (uint32_t)(row * (2 * D) + piece * 16);
-        k[i] = *(const uint4*)(s.k + (int64_t)t0 * (2 * D) + at);
-        v[i] = *(const uint4*)(s.v + (int64_t)t0 * (2 * D) + at);
-      }
+    for (int i = 0; i < LOADS; ++i) {
+      const int x = i * 512 + threadIdx.x;
+      const uint32_t at = (uint32_t)(min(x / S::PIECES, last) * (2 * D) + x % S::PIECES * 16);
+      k[i] = *(const u32x4*)(kb + at);
+      v[i] = *(const u32x4*)(vb + at);
     }
-  }
-  static __device__ __forceinline__ uint4 widen(uint4 x) {
-    if constexpr (MX) {
-      const float f = lkv::bits_to_float(x.z << 23);
-      return make_uint4(Mat<DT>::template widen<false>(x.x, f), Mat<DT>::template widen<true>(x.x, f), Mat<DT>::template widen<false>(x.y, f),
-                        Mat<DT>::template widen<true>(x.y, f));
-    }
-    return x;
   }
   // Into LDS; values of tokens behind the end as zeros, which a weight of 0 leaves.
   __device__ __forceinline__ void store(uint8_t* lds, int live) const {
 #pragma unroll
-    for (int i = 0; i < S::LOADS; ++i) {
-      const int x = i * 512 + threadIdx.x, row = x / S::PIECES, piece = (x % S::PIECES) ^ S::swizzle(row);
-      uint8_t* to = lds + row * (2 * D) + piece * 16;
-      *(uint4*)to = widen(k[i]);
-      *(uint4*)(to + S::BYTES) = row < live ? widen(v[i]) : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < LOADS; ++i) {
+      const int x = i * 512 + threadIdx.x, row = x / S::PIECES;
+      uint8_t* to = lds + row * (2 * D) + (x % S::PIECES ^ S::swizzle(row)) * 16;
+      const uint32_t keep = row < live ? ~0u : 0u;
+      *(u32x4*)to = k[i];
+      *(u32x4*)(to + S::BYTES) = v[i] & keep;
+    }
+  }
+};
+// 8 bits: 16 codes under one scale become two pieces.
+template <int DT, int D, int WR> struct StageRegs<DT, D, true, WR> {
+  using S = Stage<D, WR>;
+  static constexpr int UNITS = S::TOKENS * D / 16, LOADS = (UNITS + 511) / 512;
+  uint4 k[LOADS], v[LOADS];
+  uint32_t ks[LOADS], vs[LOADS];
+  static __device__ __forceinline__ bool mine(int i) { return UNITS % 512 == 0 || i * 512 + (int)threadIdx.x < UNITS; }
+  __device__ __forceinline__ void load(const Stream& s, int t0, int end) {
+    const int last = min(S::TOKENS, end - t0) - 1;
+    const uint8_t *kb = s.k + (int64_t)t0 * D, *vb = s.v + (int64_t)t0 * D;
+    const uint8_t *ksb = s.ks + (int64_t)t0 * (D / kMxGroup), *vsb = s.vs + (int64_t)t0 * (D / kMxGroup);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      if (!mine(i)) continue;
+      const int x = i * 512 + threadIdx.x;
+      const uint32_t at = (uint32_t)(min(x / (D / 16), last) * D + x % (D / 16) * 16);
+      k[i] = *(const uint4*)(kb + at);
+      v[i] = *(const uint4*)(vb + at);
+      ks[i] = ksb[at / kMxGroup];
+      vs[i] = vsb[at / kMxGroup];
+    }
+  }
+  static __device__ __forceinline__ uint4 widen(uint32_t lo, uint32_t hi, uint32_t scale) {
+    const float f = lkv::bits_to_float(scale << 23);
+    return make_uint4(Mat<DT>::template widen<false>(lo, f), Mat<DT>::template widen<true>(lo, f), Mat<DT>::template widen<false>(hi, f),
+                      Mat<DT>::template widen<true>(hi, f));
+  }
+  __device__ __forceinline__ void store(uint8_t* lds, int live) const {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      if (!mine(i)) continue;
+      const int x = i * 512 + threadIdx.x, row = x / (D / 16), piece = x % (D / 16) * 2, sw = S::swizzle(row);
+      uint8_t* to = lds + row * (2 * D);
+      const uint32_t keep = row < live ? ~0u : 0u;  // a code of zero is zero under any scale that is written
+      *(uint4*)(to + (piece ^ sw) * 16) = widen(k[i].x, k[i].y, ks[i]);
+      *(uint4*)(to + ((piece + 1) ^ sw) * 16) = widen(k[i].z, k[i].w, ks[i]);
+      to += S::BYTES;
+      *(uint4*)(to + (piece ^ sw) * 16) = widen(v[i].x & keep, v[i].y & keep, vs[i]);
+      *(uint4*)(to + ((piece + 1) ^ sw) * 16) = widen(v[i].z & keep, v[i].w & keep, vs[i]);
     }
   }
 };
@@ -602,7 +644,6 @@ __device__ __forceinline__ uint2 read_transposed(LdsPointer p) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
 }
 __device__ __forceinline__ uint4 read_piece(LdsPointer p) {
-  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
   const u32x4 x = *(__attribute__((address_space(3))) const u32x4*)p;
   return make_uint4(x.x, x.y, x.z, x.w);
 }
@@ -707,12 +748,12 @@ __device__ __forceinline__ void attend_wide(const Stream& s, const uint16_t* con
 template <int DT, int D, bool PMX, bool OMX, int WR>
 __global__ __launch_bounds__(512, 2) void shared_wide_kernel(SharedArgs a) {
   using S = Stage<D, WR>;
-  constexpr int STAGES = 2 * 2 * S::BYTES, JOIN = join_bytes(D, 2, S::WT, WR), OWN = join_bytes(D, 1, kWaves, 1);
+  constexpr int STAGES = 2 * 2 * S::BYTES, JOIN = finish_bytes(D, 2, S::WT, WR), OWN = finish_bytes(D, 1, 4, 1);
   constexpr int BYTES = STAGES > JOIN ? (STAGES > 2 * OWN ? STAGES : 2 * OWN) : (JOIN > 2 * OWN ? JOIN : 2 * OWN);
   __shared__ f32x4 lds[BYTES / 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int id = blockIdx.x, p_blocks = a.p_groups * 8 * a.row_tiles;
-  if (id >= p_blocks) return own_item<DT, D, OMX>(a, (int64_t)(id - p_blocks) * 2 + wave / kWaves, wave % kWaves, lds + wave / kWaves * (OWN / 16));
+  if (id >= p_blocks) return own_item<DT, D, OMX, 4>(a, (int64_t)(id - p_blocks) * 2 + wave / 4, wave % 4, lds + wave / 4 * (OWN / 16));
   const int unit = (id / (8 * a.row_tiles)) * 8 + id % 8, tile = id / 8 % a.row_tiles;
   if (unit >= a.p_parts * a.n_kv) return;
   const int part = unit / a.n_kv, h = unit % a.n_kv, wr = wave % WR, wt = wave / WR;
@@ -726,12 +767,7 @@ __global__ __launch_bounds__(512, 2) void shared_wide_kernel(SharedArgs a) {
   const int t0 = part * a.p_chunk, end = min(t0 + a.p_chunk, a.prefix_tokens);
   Result<D, 2> r;
   attend_wide<DT, D, PMX, WR>(stream_of<D, PMX>(a.prefix, 0, h), q, t0, end, wt, a.scale2, r, (uint8_t*)lds);
-  join_waves<D, 2, S::WT>(r, wt, wr, WR, lds);
-  if (wt == 0) {
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-      if (row[n] >= 0) store_row<D, true>(a, row[n], part, r.m[n], r.l[n], r.o[n]);
-  }
+  finish<D, 2, S::WT, true>(a, r, row, part, wt, wr, WR, lds);
 }
 
 // A workgroup a query row: its parts' results into one. d/4 threads take a part's channels, four each, and
@@ -813,18 +849,18 @@ Plan plan_of(const lkv_shared_desc* d) {
   const int g = d->n_q / d->n_kv;
   const int64_t rows = (int64_t)d->n_seqs * g;
   p.nr = d->prefix_tokens == 0 || rows <= 16 ? 1 : (rows <= 32 ? 2 : 0);
-  p.wr = rows <= 64 ? 2 : 4;
+  p.wr = rows <= 64 ? 2 : (rows <= 128 ? 4 : 8);
   p.row_tiles = ceil_div(rows, p.nr ? 16 * p.nr : 32 * p.wr);
   p.g_tiles = ceil_div(g, 16);
   // Tokens that a workgroup takes: as many workgroups as the card holds at once, and no fewer than one tile
   // a wave.
-  const int64_t room = p.nr == 1 ? 768 : (p.nr == 2 ? 512 : 256);
+  const int64_t room = 256;
   const int64_t tokens = (int64_t)p.row_tiles * d->n_kv * d->prefix_tokens + (p.nr ? (int64_t)d->n_seqs * d->n_kv * p.g_tiles * d->max_own : 0);
-  const int64_t least = kWaves * kTile;
+  const int64_t least = p.nr ? 128 : 256;
   int64_t chunk = (tokens / room + least - 1) / least * least;
   if (chunk < least) chunk = least;
   p.p_chunk = p.o_chunk = (int)(chunk > (1 << 30) ? (1 << 30) : chunk);
-  if (!p.nr) p.o_chunk = 1024;
+  if (!p.nr && p.o_chunk > 1024) p.o_chunk = 1024;
   p.p_parts = ceil_div(d->prefix_tokens, p.p_chunk);
   p.o_parts = ceil_div(d->max_own, p.o_chunk);
   p.p_groups = ceil_div((int64_t)p.p_parts * d->n_kv, 8);
@@ -835,7 +871,7 @@ template <int DT, int D, bool PMX, bool OMX>
 void launch(const Plan& p, dim3 grid, hipStream_t s, const SharedArgs& a) {
   auto kernel = p.nr == 1 ? shared_decode_kernel<DT, D, PMX, OMX, 1> : p.nr == 2 ? shared_decode_kernel<DT, D, PMX, OMX, 2>
               : p.wr == 2 ? shared_wide_kernel<DT, D, PMX, OMX, 2> : p.wr == 4 ? shared_wide_kernel<DT, D, PMX, OMX, 4> : shared_wide_kernel<DT, D, PMX, OMX, 8>;
-  hipLaunchKernelGGL(kernel, grid, dim3(p.nr ? 256 : 512), 0, s, a);
+  hipLaunchKernelGGL(kernel, grid, dim3(p.nr ? 64 * kWaves : 512), 0, s, a);
 }
 
 template <int DT, int D>
@@ -853,7 +889,7 @@ extern "C" size_t lkv_shared_decode_workspace_bytes(const lkv_shared_desc* desc)
   if (check_desc(desc)) return 0;
   const Plan p = plan_of(desc);
   const size_t parts = p.p_parts + p.o_parts, rows = (size_t)desc->n_seqs * desc->n_q;
-  return parts < 2 ? 16 : lkv_align_up(rows * parts * sizeof(float2), 16) + rows * parts * desc->head_dim * sizeof(float);
+  return parts < 2 ? 0 : lkv_align_up(rows * parts * sizeof(float2), 16) + rows * parts * desc->head_dim * sizeof(float);
 }
 
 extern "C" int lkv_shared_decode(uintptr_t stream, const lkv_shared_desc* desc, const void* q, int q_dtype, const lkv_kv_rows* prefix,
@@ -864,9 +900,9 @@ extern "C" int lkv_shared_decode(uintptr_t stream, const lkv_shared_desc* desc, 
   LKV_CHECK_ARG(q_dtype == LKV_F16 || q_dtype == LKV_BF16, "queries are float16 or bfloat16, got dtype %d", q_dtype);
   LKV_CHECK_ARG(lkv_is_model_dtype(out_dtype), "unsupported output dtype %d", out_dtype);
   LKV_CHECK_ARG((((uintptr_t)q | (uintptr_t)out) & 15) == 0, "queries and outputs must start on 16 bytes");
-  LKV_CHECK_ARG(ws && ws_bytes >= lkv_shared_decode_workspace_bytes(desc), "workspace of %zu bytes: %zu are needed", ws_bytes,
-                lkv_shared_decode_workspace_bytes(desc));
-  LKV_CHECK_ARG(((uintptr_t)ws & 15) == 0, "the workspace must start on 16 bytes");
+  const size_t need = lkv_shared_decode_workspace_bytes(desc);
+  LKV_CHECK_ARG(need == 0 || (ws && ws_bytes >= need), "workspace of %zu bytes: %zu are needed", ws_bytes, need);
+  LKV_CHECK_ARG(need == 0 || ((uintptr_t)ws & 15) == 0, "the workspace must start on 16 bytes");
   SharedArgs a = {};
   if (desc->prefix_tokens > 0) {
     LKV_CHECK_ARG(prefix, "a prefix of %d tokens without rows", desc->prefix_tokens);

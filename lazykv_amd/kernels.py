@@ -710,7 +710,10 @@ _NOTHING = _Nothing()
 
 def _on(index: int):  # noqa: ANN202
     """The device a launch needs as the current one, where it is another."""
-    return _NOTHING if index == torch.cuda.current_device() else torch.cuda.device(index)
+    return _NOTHING if index == _CURRENT_DEVICE() else torch.cuda.device(index)
+
+
+_CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _raw_stream(index: int) -> int:
@@ -841,7 +844,9 @@ def shared_decode(
     if not q.is_contiguous() or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
     if out is None:
-        out = torch.empty(shape, dtype=out_dtype or dtype, device=q.device)
+        out = torch.empty_like(q) if out_dtype is None or out_dtype == dtype else torch.empty_like(q, dtype=out_dtype)
+        if out.dim() == 4:
+            out = out.view(shape)
     elif not out.is_contiguous() or out.numel() != b * n_q * d or out.get_device() != index or (out_dtype is not None and out.dtype != out_dtype) or out.data_ptr() % 16:
         raise ValueError(f"out must be contiguous [{b}, {n_q}, {d}] on {rows.device}, on 16 bytes")
     if lse is None:
@@ -853,11 +858,12 @@ def shared_decode(
     lib = _lib.lib()
     desc = ctypes.byref(_lib.SharedDesc(b, n_q, rows.n_kv, d, scale, prefix_tokens, own_tokens, max_own))
     need = lib.lkv_shared_decode_workspace_bytes(desc)
-    if ws is None:
-        buf = torch.empty(max(need, 16), dtype=torch.uint8, device=q.device)
-        ws_ptr, ws_n = buf.data_ptr(), need if need > 16 else 16
-    else:
+    if ws is not None:
         ws_ptr, ws_n = ws.get(need)
+    else:
+        # Of the call's own: no other call's, on another stream or in a graph, can be in it.
+        buf = torch.empty(need, dtype=torch.uint8, device=q.device) if need else lse
+        ws_ptr, ws_n = buf.data_ptr(), need
     with _on(index):
         rc = lib.lkv_shared_decode(_raw_stream(index), desc, q.data_ptr(), rows.model_code, prefix.ref if prefix is not None else None,
                                    own.ref if own is not None else None, at, out.data_ptr(), _lib.dtype_code(out.dtype), lse.data_ptr(), ws_ptr, ws_n)
