@@ -258,10 +258,11 @@ struct Reference {
   __device__ __forceinline__ float level(float scale2) const { return limit == -INFINITY ? -INFINITY : -negative[0] * scale2; }
 };
 
-// A tile's scores of one row tile, relative to the reference, to weights, the second product's operand; the
-// reference, l and o follow. `left`: tokens that the tile has, if fewer than 32.
-template <int DT, int D>
-__device__ __forceinline__ uint4 weigh(f32x4 (&sc)[2], int left, float scale2, Reference& ref, float& l, f32x4 (&o)[D / 16]) {
+// A tile's scores of one row tile, relative to the reference, made ready for the exponential: tokens behind the end
+// without weight (`left`: tokens that the tile has, if fewer than 32), the reference moved where it must be; l and o
+// follow it.
+template <int D>
+__device__ __forceinline__ void settle(f32x4 (&sc)[2], int left, float scale2, Reference& ref, float& l, f32x4 (&o)[D / 16]) {
   if (left < kTile) {
     int mine = left - (int)(threadIdx.x & 48) / 4;
     keep_here(mine);
@@ -285,11 +286,22 @@ __device__ __forceinline__ uint4 weigh(f32x4 (&sc)[2], int left, float scale2, R
     sc[0] -= by;
     sc[1] -= by;
   }
+}
+
+// Settled scores to weights, the second product's operand.
+template <int DT>
+__device__ __forceinline__ uint4 weights(const f32x4 (&sc)[2], float scale2, float& l) {
   float w[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) w[j] = __builtin_amdgcn_exp2f(sc[j / 4][j & 3] * scale2);
   l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
   return make_uint4(Mat<DT>::pack(w[0], w[1]), Mat<DT>::pack(w[2], w[3]), Mat<DT>::pack(w[4], w[5]), Mat<DT>::pack(w[6], w[7]));
+}
+
+template <int DT, int D>
+__device__ __forceinline__ uint4 weigh(f32x4 (&sc)[2], int left, float scale2, Reference& ref, float& l, f32x4 (&o)[D / 16]) {
+  settle<D>(sc, left, scale2, ref, l, o);
+  return weights<DT>(sc, scale2, l);
 }
 
 // Loads stay on their side: moved down to where the next tile uses them, they would be waited for.
@@ -555,7 +567,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_decode_kernel(SharedArg
 // tokens of an operand lie in different banks; the values' operands are read transposed.
 template <int D, int WR> struct Stage {
   static constexpr int WT = 8 / WR;
-  static constexpr int TOKENS = WR == 8 ? 64 : 128;
+  static constexpr int TOKENS = WR == 2 ? 128 : 64;
+  static constexpr int BUFFERS = WR == 2 ? 2 : 3;
   static constexpr int TILES = TOKENS / (kTile * WT);      // of a wave in a stage
   static constexpr int PIECES = D / 8;                     // 16-byte pieces of a row
   static constexpr int BYTES = TOKENS * 2 * D;             // of keys, and of values
@@ -682,6 +695,57 @@ __device__ __forceinline__ void wide_tile(const LdsPointer (&key_at)[D / 32], co
     for (int n = 0; n < 2; ++n) r.o[n][e] = Mat<DT>::mma(make_uint4(v[e][0].x, v[e][0].y, v[e][1].x, v[e][1].y), p[n], r.o[n][e]);
 }
 
+// The scores of a tile of 32 staged tokens at offset `at` from the lane's places.
+template <int DT, int D>
+__device__ __forceinline__ void wide_scores(const uint4 (&k)[2][D / 32], const uint4 (&qf)[2][D / 32], const Reference (&ref)[2], f32x4 (&sc)[2][2]) {
+#pragma unroll
+  for (int n = 0; n < 2; ++n) sc[n][0] = sc[n][1] = ref[n].negative;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int n = 0; n < 2; ++n) sc[n][u] = Mat<DT>::mma(k[u][i], qf[n][i], sc[n][u]);
+}
+
+// One tile's step: its weights and their product with its values, and the next tile's scores, whose products fill the
+// time of this one's exponentials.
+template <int DT, int D>
+__device__ __forceinline__ void wide_step(const LdsPointer (&key_at)[D / 32], const LdsPointer (&value_at)[D / 16], int next_at, int at,
+                                          const uint4 (&qf)[2][D / 32], int left, float scale2, Reference (&ref)[2], f32x4 (&sc)[2][2], Result<D, 2>& r) {
+  uint4 k[2][D / 32];
+  uint2 v[D / 16][2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) k[u][i] = read_piece(key_at[i] + next_at + u * 16 * (2 * D));
+#pragma unroll
+  for (int e = 0; e < D / 16; ++e)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) v[e][u] = read_transposed(value_at[e] + at + u * 16 * (2 * D));
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int n = 0; n < 2; ++n) settle<D>(sc[n], left, scale2, ref[n], r.l[n], r.o[n]);
+  f32x4 next[2][2];
+  wide_scores<DT, D>(k, qf, ref, next);
+  uint4 p[2];
+#pragma unroll
+  for (int n = 0; n < 2; ++n) p[n] = weights<DT>(sc[n], scale2, r.l[n]);
+  // Products and the vector unit's work in turn.
+#pragma unroll
+  for (int i = 0; i < 4 * (D / 32); ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x2, 128 / D * 2, 0);
+    __builtin_amdgcn_sched_group_barrier(0x400, 128 / D, 0);
+  }
+#pragma unroll
+  for (int e = 0; e < D / 16; ++e)
+#pragma unroll
+    for (int n = 0; n < 2; ++n) r.o[n][e] = Mat<DT>::mma(make_uint4(v[e][0].x, v[e][0].y, v[e][1].x, v[e][1].y), p[n], r.o[n][e]);
+#pragma unroll
+  for (int n = 0; n < 2; ++n) sc[n][0] = next[n][0], sc[n][1] = next[n][1];
+}
+
 template <int DT, int D, bool MX, int WR>
 __device__ __forceinline__ void attend_wide(const Stream& s, const uint16_t* const (&q)[2], int t0, int end, int wt, float scale2, Result<D, 2>& r,
                                             uint8_t* lds) {
@@ -717,26 +781,61 @@ __device__ __forceinline__ void attend_wide(const Stream& s, const uint16_t* con
   for (int e = 0; e < D / 16; ++e) keep_here(value_at[e]);
   StageRegs<DT, D, MX, WR> regs;
   regs.load(s, t0, end);
-  // Two stages a round, one in each buffer. A stage's barrier also ends the reads of the other buffer: its readers
-  // came to this one after them.
-  for (int t = t0; t < end; t += 2 * S::TOKENS) {
-    regs.store(lds, end - t);
+  if constexpr (S::BUFFERS == 2) {
+    // Two stages a round, one in each buffer. A stage's barrier also ends the reads of the other buffer: its readers
+    // came to this one after them.
+    for (int t = t0; t < end; t += 2 * S::TOKENS) {
+      regs.store(lds, end - t);
+      __syncthreads();
+      if (t + S::TOKENS < end) regs.load(s, t + S::TOKENS, end);
+      load_fence();
+      const int left = end - t - tile0;
+      if (left > 0) wide_tile<DT, D, WR, 0>(key_at, value_at, qf, left, scale2, ref, r);
+      if (t + S::TOKENS >= end) break;
+      regs.store(lds + 2 * S::BYTES, end - t - S::TOKENS);
+      __syncthreads();
+      if (t + 2 * S::TOKENS < end) regs.load(s, t + 2 * S::TOKENS, end);
+      load_fence();
+      if (left > S::TOKENS) wide_tile<DT, D, WR, 2 * S::BYTES>(key_at, value_at, qf, left - S::TOKENS, scale2, ref, r);
+    }
+  } else {
+    // Three buffers: in stage s a wave reads its own and, for the scores ahead, the one after it, and writes the
+    // one after that, whose last readers came to this stage's barrier after their reads.
+    const int stages = (end - t0 + S::TOKENS - 1) / S::TOKENS;
+    regs.store(lds, end - t0);
+    if (stages > 1) {
+      regs.load(s, t0 + S::TOKENS, end);
+      regs.store(lds + 2 * S::BYTES, end - t0 - S::TOKENS);
+    }
+    if (stages > 2) regs.load(s, t0 + 2 * S::TOKENS, end);
     __syncthreads();
-    if (t + S::TOKENS < end) regs.load(s, t + S::TOKENS, end);
-    load_fence();
-    int left = end - t - tile0;
-    if (left > 0) wide_tile<DT, D, WR, 0>(key_at, value_at, qf, left, scale2, ref, r);
-    if constexpr (S::TILES > 1)
-      if (left > kTile) wide_tile<DT, D, WR, kTile * 2 * D>(key_at, value_at, qf, left - kTile, scale2, ref, r);
-    if (t + S::TOKENS >= end) break;
-    regs.store(lds + 2 * S::BYTES, end - t - S::TOKENS);
-    __syncthreads();
-    if (t + 2 * S::TOKENS < end) regs.load(s, t + 2 * S::TOKENS, end);
-    load_fence();
-    left -= S::TOKENS;
-    if (left > 0) wide_tile<DT, D, WR, 2 * S::BYTES>(key_at, value_at, qf, left, scale2, ref, r);
-    if constexpr (S::TILES > 1)
-      if (left > kTile) wide_tile<DT, D, WR, 2 * S::BYTES + kTile * 2 * D>(key_at, value_at, qf, left - kTile, scale2, ref, r);
+    f32x4 sc[2][2];
+    {
+      uint4 k[2][D / 32];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) k[u][i] = read_piece(key_at[i] + u * 16 * (2 * D));
+      wide_scores<DT, D>(k, qf, ref, sc);
+    }
+    int at = 0, left = end - t0 - tile0;
+    for (int stage = 0; stage < stages; ++stage) {
+      if (stage > 0) __syncthreads();
+      const int next = at == 4 * S::BYTES ? 0 : at + 2 * S::BYTES;
+      if (stage + 2 < stages) {
+        regs.store(lds + (next == 4 * S::BYTES ? 0 : next + 2 * S::BYTES), end - t0 - (stage + 2) * S::TOKENS);
+        if (stage + 3 < stages) regs.load(s, t0 + (stage + 3) * S::TOKENS, end);
+        load_fence();
+      }
+      if constexpr (S::TILES == 2) {
+        if (left > 0) wide_step<DT, D>(key_at, value_at, at + kTile * 2 * D, at, qf, left, scale2, ref, sc, r);
+        if (left > kTile) wide_step<DT, D>(key_at, value_at, next, at + kTile * 2 * D, qf, left - kTile, scale2, ref, sc, r);
+      } else {
+        if (left > 0) wide_step<DT, D>(key_at, value_at, next, at, qf, left, scale2, ref, sc, r);
+      }
+      left -= S::TOKENS;
+      at = next;
+    }
   }
 #pragma unroll
   for (int n = 0; n < 2; ++n) {
@@ -748,7 +847,7 @@ __device__ __forceinline__ void attend_wide(const Stream& s, const uint16_t* con
 template <int DT, int D, bool PMX, bool OMX, int WR>
 __global__ __launch_bounds__(512, 2) void shared_wide_kernel(SharedArgs a) {
   using S = Stage<D, WR>;
-  constexpr int STAGES = 2 * 2 * S::BYTES, JOIN = finish_bytes(D, 2, S::WT, WR), OWN = finish_bytes(D, 1, 4, 1);
+  constexpr int STAGES = S::BUFFERS * 2 * S::BYTES, JOIN = finish_bytes(D, 2, S::WT, WR), OWN = finish_bytes(D, 1, 4, 1);
   constexpr int BYTES = STAGES > JOIN ? (STAGES > 2 * OWN ? STAGES : 2 * OWN) : (JOIN > 2 * OWN ? JOIN : 2 * OWN);
   __shared__ f32x4 lds[BYTES / 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -852,13 +951,21 @@ Plan plan_of(const lkv_shared_desc* d) {
   p.wr = rows <= 64 ? 2 : (rows <= 128 ? 4 : 8);
   p.row_tiles = ceil_div(rows, p.nr ? 16 * p.nr : 32 * p.wr);
   p.g_tiles = ceil_div(g, 16);
-  // Tokens that a workgroup takes: as many workgroups as the card holds at once, and no fewer than one tile
-  // a wave.
-  const int64_t room = 256;
-  const int64_t tokens = (int64_t)p.row_tiles * d->n_kv * d->prefix_tokens + (p.nr ? (int64_t)d->n_seqs * d->n_kv * p.g_tiles * d->max_own : 0);
-  const int64_t least = p.nr ? 128 : 256;
-  int64_t chunk = (tokens / room + least - 1) / least * least;
-  if (chunk < least) chunk = least;
+  // Tokens that a workgroup takes, in steps of 128: so many that all workgroups run at once, one on each CU, and no
+  // fewer than fill it for longer than it takes to begin and end.
+  const int64_t cus = 256, items = (int64_t)d->n_seqs * d->n_kv * p.g_tiles;
+  int64_t tokens = (int64_t)p.row_tiles * d->n_kv * d->prefix_tokens, room = cus, least = 128;
+  if (p.nr) {
+    tokens += items * d->max_own;
+  } else {
+    // Own rows, two items a workgroup, beside the prefix's where that is bound by memory (16 sequences over 32K tokens with 200
+    // of their own: 43.3 us behind them, 39.7 beside) and not by the products (32 over 128K: 102 behind, 149 beside).
+    const int64_t beside = (items + 1) / 2;
+    if (d->max_own > 0 && d->max_own <= 1024 && p.wr == 2 && beside <= cus / 4) room -= beside;
+    least = 256;
+  }
+  int64_t chunk = (tokens + room - 1) / room;
+  chunk = (chunk < least ? least : chunk) + 127 & ~127;
   p.p_chunk = p.o_chunk = (int)(chunk > (1 << 30) ? (1 << 30) : chunk);
   if (!p.nr && p.o_chunk > 1024) p.o_chunk = 1024;
   p.p_parts = ceil_div(d->prefix_tokens, p.p_chunk);
