@@ -258,33 +258,45 @@ struct Reference {
   __device__ __forceinline__ float level(float scale2) const { return limit == -INFINITY ? -INFINITY : -negative[0] * scale2; }
 };
 
-// A tile's scores of one row tile, relative to the reference, made ready for the exponential: tokens behind the end
-// without weight (`left`: tokens that the tile has, if fewer than 32), the reference moved where it must be; l and o
-// follow it.
-template <int D>
-__device__ __forceinline__ void settle(f32x4 (&sc)[2], int left, float scale2, Reference& ref, float& l, f32x4 (&o)[D / 16]) {
+// A tile's scores, relative to the references, made ready for the exponential: tokens behind the end without weight
+// (`left`: tokens that the tile has, if fewer than 32), a reference moved where it must be; l and o follow it.
+template <int D, int NR>
+__device__ __forceinline__ void settle(f32x4 (&sc)[NR][2], int left, float scale2, Reference (&ref)[NR], Result<D, NR>& r) {
   if (left < kTile) {
     int mine = left - (int)(threadIdx.x & 48) / 4;
     keep_here(mine);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float x = (j < 4 ? 0 : 16) + (j & 3) < mine ? sc[j / 4][j & 3] : -INFINITY;
-      keep_here(x);
-      sc[j / 4][j & 3] = x;
-    }
-  }
-  const float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])), fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
-  if (__any(top > ref.limit)) {
-    const float up = lkv::pair_max<32>(lkv::pair_max<16>(top));
-    const bool move = up > ref.limit && up < INFINITY;
-    const float by = move ? up : 0.0f, keep = ref.limit == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-by * scale2);
-    ref.negative -= by;
-    ref.limit = move ? kSlack / scale2 : ref.limit;
-    l *= keep;
+    for (int n = 0; n < NR; ++n)
 #pragma unroll
-    for (int e = 0; e < D / 16; ++e) o[e] *= keep;
-    sc[0] -= by;
-    sc[1] -= by;
+      for (int j = 0; j < 8; ++j) {
+        float x = (j < 4 ? 0 : 16) + (j & 3) < mine ? sc[n][j / 4][j & 3] : -INFINITY;
+        keep_here(x);
+        sc[n][j / 4][j & 3] = x;
+      }
+  }
+  float top[NR];
+  bool any = false;
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    const f32x4 x = sc[n][0], y = sc[n][1];
+    top[n] = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])));
+    any |= top[n] > ref[n].limit;
+  }
+  if (__any(any)) {
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      if (!__any(top[n] > ref[n].limit)) continue;
+      const float up = lkv::pair_max<32>(lkv::pair_max<16>(top[n]));
+      const bool move = up > ref[n].limit && up < INFINITY;
+      const float by = move ? up : 0.0f, keep = ref[n].limit == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-by * scale2);
+      ref[n].negative -= by;
+      ref[n].limit = move ? kSlack / scale2 : ref[n].limit;
+      r.l[n] *= keep;
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) r.o[n][e] *= keep;
+      sc[n][0] -= by;
+      sc[n][1] -= by;
+    }
   }
 }
 
@@ -296,12 +308,6 @@ __device__ __forceinline__ uint4 weights(const f32x4 (&sc)[2], float scale2, flo
   for (int j = 0; j < 8; ++j) w[j] = __builtin_amdgcn_exp2f(sc[j / 4][j & 3] * scale2);
   l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
   return make_uint4(Mat<DT>::pack(w[0], w[1]), Mat<DT>::pack(w[2], w[3]), Mat<DT>::pack(w[4], w[5]), Mat<DT>::pack(w[6], w[7]));
-}
-
-template <int DT, int D>
-__device__ __forceinline__ uint4 weigh(f32x4 (&sc)[2], int left, float scale2, Reference& ref, float& l, f32x4 (&o)[D / 16]) {
-  settle<D>(sc, left, scale2, ref, l, o);
-  return weights<DT>(sc, scale2, l);
 }
 
 // Loads stay on their side: moved down to where the next tile uses them, they would be waited for.
@@ -359,9 +365,10 @@ __device__ __forceinline__ void attend_range(const Stream& s, const uint16_t* co
       for (int j = 0; j < 8; ++j)
         v.keep(j, t + (j < 4 ? 0 : 16) + 4 * quarter + (j & 3) < end);
     }
+    settle<D, NR>(sc, end - t, scale2, ref, r);
     uint4 p[NR];
 #pragma unroll
-    for (int n = 0; n < NR; ++n) p[n] = weigh<DT, D>(sc[n], end - t, scale2, ref[n], r.l[n], r.o[n]);
+    for (int n = 0; n < NR; ++n) p[n] = weights<DT>(sc[n], scale2, r.l[n]);
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
       uint32_t x[8];
@@ -561,14 +568,21 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_decode_kernel(SharedArg
 
 // ---- many rows: the prefix through LDS --------------------------------------------------------------
 // Each wave on its own stream of tokens reads all keys and values for its 32 rows alone: with many rows of
-// a head, the reads from L2 bound that (10 TB/s over all row tiles). Here a workgroup of eight waves, WR across 32 rows each and
-// WT = 8 / WR across tokens, stages its tokens' keys and values in LDS once, in the model dtype (8-bit
-// rows are widened on the way, once for all rows). 16-byte pieces are swizzled by the row, so that the 16
-// tokens of an operand lie in different banks; the values' operands are read transposed.
-template <int D, int WR> struct Stage {
-  static constexpr int WT = 8 / WR;
-  static constexpr int TOKENS = WR == 2 ? 128 : 64;
-  static constexpr int BUFFERS = WR == 2 ? 2 : 3;
+// a head, the reads from L2 bound that (10 TB/s over all row tiles). Here a workgroup stages its tokens' keys and
+// values in LDS once, in the model dtype (8-bit rows are widened on the way, once for all rows), for WR waves
+// across rows and WT across tokens. 16-byte pieces are swizzled by the row, so that the 16 tokens of an
+// operand lie in different banks; the values' operands are read transposed.
+//
+// Up to 64 rows the reads from memory bound it: eight waves, two across the rows, each on its own tokens of a stage of
+// 128. From there on the products and the exponentials do, and the card's power: under 256 rows of random values it
+// runs at 1.75 GHz, 2.3 with zeros. There four waves take 32 rows each of the same tokens, one on each SIMD, and a
+// second workgroup keeps each SIMD at work while the first one's waves meet at a barrier. (One workgroup of eight waves, two
+// on a SIMD, came to each barrier one wave after the other: 87,000 cycles for 32,768 tokens under 256 rows, 50,000 with
+// the barriers left out.)
+template <int D, int WR, int W> struct Stage {
+  static constexpr int THREADS = 64 * W, WT = W / WR, NR = 2;
+  static constexpr int TOKENS = W == 8 ? 128 : 64;
+  static constexpr int BUFFERS = 2;
   static constexpr int TILES = TOKENS / (kTile * WT);      // of a wave in a stage
   static constexpr int PIECES = D / 8;                     // 16-byte pieces of a row
   static constexpr int BYTES = TOKENS * 2 * D;             // of keys, and of values
@@ -576,10 +590,9 @@ template <int D, int WR> struct Stage {
 };
 
 // What a thread holds of a stage on its way to LDS.
-template <int DT, int D, bool MX, int WR> struct StageRegs;
-template <int DT, int D, int WR> struct StageRegs<DT, D, false, WR> {
-  using S = Stage<D, WR>;
-  static constexpr int LOADS = S::TOKENS * S::PIECES / 512;  // 16-byte pieces of keys, and of values
+template <int DT, int D, bool MX, class S> struct StageRegs;
+template <int DT, int D, class S> struct StageRegs<DT, D, false, S> {
+  static constexpr int LOADS = S::TOKENS * S::PIECES / S::THREADS;  // 16-byte pieces of keys, and of values
   u32x4 k[LOADS], v[LOADS];
   // Tokens t0 .. of the stream; behind `end`, its last token.
   __device__ __forceinline__ void load(const Stream& s, int t0, int end) {
@@ -587,7 +600,7 @@ template <int DT, int D, int WR> struct StageRegs<DT, D, false, WR> {
     const uint8_t *kb = s.k + (int64_t)t0 * (2 * D), *vb = s.v + (int64_t)t0 * (2 * D);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int x = i * 512 + threadIdx.x;
+      const int x = i * S::THREADS + threadIdx.x;
       const uint32_t at = (uint32_t)(min(x / S::PIECES, last) * (2 * D) + x % S::PIECES * 16);
       k[i] = *(const u32x4*)(kb + at);
       v[i] = *(const u32x4*)(vb + at);
@@ -597,7 +610,7 @@ template <int DT, int D, int WR> struct StageRegs<DT, D, false, WR> {
   __device__ __forceinline__ void store(uint8_t* lds, int live) const {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int x = i * 512 + threadIdx.x, row = x / S::PIECES;
+      const int x = i * S::THREADS + threadIdx.x, row = x / S::PIECES;
       uint8_t* to = lds + row * (2 * D) + (x % S::PIECES ^ S::swizzle(row)) * 16;
       const uint32_t keep = row < live ? ~0u : 0u;
       *(u32x4*)to = k[i];
@@ -606,12 +619,11 @@ template <int DT, int D, int WR> struct StageRegs<DT, D, false, WR> {
   }
 };
 // 8 bits: 16 codes under one scale become two pieces.
-template <int DT, int D, int WR> struct StageRegs<DT, D, true, WR> {
-  using S = Stage<D, WR>;
-  static constexpr int UNITS = S::TOKENS * D / 16, LOADS = (UNITS + 511) / 512;
+template <int DT, int D, class S> struct StageRegs<DT, D, true, S> {
+  static constexpr int UNITS = S::TOKENS * D / 16, LOADS = (UNITS + S::THREADS - 1) / S::THREADS;
   uint4 k[LOADS], v[LOADS];
   uint32_t ks[LOADS], vs[LOADS];
-  static __device__ __forceinline__ bool mine(int i) { return UNITS % 512 == 0 || i * 512 + (int)threadIdx.x < UNITS; }
+  static __device__ __forceinline__ bool mine(int i) { return UNITS % S::THREADS == 0 || i * S::THREADS + (int)threadIdx.x < UNITS; }
   __device__ __forceinline__ void load(const Stream& s, int t0, int end) {
     const int last = min(S::TOKENS, end - t0) - 1;
     const uint8_t *kb = s.k + (int64_t)t0 * D, *vb = s.v + (int64_t)t0 * D;
@@ -619,7 +631,7 @@ template <int DT, int D, int WR> struct StageRegs<DT, D, true, WR> {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       if (!mine(i)) continue;
-      const int x = i * 512 + threadIdx.x;
+      const int x = i * S::THREADS + threadIdx.x;
       const uint32_t at = (uint32_t)(min(x / (D / 16), last) * D + x % (D / 16) * 16);
       k[i] = *(const uint4*)(kb + at);
       v[i] = *(const uint4*)(vb + at);
@@ -636,7 +648,7 @@ template <int DT, int D, int WR> struct StageRegs<DT, D, true, WR> {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       if (!mine(i)) continue;
-      const int x = i * 512 + threadIdx.x, row = x / (D / 16), piece = x % (D / 16) * 2, sw = S::swizzle(row);
+      const int x = i * S::THREADS + threadIdx.x, row = x / (D / 16), piece = x % (D / 16) * 2, sw = S::swizzle(row);
       uint8_t* to = lds + row * (2 * D);
       const uint32_t keep = row < live ? ~0u : 0u;  // a code of zero is zero under any scale that is written
       *(uint4*)(to + (piece ^ sw) * 16) = widen(k[i].x, k[i].y, ks[i]);
@@ -661,107 +673,78 @@ __device__ __forceinline__ uint4 read_piece(LdsPointer p) {
   return make_uint4(x.x, x.y, x.z, x.w);
 }
 
-// One tile of 32 tokens of a staged buffer, at compile-time offset AT in LDS from the lane's places.
-template <int DT, int D, int WR, int AT>
-__device__ __forceinline__ void wide_tile(const LdsPointer (&key_at)[D / 32], const LdsPointer (&value_at)[D / 16], const uint4 (&qf)[2][D / 32],
-                                          int left, float scale2, Reference (&ref)[2], Result<D, 2>& r) {
-  // All of the tile's reads first: one by one before their products, each would be waited for.
-  uint4 k[2][D / 32];
-  uint2 v[D / 16][2];
+// The scores of a tile of 32 staged tokens, relative to the references.
+template <int DT, int D, int NR>
+__device__ __forceinline__ void wide_scores(const uint4 (&k)[2][D / 32], const uint4 (&qf)[NR][D / 32], const Reference (&ref)[NR], f32x4 (&sc)[NR][2]) {
 #pragma unroll
-  for (int u = 0; u < 2; ++u)
-#pragma unroll
-    for (int i = 0; i < D / 32; ++i) k[u][i] = read_piece(key_at[i] + AT + u * 16 * (2 * D));
-#pragma unroll
-  for (int e = 0; e < D / 16; ++e)
-#pragma unroll
-    for (int u = 0; u < 2; ++u) v[e][u] = read_transposed(value_at[e] + AT + u * 16 * (2 * D));
-  __builtin_amdgcn_sched_barrier(0);
-  f32x4 sc[2][2];
-#pragma unroll
-  for (int n = 0; n < 2; ++n) sc[n][0] = sc[n][1] = ref[n].negative;
+  for (int n = 0; n < NR; ++n) sc[n][0] = sc[n][1] = ref[n].negative;
 #pragma unroll
   for (int i = 0; i < D / 32; ++i)
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int n = 0; n < 2; ++n) sc[n][u] = Mat<DT>::mma(k[u][i], qf[n][i], sc[n][u]);
-  uint4 p[2];
-#pragma unroll
-  for (int n = 0; n < 2; ++n) p[n] = weigh<DT, D>(sc[n], left, scale2, ref[n], r.l[n], r.o[n]);
-#pragma unroll
-  for (int e = 0; e < D / 16; ++e)
-#pragma unroll
-    for (int n = 0; n < 2; ++n) r.o[n][e] = Mat<DT>::mma(make_uint4(v[e][0].x, v[e][0].y, v[e][1].x, v[e][1].y), p[n], r.o[n][e]);
+      for (int n = 0; n < NR; ++n) sc[n][u] = Mat<DT>::mma(k[u][i], qf[n][i], sc[n][u]);
 }
-
-// The scores of a tile of 32 staged tokens at offset `at` from the lane's places.
-template <int DT, int D>
-__device__ __forceinline__ void wide_scores(const uint4 (&k)[2][D / 32], const uint4 (&qf)[2][D / 32], const Reference (&ref)[2], f32x4 (&sc)[2][2]) {
-#pragma unroll
-  for (int n = 0; n < 2; ++n) sc[n][0] = sc[n][1] = ref[n].negative;
-#pragma unroll
-  for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int n = 0; n < 2; ++n) sc[n][u] = Mat<DT>::mma(k[u][i], qf[n][i], sc[n][u]);
-}
-
-// One tile's step: its weights and their product with its values, and the next tile's scores, whose products fill the
-// time of this one's exponentials.
-template <int DT, int D>
-__device__ __forceinline__ void wide_step(const LdsPointer (&key_at)[D / 32], const LdsPointer (&value_at)[D / 16], int next_at, int at,
-                                          const uint4 (&qf)[2][D / 32], int left, float scale2, Reference (&ref)[2], f32x4 (&sc)[2][2], Result<D, 2>& r) {
-  uint4 k[2][D / 32];
-  uint2 v[D / 16][2];
+// A tile's keys and values at offset `at` from the lane's places: all reads at once, for one by one before their
+// products each would be waited for.
+template <int D>
+__device__ __forceinline__ void wide_keys(const LdsPointer (&key_at)[D / 32], int at, uint4 (&k)[2][D / 32]) {
 #pragma unroll
   for (int u = 0; u < 2; ++u)
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) k[u][i] = read_piece(key_at[i] + next_at + u * 16 * (2 * D));
+    for (int i = 0; i < D / 32; ++i) k[u][i] = read_piece(key_at[i] + at + u * 16 * (2 * D));
+}
+template <int D>
+__device__ __forceinline__ void wide_values(const LdsPointer (&value_at)[D / 16], int at, uint2 (&v)[D / 16][2]) {
 #pragma unroll
   for (int e = 0; e < D / 16; ++e)
 #pragma unroll
     for (int u = 0; u < 2; ++u) v[e][u] = read_transposed(value_at[e] + at + u * 16 * (2 * D));
-  __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-  for (int n = 0; n < 2; ++n) settle<D>(sc[n], left, scale2, ref[n], r.l[n], r.o[n]);
-  f32x4 next[2][2];
-  wide_scores<DT, D>(k, qf, ref, next);
-  uint4 p[2];
-#pragma unroll
-  for (int n = 0; n < 2; ++n) p[n] = weights<DT>(sc[n], scale2, r.l[n]);
-  // Products and the vector unit's work in turn.
-#pragma unroll
-  for (int i = 0; i < 4 * (D / 32); ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(0x2, 128 / D * 2, 0);
-    __builtin_amdgcn_sched_group_barrier(0x400, 128 / D, 0);
-  }
+}
+template <int DT, int D, int NR>
+__device__ __forceinline__ void wide_sums(const uint2 (&v)[D / 16][2], const uint4 (&p)[NR], int n0, int n1, Result<D, NR>& r) {
 #pragma unroll
   for (int e = 0; e < D / 16; ++e)
 #pragma unroll
-    for (int n = 0; n < 2; ++n) r.o[n][e] = Mat<DT>::mma(make_uint4(v[e][0].x, v[e][0].y, v[e][1].x, v[e][1].y), p[n], r.o[n][e]);
-#pragma unroll
-  for (int n = 0; n < 2; ++n) sc[n][0] = next[n][0], sc[n][1] = next[n][1];
+    for (int n = n0; n < n1; ++n) r.o[n][e] = Mat<DT>::mma(make_uint4(v[e][0].x, v[e][0].y, v[e][1].x, v[e][1].y), p[n], r.o[n][e]);
 }
 
-template <int DT, int D, bool MX, int WR>
-__device__ __forceinline__ void attend_wide(const Stream& s, const uint16_t* const (&q)[2], int t0, int end, int wt, float scale2, Result<D, 2>& r,
-                                            uint8_t* lds) {
-  using S = Stage<D, WR>;
-  const int lane = threadIdx.x & 63, quarter = lane >> 4;
-  Reference ref[2];
+// One tile by itself.
+template <int DT, int D, int NR>
+__device__ __forceinline__ void wide_tile(const LdsPointer (&key_at)[D / 32], const LdsPointer (&value_at)[D / 16], int at, const uint4 (&qf)[NR][D / 32],
+                                          int left, float scale2, Reference (&ref)[NR], Result<D, NR>& r) {
+  uint4 k[2][D / 32];
+  uint2 v[D / 16][2];
+  wide_keys<D>(key_at, at, k);
+  wide_values<D>(value_at, at, v);
+  __builtin_amdgcn_sched_barrier(0);
+  f32x4 sc[NR][2];
+  wide_scores<DT, D, NR>(k, qf, ref, sc);
+  settle<D, NR>(sc, left, scale2, ref, r);
+  uint4 p[NR];
 #pragma unroll
-  for (int n = 0; n < 2; ++n) {
+  for (int n = 0; n < NR; ++n) p[n] = weights<DT>(sc[n], scale2, r.l[n]);
+  wide_sums<DT, D, NR>(v, p, 0, NR, r);
+}
+
+template <int DT, int D, bool MX, class S>
+__device__ __forceinline__ void attend_wide(const Stream& s, const uint16_t* const (&q)[S::NR], int t0, int end, int wt, float scale2, Result<D, S::NR>& r,
+                                            uint8_t* lds) {
+  constexpr int NR = S::NR;
+  const int lane = threadIdx.x & 63, quarter = lane >> 4;
+  Reference ref[NR];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
     ref[n].reset();
     r.l[n] = 0.0f;
 #pragma unroll
     for (int e = 0; e < D / 16; ++e) r.o[n][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
-  uint4 qf[2][D / 32];
+  StageRegs<DT, D, MX, S> regs;
+  regs.load(s, t0, end);
+  uint4 qf[NR][D / 32];
 #pragma unroll
-  for (int n = 0; n < 2; ++n)
+  for (int n = 0; n < NR; ++n)
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) qf[n][i] = q[n] ? *(const uint4*)(q[n] + 32 * i + 8 * quarter) : make_uint4(0, 0, 0, 0);
   // A lane's places in its wave's first tile: keys of token lane % 16 (and 16 on), values of token 4 q + (lane % 16) / 4.
@@ -779,94 +762,55 @@ __device__ __forceinline__ void attend_wide(const Stream& s, const uint16_t* con
   for (int i = 0; i < D / 32; ++i) keep_here(key_at[i]);
 #pragma unroll
   for (int e = 0; e < D / 16; ++e) keep_here(value_at[e]);
-  StageRegs<DT, D, MX, WR> regs;
-  regs.load(s, t0, end);
-  if constexpr (S::BUFFERS == 2) {
-    // Two stages a round, one in each buffer. A stage's barrier also ends the reads of the other buffer: its readers
-    // came to this one after them.
-    for (int t = t0; t < end; t += 2 * S::TOKENS) {
-      regs.store(lds, end - t);
-      __syncthreads();
-      if (t + S::TOKENS < end) regs.load(s, t + S::TOKENS, end);
-      load_fence();
-      const int left = end - t - tile0;
-      if (left > 0) wide_tile<DT, D, WR, 0>(key_at, value_at, qf, left, scale2, ref, r);
-      if (t + S::TOKENS >= end) break;
-      regs.store(lds + 2 * S::BYTES, end - t - S::TOKENS);
-      __syncthreads();
-      if (t + 2 * S::TOKENS < end) regs.load(s, t + 2 * S::TOKENS, end);
-      load_fence();
-      if (left > S::TOKENS) wide_tile<DT, D, WR, 2 * S::BYTES>(key_at, value_at, qf, left - S::TOKENS, scale2, ref, r);
-    }
-  } else {
-    // Three buffers: in stage s a wave reads its own and, for the scores ahead, the one after it, and writes the
-    // one after that, whose last readers came to this stage's barrier after their reads.
-    const int stages = (end - t0 + S::TOKENS - 1) / S::TOKENS;
-    regs.store(lds, end - t0);
-    if (stages > 1) {
-      regs.load(s, t0 + S::TOKENS, end);
-      regs.store(lds + 2 * S::BYTES, end - t0 - S::TOKENS);
-    }
-    if (stages > 2) regs.load(s, t0 + 2 * S::TOKENS, end);
-    __syncthreads();
-    f32x4 sc[2][2];
-    {
-      uint4 k[2][D / 32];
+  // Two stages a round, one in each buffer. A stage's barrier also ends the reads of the other buffer: its readers
+  // came to this one after them.
+  for (int t = t0; t < end; t += 2 * S::TOKENS) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+    for (int half = 0; half < 2; ++half) {
+      const int now = t + half * S::TOKENS, left = end - now - tile0;
+      if (half && now >= end) break;
+      regs.store(lds + half * 2 * S::BYTES, end - now);
+      __syncthreads();
+      if (now + S::TOKENS < end) regs.load(s, now + S::TOKENS, end);
+      load_fence();
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) k[u][i] = read_piece(key_at[i] + u * 16 * (2 * D));
-      wide_scores<DT, D>(k, qf, ref, sc);
-    }
-    int at = 0, left = end - t0 - tile0;
-    for (int stage = 0; stage < stages; ++stage) {
-      if (stage > 0) __syncthreads();
-      const int next = at == 4 * S::BYTES ? 0 : at + 2 * S::BYTES;
-      if (stage + 2 < stages) {
-        regs.store(lds + (next == 4 * S::BYTES ? 0 : next + 2 * S::BYTES), end - t0 - (stage + 2) * S::TOKENS);
-        if (stage + 3 < stages) regs.load(s, t0 + (stage + 3) * S::TOKENS, end);
-        load_fence();
-      }
-      if constexpr (S::TILES == 2) {
-        if (left > 0) wide_step<DT, D>(key_at, value_at, at + kTile * 2 * D, at, qf, left, scale2, ref, sc, r);
-        if (left > kTile) wide_step<DT, D>(key_at, value_at, next, at + kTile * 2 * D, qf, left - kTile, scale2, ref, sc, r);
-      } else {
-        if (left > 0) wide_step<DT, D>(key_at, value_at, next, at, qf, left, scale2, ref, sc, r);
-      }
-      left -= S::TOKENS;
-      at = next;
+      for (int tile = 0; tile < S::TILES; ++tile)
+        if (left > tile * kTile)
+          wide_tile<DT, D, NR>(key_at, value_at, half * 2 * S::BYTES + tile * kTile * 2 * D, qf, left - tile * kTile, scale2, ref, r);
     }
   }
 #pragma unroll
-  for (int n = 0; n < 2; ++n) {
+  for (int n = 0; n < NR; ++n) {
     r.l[n] = lkv::pair_sum<32>(lkv::pair_sum<16>(r.l[n]));
     r.m[n] = ref[n].level(scale2);
   }
 }
 
-template <int DT, int D, bool PMX, bool OMX, int WR>
-__global__ __launch_bounds__(512, 2) void shared_wide_kernel(SharedArgs a) {
-  using S = Stage<D, WR>;
-  constexpr int STAGES = S::BUFFERS * 2 * S::BYTES, JOIN = finish_bytes(D, 2, S::WT, WR), OWN = finish_bytes(D, 1, 4, 1);
+template <int DT, int D, bool PMX, bool OMX, int WR, int W>
+__global__ __launch_bounds__(64 * W, 2) void shared_wide_kernel(SharedArgs a) {
+  using S = Stage<D, WR, W>;
+  constexpr int OWN_WAVES = W / 2;  // two items a workgroup
+  constexpr int STAGES = S::BUFFERS * 2 * S::BYTES, JOIN = finish_bytes(D, S::NR, S::WT, WR), OWN = finish_bytes(D, 1, OWN_WAVES, 1);
   constexpr int BYTES = STAGES > JOIN ? (STAGES > 2 * OWN ? STAGES : 2 * OWN) : (JOIN > 2 * OWN ? JOIN : 2 * OWN);
   __shared__ f32x4 lds[BYTES / 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int id = blockIdx.x, p_blocks = a.p_groups * 8 * a.row_tiles;
-  if (id >= p_blocks) return own_item<DT, D, OMX, 4>(a, (int64_t)(id - p_blocks) * 2 + wave / 4, wave % 4, lds + wave / 4 * (OWN / 16));
+  if (id >= p_blocks)
+    return own_item<DT, D, OMX, OWN_WAVES>(a, (int64_t)(id - p_blocks) * 2 + wave / OWN_WAVES, wave % OWN_WAVES, lds + wave / OWN_WAVES * (OWN / 16));
   const int unit = (id / (8 * a.row_tiles)) * 8 + id % 8, tile = id / 8 % a.row_tiles;
   if (unit >= a.p_parts * a.n_kv) return;
   const int part = unit / a.n_kv, h = unit % a.n_kv, wr = wave % WR, wt = wave / WR;
-  const uint16_t* q[2];
-  int64_t row[2];
+  const uint16_t* q[S::NR];
+  int64_t row[S::NR];
 #pragma unroll
-  for (int n = 0; n < 2; ++n) {
-    row[n] = prefix_row(a, h, ((tile * WR + wr) * 2 + n) * 16 + (lane & 15));
+  for (int n = 0; n < S::NR; ++n) {
+    row[n] = prefix_row(a, h, ((tile * WR + wr) * S::NR + n) * 16 + (lane & 15));
     q[n] = row[n] >= 0 ? a.q + row[n] * D : nullptr;
   }
   const int t0 = part * a.p_chunk, end = min(t0 + a.p_chunk, a.prefix_tokens);
-  Result<D, 2> r;
-  attend_wide<DT, D, PMX, WR>(stream_of<D, PMX>(a.prefix, 0, h), q, t0, end, wt, a.scale2, r, (uint8_t*)lds);
-  finish<D, 2, S::WT, true>(a, r, row, part, wt, wr, WR, lds);
+  Result<D, S::NR> r;
+  attend_wide<DT, D, PMX, S>(stream_of<D, PMX>(a.prefix, 0, h), q, t0, end, wt, a.scale2, r, (uint8_t*)lds);
+  finish<D, S::NR, S::WT, true>(a, r, row, part, wt, wr, WR, lds);
 }
 
 // A workgroup a query row: its parts' results into one. d/4 threads take a part's channels, four each, and
@@ -940,6 +884,7 @@ int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 struct Plan {
   int nr;  // tiles of 16 rows of a wave, on its own stream; 0: through LDS
   int wr;  // there, waves across rows
+  int waves;
   int row_tiles, p_parts, p_chunk, p_groups, g_tiles, o_parts, o_chunk;
 };
 
@@ -948,7 +893,8 @@ Plan plan_of(const lkv_shared_desc* d) {
   const int g = d->n_q / d->n_kv;
   const int64_t rows = (int64_t)d->n_seqs * g;
   p.nr = d->prefix_tokens == 0 || rows <= 16 ? 1 : (rows <= 32 ? 2 : 0);
-  p.wr = rows <= 64 ? 2 : (rows <= 128 ? 4 : 8);
+  p.waves = p.nr || rows > 64 ? 4 : 8;
+  p.wr = p.waves == 8 ? 2 : 4;
   p.row_tiles = ceil_div(rows, p.nr ? 16 * p.nr : 32 * p.wr);
   p.g_tiles = ceil_div(g, 16);
   // Tokens that a workgroup takes, in steps of 128: so many that all workgroups run at once, one on each CU, and no
@@ -961,7 +907,9 @@ Plan plan_of(const lkv_shared_desc* d) {
     // Own rows, two items a workgroup, beside the prefix's where that is bound by memory (16 sequences over 32K tokens with 200
     // of their own: 43.3 us behind them, 39.7 beside) and not by the products (32 over 128K: 102 behind, 149 beside).
     const int64_t beside = (items + 1) / 2;
-    if (d->max_own > 0 && d->max_own <= 1024 && p.wr == 2 && beside <= cus / 4) room -= beside;
+    if (d->max_own > 0 && d->max_own <= 1024 && p.waves == 8 && beside <= cus / 4) room -= beside;
+    // Two workgroups of four waves a CU, where their parts stay long beside what a part costs to store and join.
+    if (p.waves == 4 && tokens >= 1024 * 2 * cus) room = 2 * cus;
     least = 256;
   }
   int64_t chunk = (tokens + room - 1) / room;
@@ -976,9 +924,11 @@ Plan plan_of(const lkv_shared_desc* d) {
 
 template <int DT, int D, bool PMX, bool OMX>
 void launch(const Plan& p, dim3 grid, hipStream_t s, const SharedArgs& a) {
-  auto kernel = p.nr == 1 ? shared_decode_kernel<DT, D, PMX, OMX, 1> : p.nr == 2 ? shared_decode_kernel<DT, D, PMX, OMX, 2>
-              : p.wr == 2 ? shared_wide_kernel<DT, D, PMX, OMX, 2> : p.wr == 4 ? shared_wide_kernel<DT, D, PMX, OMX, 4> : shared_wide_kernel<DT, D, PMX, OMX, 8>;
-  hipLaunchKernelGGL(kernel, grid, dim3(p.nr ? 64 * kWaves : 512), 0, s, a);
+  auto kernel = p.nr == 1      ? shared_decode_kernel<DT, D, PMX, OMX, 1>
+                : p.nr == 2    ? shared_decode_kernel<DT, D, PMX, OMX, 2>
+                : p.waves == 8 ? shared_wide_kernel<DT, D, PMX, OMX, 2, 8>
+                               : shared_wide_kernel<DT, D, PMX, OMX, 4, 4>;
+  hipLaunchKernelGGL(kernel, grid, dim3(64 * p.waves), 0, s, a);
 }
 
 template <int DT, int D>
