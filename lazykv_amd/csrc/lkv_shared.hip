@@ -15,13 +15,27 @@
 // weights are the second product's operand as they are. V^T takes its operand's order of tokens from
 // there: a lane holds tokens 4q .. 4q+3 and 16+4q .. 16+4q+3 (q = lane / 16), loads d/16 neighbouring
 // channels of each of these eight rows, 16 lanes a whole row, and pairs them by byte permutes.
+//
+// Weights are rounded to the model dtype for the second product (the matrix units' 16-bit form, 16 times
+// float32's rate): an output is off by no more than that one rounding of each weight, as much as its own rounding. Scores, maxima,
+// sums of weights (unrounded) and outputs are float32.
+//
+// Three forms, by the rows that share a KV head's prefix (sequences times group):
+//  - up to 16 or 32: a wave reads its own tokens from memory to registers; the workgroup's four waves, then the parts,
+//    join. Bound by memory: one sequence over 131,072 tokens of 8 KV heads, d 128, takes 54.5 us in 8 bits (277 MB, 5.1 TB/s) and
+//    96.3 in bfloat16 (537 MB, 5.6 TB/s), of which the join is 5.
+//  - up to 64: through LDS, eight waves; 16 sequences over 32,768 bfloat16 tokens 35 us (134 MB; 6.1 TB/s in the loop, 5 us
+//    before it, 3 after it and 5 for the join).
+//  - more: through LDS, four waves, two workgroups a CU; 64 sequences over 32,768 tokens 60 us, over 131,072 180 (0.76
+//    PFLOP/s; a library product of 8192^3 reaches 1.2).
+// Own rows are read as in the first form, an item for each sequence and KV head, in the same launch.
 #include "lkv_mx.h"
 
 namespace {
 
-constexpr int kWaves = 4;      // of a workgroup on streams
-constexpr int kTile = 32;      // tokens
-constexpr float kSlack = 6.0f; // a weight is at most 2^kSlack: nothing to a 16-bit weight's precision or a float32 sum's
+constexpr int kWaves = 4;       // of a workgroup whose waves read streams of their own
+constexpr int kTile = 32;       // tokens
+constexpr float kSlack = 6.0f;  // a weight is at most 2^kSlack: nothing to a 16-bit weight's precision or a float32 sum's
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -582,7 +596,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void shared_decode_kernel(SharedArg
 template <int D, int WR, int W> struct Stage {
   static constexpr int THREADS = 64 * W, WT = W / WR, NR = 2;
   static constexpr int TOKENS = W == 8 ? 128 : 64;
-  static constexpr int BUFFERS = 2;
   static constexpr int TILES = TOKENS / (kTile * WT);      // of a wave in a stage
   static constexpr int PIECES = D / 8;                     // 16-byte pieces of a row
   static constexpr int BYTES = TOKENS * 2 * D;             // of keys, and of values
@@ -701,15 +714,7 @@ __device__ __forceinline__ void wide_values(const LdsPointer (&value_at)[D / 16]
 #pragma unroll
     for (int u = 0; u < 2; ++u) v[e][u] = read_transposed(value_at[e] + at + u * 16 * (2 * D));
 }
-template <int DT, int D, int NR>
-__device__ __forceinline__ void wide_sums(const uint2 (&v)[D / 16][2], const uint4 (&p)[NR], int n0, int n1, Result<D, NR>& r) {
-#pragma unroll
-  for (int e = 0; e < D / 16; ++e)
-#pragma unroll
-    for (int n = n0; n < n1; ++n) r.o[n][e] = Mat<DT>::mma(make_uint4(v[e][0].x, v[e][0].y, v[e][1].x, v[e][1].y), p[n], r.o[n][e]);
-}
-
-// One tile by itself.
+// One tile of 32 staged tokens.
 template <int DT, int D, int NR>
 __device__ __forceinline__ void wide_tile(const LdsPointer (&key_at)[D / 32], const LdsPointer (&value_at)[D / 16], int at, const uint4 (&qf)[NR][D / 32],
                                           int left, float scale2, Reference (&ref)[NR], Result<D, NR>& r) {
@@ -724,7 +729,10 @@ __device__ __forceinline__ void wide_tile(const LdsPointer (&key_at)[D / 32], co
   uint4 p[NR];
 #pragma unroll
   for (int n = 0; n < NR; ++n) p[n] = weights<DT>(sc[n], scale2, r.l[n]);
-  wide_sums<DT, D, NR>(v, p, 0, NR, r);
+#pragma unroll
+  for (int e = 0; e < D / 16; ++e)
+#pragma unroll
+    for (int n = 0; n < NR; ++n) r.o[n][e] = Mat<DT>::mma(make_uint4(v[e][0].x, v[e][0].y, v[e][1].x, v[e][1].y), p[n], r.o[n][e]);
 }
 
 template <int DT, int D, bool MX, class S>
@@ -790,7 +798,7 @@ template <int DT, int D, bool PMX, bool OMX, int WR, int W>
 __global__ __launch_bounds__(64 * W, 2) void shared_wide_kernel(SharedArgs a) {
   using S = Stage<D, WR, W>;
   constexpr int OWN_WAVES = W / 2;  // two items a workgroup
-  constexpr int STAGES = S::BUFFERS * 2 * S::BYTES, JOIN = finish_bytes(D, S::NR, S::WT, WR), OWN = finish_bytes(D, 1, OWN_WAVES, 1);
+  constexpr int STAGES = 2 * 2 * S::BYTES, JOIN = finish_bytes(D, S::NR, S::WT, WR), OWN = finish_bytes(D, 1, OWN_WAVES, 1);
   constexpr int BYTES = STAGES > JOIN ? (STAGES > 2 * OWN ? STAGES : 2 * OWN) : (JOIN > 2 * OWN ? JOIN : 2 * OWN);
   __shared__ f32x4 lds[BYTES / 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -829,11 +837,13 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
   const float* from = a.part_o + row * parts * D + c * 4;
   for (int p0 = 0; p0 < parts; p0 += 64) {
-    float f = 0.0f;
+    float f = -1.0f;  // no part, or an empty one: its sums are not read
     if (p0 + lane < parts) {
       const float2 x = ml[p0 + lane];
-      f = join_factor(x.x, x.y, top);
-      total += x.y == 0.0f ? 0.0f : f * x.y;
+      if (x.y != 0.0f) {
+        f = join_factor(x.x, x.y, top);
+        total += f * x.y;
+      }
     }
     f32x4 x[64 / GROUPS];
     float w[64 / GROUPS];
@@ -841,8 +851,7 @@ __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
     for (int i = 0; i < 64 / GROUPS; ++i) {
       const int p = p0 + i * GROUPS + group;
       w[i] = __shfl(f, i * GROUPS + group);
-      // A part without weight is not read: an empty one holds zeros, and another's f is 0 from 150 powers of two below.
-      x[i] = p < parts && w[i] != 0.0f ? *(const f32x4*)(from + (int64_t)p * D) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      x[i] = w[i] < 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : *(const f32x4*)(from + (int64_t)p * D);
     }
 #pragma unroll
     for (int i = 0; i < 64 / GROUPS; ++i) o += x[i] * w[i];
@@ -913,7 +922,7 @@ Plan plan_of(const lkv_shared_desc* d) {
     least = 256;
   }
   int64_t chunk = (tokens + room - 1) / room;
-  chunk = (chunk < least ? least : chunk) + 127 & ~127;
+  chunk = ((chunk < least ? least : chunk) + 127) / 128 * 128;
   p.p_chunk = p.o_chunk = (int)(chunk > (1 << 30) ? (1 << 30) : chunk);
   if (!p.nr && p.o_chunk > 1024) p.o_chunk = 1024;
   p.p_parts = ceil_div(d->prefix_tokens, p.p_chunk);

@@ -394,3 +394,120 @@ def test_refusals(bad: str) -> None:
     query = {"dtype": q.bfloat16(), "head_dim": q[..., :32], "heads": q[:, :3], "batch": q[:1]}.get(bad, q)
     with pytest.raises(ValueError):
         kernels.shared_decode(query, **call)
+
+
+@pytest.mark.parametrize("seqs", [12, 20, 33, 75])
+@pytest.mark.parametrize(("model", "d", "prefix8"), [("f16", 64, False), ("f16", 128, True), ("bf16", 64, True), ("bf16", 128, False)])
+def test_prefixes_that_end_anywhere_in_a_stage(seqs: int, model: str, d: int, prefix8: bool) -> None:
+    """Rows of a KV head of 36, 60, 99 and 225 over prefixes that end at every kind of place of a stage of 64 or 128 tokens and
+    of the tiles in it, with NaN right behind the end, in parts of one stage and of several."""
+    for prefix in (1, 31, 33, 63, 65, 95, 97, 127, 129, 191, 193, 255, 257, 319, 385, 1023):
+        _case(prefix, model, d, 1, 3, prefix, [i % 3 for i in range(seqs)], prefix8, False)
+
+
+@pytest.mark.parametrize("seqs", [3, 9, 20, 70])
+def test_a_prefixs_last_values_may_be_infinite_and_what_lies_behind_is_zero(seqs: int) -> None:
+    """An infinite value in a prefix's last row comes out infinite in its channel and nowhere else, whatever the tile's other
+    tokens behind the end are."""
+    from lazykv_amd import kernels
+
+    gen = torch.Generator().manual_seed(13)
+    for prefix in (40, 65, 200):
+        p = Part(gen, 1, 2, prefix, 64, "f16", False, room=100)
+        p.store[1, 0, :, prefix - 1, 7] = float("inf")
+        q = (torch.randn((seqs, 8, 64), generator=gen) * 0.1).half().cuda()
+        out, lse = kernels.shared_decode(q, scale=0.125, prefix=p.rows, prefix_tokens=prefix)
+        torch.cuda.synchronize()
+        assert bool((out[:, :, 7] == float("inf")).all())
+        assert bool(out[:, :, [c for c in range(64) if c != 7]].isfinite().all()) and bool(lse.isfinite().all())
+
+
+def _check64(got: tuple, q: torch.Tensor, parts: list, scale: float, n: int) -> None:
+    """Against attention in 64 bits on the GPU, over lists of keys and values [h, t, d] taken piece by piece; bounds as above."""
+    b, n_q, d = q.shape
+    h = parts[0][0].shape[0]
+    g = n_q // h
+    x = q.double().view(b, h, g, d).transpose(0, 1).reshape(h, b * g, d)
+    m = torch.full((h, b * g), float("-inf"), dtype=torch.float64, device="cuda")
+    big_s, big_v = torch.zeros_like(m), 0.0
+    for k, v in parts:
+        kd = k.double().transpose(1, 2).contiguous()
+        m = torch.maximum(m, (x @ kd).amax(-1) * scale)
+        big_s = torch.maximum(big_s, (x.abs() @ kd.abs()).amax(-1) * scale)
+        big_v = max(big_v, float(v.abs().max()))
+    total, o, a = torch.zeros_like(m), torch.zeros((h, b * g, d), dtype=torch.float64, device="cuda"), torch.zeros((h, b * g, d), dtype=torch.float64, device="cuda")
+    for k, v in parts:
+        p = ((x @ k.double().transpose(1, 2).contiguous()) * scale - m.unsqueeze(-1)).exp()
+        total += p.sum(-1)
+        o += p @ v.double()
+        a += p @ v.double().abs()
+    o, a, lse = o / total.unsqueeze(-1), a / total.unsqueeze(-1), m + total.log()
+    half = {torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8}[q.dtype]
+    e = ((d + 8) * big_s + 4) * U
+    # The sums over n tokens: each lane's over its own, 32 times fewer at the least, and these joined.
+    n = n / 32 + 64
+    tol = (2 * e.unsqueeze(-1) + half + (2 * n + 16) * U) * a + n * 32 * 2.0**-25 * big_v * (q.dtype == torch.float16) / total.unsqueeze(-1) + half * o.abs()
+    tol_l = e + n * U + 16 * U * (1 + lse.abs())
+    back = lambda y: y.view(h, b, g, -1).transpose(0, 1).reshape(b, n_q, -1)  # noqa: E731
+    assert bool(((got[0].double() - back(o)).abs() <= back(tol)).all())
+    assert bool(((got[1].double() - back(lse).squeeze(-1)).abs() <= back(tol_l).squeeze(-1)).all())
+
+
+@pytest.mark.parametrize(("seqs", "prefix", "h", "eight"), [(20, 140000, 4, True), (20, 140001, 4, False), (70, 70007, 4, False)])
+def test_many_rows_over_a_long_prefix(seqs: int, prefix: int, h: int, eight: bool) -> None:
+    """Prefixes long enough for two workgroups a CU, whose last part is short."""
+    from lazykv_amd import kernels
+
+    gen = torch.Generator(device="cuda").manual_seed(14)
+    kv = [torch.randn((1, h, prefix, 64), device="cuda", generator=gen).bfloat16() for _ in range(2)]
+    q = torch.randn((seqs, 4 * h, 64), device="cuda", generator=gen).bfloat16()
+    if eight:
+        codes, scales = kernels.mx_empty(1, h, prefix, 64, "cuda")
+        rows = kernels.mx_rows(codes, scales, torch.bfloat16)
+        kernels.append_rows(rows, *kv)
+        kv = kernels.read_rows(rows, 0, prefix)
+    else:
+        rows = kernels.dense_rows(*kv)
+    got = kernels.shared_decode(q, scale=0.125, prefix=rows, prefix_tokens=prefix)
+    pieces = [tuple(x[0, :, i : i + 20000] for x in kv) for i in range(0, prefix, 20000)]
+    _check64(got, q, pieces, 0.125, prefix)
+
+
+def test_rows_past_32_bits_of_bytes() -> None:
+    """Keys and values of 4.3 GB each: one sequence of four query heads, and twelve over the same rows as a prefix."""
+    from lazykv_amd import kernels
+
+    gen = torch.Generator(device="cuda").manual_seed(15)
+    n = (1 << 25) + 77
+    kv = torch.randn((2, 1, 1, n, 64), device="cuda", generator=gen, dtype=torch.bfloat16)
+    rows = kernels.dense_rows(kv[0], kv[1])
+    for seqs, as_prefix in ((1, False), (12, True)):
+        q = (torch.randn((seqs, 4, 64), device="cuda", generator=gen) * 2).bfloat16()
+        call = dict(prefix=rows, prefix_tokens=n) if as_prefix else dict(own=rows, own_tokens=n)
+        got = kernels.shared_decode(q, scale=0.125, **call)
+        pieces = [(kv[0, 0, :, i : i + (1 << 22)], kv[1, 0, :, i : i + (1 << 22)]) for i in range(0, n, 1 << 22)]
+        _check64(got, q, pieces, 0.125, n)
+
+
+def test_a_prefix_of_no_tokens_and_no_rows() -> None:
+    from lazykv_amd import kernels
+
+    x = torch.zeros((1, 2, 5, 64), dtype=torch.float16, device="cuda")
+    out, lse = kernels.shared_decode(x.new_ones((3, 4, 64)), scale=1.0, prefix=kernels.dense_rows(x, x), prefix_tokens=0)
+    torch.cuda.synchronize()
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+
+
+def test_a_nan_far_below_the_maximum_is_not_lost() -> None:
+    """A NaN value whose weight is nothing beside another part's: it is attended, and shows, as in attention in 64 bits."""
+    from lazykv_amd import kernels
+
+    for seqs in (2, 10, 40):
+        k = torch.zeros((1, 1, 4096, 64), device="cuda", dtype=torch.float16)
+        k[:, :, 4000] = 60.0
+        v = torch.ones_like(k)
+        v[:, :, 17, 3] = float("nan")
+        q = torch.ones((seqs, 4, 64), device="cuda", dtype=torch.float16)
+        out, lse = kernels.shared_decode(q, scale=1.0, prefix=kernels.dense_rows(k, v), prefix_tokens=4096)
+        torch.cuda.synchronize()
+        assert bool(out[:, :, 3].isnan().all()) and bool((out[:, :, 4:] == 1).all()) and bool(lse.isfinite().all())
