@@ -35,7 +35,11 @@ namespace {
 
 constexpr int kWaves = 4;       // of a workgroup whose waves read streams of their own
 constexpr int kTile = 32;       // tokens
-constexpr float kSlack = 6.0f;  // a weight is at most 2^kSlack: nothing to a 16-bit weight's precision or a float32 sum's
+// How far (in base 2) a score may lie above the reference that weights are taken from. A weight is then at most 2^slack:
+// nothing to a 16-bit weight's precision or a float32 sum's. With more than 16 rows a reference that moves seldom is 2 to 8%
+// of a call's time (8 sequences over 16,411 8-bit tokens, d 64: 12.6 -> 11.6 us); with fewer it costs nothing to hold it at the
+// maximum, whose weight of 1 no rounding touches.
+constexpr float slack_of(int row_tiles) { return row_tiles == 1 ? 0.0f : 6.0f; }
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -254,16 +258,16 @@ template <int D> struct ValueRegs<D, true> {
 // channel (d/4) q + (d/16) i + e in o[n][e][i].
 template <int D, int NR> struct Result {
   f32x4 o[NR][D / 16];
-  float m[NR];  // the rows' reference, in base 2: the maximum of some tile, at most kSlack below any score
+  float m[NR];  // the rows' reference, in base 2: the maximum of some tile, at most the slack below any score
   float l[NR];  // this lane's tokens' part of the sum
 };
 
 // Rows' reference: what their scores are taken from before the exponential. It need not be a row's maximum, only
-// near it: it moves when a score is more than kSlack (in base 2) above it, so that most tiles pass without a
-// look at the other lanes. The products start from its negative, so that scores come out relative to it.
+// near it: it moves when a score is more than the slack above it, so that most tiles pass without a look at
+// the other lanes. The products start from its negative, so that scores come out relative to it.
 struct Reference {
   f32x4 negative;  // four times -reference, the products' first addend; 0 at first
-  float limit;     // kSlack in scores; -inf until there is a reference
+  float limit;     // the slack in scores; -inf until there is a reference
   __device__ __forceinline__ void reset() {
     negative = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     limit = -INFINITY;
@@ -304,7 +308,7 @@ __device__ __forceinline__ void settle(f32x4 (&sc)[NR][2], int left, float scale
       const bool move = up > ref[n].limit && up < INFINITY;
       const float by = move ? up : 0.0f, keep = ref[n].limit == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-by * scale2);
       ref[n].negative -= by;
-      ref[n].limit = move ? kSlack / scale2 : ref[n].limit;
+      ref[n].limit = move ? slack_of(NR) / scale2 : ref[n].limit;
       r.l[n] *= keep;
 #pragma unroll
       for (int e = 0; e < D / 16; ++e) r.o[n][e] *= keep;
@@ -822,42 +826,35 @@ __global__ __launch_bounds__(64 * W, 2) void shared_wide_kernel(SharedArgs a) {
 }
 
 // A workgroup a query row: its parts' results into one. d/4 threads take a part's channels, four each, and
-// the threads' groups the parts in turn, so that all loads of 64 parts are in flight together.
+// the threads' groups the parts in turn. The sums of 64 parts are under way before their weights are known: an empty
+// part has written zeros.
 template <int D>
 __global__ __launch_bounds__(256) void shared_join_kernel(SharedArgs a) {
-  constexpr int C = D / 4, GROUPS = 256 / C;
+  constexpr int C = D / 4, GROUPS = 256 / C, EACH = 64 / GROUPS;
   __shared__ f32x4 red[GROUPS][C];
   const int64_t row = blockIdx.x;
   const int lane = threadIdx.x & 63, parts = a.p_parts + a.o_parts, group = threadIdx.x / C, c = threadIdx.x % C;
   const float2* ml = a.part_ml + row * parts;
-  float top = -INFINITY;
-  for (int p = lane; p < parts; p += 64) top = fmaxf(top, ml[p].x);
-  top = lkv::wave_max_f32(top);
-  float total = 0.0f;
-  f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
   const float* from = a.part_o + row * parts * D + c * 4;
+  float top = -INFINITY, total = 0.0f;
+  f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
   for (int p0 = 0; p0 < parts; p0 += 64) {
-    float f = -1.0f;  // no part, or an empty one: its sums are not read
-    if (p0 + lane < parts) {
-      const float2 x = ml[p0 + lane];
-      if (x.y != 0.0f) {
-        f = join_factor(x.x, x.y, top);
-        total += f * x.y;
-      }
-    }
-    f32x4 x[64 / GROUPS];
-    float w[64 / GROUPS];
+    f32x4 x[EACH];
 #pragma unroll
-    for (int i = 0; i < 64 / GROUPS; ++i) {
+    for (int i = 0; i < EACH; ++i) {
       const int p = p0 + i * GROUPS + group;
-      w[i] = __shfl(f, i * GROUPS + group);
-      x[i] = w[i] < 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : *(const f32x4*)(from + (int64_t)p * D);
+      x[i] = p < parts ? *(const f32x4*)(from + (int64_t)p * D) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
+    const float2 mine = p0 + lane < parts ? ml[p0 + lane] : make_float2(-INFINITY, 0.0f);
+    const float up = fmaxf(top, lkv::wave_max_f32(mine.x));
+    const float keep = p0 == 0 ? 0.0f : join_factor(top, total, up), f = join_factor(mine.x, mine.y, up);
+    top = up;
+    total = total * keep + lkv::wave_sum_f32(mine.y == 0.0f ? 0.0f : f * mine.y);
+    o *= keep;
 #pragma unroll
-    for (int i = 0; i < 64 / GROUPS; ++i) o += x[i] * w[i];
+    for (int i = 0; i < EACH; ++i) o += x[i] * __shfl(f, i * GROUPS + group);
   }
   red[group][c] = o;
-  total = lkv::wave_sum_f32(total);
   __syncthreads();
   if (threadIdx.x >= C) return;
 #pragma unroll
@@ -922,6 +919,9 @@ Plan plan_of(const lkv_shared_desc* d) {
     least = 256;
   }
   int64_t chunk = (tokens + room - 1) / room;
+  // Few tokens and no prefix: one part, whose workgroup stores the output itself. 200 tokens (d 128, 16 bits) 8.0 -> 5.9 us, 500
+  // (d 64, 8 bits) 6.5 -> 5.4; 1,000 of those 6.5 -> 7.4.
+  if (d->prefix_tokens == 0 && (int64_t)d->max_own * d->head_dim <= 32768 && d->max_own > least) least = d->max_own;
   chunk = ((chunk < least ? least : chunk) + 127) / 128 * 128;
   p.p_chunk = p.o_chunk = (int)(chunk > (1 << 30) ? (1 << 30) : chunk);
   if (!p.nr && p.o_chunk > 1024) p.o_chunk = 1024;

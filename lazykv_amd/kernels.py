@@ -697,20 +697,12 @@ def mx_empty(seqs: int, n_kv: int, tokens: int, head_dim: int, device: torch.dev
     return codes, torch.zeros((2, seqs, n_kv, tokens, head_dim // MX_GROUP), dtype=torch.uint8, device=device)
 
 
-class _Nothing:
-    def __enter__(self) -> None:
-        return None
-
-    def __exit__(self, *exc: object) -> None:
-        return None
-
-
-_NOTHING = _Nothing()
-
-
-def _on(index: int):  # noqa: ANN202
-    """The device a launch needs as the current one, where it is another."""
-    return _NOTHING if index == _CURRENT_DEVICE() else torch.cuda.device(index)
+def _launch(index: int, fn, *args: object) -> int:  # noqa: ANN001
+    """`fn(stream, *args)` on the device's current stream, with that device as the current one."""
+    if index == _CURRENT_DEVICE():
+        return fn(_raw_stream(index), *args)
+    with torch.cuda.device(index):
+        return fn(_raw_stream(index), *args)
 
 
 _CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
@@ -761,8 +753,7 @@ def append_rows(dst: Rows, keys: torch.Tensor, values: torch.Tensor, *, start: i
     if y.stride() != st:
         x, y = torch.stack([x, y]).unbind(0)
         st = x.stride()
-    with _on(index):
-        rc = _lib.lib().lkv_append_rows(_raw_stream(index), dst.ref, x.data_ptr(), y.data_ptr(), dst.model_code, st[0], st[1], st[2], seqs, n_kv, d, n, at, start)
+    rc = _launch(index, _lib.lib().lkv_append_rows, dst.ref, x.data_ptr(), y.data_ptr(), dst.model_code, st[0], st[1], st[2], seqs, n_kv, d, n, at, start)
     if rc:
         _lib.check(rc, "append_rows")
 
@@ -776,19 +767,20 @@ def read_rows(src: Rows, first: int, n: int, out: tuple[torch.Tensor, torch.Tens
         raise ValueError(f"rows {first}..{first + n} exceed the {src.tokens} there are")
     shape, index = (src.seqs, src.n_kv, n, src.head_dim), src.device_index
     if out is None:
-        out = (torch.empty(shape, dtype=src.model_dtype, device=src.device), torch.empty(shape, dtype=src.model_dtype, device=src.device))
+        k = torch.empty(shape, dtype=src.model_dtype, device=src.device)
+        out = (k, torch.empty_like(k))
+    else:
+        for x in out:
+            if x.shape != shape or x.dtype != src.model_dtype or x.get_device() != index:
+                raise ValueError(f"out must be {src.model_dtype} {shape} on {src.device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
+        st = out[0].stride()
+        if out[1].stride() != st or st[3] != 1 or (st[0] | st[1] | st[2]) % 8 or (out[0].data_ptr() | out[1].data_ptr()) % 16:
+            raise ValueError("out's rows must be contiguous and start on 16 bytes, both with the same strides")
     k, v = out
     st = k.stride()
-    for x in out:
-        if x.shape != shape or x.dtype != src.model_dtype or x.get_device() != index:
-            raise ValueError(f"out must be {src.model_dtype} {shape} on {src.device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
-    if v.stride() != st or st[3] != 1 or (st[0] | st[1] | st[2]) % 8 or (k.data_ptr() | v.data_ptr()) % 16:
-        raise ValueError("out's rows must be contiguous and start on 16 bytes, both with the same strides")
     if 0 in shape:
         return out
-    with _on(index):
-        rc = _lib.lib().lkv_read_rows(_raw_stream(index), src.ref, src.seqs, src.n_kv, src.head_dim, first, n, k.data_ptr(), v.data_ptr(), src.model_code,
-                                      st[0], st[1], st[2])
+    rc = _launch(index, _lib.lib().lkv_read_rows, src.ref, src.seqs, src.n_kv, src.head_dim, first, n, k.data_ptr(), v.data_ptr(), src.model_code, *st[:3])
     if rc:
         _lib.check(rc, "read_rows")
     return out
@@ -864,9 +856,8 @@ def shared_decode(
         # Of the call's own: no other call's, on another stream or in a graph, can be in it.
         buf = torch.empty(need, dtype=torch.uint8, device=q.device) if need else lse
         ws_ptr, ws_n = buf.data_ptr(), need
-    with _on(index):
-        rc = lib.lkv_shared_decode(_raw_stream(index), desc, q.data_ptr(), rows.model_code, prefix.ref if prefix is not None else None,
-                                   own.ref if own is not None else None, at, out.data_ptr(), _lib.dtype_code(out.dtype), lse.data_ptr(), ws_ptr, ws_n)
+    rc = _launch(index, lib.lkv_shared_decode, desc, q.data_ptr(), rows.model_code, prefix.ref if prefix is not None else None,
+                 own.ref if own is not None else None, at, out.data_ptr(), _lib.dtype_code(out.dtype), lse.data_ptr(), ws_ptr, ws_n)
     if rc:
         _lib.check(rc, "shared_decode")
     return out, lse

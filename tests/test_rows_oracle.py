@@ -149,6 +149,26 @@ def test_shared_decode_refuses_bad_arguments(desc: dict, prefix: dict | None, ow
     assert says in lib.lkv_last_error(), lib.lkv_last_error()
 
 
+def test_every_shape_has_a_division() -> None:
+    """The division of the work and its scratch, on the host: any shape without an error, none for one part, and never more than
+    the partial results of 600 parts a row."""
+    from lazykv_amd import _lib
+
+    lib = _lib.lib()
+    for n_seqs in (0, 1, 3, 16, 65, 4096):
+        for n_q, n_kv in ((1, 1), (32, 8), (40, 1), (128, 128)):
+            for d in (64, 128):
+                for prefix in (0, 1, 127, 128, 5000, 131072, 1 << 30):
+                    for own in (0, 1, 256, 257, 513, 100000, 1 << 30):
+                        desc = _lib.SharedDesc(n_seqs, n_q, n_kv, d, 0.1, prefix, 0, own)
+                        got = lib.lkv_shared_decode_workspace_bytes(ctypes.byref(desc))
+                        rows = n_seqs * n_q
+                        if prefix == 0 and own * d <= 32768:
+                            assert got == 0
+                        if not (prefix == 1 << 30 or own == 1 << 30):
+                            assert got <= rows * 600 * (d + 2) * 4 + 16, (n_seqs, n_q, n_kv, d, prefix, own, got)
+
+
 def test_python_calls_refuse_cpu_tensors() -> None:
     from lazykv_amd import kernels
 
