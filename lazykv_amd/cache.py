@@ -278,6 +278,12 @@ class SharedLayer(CacheLayerMixin):
         if self.is_initialized:
             self._hold(*(x.index_select(1, indices) for x in self.own))
 
+    def reset(self) -> None:
+        raise RuntimeError("a shared layer is reset through its SharedPrefixCache")
+
+    def reorder_cache(self, beam_idx: torch.Tensor) -> None:
+        raise RuntimeError("a shared layer is reordered through its SharedPrefixCache")
+
     def get_mask_sizes(self, query_length: int) -> tuple[int, int]:
         return self.get_seq_length() + query_length, 0
 
@@ -303,7 +309,7 @@ class SharedPrefixCache(Cache):
     sequence that many; its attention goes sequence by sequence, over the prefix and the sequence's rows, with the causal attention
     of `attention.attend`. Sequences of different lengths: write them padded on the right and `truncate` to the lengths they have;
     later tokens are written and attended behind each one's own end (the model needs position_ids then, [n_seqs, T] from
-    `positions`)."""
+    `positions`). An attention_mask is not looked at: padding on the left is attended."""
 
     batched = True  # the attention function takes a batch from this selector
     policy_name = "shared_prefix"
@@ -313,6 +319,8 @@ class SharedPrefixCache(Cache):
             raise ValueError(f"unknown precision {quant!r}; expected one of {QUANTS}")
         if n_seqs <= 0 or max_new <= 0:
             raise ValueError(f"a batch needs sequences and room for their tokens, got n_seqs={n_seqs}, max_new={max_new}")
+        if not isinstance(prefix, FullGPUCache):
+            raise ValueError(f"the prefix must hold every layer densely (FullGPUCache, MXFP8Cache), got {type(prefix).__name__}")
         lengths = {layer.get_seq_length() if layer.is_initialized else 0 for layer in prefix.layers}
         if len(lengths) != 1 or 0 in lengths:
             raise ValueError(f"the prefix must be prefilled, every layer with as many tokens; they hold {sorted(lengths)}")
@@ -323,6 +331,7 @@ class SharedPrefixCache(Cache):
         self._base = [0] * n_seqs  # own lengths as last set; a layer has `added` more
         self._starts: torch.Tensor | None = None  # those on the device, where they differ
         self._scratch: tuple[torch.Tensor, torch.Tensor] | None = None
+        self._unattended: int | None = None  # the layer whose new tokens `select` has not seen yet
 
     # -- lengths ----------------------------------------------------------------------------------
 
@@ -361,6 +370,17 @@ class SharedPrefixCache(Cache):
         self.n_seqs = len(chosen)
         self._set([now[i] for i in chosen])
 
+    def reorder_cache(self, beam_idx: torch.Tensor) -> None:
+        self.keep(beam_idx)
+
+    def batch_select_indices(self, indices: torch.Tensor) -> None:
+        self.keep(indices)
+
+    def reset(self) -> None:
+        """Forget every sequence's own tokens; the prefix stays."""
+        self._unattended = None
+        self._set([0] * self.n_seqs)
+
     def _whole(self) -> list[int]:
         if len({layer.added for layer in self.layers}) != 1:
             raise RuntimeError("lengths are set between forwards: the layers hold different numbers of tokens")
@@ -379,6 +399,9 @@ class SharedPrefixCache(Cache):
         """The tokens' keys and values [n_seqs, h, T, d] behind each sequence's own. What is returned is the new tokens' alone:
         the attention is `select`'s."""
         layer = self.layers[layer_idx]
+        if self._unattended is not None:
+            raise RuntimeError(f"layer {self._unattended}'s attention did not come from this cache: the forward needs **cache.model_kwargs() and this "
+                               "library's attention function")
         if not layer.is_initialized:
             layer.lazy_initialization(key_states, value_states)
         n_new = key_states.shape[-2]
@@ -387,6 +410,7 @@ class SharedPrefixCache(Cache):
             raise RuntimeError(f"sequences full: appending {n_new} tokens to {most} exceeds their {self.max_new}-token capacity")
         kernels.append_rows(layer.own_rows, key_states, value_states, start=start, starts=self._starts)
         layer.added += n_new
+        self._unattended = layer_idx
         return key_states, value_states
 
     def get_seq_length(self, layer_idx: int = 0) -> int:
@@ -404,6 +428,9 @@ class SharedPrefixCache(Cache):
         layer = self.layers[layer_idx]
         if query.shape[0] != self.n_seqs:
             raise ValueError(f"queries of {query.shape[0]} sequences, the cache holds {self.n_seqs}")
+        if layer.prefix.length < self.prefix_tokens:
+            raise RuntimeError(f"the prefix was cut to {layer.prefix.length} tokens; the batch was made over {self.prefix_tokens}")
+        self._unattended = None
         _, n_q, n_new, d = query.shape
         scale = scaling if scaling is not None else d**-0.5
         if n_new > 1:

@@ -876,7 +876,7 @@ int check_desc(const lkv_shared_desc* d) {
   LKV_CHECK_ARG(d->n_seqs >= 0 && d->n_kv > 0 && d->n_q > 0 && d->n_q % d->n_kv == 0, "bad shape: %d sequences, %d query heads over %d",
                 d->n_seqs, d->n_q, d->n_kv);
   LKV_CHECK_ARG((int64_t)d->n_seqs * d->n_q <= (1 << 24), "%lld query rows in one call", (long long)d->n_seqs * d->n_q);
-  LKV_CHECK_ARG(d->scale > 0.0f && d->scale < INFINITY, "scale %g: positive and finite", (double)d->scale);
+  LKV_CHECK_ARG(d->scale > 0.0f && d->scale * lkv::kLog2e < INFINITY, "scale %g: positive and finite", (double)d->scale);
   LKV_CHECK_ARG(d->prefix_tokens >= 0 && d->max_own >= 0 && d->own_tokens >= 0, "bad extent: prefix %d, own %d of at most %d",
                 d->prefix_tokens, d->own_tokens, d->max_own);
   LKV_CHECK_ARG(d->prefix_tokens <= (1 << 30) && d->max_own <= (1 << 30), "at most %d tokens: prefix %d, own %d", 1 << 30, d->prefix_tokens,

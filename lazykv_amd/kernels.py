@@ -724,6 +724,12 @@ def _placed(x: torch.Tensor) -> torch.Tensor:
     return x
 
 
+def _int32(name: str, x: int) -> None:
+    """Refuses an integer that a C argument of 32 bits would cut."""
+    if not -(1 << 31) <= x < 1 << 31:
+        raise ValueError(f"{name} = {x} is out of range")
+
+
 def _counts(x: torch.Tensor | None, seqs: int, device: int, name: str) -> int | None:
     """The address of a count for each sequence, int32 on the device."""
     if x is None:
@@ -745,6 +751,7 @@ def append_rows(dst: Rows, keys: torch.Tensor, values: torch.Tensor, *, start: i
         raise ValueError(f"keys/values {tuple(shape)} do not match rows of {dst.seqs} sequences, {dst.n_kv} heads and head_dim {dst.head_dim}")
     if keys.get_device() != index or values.get_device() != index:
         raise ValueError(f"keys/values on {keys.device} / {values.device}, the cache on {dst.device}")
+    _int32("start", start)
     at = _counts(starts, seqs, index, "starts")
     if 0 in shape:
         return
@@ -831,6 +838,9 @@ def shared_decode(
         raise ValueError(f"a prefix of {prefix.seqs} sequences, {prefix.n_kv} heads, head_dim {prefix.head_dim}, {prefix.model_dtype} on {prefix.device} "
                          f"does not match one of {rows.n_kv}, {d}, {dtype} on {rows.device}")
     at = _counts(lengths, b, index, "lengths")
+    if (prefix_tokens | own_tokens | max_own) >> 31:
+        for name, n in (("prefix_tokens", prefix_tokens), ("own_tokens", own_tokens), ("max_own", max_own)):
+            _int32(name, n)
     if lengths is None and own_tokens > max_own:
         raise ValueError(f"own_tokens={own_tokens} exceed max_own={max_own}")
     if not q.is_contiguous() or q.data_ptr() % 16:

@@ -13,6 +13,8 @@ import numpy as np
 import pytest
 import torch
 
+from lazykv_amd.cache import Decoded
+from oracle import reference as R
 from oracle import rows as O
 
 pytestmark = pytest.mark.gpu
@@ -107,6 +109,40 @@ def test_8_bit_cache_truncates_and_resets(tiny) -> None:  # noqa: ANN001
         _forward(model, cache, _ids(3, 1, 40))
 
 
+def _follow(cache, ref) -> None:  # noqa: ANN001
+    """Has `ref`'s tiers attend the blocks that `cache`'s choose, which must be their own choice up to near ties: the two hold queries
+    and keys that differ by roundings, and a swap at a tie moves an output by any amount. With Delta the largest difference of
+    the two bounds (64 bits) and e the float32 bound's error, a block that `cache` chooses has a bound of at least its K-th - e
+    there, so of at least the K-th - e - 2 Delta in `ref` (the K-th largest moves by Delta at most)."""
+    chosen = {}
+    ours = cache.select
+
+    def bound(tier, query):  # noqa: ANN001, ANN202
+        n, _ = tier.candidates()
+        lo, hi = (x.double().cpu().numpy().reshape(tier.h, -1, tier.d)[:, 1:n] for x in (tier.kmin, tier.kmax))
+        q = query.double().cpu().numpy().reshape(-1, tier.d)
+        return R.quest_bound(q, lo, hi), float(np.abs(q).max() * np.maximum(np.abs(lo), np.abs(hi)).sum(-1).max()) * 2.0**-19
+
+    def record(layer, query, *args):  # noqa: ANN001, ANN002, ANN202
+        tier = cache.tiers.get(layer)
+        if tier is not None:
+            chosen[layer] = (tier.rank(query).clone(), bound(tier, query))
+        return ours(layer, query, *args)
+
+    def follow(layer, query, key=None, value=None, scaling=None):  # noqa: ANN001, ANN202
+        tier = ref.tiers.get(layer)
+        if tier is None:
+            return None
+        idx, (theirs, _) = chosen[layer]
+        own, err = bound(tier, query)
+        for j in range(tier.h):
+            assert R.selection_ok(idx[j].cpu().numpy() - 1, own[j], tier.k, abs_err=err + 2 * float(np.abs(theirs - own).max()))[0], (layer, j)
+        out, lse = tier.decode(query, scaling, idx=idx)
+        return Decoded(out.view(1, -1, 1, tier.d), lse.view(1, -1))
+
+    cache.select, ref.select = record, follow
+
+
 def test_8_bit_dense_layers_of_a_tiered_cache(tiny) -> None:  # noqa: ANN001
     """A tier whose dense layers stay in 8 bits, from a layer-major prefill and from a prefilled cache: the same tier either way as
     from dense layers of those rows, and the same decode."""
@@ -127,6 +163,7 @@ def test_8_bit_dense_layers_of_a_tiered_cache(tiny) -> None:  # noqa: ANN001
         for a in range(0, prompt, chunk):
             _forward(model, ref, ids[:, a : min(prompt, a + chunk)])
         tier = TieredCache(ref, k, bs, 512, dense_layers=1, fetch="resident")
+        _follow(got.cache, tier)
         for i in range(prompt, prompt + 12):
             a, b = (_forward(model, c, ids[:, i : i + 1], **c.model_kwargs()) for c in (got.cache, tier))
             assert float((a - b).abs().max()) < TOL, i
@@ -331,3 +368,65 @@ def test_eight_bit_layers_hold_rows_independent_of_how_they_came() -> None:
     want = [O.mx_decode(*O.mx_encode(x.double().cpu().numpy(), "bf16")) for x in kv]
     for x, y in zip(a.dense(), want):
         assert np.array_equal(x.double().cpu().numpy(), y)
+
+
+def test_a_forward_without_the_selector_is_refused(tiny) -> None:  # noqa: ANN001
+    """With another attention function too, which would attend the new token alone."""
+    from lazykv_amd.attention import IMPLEMENTATION_NAME
+    from lazykv_amd.cache import FullGPUCache, SharedPrefixCache
+
+    cfg, model = tiny
+    full = FullGPUCache(cfg.num_hidden_layers, 64)
+    _forward(model, full, _ids(20, 1, 20))
+    cache = SharedPrefixCache(full, 1, 8)
+    model.set_attn_implementation("sdpa")
+    try:
+        with pytest.raises(RuntimeError, match="model_kwargs"):
+            _forward(model, cache, _ids(21, 1, 1), position_ids=cache.positions())
+    finally:
+        model.set_attn_implementation(IMPLEMENTATION_NAME)
+    cache.reset()
+    assert bool(_forward(model, cache, _ids(21, 1, 1), **cache.model_kwargs()).isfinite().all()) and cache.lengths() == [1]
+
+
+def test_a_prefix_that_was_cut_and_one_that_is_not_dense_are_refused(tiny) -> None:  # noqa: ANN001
+    from lazykv_amd.cache import FullGPUCache, SharedPrefixCache
+    from lazykv_amd.tiered import TieredCache
+
+    cfg, model = tiny
+    full = FullGPUCache(cfg.num_hidden_layers, 64)
+    _forward(model, full, _ids(22, 1, 20))
+    cache = SharedPrefixCache(full, 2, 8)
+    full.truncate(19)
+    with pytest.raises(RuntimeError, match="cut to 19"):
+        _forward(model, cache, _ids(23, 2, 1), **cache.model_kwargs())
+    _forward(model, full, _ids(24, 1, 1))
+    tier = TieredCache(full, 1, 4, 64, dense_layers=1, fetch="resident")
+    with pytest.raises(ValueError, match="densely"):
+        SharedPrefixCache(tier, 2, 8)
+
+
+@pytest.mark.parametrize("quant", [None, "mxfp8"])
+def test_a_batch_is_reset_and_reordered_as_transformers_caches_are(tiny, quant: str | None) -> None:  # noqa: ANN001
+    from lazykv_amd.cache import FullGPUCache, SharedPrefixCache
+
+    cfg, model = tiny
+    full = FullGPUCache(cfg.num_hidden_layers, 64)
+    _forward(model, full, _ids(25, 1, 33))
+    cache = SharedPrefixCache(full, 3, 8, quant=quant)
+    ids, order = _ids(26, 3, 2), torch.tensor([2, 0, 2], device="cuda")
+    first = _forward(model, cache, ids[:, :1], **cache.model_kwargs())
+    cache.reorder_cache(order)
+    got = _forward(model, cache, ids[:, 1:], **cache.model_kwargs())
+    cache.reset()
+    assert cache.lengths() == [0, 0, 0] and cache.get_seq_length() == 33
+    assert torch.equal(_forward(model, cache, ids[:, :1], **cache.model_kwargs()), first)
+    cache.reset()
+    _forward(model, cache, ids[order][:, :1], **cache.model_kwargs())
+    assert torch.equal(_forward(model, cache, ids[:, 1:], **cache.model_kwargs()), got)
+    cache.batch_select_indices(torch.tensor([1], device="cuda"))
+    assert cache.lengths() == [2] and cache.n_seqs == 1
+    for layer in cache.layers:
+        for call in (layer.reset, lambda layer=layer: layer.reorder_cache(order)):
+            with pytest.raises(RuntimeError, match="through its SharedPrefixCache"):
+                call()

@@ -269,3 +269,26 @@ def test_python_refusals(bad: str) -> None:
         else:
             kernels.read_rows(rows, 0, 3, out=(x.bfloat16(), x.bfloat16()))
     assert bool((codes.view(torch.uint8) == 0x55).all())
+
+
+@pytest.mark.parametrize("bad", ["start", "start_with_starts", "same_sequences", "same_tensor", "out_same_heads", "out_same_tensor"])
+def test_cut_integers_and_rows_written_twice_are_refused(bad: str) -> None:
+    from lazykv_amd import kernels
+
+    codes, scales, rows = _cache(2, 2, 8, 64, "f16")
+    x = torch.zeros((2, 2, 3, 64), dtype=torch.float16, device="cuda")
+    with pytest.raises(ValueError):
+        if bad == "start":
+            kernels.append_rows(rows, x, x, start=1 << 32)
+        elif bad == "start_with_starts":
+            kernels.append_rows(rows, x, x, start=-(1 << 32), starts=torch.zeros(2, dtype=torch.int32, device="cuda"))
+        elif bad == "same_sequences":
+            kernels.append_rows(kernels.mx_rows(codes[:, :1].expand(2, 2, 2, 8, 64), scales[:, :1].expand(2, 2, 2, 8, 2), torch.float16), x, x)
+        elif bad == "same_tensor":
+            kernels.append_rows(kernels.dense_rows(x, x), x, x.clone())
+        elif bad == "out_same_heads":
+            y = torch.zeros((2, 2, 1, 3, 64), dtype=torch.float16, device="cuda").expand(2, 2, 2, 3, 64)
+            kernels.read_rows(rows, 0, 3, out=(y[0], y[1]))
+        else:
+            kernels.read_rows(rows, 0, 3, out=(x, x))
+    assert bool((codes.view(torch.uint8) == 0x55).all())

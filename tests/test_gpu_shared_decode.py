@@ -511,3 +511,47 @@ def test_a_nan_far_below_the_maximum_is_not_lost() -> None:
         out, lse = kernels.shared_decode(q, scale=1.0, prefix=kernels.dense_rows(k, v), prefix_tokens=4096)
         torch.cuda.synchronize()
         assert bool(out[:, :, 3].isnan().all()) and bool((out[:, :, 4:] == 1).all()) and bool(lse.isfinite().all())
+
+
+@pytest.mark.parametrize("name", ["prefix_tokens", "own_tokens", "max_own"])
+@pytest.mark.parametrize("by", [1 << 31, 1 << 32, -(1 << 32)])
+def test_counts_beyond_32_bits_are_refused(name: str, by: int) -> None:
+    """2^32 more than a valid count is that count in 32 bits."""
+    from lazykv_amd import kernels
+
+    x = torch.zeros((2, 2, 5, 64), dtype=torch.float16, device="cuda")
+    lengths = torch.zeros(2, dtype=torch.int32, device="cuda")
+    call = dict(scale=0.1, prefix=kernels.dense_rows(x[:1], x[:1]), prefix_tokens=5, own=kernels.dense_rows(x, x), own_tokens=5, max_own=5, lengths=lengths)
+    call[name] += by
+    with pytest.raises(ValueError):
+        kernels.shared_decode(x.new_zeros((2, 4, 64)), **call)
+
+
+def test_rows_that_sequences_share_are_read() -> None:
+    """The same rows for every sequence, by a stride of 0: as copies of them."""
+    from lazykv_amd import kernels
+
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    kv = torch.randn((2, 1, 2, 77, 64), device="cuda", generator=gen).half()
+    q = torch.randn((5, 4, 64), device="cuda", generator=gen).half()
+    shared = kernels.dense_rows(kv[0].expand(5, 2, 77, 64), kv[1].expand(5, 2, 77, 64))
+    copies = kernels.dense_rows(kv[0].repeat(5, 1, 1, 1), kv[1].repeat(5, 1, 1, 1))
+    a, b = (kernels.shared_decode(q, scale=0.125, own=r, own_tokens=77) for r in (shared, copies))
+    torch.cuda.synchronize()
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_an_output_in_the_querys_place() -> None:
+    from lazykv_amd import kernels
+
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    for n, seqs in ((100, 1), (3000, 2), (300, 40)):
+        kv = torch.randn((2, 1, 2, n, 64), device="cuda", generator=gen).half()
+        q = torch.randn((seqs, 8, 64), device="cuda", generator=gen).half()
+        rows = kernels.dense_rows(kv[0], kv[1])
+        call = dict(own=rows, own_tokens=n) if seqs == 1 else dict(prefix=rows, prefix_tokens=n)
+        want, _ = kernels.shared_decode(q, scale=0.125, **call)
+        got = q.clone()
+        kernels.shared_decode(got, scale=0.125, out=got, **call)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)

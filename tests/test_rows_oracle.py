@@ -114,6 +114,30 @@ def test_rows_calls_refuse_bad_arguments(fn: str, change: dict, call: dict, says
     assert says in lib.lkv_last_error(), lib.lkv_last_error()
 
 
+@pytest.mark.parametrize(("fn", "change", "call"), [
+    ("append", dict(seq_stride=0), {}),
+    ("append", dict(head_stride=0), {}),
+    ("append", dict(v=4096), {}),
+    ("read", {}, dict(v=4096)),
+    ("read", {}, dict(strides=(0, 1 << 16, 128))),
+    ("read", {}, dict(strides=(1 << 20, 0, 128))),
+    ("read", {}, dict(strides=(1 << 20, 1 << 16, 0))),
+])
+def test_rows_that_are_written_must_be_distinct(fn: str, change: dict, call: dict) -> None:
+    from lazykv_amd import _lib
+
+    lib = _lib.lib()
+    have = dict(k=4096, v=8192, strides=(1 << 20, 1 << 16, 128))
+    have.update(call)
+    r = _rows(**change)
+    if fn == "append":
+        rc = lib.lkv_append_rows(0, ctypes.byref(r), have["k"], have["v"], _lib.BF16, *have["strides"], 2, 8, 128, 10, None, 0)
+    else:
+        rc = lib.lkv_read_rows(0, ctypes.byref(r), 2, 8, 128, 0, 10, have["k"], have["v"], _lib.BF16, *have["strides"])
+    assert rc == _lib.LKV_ERR_INVALID
+    assert b"share an address" in lib.lkv_last_error()
+
+
 @pytest.mark.parametrize(("desc", "prefix", "own", "more", "says"), [
     (dict(head_dim=80), {}, {}, {}, b"head_dim 80"),
     (dict(n_q=30), {}, {}, {}, b"30 query heads over 8"),
@@ -147,6 +171,15 @@ def test_shared_decode_refuses_bad_arguments(desc: dict, prefix: dict | None, ow
     rc = lib.lkv_shared_decode(0, ctypes.byref(d), a["q"], a["q_dtype"], p, o, None, 4096, a["out_dtype"], 4096, 4096, a["ws_bytes"])
     assert rc == _lib.LKV_ERR_INVALID
     assert says in lib.lkv_last_error(), lib.lkv_last_error()
+
+
+def test_a_scale_that_leaves_float32_in_base_2_is_refused() -> None:
+    from lazykv_amd import _lib
+
+    lib = _lib.lib()
+    d = _lib.SharedDesc(1, 8, 8, 64, 3.0e38, 0, 0, 0)
+    assert lib.lkv_shared_decode(0, ctypes.byref(d), 4096, _lib.F16, None, None, None, 4096, _lib.F16, 4096, None, 0) == _lib.LKV_ERR_INVALID
+    assert b"scale" in lib.lkv_last_error()
 
 
 def test_every_shape_has_a_division() -> None:
