@@ -22,8 +22,9 @@
 //
 // Three forms, by the rows that share a KV head's prefix (sequences times group):
 //  - up to 16 or 32: a wave reads its own tokens from memory to registers; the workgroup's four waves, then the parts,
-//    join. Bound by memory: one sequence over 131,072 tokens of 8 KV heads, d 128, takes 54.5 us in 8 bits (277 MB, 5.1 TB/s) and
-//    96.3 in bfloat16 (537 MB, 5.6 TB/s), of which the join is 5.
+//    join. Bound by memory: one sequence over 131,072 tokens of 8 KV heads, d 128, takes 52.4 us in 8 bits (277 MB, 5.3 TB/s) and
+//    95.8 in bfloat16 (537 MB, 5.6 TB/s), of which the join is 5. (64 rows a wave, one wave a SIMD: 16 sequences over
+//    32,768 bfloat16 tokens 32.4 us where the next form takes 29.7, launches left out.)
 //  - up to 64: through LDS, eight waves; 16 sequences over 32,768 bfloat16 tokens 35 us (134 MB; 6.1 TB/s in the loop, 5 us
 //    before it, 3 after it and 5 for the join).
 //  - more: through LDS, four waves, two workgroups a CU; 64 sequences over 32,768 tokens 60 us, over 131,072 180 (0.76
@@ -491,6 +492,7 @@ __device__ __forceinline__ void finish(const SharedArgs& a, const Result<D, NR>&
     }
     return;
   } else {
+    static_assert(FOURS % GROUPS == 0, "every wave takes as many channels");
     float2* const ml = (float2*)(lds + GROUPS * width * NR * FOURS * 64);
     __syncthreads();  // what LDS held before is read no more
     const int mine = (group * width + slot) * NR;
@@ -520,9 +522,8 @@ __device__ __forceinline__ void finish(const SharedArgs& a, const Result<D, NR>&
       }
       if (group == 0 && quarter == 0 && row[n] >= 0) store_sums(a, row[n], part, top, total);
 #pragma unroll
-      for (int j = 0; j < (FOURS + GROUPS - 1) / GROUPS; ++j) {
+      for (int j = 0; j < FOURS / GROUPS; ++j) {
         const int k = j * GROUPS + group;
-        if (FOURS % GROUPS != 0 && k >= FOURS) break;
         f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int i = 0; i < GROUPS; ++i) o += lds[(((i * width + slot) * NR + n) * FOURS + k) * 64 + lane] * x[i].x;
@@ -637,17 +638,16 @@ template <int DT, int D, class S> struct StageRegs<DT, D, false, S> {
 };
 // 8 bits: 16 codes under one scale become two pieces.
 template <int DT, int D, class S> struct StageRegs<DT, D, true, S> {
-  static constexpr int UNITS = S::TOKENS * D / 16, LOADS = (UNITS + S::THREADS - 1) / S::THREADS;
+  static constexpr int LOADS = S::TOKENS * D / 16 / S::THREADS;
+  static_assert(LOADS * S::THREADS * 16 == S::TOKENS * D, "whole loads of every thread");
   uint4 k[LOADS], v[LOADS];
   uint32_t ks[LOADS], vs[LOADS];
-  static __device__ __forceinline__ bool mine(int i) { return UNITS % S::THREADS == 0 || i * S::THREADS + (int)threadIdx.x < UNITS; }
   __device__ __forceinline__ void load(const Stream& s, int t0, int end) {
     const int last = min(S::TOKENS, end - t0) - 1;
     const uint8_t *kb = s.k + (int64_t)t0 * D, *vb = s.v + (int64_t)t0 * D;
     const uint8_t *ksb = s.ks + (int64_t)t0 * (D / kMxGroup), *vsb = s.vs + (int64_t)t0 * (D / kMxGroup);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      if (!mine(i)) continue;
       const int x = i * S::THREADS + threadIdx.x;
       const uint32_t at = (uint32_t)(min(x / (D / 16), last) * D + x % (D / 16) * 16);
       k[i] = *(const uint4*)(kb + at);
@@ -664,7 +664,6 @@ template <int DT, int D, class S> struct StageRegs<DT, D, true, S> {
   __device__ __forceinline__ void store(uint8_t* lds, int live) const {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      if (!mine(i)) continue;
       const int x = i * S::THREADS + threadIdx.x, row = x / (D / 16), piece = x % (D / 16) * 2, sw = S::swizzle(row);
       uint8_t* to = lds + row * (2 * D);
       const uint32_t keep = row < live ? ~0u : 0u;  // a code of zero is zero under any scale that is written
