@@ -636,14 +636,12 @@ class Rows:
 
     __slots__ = ("seqs", "n_kv", "tokens", "head_dim", "dtype", "model_dtype", "model_code", "device_index", "owners", "struct", "ref")
 
-    def __init__(self, k: int, v: int, k_scale: int | None, v_scale: int | None, seq_stride: int, head_stride: int, shape: tuple, dtype: int,
-                 model_dtype: torch.dtype, device_index: int, owners: tuple) -> None:
-        self.seqs, self.n_kv, self.tokens, self.head_dim = shape
+    def __init__(self, k: int, v: int, k_scale: int | None, v_scale: int | None, strides: tuple, seqs: int, n_kv: int, tokens: int, head_dim: int,
+                 dtype: int, model_dtype: torch.dtype, model_code: int, device_index: int, owners: tuple) -> None:
+        self.seqs, self.n_kv, self.tokens, self.head_dim = seqs, n_kv, tokens, head_dim
         self.dtype = dtype  # _lib.F16, _lib.BF16 or _lib.MXFP8
-        self.model_dtype, self.model_code = model_dtype, _ROW_DTYPES[model_dtype]
-        self.device_index = device_index
-        self.owners = owners
-        self.struct = _lib.KVRows(k, v, k_scale, v_scale, seq_stride, head_stride, self.tokens, self.seqs, dtype, self.model_code)
+        self.model_dtype, self.model_code, self.device_index, self.owners = model_dtype, model_code, device_index, owners
+        self.struct = _lib.KVRows(k, v, k_scale, v_scale, *strides, tokens, seqs, dtype, model_code)
         self.ref = ctypes.byref(self.struct)
 
     @property
@@ -666,29 +664,31 @@ def dense_rows(keys: torch.Tensor, values: torch.Tensor) -> Rows:
     """Rows in the model dtype: keys and values `[seqs, h, T, d]`, contiguous rows d elements apart, any strides above
     that are multiples of 32 elements and the same for both."""
     _lib.require_cuda(keys, values)
-    shape, ks, device, dtype = keys.shape, keys.stride(), keys.get_device(), keys.dtype
+    shape, st, device, dtype = keys.shape, keys.stride(), keys.get_device(), keys.dtype
     if len(shape) != 4 or values.shape != shape or values.dtype != dtype or values.get_device() != device:
         raise ValueError(f"expected matching [seqs, h, T, d] keys/values, got {tuple(shape)} {dtype} / {tuple(values.shape)} {values.dtype}")
-    if ks[3] != 1 or ks[2] != shape[3] or values.stride() != ks:
+    seqs, h, tokens, d = shape
+    if st[3] != 1 or st[2] != d or values.stride() != st:
         raise ValueError("rows must be contiguous with a token stride of head_dim, keys and values with the same strides")
-    return Rows(keys.data_ptr(), values.data_ptr(), None, None, ks[0], ks[1], shape, _row_dtype(dtype), dtype, device, (keys, values))
+    code = _row_dtype(dtype)
+    return Rows(keys.data_ptr(), values.data_ptr(), None, None, st[:2], seqs, h, tokens, d, code, dtype, code, device, (keys, values))
 
 
 def mx_rows(codes: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype) -> Rows:
     """Rows in 8 bits: codes `[2, seqs, h, T, d]` (keys, values; float8_e4m3fn or uint8) and scales `[2, seqs, h, T, d / 32]`
     (uint8), for a model of `dtype`. Views are fine whose scales are cut like their codes."""
     _lib.require_cuda(codes, scales)
-    _row_dtype(dtype)
+    model = _row_dtype(dtype)
     shape, cs, ss, device = codes.shape, codes.stride(), scales.stride(), codes.get_device()
     if len(shape) != 5 or shape[0] != 2 or codes.dtype not in _CODE_DTYPES or scales.dtype != torch.uint8 or scales.get_device() != device:
         raise ValueError(f"expected codes [2, seqs, h, T, d] and uint8 scales, got {tuple(shape)} {codes.dtype} / {tuple(scales.shape)} {scales.dtype}")
-    d = shape[4]
-    if d % MX_GROUP or scales.shape != shape[:4] + (d // MX_GROUP,):
-        raise ValueError(f"codes {tuple(shape)} take scales {tuple(shape[:4]) + (d // MX_GROUP,)}, got {tuple(scales.shape)}")
+    _, seqs, h, tokens, d = shape
+    if d % MX_GROUP or scales.shape != (2, seqs, h, tokens, d // MX_GROUP):
+        raise ValueError(f"codes {tuple(shape)} take scales {(2, seqs, h, tokens, d // MX_GROUP)}, got {tuple(scales.shape)}")
     if cs[4] != 1 or cs[3] != d or ss[4] != 1 or ss[3] * MX_GROUP != d or ss[1] * MX_GROUP != cs[1] or ss[2] * MX_GROUP != cs[2]:
         raise ValueError("codes' and scales' rows must be contiguous, and their strides alike")
     k, k_scale = codes.data_ptr(), scales.data_ptr()
-    return Rows(k, k + cs[0], k_scale, k_scale + ss[0], cs[1], cs[2], shape[1:], _lib.MXFP8, dtype, device, (codes, scales))
+    return Rows(k, k + cs[0], k_scale, k_scale + ss[0], cs[1:3], seqs, h, tokens, d, _lib.MXFP8, dtype, model, device, (codes, scales))
 
 
 def mx_empty(seqs: int, n_kv: int, tokens: int, head_dim: int, device: torch.device | str) -> tuple[torch.Tensor, torch.Tensor]:
