@@ -17,8 +17,10 @@
 // channels of each of these eight rows, 16 lanes a whole row, and pairs them by byte permutes.
 //
 // Weights are rounded to the model dtype for the second product (the matrix units' 16-bit form, 16 times
-// float32's rate): an output is off by no more than that one rounding of each weight, as much as its own rounding. Scores, maxima,
-// sums of weights (unrounded) and outputs are float32.
+// float32's rate): with h = 2^-8 (bfloat16) or 2^-11 (float16) an output is off by at most h sum p_t |v_t| for it and, in float16, whose
+// small numbers have fewer bits, by 2^-38 max |v| more for each token that is 2^-27 of the largest or less (2^-40 and 2^-29 with up to 16
+// rows; `lift_of`). Where values cancel, that is more than the output's own rounding. Scores, maxima, sums of
+// weights (unrounded) and outputs are float32.
 //
 // Three forms, by the rows that share a KV head's prefix (sequences times group):
 //  - up to 16 or 32: a wave reads its own tokens from memory to registers; the workgroup's four waves, then the parts,
@@ -39,8 +41,14 @@ constexpr int kTile = 32;       // tokens
 // How far (in base 2) a score may lie above the reference that weights are taken from. A weight is then at most 2^slack:
 // nothing to a 16-bit weight's precision or a float32 sum's. With more than 16 rows a reference that moves seldom is 2 to 8%
 // of a call's time (8 sequences over 16,411 8-bit tokens, d 64: 12.6 -> 11.6 us); with fewer it costs nothing to hold it at the
-// maximum, whose weight of 1 no rounding touches.
-constexpr float slack_of(int row_tiles) { return row_tiles == 1 ? 0.0f : 6.0f; }
+// maximum, whose weight of 1 no rounding touches. Float16 pays for slack with the range of its weights (`lift_of`): 2 for 4 more powers of two
+// than 6 leaves, at no time up to 32 rows, 64 sequences over 32,768 tokens, d 128, 71.9 -> 73.4 us, 32 over 65,536 8-bit tokens, d 64, 37.1 -> 39.5.
+constexpr float slack_of(int dt, int row_tiles) { return row_tiles == 1 ? 0.0f : (dt == LKV_F16 ? 2.0f : 6.0f); }
+// Float16 weights are held 2^lift larger than they are, the largest at 2^15, and the sums scaled back at the end (exactly): of float16's
+// 30 powers of two above its subnormal numbers all but one then lie below the largest weight. Held as they are, weights below 2^-14 of it would
+// lose bits and those below 2^-25 be lost from the products though not from the sum: one token 17.4 above the others in score, as the
+// first of a prompt often is, would leave nothing of them. The lift is the exponential's addend, a multiplication's cost.
+constexpr float lift_of(int dt, int row_tiles) { return dt == LKV_F16 ? 15.0f - slack_of(dt, row_tiles) : 0.0f; }
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -279,7 +287,7 @@ struct Reference {
 
 // A tile's scores, relative to the references, made ready for the exponential: tokens behind the end without weight
 // (`left`: tokens that the tile has, if fewer than 32), a reference moved where it must be; l and o follow it.
-template <int D, int NR>
+template <int DT, int D, int NR>
 __device__ __forceinline__ void settle(f32x4 (&sc)[NR][2], int left, float scale2, Reference (&ref)[NR], Result<D, NR>& r) {
   if (left < kTile) {
     int mine = left - (int)(threadIdx.x & 48) / 4;
@@ -309,7 +317,7 @@ __device__ __forceinline__ void settle(f32x4 (&sc)[NR][2], int left, float scale
       const bool move = up > ref[n].limit && up < INFINITY;
       const float by = move ? up : 0.0f, keep = ref[n].limit == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(-by * scale2);
       ref[n].negative -= by;
-      ref[n].limit = move ? slack_of(NR) / scale2 : ref[n].limit;
+      ref[n].limit = move ? slack_of(DT, NR) / scale2 : ref[n].limit;
       r.l[n] *= keep;
 #pragma unroll
       for (int e = 0; e < D / 16; ++e) r.o[n][e] *= keep;
@@ -320,13 +328,31 @@ __device__ __forceinline__ void settle(f32x4 (&sc)[NR][2], int left, float scale
 }
 
 // Settled scores to weights, the second product's operand.
-template <int DT>
+template <int DT, int NR>
 __device__ __forceinline__ uint4 weights(const f32x4 (&sc)[2], float scale2, float& l) {
   float w[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) w[j] = __builtin_amdgcn_exp2f(sc[j / 4][j & 3] * scale2);
+  for (int j = 0; j < 8; ++j) {
+    const float x = sc[j / 4][j & 3];
+    w[j] = __builtin_amdgcn_exp2f(lift_of(DT, NR) != 0.0f ? __builtin_fmaf(x, scale2, lift_of(DT, NR)) : x * scale2);
+  }
   l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
   return make_uint4(Mat<DT>::pack(w[0], w[1]), Mat<DT>::pack(w[2], w[3]), Mat<DT>::pack(w[4], w[5]), Mat<DT>::pack(w[6], w[7]));
+}
+
+// A range's sums and references as partial results carry them.
+template <int DT, int D, int NR>
+__device__ __forceinline__ void conclude(float scale2, const Reference (&ref)[NR], Result<D, NR>& r) {
+  constexpr float down = 1.0f / (float)(1 << (int)lift_of(DT, NR));
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    r.l[n] = lkv::pair_sum<32>(lkv::pair_sum<16>(r.l[n])) * down;
+    r.m[n] = ref[n].level(scale2);
+    if constexpr (down != 1.0f) {
+#pragma unroll
+      for (int e = 0; e < D / 16; ++e) r.o[n][e] *= down;
+    }
+  }
 }
 
 // Loads stay on their side: moved down to where the next tile uses them, they would be waited for.
@@ -384,10 +410,10 @@ __device__ __forceinline__ void attend_range(const Stream& s, const uint16_t* co
       for (int j = 0; j < 8; ++j)
         v.keep(j, t + (j < 4 ? 0 : 16) + 4 * quarter + (j & 3) < end);
     }
-    settle<D, NR>(sc, end - t, scale2, ref, r);
+    settle<DT, D, NR>(sc, end - t, scale2, ref, r);
     uint4 p[NR];
 #pragma unroll
-    for (int n = 0; n < NR; ++n) p[n] = weights<DT>(sc[n], scale2, r.l[n]);
+    for (int n = 0; n < NR; ++n) p[n] = weights<DT, NR>(sc[n], scale2, r.l[n]);
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
       uint32_t x[8];
@@ -406,11 +432,7 @@ __device__ __forceinline__ void attend_range(const Stream& s, const uint16_t* co
     v.load(s, next, at);
     load_fence();
   }
-#pragma unroll
-  for (int n = 0; n < NR; ++n) {
-    r.l[n] = lkv::pair_sum<32>(lkv::pair_sum<16>(r.l[n]));
-    r.m[n] = ref[n].level(scale2);
-  }
+  conclude<DT, D, NR>(scale2, ref, r);
 }
 
 __device__ __forceinline__ float join_factor(float m, float l, float top) {
@@ -728,10 +750,10 @@ __device__ __forceinline__ void wide_tile(const LdsPointer (&key_at)[D / 32], co
   __builtin_amdgcn_sched_barrier(0);
   f32x4 sc[NR][2];
   wide_scores<DT, D, NR>(k, qf, ref, sc);
-  settle<D, NR>(sc, left, scale2, ref, r);
+  settle<DT, D, NR>(sc, left, scale2, ref, r);
   uint4 p[NR];
 #pragma unroll
-  for (int n = 0; n < NR; ++n) p[n] = weights<DT>(sc[n], scale2, r.l[n]);
+  for (int n = 0; n < NR; ++n) p[n] = weights<DT, NR>(sc[n], scale2, r.l[n]);
 #pragma unroll
   for (int e = 0; e < D / 16; ++e)
 #pragma unroll
@@ -790,11 +812,7 @@ __device__ __forceinline__ void attend_wide(const Stream& s, const uint16_t* con
           wide_tile<DT, D, NR>(key_at, value_at, half * 2 * S::BYTES + tile * kTile * 2 * D, qf, left - tile * kTile, scale2, ref, r);
     }
   }
-#pragma unroll
-  for (int n = 0; n < NR; ++n) {
-    r.l[n] = lkv::pair_sum<32>(lkv::pair_sum<16>(r.l[n]));
-    r.m[n] = ref[n].level(scale2);
-  }
+  conclude<DT, D, NR>(scale2, ref, r);
 }
 
 template <int DT, int D, bool PMX, bool OMX, int WR, int W>
