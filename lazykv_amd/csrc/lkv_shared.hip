@@ -941,7 +941,15 @@ Plan plan_of(const lkv_shared_desc* d) {
   if (d->prefix_tokens == 0 && (int64_t)d->max_own * d->head_dim <= 32768 && d->max_own > least) least = d->max_own;
   chunk = ((chunk < least ? least : chunk) + 127) / 128 * 128;
   p.p_chunk = p.o_chunk = (int)(chunk > (1 << 30) ? (1 << 30) : chunk);
-  if (!p.nr && p.o_chunk > 1024) p.o_chunk = 1024;
+  if (!p.nr) {
+    // Own rows in about as many pieces as the card takes at once, four a CU, however many rows there is room for: each stores its
+    // partial result, rows or none. Pieces of the prefix's size gave 398 MiB of scratch for 64 sequences with room for 100,000 tokens. 64
+    // sequences of 32,768 tokens behind 1,021, d 128, 8 bits: 905 us in pieces of 256 tokens, 740, 729 and 727 in 16, 8 and 4 pieces a CU; 16 of
+    // up to 16,384 behind 32,768: 118, 118, 118 and 109.
+    const int64_t piece = (items * d->max_own + 4 * cus - 1) / (4 * cus);
+    p.o_chunk = p.o_chunk > 1024 ? 1024 : p.o_chunk;
+    if (piece > p.o_chunk) p.o_chunk = (int)((piece > (1 << 30) ? (1 << 30) : piece) + 127) / 128 * 128;
+  }
   p.p_parts = ceil_div(d->prefix_tokens, p.p_chunk);
   p.o_parts = ceil_div(d->max_own, p.o_chunk);
   p.p_groups = ceil_div((int64_t)p.p_parts * d->n_kv, 8);
