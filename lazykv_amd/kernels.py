@@ -669,7 +669,9 @@ def dense_rows(keys: torch.Tensor, values: torch.Tensor) -> Rows:
         raise ValueError(f"expected matching [seqs, h, T, d] keys/values, got {tuple(shape)} {dtype} / {tuple(values.shape)} {values.dtype}")
     seqs, h, tokens, d = shape
     if st[3] != 1 or st[2] != d or values.stride() != st:
-        raise ValueError("rows must be contiguous with a token stride of head_dim, keys and values with the same strides")
+        st, vt = _meant(shape, st), _meant(shape, values.stride())
+        if st[3] != 1 or (st[2] != d and tokens != 1) or vt != st:
+            raise ValueError("rows must be contiguous with a token stride of head_dim, keys and values with the same strides")
     code = _row_dtype(dtype)
     return Rows(keys.data_ptr(), values.data_ptr(), None, None, st[:2], seqs, h, tokens, d, code, dtype, code, device, (keys, values))
 
@@ -716,12 +718,19 @@ def _raw_stream(index: int) -> int:
 _GET_RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def _placed(x: torch.Tensor) -> torch.Tensor:
-    """`x` as the row kernels read it: contiguous channels, rows on 16 bytes. A copy where it lies otherwise."""
-    st = x.stride()
+def _meant(shape: tuple, strides: tuple) -> tuple:
+    """A tensor's strides with 0 for dimensions of size 1, whose strides mean nothing: a decode token's keys and values, one contiguous and
+    one a projection's transposed view, differ in those alone. The last dimension's stays."""
+    return (*(s if n != 1 else 0 for n, s in zip(shape[:-1], strides)), strides[-1])
+
+
+def _placed(x: torch.Tensor) -> tuple[torch.Tensor, tuple]:
+    """`x` as the row kernels read it, and its strides: contiguous channels, rows on 16 bytes. A copy where it lies otherwise."""
+    st = _meant(x.shape, x.stride())
     if st[3] != 1 or (st[0] | st[1] | st[2]) % 8 or x.data_ptr() % 16:
-        return x.clone(memory_format=torch.contiguous_format)
-    return x
+        x = x.clone(memory_format=torch.contiguous_format)
+        st = _meant(x.shape, x.stride())
+    return x, st
 
 
 def _int32(name: str, x: int) -> None:
@@ -755,11 +764,12 @@ def append_rows(dst: Rows, keys: torch.Tensor, values: torch.Tensor, *, start: i
     at = _counts(starts, seqs, index, "starts")
     if 0 in shape:
         return
-    x, y = _placed(keys), _placed(values)
-    st = x.stride()
-    if y.stride() != st:
-        x, y = torch.stack([x, y]).unbind(0)
-        st = x.stride()
+    x, y, st = keys, values, keys.stride()
+    if values.stride() != st or st[3] != 1 or (st[0] | st[1] | st[2]) % 8 or (x.data_ptr() | y.data_ptr()) % 16:
+        (x, st), (y, yt) = _placed(x), _placed(y)
+        if yt != st:
+            x, y = torch.stack([x, y]).unbind(0)
+            st = x.stride()
     rc = _launch(index, _lib.lib().lkv_append_rows, dst.ref, x.data_ptr(), y.data_ptr(), dst.model_code, st[0], st[1], st[2], seqs, n_kv, d, n, at, start)
     if rc:
         _lib.check(rc, "append_rows")
@@ -775,16 +785,16 @@ def read_rows(src: Rows, first: int, n: int, out: tuple[torch.Tensor, torch.Tens
     shape, index = (src.seqs, src.n_kv, n, src.head_dim), src.device_index
     if out is None:
         k = torch.empty(shape, dtype=src.model_dtype, device=src.device)
-        out = (k, torch.empty_like(k))
+        v = torch.empty_like(k)
+        out, st = (k, v), k.stride()
     else:
         for x in out:
             if x.shape != shape or x.dtype != src.model_dtype or x.get_device() != index:
                 raise ValueError(f"out must be {src.model_dtype} {shape} on {src.device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
-        st = out[0].stride()
-        if out[1].stride() != st or st[3] != 1 or (st[0] | st[1] | st[2]) % 8 or (out[0].data_ptr() | out[1].data_ptr()) % 16:
+        k, v = out
+        st, vt = _meant(shape, k.stride()), _meant(shape, v.stride())
+        if vt != st or st[3] != 1 or (st[0] | st[1] | st[2]) % 8 or (k.data_ptr() | v.data_ptr()) % 16:
             raise ValueError("out's rows must be contiguous and start on 16 bytes, both with the same strides")
-    k, v = out
-    st = k.stride()
     if 0 in shape:
         return out
     rc = _launch(index, _lib.lib().lkv_read_rows, src.ref, src.seqs, src.n_kv, src.head_dim, first, n, k.data_ptr(), v.data_ptr(), src.model_code, *st[:3])
