@@ -84,3 +84,50 @@ def test_rows_of_one_token_or_head_are_described_and_read_into() -> None:
     kernels.read_rows(rows, 0, 1, out=out)
     torch.cuda.synchronize()
     assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+@pytest.mark.parametrize(("seqs", "prefix"), [(1, False), (6, True), (12, True), (20, True)])
+@pytest.mark.parametrize("eight", [False, True])
+def test_rows_behind_32_bits_of_bytes_decide_the_result(seqs: int, prefix: bool, eight: bool) -> None:
+    """The last 77 of 2^25 + 77 rows of 128 bytes lie behind 2^32 bytes, those of the second head behind 2^33. Their keys score 40, all
+    others' 0 but the first 77's, which lie where a 32-bit offset would look for them and score -40: the others' share, 2^25 e^-40, is below
+    2^-32, and the output is the last rows' value, 2. Its weights are alike, so rounded alike; products and sums of up to 77 such are exact, and what is
+    left is the division's roundings and the output's: 2 (2^-22 + 2^-8) at most. lse: as in test_gpu_shared_decode.py, with n = 77, as the other
+    rows' sum is nothing."""
+    from lazykv_amd import kernels
+
+    n, last, h, d = (1 << 25) + 77, 77, 2, 128 if eight else 64
+    k, v = torch.zeros((1, h, last, d), dtype=torch.bfloat16, device="cuda"), torch.full((1, h, last, d), 2.0, dtype=torch.bfloat16, device="cuda")
+    k[..., 0] = 40.0
+    if eight:
+        codes, scales = kernels.mx_empty(1, h, n, d, "cuda")
+        rows = kernels.mx_rows(codes, scales, torch.bfloat16)
+    else:
+        store = torch.zeros((2, 1, h, n, d), dtype=torch.bfloat16, device="cuda")
+        store[1] = 1.0
+        rows = kernels.dense_rows(store[0], store[1])
+    kernels.append_rows(rows, -k, -v)
+    kernels.append_rows(rows, k, v, start=n - last)
+    q = torch.zeros((seqs, 4 * h, d), dtype=torch.bfloat16, device="cuda")
+    q[..., 0] = 1.0
+    out, lse = kernels.shared_decode(q, scale=1.0, **(dict(prefix=rows, prefix_tokens=n) if prefix else dict(own=rows, own_tokens=n)))
+    torch.cuda.synchronize()
+    assert float((out.double() - 2.0).abs().max()) <= 2 * (2.0**-22 + 2.0**-8)
+    want = 40.0 + np.log(77.0)
+    assert float((lse.double() - want).abs().max()) <= (3 * 40 + 4 + 77 + 16 * (1 + want)) * 2.0**-24
+
+
+def test_sequences_of_their_own_behind_32_bits_of_bytes() -> None:
+    """The third sequence's rows begin behind 2^32 bytes and hold another value than the first's: each gets its own."""
+    from lazykv_amd import kernels
+
+    n = (1 << 24) + 5
+    store = torch.zeros((2, 3, 1, n, 64), dtype=torch.bfloat16, device="cuda")
+    for b in range(3):
+        store[1, b] = 1.0 + b
+    q = torch.ones((3, 4, 64), dtype=torch.bfloat16, device="cuda")
+    lengths = torch.tensor([200, 3, 200], dtype=torch.int32, device="cuda")
+    out, _ = kernels.shared_decode(q, scale=1.0, own=kernels.dense_rows(store[0], store[1]), lengths=lengths, max_own=200)
+    torch.cuda.synchronize()
+    for b in range(3):
+        assert bool((out[b] == 1.0 + b).all())
