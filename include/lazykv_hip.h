@@ -313,14 +313,16 @@ typedef struct lkv_kv_rows {
  * group's finite values; the code is x * 2^(127 - X) rounded to the nearest E4M3 value, ties to even,
  * after x is limited to the largest four-bit significand of the model dtype (61440 in float16), so that
  * every finite row reads back finite; what is not finite becomes the NaN code. A model-dtype dst takes
- * the values as they are. A dst whose sequences, heads or keys and values share rows is refused. */
+ * the values as they are. A dst of which two rows (or scales) overlap, of any sequences and heads, keys and values, is
+ * refused; so is a layout of more than 65,536 combinations whose strides do not nest (each at least what the
+ * smaller ones reach), of which that cannot be told. */
 int lkv_append_rows(uintptr_t stream, const lkv_kv_rows* dst, const void* k, const void* v, int dtype, int64_t seq_stride,
                     int64_t head_stride, int64_t token_stride, int n_seqs, int n_kv, int head_dim, int tokens,
                     const int32_t* starts, int start);
 
 /* Rows first .. first + tokens - 1 of an LKV_MXFP8 src, each code times its scale, in the model dtype
  * (exact there, but for bfloat16 values below its normal range, which are rounded) to k / v, laid out
- * as in lkv_append_rows, no two rows at one address. */
+ * as in lkv_append_rows; rows that overlap are refused in the same way. */
 int lkv_read_rows(uintptr_t stream, const lkv_kv_rows* src, int n_seqs, int n_kv, int head_dim, int first, int tokens, void* k,
                   void* v, int dtype, int64_t seq_stride, int64_t head_stride, int64_t token_stride);
 

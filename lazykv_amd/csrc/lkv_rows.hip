@@ -110,11 +110,69 @@ __global__ __launch_bounds__(256) void read_rows_kernel(RowPlan p, const uint8_t
   }
 }
 
-// Two rows that are written must not be one.
-int distinct_rows(const char* what, const void* k, const void* v, int n_seqs, int n_kv, int tokens, int64_t seq_stride, int64_t head_stride,
-                  int64_t token_stride) {
-  LKV_CHECK_ARG(k != v && (n_seqs == 1 || seq_stride) && (n_kv == 1 || head_stride) && (tokens == 1 || token_stride),
-                "%s: rows that are written share an address", what);
+// One dimension of a set of rows: `count` of them, `stride` apart.
+struct Dim {
+  int64_t count, stride;
+};
+
+// Whether no two of the spans of `length` that start at sums of the dimensions' multiples share an address. Strides that nest, each at least
+// what the smaller ones reach, are seen at once: slices, steps and permutations of contiguous tensors have such. Otherwise every difference of
+// two spans is tried, along the longest dimension only the multiples that come next to zero; over 65,536 tries are not made,
+// and the spans not taken for apart.
+bool rows_apart(Dim (&dims)[4], int64_t length) {
+  for (int i = 0; i < 4; ++i) {
+    if (dims[i].count < 2) dims[i] = {1, 0};
+    dims[i].stride = dims[i].stride < 0 ? -dims[i].stride : dims[i].stride;  // the same differences
+    for (int j = i; j > 0 && dims[j].stride < dims[j - 1].stride; --j) {
+      const Dim x = dims[j];
+      dims[j] = dims[j - 1];
+      dims[j - 1] = x;
+    }
+  }
+  __int128 reach = length;
+  bool nested = true;
+  for (const Dim& d : dims) {
+    if (d.count < 2) continue;
+    nested = nested && d.stride >= reach;
+    reach += (__int128)d.stride * (d.count - 1);
+  }
+  if (nested) return true;
+  int most = 0;
+  for (int i = 1; i < 4; ++i)
+    if (dims[i].count > dims[most].count) most = i;
+  __int128 tries = 1;
+  for (int i = 0; i < 4; ++i)
+    if (i != most) tries *= 2 * dims[i].count - 1;
+  const Dim along = dims[most];
+  if (tries > (1 << 16) || along.stride == 0 || along.stride < length) return false;
+  dims[most] = {1, 0};
+  for (int64_t t = 0; t < (int64_t)tries; ++t) {
+    __int128 at = 0;
+    int64_t rest = t;
+    bool same = true;
+    for (const Dim& d : dims) {
+      const int64_t by = rest % (2 * d.count - 1) - (d.count - 1);
+      rest /= 2 * d.count - 1;
+      at += (__int128)by * d.stride;
+      same = same && by == 0;
+    }
+    if (same) continue;  // along one dimension: a stride of `length` or more
+    const __int128 m = -at / along.stride;
+    for (__int128 x = m - 1; x <= m + 1; ++x) {
+      const __int128 gap = at + x * along.stride;
+      if (x > -along.count && x < along.count && gap < length && gap > -length) return false;
+    }
+  }
+  return true;
+}
+
+// Two rows that are written must not share an address. Strides and head_dim are in elements of `bytes` bytes.
+int distinct_rows(const char* what, const void* k, const void* v, int bytes, int n_seqs, int n_kv, int64_t tokens, int head_dim, int64_t seq_stride,
+                  int64_t head_stride, int64_t token_stride) {
+  const int64_t apart = (int64_t)((uintptr_t)v - (uintptr_t)k);
+  Dim dims[4] = {{2, apart}, {n_seqs, seq_stride * bytes}, {n_kv, head_stride * bytes}, {tokens, token_stride * bytes}};
+  if (token_stride == head_dim) dims[3] = {1, 0};
+  LKV_CHECK_ARG(rows_apart(dims, (token_stride == head_dim ? tokens : 1) * head_dim * bytes), "%s: rows that are written share an address", what);
   return LKV_OK;
 }
 
@@ -144,7 +202,13 @@ extern "C" int lkv_append_rows(uintptr_t stream, const lkv_kv_rows* dst, const v
   if (!starts) LKV_CHECK_ARG(start >= 0 && (int64_t)start + tokens <= dst->tokens, "rows %d..%lld exceed the %lld there are", start,
                              (long long)start + tokens, (long long)dst->tokens);
   if (p.rows == 0) return LKV_OK;
-  if (int rc = distinct_rows("dst", dst->k, dst->v, n_seqs, n_kv, tokens, dst->seq_stride, dst->head_stride, head_dim)) return rc;
+  const int es = dst->dtype == LKV_MXFP8 ? 1 : 2;
+  if (int rc = distinct_rows("dst", dst->k, dst->v, es, n_seqs, n_kv, dst->tokens, head_dim, dst->seq_stride, dst->head_stride, head_dim)) return rc;
+  if (es == 1) {
+    if (int rc = distinct_rows("dst's scales", dst->k_scale, dst->v_scale, 1, n_seqs, n_kv, dst->tokens, head_dim / kMxGroup, dst->seq_stride / kMxGroup,
+                               dst->head_stride / kMxGroup, head_dim / kMxGroup))
+      return rc;
+  }
   p.start = start;
   p.starts = starts;
   const bool mx = dst->dtype == LKV_MXFP8, half = dtype == LKV_F16, wide = head_dim == 128;
@@ -166,7 +230,7 @@ extern "C" int lkv_read_rows(uintptr_t stream, const lkv_kv_rows* src, int n_seq
   LKV_CHECK_ARG(first >= 0 && (int64_t)first + tokens <= src->tokens, "rows %d..%lld exceed the %lld there are", first,
                 (long long)first + tokens, (long long)src->tokens);
   if (p.rows == 0) return LKV_OK;
-  if (int rc = distinct_rows("out", k, v, n_seqs, n_kv, tokens, seq_stride, head_stride, token_stride)) return rc;
+  if (int rc = distinct_rows("out", k, v, 2, n_seqs, n_kv, tokens, head_dim, seq_stride, head_stride, token_stride)) return rc;
   p.start = first;
   const bool half = dtype == LKV_F16, wide = head_dim == 128;
   auto kernel = half ? (wide ? read_rows_kernel<LKV_F16, 128> : read_rows_kernel<LKV_F16, 64>)

@@ -131,3 +131,56 @@ def test_sequences_of_their_own_behind_32_bits_of_bytes() -> None:
     torch.cuda.synchronize()
     for b in range(3):
         assert bool((out[b] == 1.0 + b).all())
+
+
+def _overlap(shape: tuple, strides: tuple, apart: int, d: int) -> bool:
+    """Whether any two of the rows of d elements at these strides, of keys and of values `apart` elements on, share an element."""
+    at = np.zeros((), dtype=np.int64)
+    for n, s in zip((2, *shape), (apart, *strides)):
+        at = at[..., None] + np.arange(n) * s
+    at = np.sort(at.ravel())
+    return bool((np.diff(at) < d).any())
+
+
+@pytest.mark.parametrize("seed", range(24))
+def test_layouts_that_are_written_are_those_whose_rows_are_apart(seed: int) -> None:
+    """Random strides of one buffer, which may interleave sequences, heads, keys and values or make them overlap: the write of a cache and the
+    output of a read-back are taken where no two rows overlap, and then hold what they should, and refused otherwise."""
+    from lazykv_amd import kernels
+
+    rng = np.random.default_rng(seed)
+    taken = refused = 0
+    for _ in range(40):
+        seqs, h, n, d = int(rng.integers(1, 4)), int(rng.integers(1, 4)), int(rng.integers(1, 6)), 64
+        unit = n * d
+        ss, hs, apart = (int(x) * unit + int(rng.choice([0, 0, 0, 32, d])) for x in rng.integers(0, 13, 3))
+        buf = torch.zeros(400 * d, dtype=torch.float16, device="cuda")
+        k = torch.randn((seqs, h, n, d), device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed)).half()
+        dst = [buf.as_strided((seqs, h, n, d), (ss, hs, d, 1), off) for off in (0, apart)]
+        bad = _overlap((seqs, h, n), (ss, hs, d), apart, d)
+        if (seqs == 1 or ss % 32 == 0) and (h == 1 or hs % 32 == 0) and apart % 8 == 0:
+            if bad:
+                with pytest.raises(ValueError, match="share an address"):
+                    kernels.append_rows(kernels.dense_rows(*dst), k, -k)
+            else:
+                kernels.append_rows(kernels.dense_rows(*dst), k, -k)
+                torch.cuda.synchronize()
+                assert torch.equal(dst[0], k) and torch.equal(dst[1], -k)
+            taken, refused = taken + (not bad), refused + bad
+        # The read-back's output, with a token stride of its own.
+        ts = d * int(rng.integers(1, 4)) + int(rng.choice([0, 8]))
+        codes, scales = kernels.mx_empty(seqs, h, n, d, "cuda")
+        rows = kernels.mx_rows(codes, scales, torch.float16)
+        kernels.append_rows(rows, k, -k)
+        want = kernels.read_rows(rows, 0, n)
+        out = [buf.zero_().as_strided((seqs, h, n, d), (ss, hs, ts, 1), off) for off in (0, apart)]
+        bad = _overlap((seqs, h, n), (ss, hs, ts), apart, d)
+        if bad:
+            with pytest.raises(ValueError, match="share an address"):
+                kernels.read_rows(rows, 0, n, out=tuple(out))
+        else:
+            kernels.read_rows(rows, 0, n, out=tuple(out))
+            torch.cuda.synchronize()
+            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+        taken, refused = taken + (not bad), refused + bad
+    assert taken > 5 and refused > 5

@@ -37,3 +37,42 @@ def test_a_short_prefix_does_not_cut_long_rows_behind_it_into_small_parts(prefix
     assert _scratch(64, 32, 8, 128, prefix, own) <= 45 << 20
     if prefix <= 1021:
         assert _scratch(64, 32, 8, 128, prefix, own) <= 10 << 20
+
+
+@pytest.mark.parametrize(("fn", "change", "call"), [
+    ("append", dict(head_stride=32), {}),
+    ("append", dict(head_stride=99 * 128), {}),
+    ("append", dict(seq_stride=7 * (1 << 14) + 99 * 128), {}),
+    ("append", dict(seq_stride=3 * (1 << 14)), {}),
+    ("append", dict(head_stride=-99 * 128), {}),
+    ("append", dict(v_off=128), {}),
+    ("append", dict(v_off=-128), {}),
+    ("append", dict(v_off=5 * (1 << 14)), {}),
+    ("append", dict(v_scale_off=4), {}),
+    ("append", dict(v_scale_off=-(1 << 9)), {}),
+    ("read", {}, dict(v_off=256)),
+    ("read", {}, dict(v_off=9 * 256)),
+    ("read", {}, dict(strides=(1 << 20, 8, 128))),
+    ("read", {}, dict(strides=(1 << 20, 1 << 16, 8))),
+    ("read", {}, dict(strides=(128, 1 << 16, 128))),
+    ("read", {}, dict(strides=(1 << 20, 1 << 16, 120))),
+    ("read", {}, dict(strides=(1 << 16, 1 << 16, 128))),
+])
+def test_rows_that_overlap_are_not_written(fn: str, change: dict, call: dict) -> None:
+    """Strides and addresses that are all different and none 0: a row's end in another's, a head's last rows another's first, values in
+    the keys' place of another head."""
+    from lazykv_amd import _lib
+
+    lib = _lib.lib()
+    at = dict(k=1 << 40, v_off=1 << 30, k_scale=1 << 42, v_scale_off=1 << 30, seq_stride=8 << 14, head_stride=1 << 14)
+    at.update(change)
+    r = _lib.KVRows(at["k"], at["k"] + at["v_off"], at["k_scale"], at["k_scale"] + at["v_scale_off"], at["seq_stride"], at["head_stride"], 100, 2, _lib.MXFP8,
+                    _lib.BF16)
+    have = dict(k=1 << 41, v_off=1 << 30, strides=(1 << 20, 1 << 16, 128))
+    have.update(call)
+    if fn == "append":
+        rc = lib.lkv_append_rows(0, ctypes.byref(r), have["k"], have["k"] + have["v_off"], _lib.BF16, *have["strides"], 2, 8, 128, 10, None, 0)
+    else:
+        rc = lib.lkv_read_rows(0, ctypes.byref(r), 2, 8, 128, 0, 10, have["k"], have["k"] + have["v_off"], _lib.BF16, *have["strides"])
+    assert rc == _lib.LKV_ERR_INVALID
+    assert b"share an address" in lib.lkv_last_error()
