@@ -308,8 +308,8 @@ typedef struct lkv_kv_rows {
 /* New rows into dst (whose buffers are written): token t of sequence b, of `tokens` each, becomes row
  * start + starts[b] + t (starts, int32 on the device, may be NULL: 0); rows outside 0 .. dst->tokens-1
  * are dropped. k / v: keys and values in the model dtype, element (b, h, t, c) at
- * b * seq_stride + h * head_stride + t * token_stride + c, 16-byte aligned, strides multiples of 8.
- * LKV_MXFP8: X is the least exponent (0 at the least) with max |x| <= 448 * 2^(X - 127) over the
+ * b * seq_stride + h * head_stride + t * token_stride + c, 16-byte aligned, strides multiples of 8;
+ * rows that the call writes must not be among them. LKV_MXFP8: X is the least exponent (0 at the least) with max |x| <= 448 * 2^(X - 127) over the
  * group's finite values; the code is x * 2^(127 - X) rounded to the nearest E4M3 value, ties to even,
  * after x is limited to the largest four-bit significand of the model dtype (61440 in float16), so that
  * every finite row reads back finite; what is not finite becomes the NaN code. A model-dtype dst takes

@@ -733,6 +733,12 @@ def _placed(x: torch.Tensor) -> tuple[torch.Tensor, tuple]:
     return x, st
 
 
+def _of_storage(x: torch.Tensor, owners: tuple) -> bool:
+    """Whether `x` is a view of one of the tensors' memory."""
+    at = x.untyped_storage().data_ptr()
+    return any(t.untyped_storage().data_ptr() == at for t in owners)
+
+
 def _int32(name: str, x: int) -> None:
     """Refuses an integer that a C argument of 32 bits would cut."""
     if not -(1 << 31) <= x < 1 << 31:
@@ -751,7 +757,8 @@ def _counts(x: torch.Tensor | None, seqs: int, device: int, name: str) -> int | 
 def append_rows(dst: Rows, keys: torch.Tensor, values: torch.Tensor, *, start: int = 0, starts: torch.Tensor | None = None) -> None:
     """New tokens' keys and values `[seqs, h, T, d]` into a cache's rows (lkv_append_rows): token t of sequence b becomes row
     `start + starts[b] + t`. Without `starts` the rows must exist (ValueError); with it, rows outside the cache are dropped. An
-    8-bit cache takes them as E4M3 codes with a power-of-two scale for every 32 channels, another one as they are."""
+    8-bit cache takes them as E4M3 codes with a power-of-two scale for every 32 channels, another one as they are; they may be rows of
+    that cache itself."""
     shape, dtype, index = keys.shape, dst.model_dtype, dst.device_index
     if len(shape) != 4 or values.shape != shape or keys.dtype != dtype or values.dtype != dtype:
         raise ValueError(f"expected matching {dtype} keys/values [seqs, h, T, d], got {tuple(shape)} {keys.dtype} / {tuple(values.shape)} {values.dtype}")
@@ -770,6 +777,9 @@ def append_rows(dst: Rows, keys: torch.Tensor, values: torch.Tensor, *, start: i
         if yt != st:
             x, y = torch.stack([x, y]).unbind(0)
             st = x.stride()
+    if dst.dtype != _lib.MXFP8 and (_of_storage(x, dst.owners) or _of_storage(y, dst.owners)):
+        x, y = torch.stack([x, y]).unbind(0)  # the cache's own rows, moved: none is written before all are read
+        st = x.stride()
     rc = _launch(index, _lib.lib().lkv_append_rows, dst.ref, x.data_ptr(), y.data_ptr(), dst.model_code, st[0], st[1], st[2], seqs, n_kv, d, n, at, start)
     if rc:
         _lib.check(rc, "append_rows")

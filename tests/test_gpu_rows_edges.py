@@ -184,3 +184,20 @@ def test_layouts_that_are_written_are_those_whose_rows_are_apart(seed: int) -> N
             assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
         taken, refused = taken + (not bad), refused + bad
     assert taken > 5 and refused > 5
+
+
+@pytest.mark.parametrize("by", [1, -1, 8, 300])
+def test_a_caches_own_rows_are_moved_within_it(by: int) -> None:
+    """A block of rows to a place that overlaps it, keys and values swapped: what was read is what stood there before."""
+    from lazykv_amd import kernels
+
+    gen = torch.Generator(device="cuda").manual_seed(by + 2)
+    store = torch.randn((2, 3, 4, 4000, 64), device="cuda", generator=gen).half()
+    before = store.clone()
+    rows = kernels.dense_rows(store[0], store[1])
+    part = store[:, :, :, 500:3500]
+    kernels.append_rows(rows, part[1], part[0], start=500 + by)
+    torch.cuda.synchronize()
+    want = before.clone()
+    want[:, :, :, 500 + by : 3500 + by] = before[:, :, :, 500:3500].flip(0)
+    assert torch.equal(store, want)
