@@ -733,6 +733,17 @@ def _placed(x: torch.Tensor) -> tuple[torch.Tensor, tuple]:
     return x, st
 
 
+def _no_gradients(what: str, *tensors: torch.Tensor) -> None:
+    """Refuses tensors that autograd follows, in either mode: the calls over rows have no derivative, and leaving it out would be silent."""
+    if torch.is_grad_enabled():
+        for x in tensors:
+            if x.requires_grad:
+                raise RuntimeError(f"{what} has no gradient: call it (and a forward over its caches) under torch.no_grad() or inference_mode(), or detach "
+                                   "its inputs")
+    if _forward_level() >= 0 and any(torch.autograd.forward_ad.unpack_dual(x).tangent is not None for x in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative; its inputs carry tangents")
+
+
 def _of_storage(x: torch.Tensor, owners: tuple) -> bool:
     """Whether `x` is a view of one of the tensors' memory."""
     at = x.untyped_storage().data_ptr()
@@ -768,6 +779,7 @@ def append_rows(dst: Rows, keys: torch.Tensor, values: torch.Tensor, *, start: i
     if keys.get_device() != index or values.get_device() != index:
         raise ValueError(f"keys/values on {keys.device} / {values.device}, the cache on {dst.device}")
     _int32("start", start)
+    _no_gradients("append_rows", keys, values, *dst.owners)
     at = _counts(starts, seqs, index, "starts")
     if 0 in shape:
         return
@@ -780,6 +792,7 @@ def append_rows(dst: Rows, keys: torch.Tensor, values: torch.Tensor, *, start: i
     if dst.dtype != _lib.MXFP8 and (_of_storage(x, dst.owners) or _of_storage(y, dst.owners)):
         x, y = torch.stack([x, y]).unbind(0)  # the cache's own rows, moved: none is written before all are read
         st = x.stride()
+    torch.autograd.graph.increment_version(dst.owners)  # a graph that saved one of them sees the write, as after copy_
     rc = _launch(index, _lib.lib().lkv_append_rows, dst.ref, x.data_ptr(), y.data_ptr(), dst.model_code, st[0], st[1], st[2], seqs, n_kv, d, n, at, start)
     if rc:
         _lib.check(rc, "append_rows")
@@ -793,6 +806,7 @@ def read_rows(src: Rows, first: int, n: int, out: tuple[torch.Tensor, torch.Tens
     if first < 0 or n < 0 or first + n > src.tokens:
         raise ValueError(f"rows {first}..{first + n} exceed the {src.tokens} there are")
     shape, index = (src.seqs, src.n_kv, n, src.head_dim), src.device_index
+    _no_gradients("read_rows", *src.owners, *(out or ()))
     if out is None:
         k = torch.empty(shape, dtype=src.model_dtype, device=src.device)
         v = torch.empty_like(k)
@@ -805,6 +819,7 @@ def read_rows(src: Rows, first: int, n: int, out: tuple[torch.Tensor, torch.Tens
         st, vt = _meant(shape, k.stride()), _meant(shape, v.stride())
         if vt != st or st[3] != 1 or (st[0] | st[1] | st[2]) % 8 or (k.data_ptr() | v.data_ptr()) % 16:
             raise ValueError("out's rows must be contiguous and start on 16 bytes, both with the same strides")
+        torch.autograd.graph.increment_version(out)
     if 0 in shape:
         return out
     rc = _launch(index, _lib.lib().lkv_read_rows, src.ref, src.seqs, src.n_kv, src.head_dim, first, n, k.data_ptr(), v.data_ptr(), src.model_code, *st[:3])
@@ -833,7 +848,7 @@ def shared_decode(
     0 .. own_tokens + lengths[b] - 1 of its own in `own`, at most `max_own` of them (default: own_tokens without
     `lengths`, else all that `own` holds; a bound near the lengths divides the work better). Either may be left out: B = 1 over
     `own` alone is plain decode over an 8-bit cache. Returns (out [B, n_q, d], lse [B, n_q] float32, natural log); a sequence
-    without any rows gets zeros and -inf. Without `ws` the scratch is torch's, so calls on several streams and in several graphs
+    without any rows gets zeros and -inf. No gradient: inputs that autograd follows are refused. Without `ws` the scratch is torch's, so calls on several streams and in several graphs
     do not meet."""
     rows = own if own is not None else prefix
     if rows is None:
@@ -857,6 +872,8 @@ def shared_decode(
     if prefix is not None and (prefix.seqs != 1 or prefix.n_kv != rows.n_kv or prefix.head_dim != d or prefix.model_dtype != dtype or prefix.device_index != index):
         raise ValueError(f"a prefix of {prefix.seqs} sequences, {prefix.n_kv} heads, head_dim {prefix.head_dim}, {prefix.model_dtype} on {prefix.device} "
                          f"does not match one of {rows.n_kv}, {d}, {dtype} on {rows.device}")
+    given = [x for x in (out, lse) if x is not None]
+    _no_gradients("shared_decode", q, *(own.owners if own is not None else ()), *(prefix.owners if prefix is not None else ()), *given)
     at = _counts(lengths, b, index, "lengths")
     if (prefix_tokens | own_tokens | max_own) >> 31:
         for name, n in (("prefix_tokens", prefix_tokens), ("own_tokens", own_tokens), ("max_own", max_own)):
@@ -877,6 +894,8 @@ def shared_decode(
         raise ValueError(f"lse must be contiguous float32 [{b}, {n_q}] on {rows.device}")
     if b == 0:
         return out, lse
+    if given:
+        torch.autograd.graph.increment_version(given)
     lib = _lib.lib()
     desc = ctypes.byref(_lib.SharedDesc(b, n_q, rows.n_kv, d, scale, prefix_tokens, own_tokens, max_own))
     need = lib.lkv_shared_decode_workspace_bytes(desc)

@@ -1,0 +1,109 @@
+"""The 8-bit cache and the batch over a shared prefix at the edges of what their documentation allows, on the GPU."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def tiny():  # noqa: ANN201
+    from transformers import LlamaConfig, LlamaForCausalLM
+
+    from lazykv_amd.attention import IMPLEMENTATION_NAME, install
+
+    install()
+    torch.manual_seed(0)
+    cfg = LlamaConfig(hidden_size=256, intermediate_size=512, num_hidden_layers=3, num_attention_heads=4, num_key_value_heads=2, head_dim=64,
+                      vocab_size=512, max_position_embeddings=4096)
+    with torch.device("cuda"):
+        model = LlamaForCausalLM(cfg)
+    model.set_attn_implementation(IMPLEMENTATION_NAME)
+    return model.to(dtype=torch.float16).eval()
+
+
+def _ids(seed: int, *shape: int) -> torch.Tensor:
+    return torch.randint(0, 512, shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed))
+
+
+def _forward(model, cache, ids: torch.Tensor, **kw) -> torch.Tensor:  # noqa: ANN001, ANN003
+    with torch.inference_mode():
+        return model(input_ids=ids, past_key_values=cache, use_cache=True, **kw).logits
+
+
+def _prefilled(model, tokens: int, cap: int = 256, seed: int = 1):  # noqa: ANN001, ANN202
+    from lazykv_amd.cache import FullGPUCache
+
+    full = FullGPUCache(3, cap)
+    _forward(model, full, _ids(seed, 1, tokens))
+    return full
+
+
+def test_gradients_are_refused_not_dropped(tiny) -> None:  # noqa: ANN001
+    """Inputs, caches and outputs that autograd follows, in both modes; under no_grad, and without a gradient, the calls go on."""
+    import torch.autograd.forward_ad as fwd
+
+    from lazykv_amd import kernels
+    from lazykv_amd.cache import MXFP8Cache, SharedPrefixCache
+
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    kv = torch.randn((2, 1, 2, 5, 64), device="cuda", generator=gen).half()
+    q = torch.randn((1, 4, 64), device="cuda", generator=gen).half()
+    leaf = lambda x: x.clone().requires_grad_()  # noqa: E731
+    codes, scales = kernels.mx_empty(1, 2, 5, 64, "cuda")
+    rows = kernels.mx_rows(codes, scales, torch.float16)
+    dense = kernels.dense_rows(kv[0], kv[1])
+    followed = leaf(kv)
+    calls = [
+        lambda: kernels.append_rows(rows, leaf(kv[0]), kv[1]), lambda: kernels.append_rows(rows, kv[0], leaf(kv[1])),
+        lambda: kernels.append_rows(kernels.dense_rows(followed[0], followed[1]), kv[0], kv[1]),
+        lambda: kernels.read_rows(rows, 0, 5, out=(leaf(kv[0]), kv[1].clone())),
+        lambda: kernels.shared_decode(leaf(q), scale=0.1, own=dense, own_tokens=5),
+        lambda: kernels.shared_decode(q, scale=0.1, prefix=kernels.dense_rows(followed[0], followed[1]), prefix_tokens=5),
+        lambda: kernels.shared_decode(q, scale=0.1, own=dense, own_tokens=5, out=leaf(q)),
+    ]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call()
+        with torch.no_grad():
+            call()
+    with fwd.dual_level():
+        kernels.append_rows(rows, kv[0], kv[1])
+        with pytest.raises(RuntimeError, match="tangents"):
+            kernels.append_rows(rows, fwd.make_dual(kv[0].clone(), kv[1].clone()), kv[1])
+        with pytest.raises(RuntimeError, match="tangents"):
+            kernels.shared_decode(fwd.make_dual(q.clone(), q.clone()), scale=0.1, own=dense, own_tokens=5)
+    # A model whose weights have gradients.
+    mx = MXFP8Cache(3, 64)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        tiny(input_ids=_ids(3, 1, 9), past_key_values=mx, use_cache=True)
+    batch = SharedPrefixCache(_prefilled(tiny, 20), 2, 8)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        tiny(input_ids=_ids(3, 2, 1), past_key_values=batch, use_cache=True, **batch.model_kwargs())
+
+
+def test_writes_are_seen_by_graphs_that_saved_what_they_change() -> None:
+    """A backward pass that needs a tensor as it was fails, as after any write in place, instead of going on with other values."""
+    from lazykv_amd import kernels
+
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    w = torch.randn((1, 2, 5, 64), device="cuda", generator=gen).half().requires_grad_()
+    new = torch.ones((1, 2, 5, 64), device="cuda").half()
+    q = torch.ones((1, 4, 64), device="cuda").half()
+    store = torch.zeros((2, 1, 2, 5, 64), device="cuda").half()
+    codes, scales = kernels.mx_empty(1, 2, 5, 64, "cuda")
+    mx = kernels.mx_rows(codes, scales, torch.float16)
+    out = (torch.zeros_like(store[0]), torch.zeros_like(store[0]))
+    got, lse = torch.ones((1, 4, 64), device="cuda").half(), torch.ones((1, 4), device="cuda")
+    for saved, write in (
+        (store[0], lambda: kernels.append_rows(kernels.dense_rows(store[0], store[1]), new, new)),
+        (out[1], lambda: kernels.read_rows(mx, 0, 5, out=out)),
+        (got, lambda: kernels.shared_decode(q, scale=1.0, own=mx, own_tokens=5, out=got, lse=lse)),
+    ):
+        y = (w[:, :1, :4] * saved.view(1, -1, 4, 64)[:, :1]).sum() if saved is got else (w * saved).sum()
+        with torch.no_grad():
+            write()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
