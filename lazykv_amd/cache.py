@@ -21,6 +21,7 @@ rows of its own behind it.
 
 from __future__ import annotations
 
+import weakref
 from dataclasses import dataclass
 
 import torch
@@ -54,6 +55,15 @@ class CacheStats:
         return self.gpu_resident_kv_bytes / held if held else 1.0
 
 
+class Held:
+    """The fewest tokens that a dense layer has held since this was made (`DenseLayer.held`): rows below it are still the same."""
+
+    __slots__ = ("least", "__weakref__")
+
+    def __init__(self, least: int) -> None:
+        self.least = least
+
+
 class DenseLayer(CacheLayerMixin):
     """One layer's KV in a single preallocated slab (the reference's `PreallocatedLayer`)."""
 
@@ -64,6 +74,7 @@ class DenseLayer(CacheLayerMixin):
         self.max_len = max_len
         self.length = 0
         self.slab: torch.Tensor | None = None
+        self._held: weakref.WeakSet[Held] = weakref.WeakSet()
 
     # -- storage ----------------------------------------------------------------------------------
 
@@ -107,10 +118,18 @@ class DenseLayer(CacheLayerMixin):
         if n < 0 or n > self.length:
             raise ValueError(f"a dense layer of {self.length} tokens cannot be cut to {n}")
         self.length = n
+        for held in self._held:
+            held.least = min(held.least, n)
 
     def reset(self) -> None:
         """Forget every token; the slab is kept (only the live prefix is ever read)."""
-        self.length = 0
+        self._set_length(0)
+
+    def held(self) -> Held:
+        """From now on, which of the rows stay: what reads them later sees by it that they were cut, filled again or not."""
+        held = Held(self.length)
+        self._held.add(held)
+        return held
 
     def truncate(self, length: int) -> None:
         """Forget the tokens past `length`, so one prefill can be decoded from more than once."""
@@ -239,6 +258,7 @@ class SharedLayer(CacheLayerMixin):
         self.prefix = prefix
         self.prefix_tokens = prefix.get_seq_length()
         self.prefix_rows = prefix.rows()
+        self.prefix_held = prefix.held()
         self.n_seqs, self.max_new, self.quant = n_seqs, max_new, quant
         self.base = 0  # the longest sequence's own tokens when lengths were last set
         self.added = 0  # tokens of every sequence since then
@@ -302,7 +322,8 @@ class SharedPrefixCache(Cache):
     """A batch of `n_seqs` sequences that continue one prefilled cache, the prefix: samples of one prompt, questions about one
     document. The prefix is held once, however many sequences there are, and is not written to; each sequence has up to `max_new`
     rows of its own behind it, in the model dtype or, with `quant="mxfp8"`, in 8 bits (what the prefix is held in is its own
-    matter: a FullGPUCache or an MXFP8Cache). It must not be cut below the length it had here while the batch lives.
+    matter: a FullGPUCache or an MXFP8Cache). It may grow and be cut back, but once it was cut below the length it had here the
+    batch goes no further (RuntimeError), whatever it was filled with again.
 
     A decode forward (input_ids [n_seqs, 1], `**cache.model_kwargs()`) writes each sequence's token and attends in one call, the
     prefix's keys and values read once for all sequences (`kernels.shared_decode`). A forward of several tokens gives every
@@ -404,6 +425,7 @@ class SharedPrefixCache(Cache):
                                "library's attention function")
         if not layer.is_initialized:
             layer.lazy_initialization(key_states, value_states)
+        self._prefix_whole(layer)
         n_new = key_states.shape[-2]
         start, most = self._room(layer)
         if most + n_new > self.max_new:
@@ -412,6 +434,10 @@ class SharedPrefixCache(Cache):
         layer.added += n_new
         self._unattended = layer_idx
         return key_states, value_states
+
+    def _prefix_whole(self, layer: SharedLayer) -> None:
+        if layer.prefix_held.least < self.prefix_tokens:
+            raise RuntimeError(f"the prefix was cut to {layer.prefix_held.least} tokens; the batch was made over {self.prefix_tokens}")
 
     def get_seq_length(self, layer_idx: int = 0) -> int:
         """The longest sequence's tokens, the prefix's among them."""
@@ -428,8 +454,7 @@ class SharedPrefixCache(Cache):
         layer = self.layers[layer_idx]
         if query.shape[0] != self.n_seqs:
             raise ValueError(f"queries of {query.shape[0]} sequences, the cache holds {self.n_seqs}")
-        if layer.prefix.length < self.prefix_tokens:
-            raise RuntimeError(f"the prefix was cut to {layer.prefix.length} tokens; the batch was made over {self.prefix_tokens}")
+        self._prefix_whole(layer)
         self._unattended = None
         _, n_q, n_new, d = query.shape
         scale = scaling if scaling is not None else d**-0.5

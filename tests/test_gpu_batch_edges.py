@@ -107,3 +107,46 @@ def test_writes_are_seen_by_graphs_that_saved_what_they_change() -> None:
             write()
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             y.backward()
+
+
+@pytest.mark.parametrize("cut", ["reset", "truncate", "layer"])
+def test_a_prefix_that_was_cut_and_filled_again_is_noticed(tiny, cut: str) -> None:  # noqa: ANN001
+    """Another prompt of the same length in the prefix's place: the batch would answer about the wrong one."""
+    from lazykv_amd.cache import SharedPrefixCache
+
+    full = _prefilled(tiny, 30)
+    batch = SharedPrefixCache(full, 2, 8)
+    _forward(tiny, batch, _ids(5, 2, 1), **batch.model_kwargs())
+    if cut == "reset":
+        for layer in full.layers:
+            layer.reset()
+        _forward(tiny, full, _ids(6, 1, 30))
+    elif cut == "truncate":
+        full.truncate(29)
+        _forward(tiny, full, _ids(6, 1, 1))
+    else:
+        full.layers[2].truncate(0)
+        with torch.inference_mode():
+            full.layers[2].store(*(torch.zeros((1, 2, 30, 64), device="cuda").half() for _ in range(2)))
+    assert full.get_seq_length() == 30
+    with pytest.raises(RuntimeError, match="the prefix was cut"):
+        _forward(tiny, batch, _ids(5, 2, 1), **batch.model_kwargs())
+    fresh = SharedPrefixCache(full, 2, 8)  # a batch over what is there now
+    assert bool(_forward(tiny, fresh, _ids(5, 2, 1), **fresh.model_kwargs()).isfinite().all())
+
+
+def test_a_prefix_may_grow_and_be_cut_back(tiny) -> None:  # noqa: ANN001
+    """Tokens behind the batch's prefix come and go without a change to it, also under a second batch over more of them."""
+    from lazykv_amd.cache import SharedPrefixCache
+
+    full, ids = _prefilled(tiny, 30), _ids(7, 2, 2)
+    batch = SharedPrefixCache(full, 2, 8)
+    _forward(tiny, batch, ids[:, :1], **batch.model_kwargs())
+    want = _forward(tiny, batch, ids[:, 1:], **batch.model_kwargs())
+    batch.truncate(1)
+    _forward(tiny, full, _ids(8, 1, 5))
+    longer = SharedPrefixCache(full, 2, 8)
+    full.truncate(30)
+    assert torch.equal(_forward(tiny, batch, ids[:, 1:], **batch.model_kwargs()), want)
+    with pytest.raises(RuntimeError, match="cut to 30"):
+        _forward(tiny, longer, ids[:, :1], **longer.model_kwargs())
