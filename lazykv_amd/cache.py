@@ -262,6 +262,7 @@ class SharedLayer(CacheLayerMixin):
         self.n_seqs, self.max_new, self.quant = n_seqs, max_new, quant
         self.base = 0  # the longest sequence's own tokens when lengths were last set
         self.added = 0  # tokens of every sequence since then
+        self.attended = 0  # of these, the ones whose attention was taken: those of whole forwards, once all layers have as many
         self.own: tuple[torch.Tensor, ...] = ()  # keys, values, or codes and scales
         self.own_rows: kernels.Rows | None = None
 
@@ -353,6 +354,7 @@ class SharedPrefixCache(Cache):
         self._starts: torch.Tensor | None = None  # those on the device, where they differ
         self._scratch: tuple[torch.Tensor, torch.Tensor] | None = None
         self._unattended: int | None = None  # the layer whose new tokens `select` has not seen yet
+        self._ended, self._written = 0, 0  # tokens that every layer has since lengths were set, layers that have the current forward's
 
     # -- lengths ----------------------------------------------------------------------------------
 
@@ -397,20 +399,27 @@ class SharedPrefixCache(Cache):
     def batch_select_indices(self, indices: torch.Tensor) -> None:
         self.keep(indices)
 
+    def rollback(self) -> None:
+        """Forget the tokens of a forward that raised before its last layer's attention: every sequence has what it had before it. (A forward
+        that got further has ended here; `truncate` takes it back.)"""
+        whole = min(layer.attended for layer in self.layers)
+        self._set([n + whole for n in self._base])
+
     def reset(self) -> None:
         """Forget every sequence's own tokens; the prefix stays."""
-        self._unattended = None
         self._set([0] * self.n_seqs)
 
     def _whole(self) -> list[int]:
         if len({layer.added for layer in self.layers}) != 1:
-            raise RuntimeError("lengths are set between forwards: the layers hold different numbers of tokens")
+            raise RuntimeError("lengths are set between forwards: the layers hold different numbers of tokens; rollback() forgets those of a forward that "
+                               "did not end")
         return self.lengths()
 
     def _set(self, lengths: list[int]) -> None:
         self._base = lengths
         for layer in self.layers:
-            layer.base, layer.added = max(lengths), 0
+            layer.base, layer.added, layer.attended = max(lengths), 0, 0
+        self._ended, self._written, self._unattended = 0, 0, None
         same = len(set(lengths)) == 1
         self._starts = None if same else torch.tensor(lengths, dtype=torch.int32, device=self.layers[0].prefix_rows.device)
 
@@ -422,7 +431,9 @@ class SharedPrefixCache(Cache):
         layer = self.layers[layer_idx]
         if self._unattended is not None:
             raise RuntimeError(f"layer {self._unattended}'s attention did not come from this cache: the forward needs **cache.model_kwargs() and this "
-                               "library's attention function")
+                               "library's attention function (rollback() forgets the token it wrote)")
+        if layer.added != self._ended:
+            raise RuntimeError(f"layer {layer_idx} holds tokens of a forward that did not end; rollback() forgets them")
         if not layer.is_initialized:
             layer.lazy_initialization(key_states, value_states)
         self._prefix_whole(layer)
@@ -433,6 +444,9 @@ class SharedPrefixCache(Cache):
         kernels.append_rows(layer.own_rows, key_states, value_states, start=start, starts=self._starts)
         layer.added += n_new
         self._unattended = layer_idx
+        self._written += 1
+        if self._written == len(self.layers):
+            self._ended, self._written = layer.added, 0
         return key_states, value_states
 
     def _prefix_whole(self, layer: SharedLayer) -> None:
@@ -459,10 +473,13 @@ class SharedPrefixCache(Cache):
         _, n_q, n_new, d = query.shape
         scale = scaling if scaling is not None else d**-0.5
         if n_new > 1:
-            return self._select_many(layer, query, scale)
+            got = self._select_many(layer, query, scale)
+            layer.attended = layer.added
+            return got
         start, most = self._room(layer)
         out, lse = kernels.shared_decode(query, scale=scale, prefix=layer.prefix_rows, prefix_tokens=self.prefix_tokens, own=layer.own_rows,
                                          own_tokens=start, lengths=self._starts, max_own=most)
+        layer.attended = layer.added
         return Decoded(out.view(self.n_seqs, n_q, 1, d), lse)
 
     def _select_many(self, layer: SharedLayer, query: torch.Tensor, scale: float) -> Decoded:

@@ -150,3 +150,73 @@ def test_a_prefix_may_grow_and_be_cut_back(tiny) -> None:  # noqa: ANN001
     assert torch.equal(_forward(tiny, batch, ids[:, 1:], **batch.model_kwargs()), want)
     with pytest.raises(RuntimeError, match="cut to 30"):
         _forward(tiny, longer, ids[:, :1], **longer.model_kwargs())
+
+
+class _Stop(Exception):
+    pass
+
+
+def _stop_at(model, layer: int, after: bool):  # noqa: ANN001, ANN202
+    """A forward that raises at a layer: before its attention has begun, or after it."""
+    def hook(*args: object) -> None:
+        raise _Stop
+
+    module = model.model.layers[layer].self_attn
+    return module.register_forward_hook(hook) if after else module.register_forward_pre_hook(hook)
+
+
+@pytest.mark.parametrize("n", [1, 3])
+@pytest.mark.parametrize(("layer", "after"), [(0, False), (0, True), (1, False), (2, False), (2, True)])
+def test_a_forward_that_raised_is_rolled_back(tiny, layer: int, after: bool, n: int) -> None:  # noqa: ANN001
+    """Behind ragged lengths, one token or several; the batch then goes on as if that forward had not been. Without the rollback
+    another forward is refused where it would leave layers with tokens of both."""
+    from lazykv_amd.cache import SharedPrefixCache
+
+    batch = SharedPrefixCache(_prefilled(tiny, 25), 3, 32, quant="mxfp8")
+    _forward(tiny, batch, _ids(9, 3, 4), **batch.model_kwargs())
+    batch.truncate([4, 1, 2])
+    _forward(tiny, batch, _ids(10, 3, 1), position_ids=batch.positions(), **batch.model_kwargs())
+    call = dict(position_ids=batch.positions(n), **batch.model_kwargs())
+    want = _forward(tiny, batch, _ids(11, 3, n), **call)
+    batch.truncate([5, 2, 3])
+    hook = _stop_at(tiny, layer, after)
+    try:
+        with pytest.raises(_Stop):
+            _forward(tiny, batch, _ids(12, 3, n), **call)
+    finally:
+        hook.remove()
+    if (layer, after) not in ((0, False), (2, True)):  # nothing written yet, everything attended
+        with pytest.raises(RuntimeError, match="rollback"):
+            batch.truncate([5, 2, 3])
+        with pytest.raises(RuntimeError, match="rollback"):
+            _forward(tiny, batch, _ids(12, 3, n), **call)
+    batch.rollback()
+    if (layer, after) == (2, True):  # ended: taken back as any other
+        batch.truncate([5, 2, 3])
+    assert batch.lengths() == [5, 2, 3] and batch.get_seq_length() == 30
+    assert torch.equal(_forward(tiny, batch, _ids(11, 3, n), **call), want)
+    batch.rollback()  # of nothing
+    assert batch.lengths() == [5 + n, 2 + n, 3 + n]
+
+
+@pytest.mark.parametrize("by_length", [False, True])
+def test_a_layers_attention_that_raised_is_rolled_back(tiny, by_length: bool) -> None:  # noqa: ANN001
+    """The last layer's tokens written, its attention refused: every layer has them, and none is left after the rollback, or after
+    lengths without them are set."""
+    from lazykv_amd.cache import SharedPrefixCache
+
+    batch = SharedPrefixCache(_prefilled(tiny, 25), 2, 8)
+    kv = torch.randn((2, 2, 2, 1, 64), device="cuda").half()
+    q = torch.randn((2, 4, 1, 64), device="cuda").half()
+    for layer in range(3):
+        batch.update(kv[0], kv[1], layer)
+        if layer < 2:
+            batch.select(layer, q)
+    with pytest.raises(ValueError, match="sequences"):
+        batch.select(2, q[:1])
+    if by_length:
+        batch.truncate(0)
+    else:
+        batch.rollback()
+    assert batch.lengths() == [0, 0]
+    assert bool(_forward(tiny, batch, _ids(13, 2, 1), **batch.model_kwargs()).isfinite().all()) and batch.lengths() == [1, 1]
