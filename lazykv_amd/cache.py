@@ -368,9 +368,10 @@ class SharedPrefixCache(Cache):
         return [n + self.layers[layer_idx].added for n in self._base]
 
     def positions(self, n_new: int = 1) -> torch.Tensor:
-        """position_ids [n_seqs, n_new] of each sequence's next tokens."""
-        start = torch.tensor(self.lengths(), device=self.layers[0].prefix_rows.device) + self.prefix_tokens
-        return start[:, None] + torch.arange(n_new, device=start.device)
+        """position_ids [n_seqs, n_new] of each sequence's next tokens, made on the device: nothing is waited for."""
+        first = self.prefix_tokens + self._room(self.layers[0])[0]
+        new = torch.arange(first, first + n_new, device=self.layers[0].prefix_rows.device)
+        return new.repeat(self.n_seqs, 1) if self._starts is None else self._starts[:, None] + new
 
     def truncate(self, lengths: int | list[int]) -> None:
         """Forget each sequence's own tokens past its length (one for all, or one each), between forwards."""

@@ -220,3 +220,28 @@ def test_a_layers_attention_that_raised_is_rolled_back(tiny, by_length: bool) ->
         batch.rollback()
     assert batch.lengths() == [0, 0]
     assert bool(_forward(tiny, batch, _ids(13, 2, 1), **batch.model_kwargs()).isfinite().all()) and batch.lengths() == [1, 1]
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+def test_the_documented_loop_never_waits_for_the_device(tiny, ragged: bool) -> None:  # noqa: ANN001
+    """Whole forwards of one token, with the positions that the cache gives."""
+    from lazykv_amd.cache import SharedPrefixCache
+
+    batch = SharedPrefixCache(_prefilled(tiny, 40), 3, 16)
+    _forward(tiny, batch, _ids(14, 3, 4), position_ids=batch.positions(4), **batch.model_kwargs())
+    batch.truncate([4, 2, 3] if ragged else 3)
+    ids = _ids(15, 3, 1)
+    _forward(tiny, batch, ids, position_ids=batch.positions(), **batch.model_kwargs())
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        for _ in range(3):
+            ids = _forward(tiny, batch, ids, position_ids=batch.positions(), **batch.model_kwargs())[:, -1:].argmax(-1)
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    lengths = [8, 6, 7] if ragged else [7, 7, 7]
+    assert batch.lengths() == lengths
+    for n in (1, 5):
+        got = batch.positions(n)
+        assert got.dtype == torch.int64 and got.is_contiguous()
+        assert got.tolist() == [[40 + m + t for t in range(n)] for m in lengths]
