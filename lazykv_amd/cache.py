@@ -420,7 +420,7 @@ class SharedPrefixCache(Cache):
         self._base = lengths
         for layer in self.layers:
             layer.base, layer.added, layer.attended = max(lengths), 0, 0
-        self._ended, self._written, self._unattended = 0, 0, None
+        self._ended, self._written, self._unattended, self._scratch = 0, 0, None, None
         same = len(set(lengths)) == 1
         self._starts = None if same else torch.tensor(lengths, dtype=torch.int32, device=self.layers[0].prefix_rows.device)
 
@@ -476,6 +476,8 @@ class SharedPrefixCache(Cache):
         if n_new > 1:
             got = self._select_many(layer, query, scale)
             layer.attended = layer.added
+            if self._written == 0:  # the last layer of this forward
+                self._scratch = None
             return got
         start, most = self._room(layer)
         out, lse = kernels.shared_decode(query, scale=scale, prefix=layer.prefix_rows, prefix_tokens=self.prefix_tokens, own=layer.own_rows,
@@ -484,13 +486,15 @@ class SharedPrefixCache(Cache):
         return Decoded(out.view(self.n_seqs, n_q, 1, d), lse)
 
     def _select_many(self, layer: SharedLayer, query: torch.Tensor, scale: float) -> Decoded:
-        """Several tokens of each sequence: the prefix into one dense buffer, then each sequence's rows behind it in turn."""
+        """Several tokens of each sequence: the prefix into one dense buffer in the model dtype, which the layers of a forward share, then each
+        sequence's rows behind it in turn. The buffer goes with the forward."""
         from lazykv_amd.attention import attend
 
         p, r = self.prefix_tokens, layer.prefix_rows
         lengths = [n + layer.added for n in self._base]
         total = p + max(lengths)
-        if self._scratch is None or self._scratch[0].shape[1] != r.n_kv or self._scratch[0].shape[2] < total:
+        kept = self._scratch[0] if self._scratch is not None else None
+        if kept is None or kept.shape[1] != r.n_kv or kept.shape[2] < total or kept.shape[3] != r.head_dim or kept.dtype != r.model_dtype or kept.device != r.device:
             shape = (1, r.n_kv, -(-total // 256) * 256, r.head_dim)
             self._scratch = (torch.empty(shape, dtype=r.model_dtype, device=r.device), torch.empty(shape, dtype=r.model_dtype, device=r.device))
         k, v = self._scratch
@@ -508,9 +512,10 @@ class SharedPrefixCache(Cache):
         return Decoded(torch.cat(outs), torch.empty(0, device=r.device))
 
     def stats(self) -> CacheStats:
-        """The prefix's bytes, once, and the sequences' own."""
+        """The prefix's bytes, once, and the sequences' own; allocated, also a buffer that a forward of several tokens holds until it ends."""
         p = self.full.stats()
         own = sum(layer.own_bytes() for layer in self.layers)
         used = own * sum(self.lengths()) // (self.n_seqs * self.max_new)
+        own += sum(x.numel() * x.element_size() for x in self._scratch or ())
         return CacheStats(seq_len=self.get_seq_length(), gpu_resident_kv_bytes=p.gpu_resident_kv_bytes + used, host_kv_bytes=0,
                           gpu_allocated_kv_bytes=p.gpu_allocated_kv_bytes + own)

@@ -245,3 +245,56 @@ def test_the_documented_loop_never_waits_for_the_device(tiny, ragged: bool) -> N
         got = batch.positions(n)
         assert got.dtype == torch.int64 and got.is_contiguous()
         assert got.tolist() == [[40 + m + t for t in range(n)] for m in lengths]
+
+
+def test_a_forward_of_several_tokens_leaves_no_buffer(tiny) -> None:  # noqa: ANN001
+    """The prefix's copy in the model dtype is counted while a forward holds it, and goes with its last layer, or with a rollback."""
+    from lazykv_amd.cache import SharedPrefixCache
+
+    batch = SharedPrefixCache(_prefilled(tiny, 200), 2, 32)
+    call = dict(position_ids=batch.positions(3), **batch.model_kwargs())
+    own = 3 * 2 * 2 * 2 * 32 * 64 * 2  # layers, keys and values, sequences, heads, tokens, channels, bytes
+    full = batch.full.stats().gpu_allocated_kv_bytes
+    seen = []
+    hook = tiny.model.layers[0].register_forward_hook(lambda *a: seen.append(batch.stats().gpu_allocated_kv_bytes))
+    try:
+        _forward(tiny, batch, _ids(16, 2, 3), **call)
+        assert seen == [full + own // 3 + 2 * 2 * 256 * 64 * 2]  # the other layers hold nothing yet
+        assert batch.stats().gpu_allocated_kv_bytes == full + own
+    finally:
+        hook.remove()
+    hook = _stop_at(tiny, 1, True)
+    try:
+        with pytest.raises(_Stop):
+            _forward(tiny, batch, _ids(16, 2, 3), **call)
+    finally:
+        hook.remove()
+    assert batch.stats().gpu_allocated_kv_bytes > full + own
+    batch.rollback()
+    assert batch.stats().gpu_allocated_kv_bytes == full + own
+
+
+def test_layers_of_different_shapes_share_no_buffer() -> None:
+    """Layers whose head_dim, dtype or heads differ, each against its tokens in 64 bits: softmax weights of 3 + 2 (causal) rows; float16 /
+    bfloat16 outputs of torch's attention, within 4 half steps of the largest value."""
+    from lazykv_amd.cache import FullGPUCache, SharedPrefixCache
+
+    gen = torch.Generator(device="cuda").manual_seed(17)
+    shapes = [(2, 64, torch.float16), (2, 128, torch.float16), (2, 128, torch.bfloat16), (1, 128, torch.bfloat16), (2, 64, torch.float16)]
+    full = FullGPUCache(len(shapes), 16)
+    made = []
+    for layer, (h, d, t) in zip(full.layers, shapes):
+        kv = torch.randn((2, 1, h, 3, d), device="cuda", generator=gen).to(t)
+        layer.store(kv[0], kv[1])
+        made.append((kv, torch.randn((2, 2, h, 2, d), device="cuda", generator=gen).to(t), torch.randn((2, 2 * h, 2, d), device="cuda", generator=gen).to(t)))
+    batch = SharedPrefixCache(full, 2, 8)
+    for i, (kv, new, q) in enumerate(made):
+        batch.update(new[0], new[1], i)
+        got = batch.select(i, q).out.double().cpu().view(q.shape)
+        for b in range(2):
+            for j in range(q.shape[1]):
+                k, v = (torch.cat([kv[w, 0, j // 2], new[w, b, j // 2]]).double().cpu() for w in range(2))
+                for t in range(2):
+                    p = torch.softmax(k[: 4 + t] @ q[b, j, t].double().cpu() * q.shape[3] ** -0.5, 0)
+                    tol = 4 * torch.finfo(q.dtype).eps / 2 * float(v.abs().max())
+                    assert float((got[b, j, t] - p @ v[: 4 + t]).abs().max()) <= tol, (i, b, j, t)
