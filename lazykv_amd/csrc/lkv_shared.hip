@@ -915,6 +915,10 @@ Plan plan_of(const lkv_shared_desc* d) {
   Plan p = {};
   const int g = d->n_q / d->n_kv;
   const int64_t rows = (int64_t)d->n_seqs * g;
+  // Rows of a KV head to a form. Up to 32 on streams of the waves' own: 32 rows over 131,072 tokens (d 128, 8 bits / 16; 8 KV heads here
+  // and below) take 54 / 96 us, in LDS by eight waves 67 / 97; 40 rows 79 / 110 against 67 / 97. Up to 64 by eight waves: 64 rows take 75 / 107,
+  // by four 86 / 105; 80 rows 106 / 133 against 88 / 107. Over 32,768 tokens the order is the same but for 64 rows of 8 bits (26.8 in LDS, 24.6 as
+  // streams); up to 4,099 all are within 1 us.
   p.nr = d->prefix_tokens == 0 || rows <= 16 ? 1 : (rows <= 32 ? 2 : 0);
   p.waves = p.nr || rows > 64 ? 4 : 8;
   p.wr = p.waves == 8 ? 2 : 4;
@@ -927,12 +931,18 @@ Plan plan_of(const lkv_shared_desc* d) {
   if (p.nr) {
     tokens += items * d->max_own;
   } else {
-    // Own rows, two items a workgroup, beside the prefix's where that is bound by memory (16 sequences over 32K tokens with 200
-    // of their own: 43.3 us behind them, 39.7 beside) and not by the products (32 over 128K: 102 behind, 149 beside).
+    // Own rows, two items a workgroup, beside the prefix's where that is bound by memory and not by the products (32 sequences over 128K
+    // tokens: 102 us behind them, 149 beside). 12 sequences over 32,768 tokens with room for 50, 384, 1,024 and 3,000 of their own: 31.8,
+    // 41.1, 56.3 and 61.1 behind, 29.6, 32.5, 37.8 and 62.6 beside; over 131,072: 99, 107, 120 and 124 against 102, 103, 104 and 113.
     const int64_t beside = (items + 1) / 2;
     if (d->max_own > 0 && d->max_own <= 1024 && p.waves == 8 && beside <= cus / 4) room -= beside;
-    // Two workgroups of four waves a CU, where their parts stay long beside what a part costs to store and join.
-    if (p.waves == 4 && tokens >= 1024 * 2 * cus) room = 2 * cus;
+    // Two workgroups of four waves a CU, where their parts stay long beside what a part costs to store and join: of 512 tokens, or of 1,024
+    // for one tile of 128 rows of d 128, whose 16-bit form is bound by memory. One workgroup / two, us, at parts of 256 (with two), 512 and 1,024:
+    // two tiles, d 128, 16 bits 26.6/28.7, 37.6/36.5, 64.0/56.2, 8 bits 29.4/31.6, 38.7/36.8, 62.8/54.3; one tile, d 64, 8 bits 22.2/24.0, 28.6/28.0,
+    // 44.9/40.0; one tile, d 128, 16 bits 25.9/29.6, 39.8/42.3, 64.1/68.5, 8 bits 26.5/29.4, 37.9/36.9, 64.2/56.6 (the call does not tell
+    // the two apart here: scratch is asked for without the rows).
+    const int64_t enough = p.row_tiles == 1 && d->head_dim == 128 ? 1024 : 512;
+    if (p.waves == 4 && tokens >= enough * 2 * cus) room = 2 * cus;
     least = 256;
   }
   int64_t chunk = (tokens + room - 1) / room;
