@@ -621,7 +621,10 @@ _PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 def _forward_level() -> int:
     """The level of forward-mode differentiation, whose tangents a launch would leave behind; negative outside of any."""
-    return getattr(torch.autograd.forward_ad, "_current_level", 0)
+    return getattr(_FORWARD_AD, "_current_level", 0)
+
+
+_FORWARD_AD = torch.autograd.forward_ad
 
 
 # -- rows of dense caches: 8 bits as tokens arrive, and a batch over a shared prefix ---------------------
@@ -634,13 +637,15 @@ class Rows:
     """A `lkv_kv_rows`: the keys' and values' rows of `seqs` sequences, one per token, in the model dtype or in 8 bits
     (`dense_rows`, `mx_rows`). It describes the tensors it was made of and keeps them; a program may keep it."""
 
-    __slots__ = ("seqs", "n_kv", "tokens", "head_dim", "dtype", "model_dtype", "model_code", "device_index", "owners", "struct", "ref")
+    __slots__ = ("seqs", "n_kv", "tokens", "head_dim", "dtype", "model_dtype", "model_code", "device_index", "owners", "span", "struct", "ref")
 
     def __init__(self, k: int, v: int, k_scale: int | None, v_scale: int | None, strides: tuple, seqs: int, n_kv: int, tokens: int, head_dim: int,
                  dtype: int, model_dtype: torch.dtype, model_code: int, device_index: int, owners: tuple) -> None:
         self.seqs, self.n_kv, self.tokens, self.head_dim = seqs, n_kv, tokens, head_dim
         self.dtype = dtype  # _lib.F16, _lib.BF16 or _lib.MXFP8
         self.model_dtype, self.model_code, self.device_index, self.owners = model_dtype, model_code, device_index, owners
+        # Where model-dtype rows lie: the first addresses, and the bytes that they reach.
+        self.span = (k, v, 2 * ((seqs - 1) * strides[0] + (n_kv - 1) * strides[1] + tokens * head_dim)) if k_scale is None else None
         self.struct = _lib.KVRows(k, v, k_scale, v_scale, *strides, tokens, seqs, dtype, model_code)
         self.ref = ctypes.byref(self.struct)
 
@@ -733,21 +738,19 @@ def _placed(x: torch.Tensor) -> tuple[torch.Tensor, tuple]:
     return x, st
 
 
-def _no_gradients(what: str, *tensors: torch.Tensor) -> None:
+def _no_gradients(what: str, tensors: tuple) -> None:
     """Refuses tensors that autograd follows, in either mode: the calls over rows have no derivative, and leaving it out would be silent."""
-    if torch.is_grad_enabled():
+    if _GRAD_ENABLED():
         for x in tensors:
             if x.requires_grad:
                 raise RuntimeError(f"{what} has no gradient: call it (and a forward over its caches) under torch.no_grad() or inference_mode(), or detach "
                                    "its inputs")
-    if _forward_level() >= 0 and any(torch.autograd.forward_ad.unpack_dual(x).tangent is not None for x in tensors):
+    if _forward_level() >= 0 and any(_FORWARD_AD.unpack_dual(x).tangent is not None for x in tensors):
         raise RuntimeError(f"{what} has no forward-mode derivative; its inputs carry tangents")
 
 
-def _of_storage(x: torch.Tensor, owners: tuple) -> bool:
-    """Whether `x` is a view of one of the tensors' memory."""
-    at = x.untyped_storage().data_ptr()
-    return any(t.untyped_storage().data_ptr() == at for t in owners)
+_GRAD_ENABLED = torch.is_grad_enabled
+_WRITTEN = getattr(torch._C, "_increment_version", torch.autograd.graph.increment_version)  # a graph that saved one of them sees the write, as after copy_
 
 
 def _int32(name: str, x: int) -> None:
@@ -779,21 +782,27 @@ def append_rows(dst: Rows, keys: torch.Tensor, values: torch.Tensor, *, start: i
     if keys.get_device() != index or values.get_device() != index:
         raise ValueError(f"keys/values on {keys.device} / {values.device}, the cache on {dst.device}")
     _int32("start", start)
-    _no_gradients("append_rows", keys, values, *dst.owners)
+    _no_gradients("append_rows", (keys, values, *dst.owners))
     at = _counts(starts, seqs, index, "starts")
     if 0 in shape:
         return
     x, y, st = keys, values, keys.stride()
-    if values.stride() != st or st[3] != 1 or (st[0] | st[1] | st[2]) % 8 or (x.data_ptr() | y.data_ptr()) % 16:
+    at_x, at_y = x.data_ptr(), y.data_ptr()
+    if values.stride() != st or st[3] != 1 or (st[0] | st[1] | st[2]) % 8 or (at_x | at_y) % 16:
         (x, st), (y, yt) = _placed(x), _placed(y)
         if yt != st:
             x, y = torch.stack([x, y]).unbind(0)
             st = x.stride()
-    if dst.dtype != _lib.MXFP8 and (_of_storage(x, dst.owners) or _of_storage(y, dst.owners)):
-        x, y = torch.stack([x, y]).unbind(0)  # the cache's own rows, moved: none is written before all are read
-        st = x.stride()
-    torch.autograd.graph.increment_version(dst.owners)  # a graph that saved one of them sees the write, as after copy_
-    rc = _launch(index, _lib.lib().lkv_append_rows, dst.ref, x.data_ptr(), y.data_ptr(), dst.model_code, st[0], st[1], st[2], seqs, n_kv, d, n, at, start)
+        at_x, at_y = x.data_ptr(), y.data_ptr()
+    if dst.span is not None:
+        k, v, span = dst.span
+        n_bytes = 2 * ((seqs - 1) * st[0] + (n_kv - 1) * st[1] + (n - 1) * st[2] + d)
+        if min(at_x, at_y) < max(k, v) + span and max(at_x, at_y) + n_bytes > min(k, v) and any(
+                a < b + span and b < a + n_bytes for a in (at_x, at_y) for b in (k, v)):
+            x, y = torch.stack([x, y]).unbind(0)  # the cache's own rows, moved: none is written before all are read
+            st, at_x, at_y = x.stride(), x.data_ptr(), y.data_ptr()
+    _WRITTEN(dst.owners)
+    rc = _launch(index, _lib.lib().lkv_append_rows, dst.ref, at_x, at_y, dst.model_code, st[0], st[1], st[2], seqs, n_kv, d, n, at, start)
     if rc:
         _lib.check(rc, "append_rows")
 
@@ -806,7 +815,7 @@ def read_rows(src: Rows, first: int, n: int, out: tuple[torch.Tensor, torch.Tens
     if first < 0 or n < 0 or first + n > src.tokens:
         raise ValueError(f"rows {first}..{first + n} exceed the {src.tokens} there are")
     shape, index = (src.seqs, src.n_kv, n, src.head_dim), src.device_index
-    _no_gradients("read_rows", *src.owners, *(out or ()))
+    _no_gradients("read_rows", src.owners if out is None else (*src.owners, *out))
     if out is None:
         k = torch.empty(shape, dtype=src.model_dtype, device=src.device)
         v = torch.empty_like(k)
@@ -819,7 +828,7 @@ def read_rows(src: Rows, first: int, n: int, out: tuple[torch.Tensor, torch.Tens
         st, vt = _meant(shape, k.stride()), _meant(shape, v.stride())
         if vt != st or st[3] != 1 or (st[0] | st[1] | st[2]) % 8 or (k.data_ptr() | v.data_ptr()) % 16:
             raise ValueError("out's rows must be contiguous and start on 16 bytes, both with the same strides")
-        torch.autograd.graph.increment_version(out)
+        _WRITTEN(out)
     if 0 in shape:
         return out
     rc = _launch(index, _lib.lib().lkv_read_rows, src.ref, src.seqs, src.n_kv, src.head_dim, first, n, k.data_ptr(), v.data_ptr(), src.model_code, *st[:3])
@@ -872,8 +881,8 @@ def shared_decode(
     if prefix is not None and (prefix.seqs != 1 or prefix.n_kv != rows.n_kv or prefix.head_dim != d or prefix.model_dtype != dtype or prefix.device_index != index):
         raise ValueError(f"a prefix of {prefix.seqs} sequences, {prefix.n_kv} heads, head_dim {prefix.head_dim}, {prefix.model_dtype} on {prefix.device} "
                          f"does not match one of {rows.n_kv}, {d}, {dtype} on {rows.device}")
-    given = [x for x in (out, lse) if x is not None]
-    _no_gradients("shared_decode", q, *(own.owners if own is not None else ()), *(prefix.owners if prefix is not None else ()), *given)
+    given = () if out is None and lse is None else tuple(x for x in (out, lse) if x is not None)
+    _no_gradients("shared_decode", (q, *rows.owners, *(prefix.owners if prefix is not None else ()), *given))
     at = _counts(lengths, b, index, "lengths")
     if (prefix_tokens | own_tokens | max_own) >> 31:
         for name, n in (("prefix_tokens", prefix_tokens), ("own_tokens", own_tokens), ("max_own", max_own)):
@@ -895,7 +904,7 @@ def shared_decode(
     if b == 0:
         return out, lse
     if given:
-        torch.autograd.graph.increment_version(given)
+        _WRITTEN(given)
     lib = _lib.lib()
     desc = ctypes.byref(_lib.SharedDesc(b, n_q, rows.n_kv, d, scale, prefix_tokens, own_tokens, max_own))
     need = lib.lkv_shared_decode_workspace_bytes(desc)
