@@ -21,7 +21,7 @@ rows of its own behind it.
 
 from __future__ import annotations
 
-import weakref
+from bisect import bisect_left
 from dataclasses import dataclass
 
 import torch
@@ -55,15 +55,6 @@ class CacheStats:
         return self.gpu_resident_kv_bytes / held if held else 1.0
 
 
-class Held:
-    """The fewest tokens that a dense layer has held since this was made (`DenseLayer.held`): rows below it are still the same."""
-
-    __slots__ = ("least", "__weakref__")
-
-    def __init__(self, least: int) -> None:
-        self.least = least
-
-
 class DenseLayer(CacheLayerMixin):
     """One layer's KV in a single preallocated slab (the reference's `PreallocatedLayer`)."""
 
@@ -74,7 +65,8 @@ class DenseLayer(CacheLayerMixin):
         self.max_len = max_len
         self.length = 0
         self.slab: torch.Tensor | None = None
-        self._held: weakref.WeakSet[Held] = weakref.WeakSet()
+        self.cuts = 0  # how often tokens were forgotten
+        self._least: list[tuple[int, int]] = []  # (number of the cut, tokens left) of those that no later one went below
 
     # -- storage ----------------------------------------------------------------------------------
 
@@ -118,18 +110,20 @@ class DenseLayer(CacheLayerMixin):
         if n < 0 or n > self.length:
             raise ValueError(f"a dense layer of {self.length} tokens cannot be cut to {n}")
         self.length = n
-        for held in self._held:
-            held.least = min(held.least, n)
+        while self._least and self._least[-1][1] >= n:
+            self._least.pop()
+        self._least.append((self.cuts, n))
+        self.cuts += 1
 
     def reset(self) -> None:
         """Forget every token; the slab is kept (only the live prefix is ever read)."""
         self._set_length(0)
 
-    def held(self) -> Held:
-        """From now on, which of the rows stay: what reads them later sees by it that they were cut, filled again or not."""
-        held = Held(self.length)
-        self._held.add(held)
-        return held
+    def least_since(self, cuts: int) -> int:
+        """The fewest tokens that a cut has left since `cuts` was this many (what there is now, without one): of the rows there were then, those
+        below are the same, those from there on may have been filled again."""
+        i = bisect_left(self._least, (cuts, -1))
+        return self._least[i][1] if i < len(self._least) else self.length
 
     def truncate(self, length: int) -> None:
         """Forget the tokens past `length`, so one prefill can be decoded from more than once."""
@@ -258,7 +252,7 @@ class SharedLayer(CacheLayerMixin):
         self.prefix = prefix
         self.prefix_tokens = prefix.get_seq_length()
         self.prefix_rows = prefix.rows()
-        self.prefix_held = prefix.held()
+        self.prefix_cuts = prefix.cuts
         self.n_seqs, self.max_new, self.quant = n_seqs, max_new, quant
         self.base = 0  # the longest sequence's own tokens when lengths were last set
         self.added = 0  # tokens of every sequence since then
@@ -451,8 +445,11 @@ class SharedPrefixCache(Cache):
         return key_states, value_states
 
     def _prefix_whole(self, layer: SharedLayer) -> None:
-        if layer.prefix_held.least < self.prefix_tokens:
-            raise RuntimeError(f"the prefix was cut to {layer.prefix_held.least} tokens; the batch was made over {self.prefix_tokens}")
+        if layer.prefix.cuts == layer.prefix_cuts:
+            return
+        least = layer.prefix.least_since(layer.prefix_cuts)
+        if least < self.prefix_tokens:
+            raise RuntimeError(f"the prefix was cut to {least} tokens; the batch was made over {self.prefix_tokens}")
 
     def get_seq_length(self, layer_idx: int = 0) -> int:
         """The longest sequence's tokens, the prefix's among them."""
