@@ -25,7 +25,7 @@
 // Three forms, by the rows that share a KV head's prefix (sequences times group):
 //  - up to 16 or 32: a wave reads its own tokens from memory to registers; the workgroup's four waves, then the parts,
 //    join. Bound by memory: one sequence over 131,072 tokens of 8 KV heads, d 128, takes 52.4 us in 8 bits (277 MB, 5.3 TB/s) and
-//    95.8 in bfloat16 (537 MB, 5.6 TB/s), of which the join is 5. (64 rows a wave, one wave a SIMD: 16 sequences over
+//    93.5 in bfloat16 (537 MB, 5.7 TB/s), of which the join is 5. (64 rows a wave, one wave a SIMD: 16 sequences over
 //    32,768 bfloat16 tokens 32.4 us where the next form takes 29.7, launches left out.)
 //  - up to 64: through LDS, eight waves; 16 sequences over 32,768 bfloat16 tokens 35 us (134 MB; 6.1 TB/s in the loop, 5 us
 //    before it, 3 after it and 5 for the join).
