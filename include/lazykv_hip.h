@@ -309,13 +309,14 @@ typedef struct lkv_kv_rows {
  * start + starts[b] + t (starts, int32 on the device, may be NULL: 0); rows outside 0 .. dst->tokens-1
  * are dropped. k / v: keys and values in the model dtype, element (b, h, t, c) at
  * b * seq_stride + h * head_stride + t * token_stride + c, 16-byte aligned, strides multiples of 8;
- * rows that the call writes must not be among them. LKV_MXFP8: X is the least exponent (0 at the least) with max |x| <= 448 * 2^(X - 127) over the
- * group's finite values; the code is x * 2^(127 - X) rounded to the nearest E4M3 value, ties to even,
- * after x is limited to the largest four-bit significand of the model dtype (61440 in float16), so that
- * every finite row reads back finite; what is not finite becomes the NaN code. A model-dtype dst takes
- * the values as they are. A dst of which two rows (or scales) overlap, of any sequences and heads, keys and values, is
- * refused; so is a layout of more than 65,536 combinations whose strides do not nest (each at least what the
- * smaller ones reach), of which that cannot be told. */
+ * rows that the call writes must not be among them. LKV_MXFP8: X is the least exponent (0 at the least)
+ * with max |x| <= 448 * 2^(X - 127) over the group's finite values; the code is x * 2^(127 - X) rounded
+ * to the nearest E4M3 value, ties to even, after x is limited to the largest four-bit significand of the
+ * model dtype (61440 in float16), so that every finite row reads back finite; what is not finite becomes
+ * the NaN code. A model-dtype dst takes the values as they are. A dst of which two rows (or scales)
+ * overlap, of any sequences and heads, keys and values, is refused; so is a layout of more than 65,536
+ * combinations whose strides do not nest (each at least what the smaller ones reach), of which that
+ * cannot be told. */
 int lkv_append_rows(uintptr_t stream, const lkv_kv_rows* dst, const void* k, const void* v, int dtype, int64_t seq_stride,
                     int64_t head_stride, int64_t token_stride, int n_seqs, int n_kv, int head_dim, int tokens,
                     const int32_t* starts, int start);
