@@ -351,6 +351,83 @@ int lkv_shared_decode(uintptr_t stream, const lkv_shared_desc* desc, const void*
                       const lkv_kv_rows* own, const int32_t* lengths, void* out, int out_dtype, float* lse, void* ws,
                       size_t ws_bytes);
 
+/* ---- a layer's forward of several tokens over a bounded cache in pages: keys and queries normalised and rotated
+ * on their way (lkv_rotate_append), a chunk of new tokens attended (lkv_chunk_attend), the weights that rows get
+ * summed up (lkv_weigh_rows), rows over a budget evicted by them (lkv_evict_rows). No counterpart in the reference, whose
+ * forwards of several tokens go to torch (lazykv/attention.py:97-136) and whose dense store keeps every row.
+ *
+ * Where a call takes pages, `rows` is a pool: its sequences are pages of rows->tokens tokens (a multiple of 16, at most 16384),
+ * and row i of sequence b is row i % tokens of page table[b * seq_stride + i / tokens] (int32 on the device). An entry that is no
+ * page of the pool (negative, or rows->seqs or more) stands for rows that are not there: not attended, not written. A page may
+ * be in several tables where it is only read. pages == NULL: the sequences' rows one after the other, as lkv_kv_rows says. */
+typedef struct lkv_pages {
+  const int32_t* table;
+  int64_t seq_stride;
+  int64_t n_pages; /* of a sequence */
+} lkv_pages;
+
+/* New tokens' queries, keys and values [n_seqs, heads, tokens, head_dim] (element (b, h, t, c) at b * seq_stride + h *
+ * head_stride + t * token_stride + c; 16-byte aligned, strides multiples of 8): queries and keys normalised over each head
+ * (y = x / sqrt(mean x^2 + eps) * weight, where weights [head_dim] are given), their first `rotary` channels rotated (channel i < rotary / 2 to
+ * y_i cos_i - y_(i + rotary / 2) sin_i, i + rotary / 2 to y_(i + rotary / 2) cos_(i + rotary / 2) + y_i sin_(i + rotary / 2); cos and sin
+ * [n_seqs or 1, tokens, rotary] at b * table_seq_stride + t * rotary), in float32 and rounded to the model dtype once. Queries go to
+ * q_out (strides of its own), keys and values to rows start + starts[b] + t of `dst` as in lkv_append_rows; tokens from counts[b] on
+ * go to no row (counts NULL: all go). Of two tokens that go to one row (a page in two tables) either may be what it holds. */
+typedef struct lkv_rotate_desc {
+  int32_t n_seqs, n_q, n_kv, head_dim, tokens;
+  int32_t dtype;        /* of q, k, v, q_out */
+  int32_t rotary;       /* 0, or a multiple of 16 up to head_dim */
+  int32_t table_dtype;  /* of cos and sin: dtype or LKV_F32 */
+  int32_t weight_dtype; /* of the weights: dtype or LKV_F32 */
+  float eps;
+  int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3]; /* sequence, head, token */
+  int64_t table_seq_stride;                                     /* 0: one table for all */
+} lkv_rotate_desc;
+int lkv_rotate_append(uintptr_t stream, const lkv_rotate_desc* desc, const void* q, const void* k, const void* v, const void* cos, const void* sin,
+                      const void* q_weight, const void* k_weight, void* q_out, const lkv_kv_rows* dst, const lkv_pages* pages,
+                      const int32_t* starts, int start, const int32_t* counts);
+
+/* A chunk of new tokens of each sequence over its rows: sequence b has len = tokens + lengths[b] rows (lengths NULL: 0; limited to
+ * 0 .. max_tokens), the last n = counts[b] (counts NULL: new_tokens; limited to 0 .. new_tokens) of them the call's own. Its token t
+ * attends rows 0 .. len - n + t. q [n_seqs, n_q, new_tokens, head_dim] with strides; out [n_seqs, n_q, new_tokens, head_dim] (out_dtype) and
+ * lse [n_seqs, n_q, new_tokens] (float32, natural log) contiguous. Tokens from n on and tokens without any row get zeros and -inf. What rows hold that a token
+ * does not attend does not reach it, NaN or not. The launch depends on max_tokens and new_tokens, not on what is on the device. */
+typedef struct lkv_chunk_desc {
+  int32_t n_seqs, n_q, n_kv, head_dim, new_tokens;
+  float scale; /* positive */
+  int32_t tokens, max_tokens;
+  int64_t q_stride[3]; /* sequence, head, token */
+} lkv_chunk_desc;
+size_t lkv_chunk_attend_workspace_bytes(const lkv_chunk_desc* desc);
+int lkv_chunk_attend(uintptr_t stream, const lkv_chunk_desc* desc, const void* q, int q_dtype, const lkv_kv_rows* rows, const lkv_pages* pages,
+                     const int32_t* lengths, const int32_t* counts, void* out, int out_dtype, float* lse, void* ws, size_t ws_bytes);
+
+/* The weights that rows get from a chunk's tokens, summed up: with lse [n_seqs, n_q, new_tokens] as lkv_chunk_attend gives it, row i of KV
+ * head h of sequence b gets  sum over the head's query heads and the tokens that attend i of  exp(scale q . k_i - lse), added
+ * to sums for rows from before the chunk and by itself for the chunk's own, into out; a token whose lse is -inf adds nothing. sums (NULL: 0) and
+ * out are float32, element (b, h, i) at b * sums_stride[0] + h * sums_stride[1] + i; they may be the same; rows from len on are left as they are.
+ * positions (int32, laid out the same; may be NULL) of the chunk's own rows are set to seen[b] + their place in it (seen NULL:
+ * len - n, the rows before). */
+int lkv_weigh_rows(uintptr_t stream, const lkv_chunk_desc* desc, const void* q, int q_dtype, const float* lse, const lkv_kv_rows* rows, const lkv_pages* pages,
+                   const int32_t* lengths, const int32_t* counts, const float* sums, const int64_t* sums_stride, float* out, const int64_t* out_stride,
+                   int32_t* positions, const int64_t* positions_stride, const int32_t* seen, void* ws, size_t ws_bytes);
+size_t lkv_weigh_rows_workspace_bytes(const lkv_chunk_desc* desc);
+
+/* Of each sequence's len rows (as above) every KV head keeps `keep`: rows whose position is below `sinks` or among the `recent` that end with the
+ * head's largest, then those with the largest sums, ties to the lowest row, NaN after all others. A kept row behind row keep - 1 moves to a row before
+ * it that is not kept, the first to the first: keys and values, their sums and positions into sums_out and positions_out (laid out as
+ * the inputs, may be them; rows that stay are copied there where they differ). Rows from keep on are left as they are: min(len, keep) are
+ * the sequence's now. A page that the call moves rows of or to must be in one place of one table. */
+typedef struct lkv_evict_desc {
+  int32_t n_seqs, n_kv, head_dim, dtype; /* the rows' model dtype */
+  int32_t keep, sinks, recent;
+  int32_t tokens, max_tokens;
+} lkv_evict_desc;
+size_t lkv_evict_rows_workspace_bytes(const lkv_evict_desc* desc);
+int lkv_evict_rows(uintptr_t stream, const lkv_evict_desc* desc, const lkv_kv_rows* rows, const lkv_pages* pages, const int32_t* lengths, const float* sums,
+                   const int64_t* sums_stride, const int32_t* positions, const int64_t* positions_stride, float* sums_out, const int64_t* sums_out_stride,
+                   int32_t* positions_out, const int64_t* positions_out_stride, void* ws, size_t ws_bytes);
+
 /* ---- measurement: a streaming read of `bytes` at `src` (HBM or mapped host memory), the
  * device-side probe of the link asymptote that the byte roofline uses; no reference
  * counterpart (the reference quotes a probe figure at configs/phase23.yaml:13). Writes one

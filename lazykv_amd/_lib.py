@@ -148,6 +148,73 @@ class SharedDesc(ctypes.Structure):
     ]
 
 
+class Pages(ctypes.Structure):
+    """lkv_pages: which pages of a pool hold each sequence's rows (see include/lazykv_hip.h)."""
+
+    _fields_ = [
+        ("table", ctypes.c_void_p),
+        ("seq_stride", ctypes.c_int64),
+        ("n_pages", ctypes.c_int64),
+    ]
+
+
+class RotateDesc(ctypes.Structure):
+    """lkv_rotate_desc: shapes, types and strides of new tokens on their way into a cache."""
+
+    _fields_ = [
+        ("n_seqs", ctypes.c_int32),
+        ("n_q", ctypes.c_int32),
+        ("n_kv", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("tokens", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("rotary", ctypes.c_int32),
+        ("table_dtype", ctypes.c_int32),
+        ("weight_dtype", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("v_stride", ctypes.c_int64 * 3),
+        ("out_stride", ctypes.c_int64 * 3),
+        ("table_seq_stride", ctypes.c_int64),
+    ]
+
+
+class ChunkDesc(ctypes.Structure):
+    """lkv_chunk_desc: shape and extent of a chunk of new tokens over a cache's rows."""
+
+    _fields_ = [
+        ("n_seqs", ctypes.c_int32),
+        ("n_q", ctypes.c_int32),
+        ("n_kv", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("new_tokens", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("tokens", ctypes.c_int32),
+        ("max_tokens", ctypes.c_int32),
+        ("q_stride", ctypes.c_int64 * 3),
+    ]
+
+
+class EvictDesc(ctypes.Structure):
+    """lkv_evict_desc: which of a cache's rows stay."""
+
+    _fields_ = [
+        ("n_seqs", ctypes.c_int32),
+        ("n_kv", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("keep", ctypes.c_int32),
+        ("sinks", ctypes.c_int32),
+        ("recent", ctypes.c_int32),
+        ("tokens", ctypes.c_int32),
+        ("max_tokens", ctypes.c_int32),
+    ]
+
+
+Pair = ctypes.c_int64 * 2
+Triple = ctypes.c_int64 * 3
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _I64 = ctypes.c_int64
@@ -205,6 +272,27 @@ SIGNATURES: dict[str, tuple] = {
     "lkv_shared_decode": (
         _I,
         [_U, ctypes.POINTER(SharedDesc), _P, _I, ctypes.POINTER(KVRows), ctypes.POINTER(KVRows), _P, _P, _I, _P, _P, _SZ],
+    ),
+    "lkv_rotate_append": (
+        _I,
+        [_U, ctypes.POINTER(RotateDesc), _P, _P, _P, _P, _P, _P, _P, _P, ctypes.POINTER(KVRows), ctypes.POINTER(Pages), _P, _I, _P],
+    ),
+    "lkv_chunk_attend_workspace_bytes": (_SZ, [ctypes.POINTER(ChunkDesc)]),
+    "lkv_chunk_attend": (
+        _I,
+        [_U, ctypes.POINTER(ChunkDesc), _P, _I, ctypes.POINTER(KVRows), ctypes.POINTER(Pages), _P, _P, _P, _I, _P, _P, _SZ],
+    ),
+    "lkv_weigh_rows_workspace_bytes": (_SZ, [ctypes.POINTER(ChunkDesc)]),
+    "lkv_weigh_rows": (
+        _I,
+        [_U, ctypes.POINTER(ChunkDesc), _P, _I, _P, ctypes.POINTER(KVRows), ctypes.POINTER(Pages), _P, _P, _P, ctypes.POINTER(_I64), _P,
+         ctypes.POINTER(_I64), _P, ctypes.POINTER(_I64), _P, _P, _SZ],
+    ),
+    "lkv_evict_rows_workspace_bytes": (_SZ, [ctypes.POINTER(EvictDesc)]),
+    "lkv_evict_rows": (
+        _I,
+        [_U, ctypes.POINTER(EvictDesc), ctypes.POINTER(KVRows), ctypes.POINTER(Pages), _P, _P, ctypes.POINTER(_I64), _P, ctypes.POINTER(_I64), _P,
+         ctypes.POINTER(_I64), _P, ctypes.POINTER(_I64), _P, _SZ],
     ),
     "lkv_stream_read": (_I, [_U, _P, _SZ, _I, _P]),
 }

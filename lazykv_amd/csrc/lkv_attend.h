@@ -104,6 +104,13 @@ template <int D> struct KeyRegs<D, false> {
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) w[u][i] = *(const uint4*)(base + at.key[u] + i * 64);
   }
+  // The tile's halves of 16 tokens from streams of their own, each placed as if the tile lay together.
+  __device__ __forceinline__ void load(const Stream (&s)[2], const LaneOffsets<D, false>& at) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) w[u][i] = *(const uint4*)(s[u].k + at.key[u] + i * 64);
+  }
   template <int DT> __device__ __forceinline__ uint4 operand(int u, int i) const { return w[u][i]; }
   static __device__ __forceinline__ int channel(int q, int i) { return 32 * i + 8 * q; }
 };
@@ -117,6 +124,14 @@ template <int D> struct KeyRegs<D, true> {
 #pragma unroll
       for (int i = 0; i < D / 64; ++i) w[u][i] = *(const uint4*)(base + at.key[u] + i * 16);
       scale[u] = scales[at.key[u] / kMxGroup];
+    }
+  }
+  __device__ __forceinline__ void load(const Stream (&s)[2], const LaneOffsets<D, true>& at) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) w[u][i] = *(const uint4*)(s[u].k + at.key[u] + i * 16);
+      scale[u] = s[u].ks[at.key[u] / kMxGroup];
     }
   }
   template <int DT> __device__ __forceinline__ uint4 operand(int u, int i) const {
@@ -142,6 +157,19 @@ template <int D> struct ValueRegs<D, false> {
         w[j][0] = x.x, w[j][1] = x.y, w[j][2] = x.z, w[j][3] = x.w;
       } else {
         const uint2 x = *(const uint2*)(base + at.value[j]);
+        w[j][0] = x.x, w[j][1] = x.y;
+      }
+    }
+  }
+  __device__ __forceinline__ void load(const Stream (&s)[2], const LaneOffsets<D, false>& at) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint8_t* from = s[j / 4].v + at.value[j];
+      if constexpr (D == 128) {
+        const uint4 x = *(const uint4*)from;
+        w[j][0] = x.x, w[j][1] = x.y, w[j][2] = x.z, w[j][3] = x.w;
+      } else {
+        const uint2 x = *(const uint2*)from;
         w[j][0] = x.x, w[j][1] = x.y;
       }
     }
@@ -189,6 +217,37 @@ template <int D> struct ValueRegs<D, true> {
           } else {
             uint16_t x;
             __builtin_memcpy(&x, scales + row, 2);
+            scale[u][j / 2] = j & 1 ? scale[u][j / 2] | (uint32_t)x << 16 : x;
+          }
+        }
+    }
+  }
+  __device__ __forceinline__ void load(const Stream (&s)[2], const LaneOffsets<D, true>& at) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint8_t* from = s[j / 4].v + at.value[j];
+      if constexpr (D == 128) {
+        const uint2 x = *(const uint2*)from;
+        w[j][0] = x.x, w[j][1] = x.y;
+      } else {
+        w[j][0] = *(const uint32_t*)from;
+      }
+    }
+    if (!at.cut) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        __builtin_memcpy(scale[u], s[u].vs + (uint32_t)(((threadIdx.x & 48) / 4 + 16 * u) * (D / kMxGroup)), sizeof(scale[u]));
+    } else {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint8_t* from = s[u].vs + at.value[4 * u + j] / D * (D / kMxGroup);
+          if constexpr (D == 128) {
+            __builtin_memcpy(&scale[u][j], from, 4);
+          } else {
+            uint16_t x;
+            __builtin_memcpy(&x, from, 2);
             scale[u][j / 2] = j & 1 ? scale[u][j / 2] | (uint32_t)x << 16 : x;
           }
         }

@@ -1,0 +1,717 @@
+// A chunk of new tokens of each sequence of a batch over its rows, which lie in pages or one after the other (lkv_chunk_attend).
+//
+// Token t of a sequence's n new ones, of len rows in all, attends rows 0 .. len - n + t:
+//   s_i = scale * q . k_i,  m = max s_i,  out = sum exp(s_i - m) v_i / sum exp(s_i - m),  lse = m + ln sum exp(s_i - m),
+// in one pass over the rows, base 2, as in the batch decode (lkv_shared.hip), whose rounding of weights and lift in float16 it has too.
+//
+// The query rows of a KV head are its g heads of every token, x = t * g + j, so that a tile of them spans few tokens: the rows
+// that some of them attend and others do not are few.
+#include "lkv_attend.h"
+#include "lkv_pages.h"
+
+namespace {
+
+using namespace lkv;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kWaves = 4;
+
+struct ChunkArgs {
+  const uint16_t* q;
+  PagedRows rows;
+  const int32_t* lengths;
+  const int32_t* counts;
+  void* out;
+  float* lse;
+  float2* part_ml;  // [query rows][parts]: a part's maximum (base 2) and sum
+  float* part_o;    // [query rows][parts][d]
+  int64_t q_stride[3];
+  float scale2;  // scale * log2(e)
+  int32_t n_seqs, n_q, n_kv, g, new_tokens, tokens, max_tokens, out_dtype;
+  int32_t tiles, parts, chunk;  // row tiles of a KV head; its rows in `parts` ranges of `chunk`
+};
+
+// What a sequence has: rows in all, and the call's own among them.
+struct Extent {
+  int len, n;
+};
+__device__ __forceinline__ Extent extent_of(const ChunkArgs& a, int b) {
+  const int64_t len = (int64_t)a.tokens + (a.lengths ? a.lengths[b] : 0);
+  const int n = a.counts ? a.counts[b] : a.new_tokens;
+  return {(int)(len < 0 ? 0 : (len > a.max_tokens ? a.max_tokens : len)), n < 0 ? 0 : (n > a.new_tokens ? a.new_tokens : n)};
+}
+
+// A lane's query row.
+struct QueryRow {
+  int64_t row;  // of out and lse; -1 for none
+  int limit;    // rows that it attends
+  const uint16_t* q;
+};
+__device__ __forceinline__ QueryRow query_row(const ChunkArgs& a, const Extent& e, int b, int h, int x) {
+  const int t = x / a.g, j = h * a.g + (x - t * a.g);
+  if (t >= a.new_tokens) return {-1, 0, nullptr};
+  const int64_t row = ((int64_t)b * a.n_q + j) * a.new_tokens + t;
+  const int limit = t < e.n ? max(e.len - e.n + t + 1, 0) : 0;
+  return {row, limit, a.q + b * a.q_stride[0] + j * a.q_stride[1] + t * a.q_stride[2]};
+}
+
+// Four channels of a row: a part's, or, where it is the only part, the output's.
+template <int D>
+__device__ __forceinline__ void store_part(const ChunkArgs& a, int64_t row, int part, int channel, float l, f32x4 x) {
+  if (a.parts > 1) {
+    *(f32x4*)(a.part_o + (row * a.parts + part) * D + channel) = x;
+    return;
+  }
+  x = l == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : x * (1.0f / l);
+  if (a.out_dtype == LKV_F32) {
+    store_four<LKV_F32>(a.out, row * D + channel, x);
+  } else if (a.out_dtype == LKV_BF16) {
+    store_four<LKV_BF16>(a.out, row * D + channel, x);
+  } else {
+    store_four<LKV_F16>(a.out, row * D + channel, x);
+  }
+}
+__device__ __forceinline__ void store_sums(const ChunkArgs& a, int64_t row, int part, float m, float l) {
+  if (a.parts > 1) {
+    a.part_ml[row * a.parts + part] = make_float2(m, l);
+  } else {
+    a.lse[row] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+  }
+}
+
+// Values that are not finite, in a tile whose rows not all attend: a weight of 0 would make NaN of them in rows that do not attend them. They are
+// taken out of the product, and what they are is added by products of their own, with 1 for a row that attends and 0 for one that does not.
+template <int DT> constexpr uint32_t kInfBits = DT == LKV_BF16 ? 0x7f80u : 0x7c00u;
+template <int DT> constexpr uint32_t kOneBits = DT == LKV_BF16 ? 0x3f80u : 0x3c00u;
+// For each half of a word: all ones where it satisfies.
+template <int DT> __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+  constexpr uint32_t I = kInfBits<DT>;
+  return ((w & I) == I ? 0xffffu : 0u) | ((w >> 16 & I) == I ? 0xffff0000u : 0u);
+}
+template <int DT> __device__ __forceinline__ uint32_t ones_where(uint32_t w, uint32_t value) {
+  return ((w & 0xffffu) == value ? kOneBits<DT> : 0u) | (w >> 16 == value ? kOneBits<DT> << 16 : 0u);
+}
+template <int DT> __device__ __forceinline__ uint32_t ones_where_nan(uint32_t w) {
+  constexpr uint32_t I = kInfBits<DT>;
+  return ((w & 0x7fffu) > I ? kOneBits<DT> : 0u) | ((w >> 16 & 0x7fffu) > I ? kOneBits<DT> << 16 : 0u);
+}
+template <int DT> __device__ __forceinline__ bool any_not_finite(uint4 x) { return (not_finite<DT>(x.x) | not_finite<DT>(x.y) | not_finite<DT>(x.z) | not_finite<DT>(x.w)) != 0; }
+
+template <int DT, class ACC, class MMA>
+__device__ __forceinline__ void add_not_finite(uint4 v, uint4 attended, ACC& o, MMA mma) {
+  const auto add = [&](uint4 ones, float what) {
+    ACC zero;
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(ACC) / 4); ++i) zero[i] = 0.0f;
+    const ACC n = mma(ones, attended, zero);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(ACC) / 4); ++i) o[i] += n[i] > 0.0f ? what : 0.0f;
+  };
+  constexpr uint32_t I = kInfBits<DT>;
+  add(make_uint4(ones_where<DT>(v.x, I), ones_where<DT>(v.y, I), ones_where<DT>(v.z, I), ones_where<DT>(v.w, I)), INFINITY);
+  add(make_uint4(ones_where<DT>(v.x, I | 0x8000u), ones_where<DT>(v.y, I | 0x8000u), ones_where<DT>(v.z, I | 0x8000u), ones_where<DT>(v.w, I | 0x8000u)), -INFINITY);
+  add(make_uint4(ones_where_nan<DT>(v.x), ones_where_nan<DT>(v.y), ones_where_nan<DT>(v.z), ones_where_nan<DT>(v.w)), NAN);
+}
+
+// ---- few rows: every wave on its own stream of tokens, straight from memory to registers -----------------
+
+// The two halves of a wave's tile of 32 rows, each in one page; a half that is not there reads the other's rows, or the pool's first.
+template <int D, bool MX> struct Halves {
+  Stream s[2];
+  bool there[2];
+  // Rows 16 group .. of which `last` (0 .. 31) is the last one there is.
+  __device__ __forceinline__ void find(const PagedRows& p, int b, int h, int group, int last) {
+    Sixteen x[2];
+    x[0] = sixteen_of<D>(p, b, h, group);
+    x[1] = last >= 16 ? sixteen_of<D>(p, b, h, group + 1) : Sixteen{x[0].at + 16 * D, x[0].there};
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int64_t at = x[u].at - u * 16 * D;  // as if the tile lay together
+      s[u] = {(const uint8_t*)p.rows.k + (MX ? at : 2 * at), (const uint8_t*)p.rows.v + (MX ? at : 2 * at), MX ? p.rows.k_scale + at / kMxGroup : nullptr,
+              MX ? p.rows.v_scale + at / kMxGroup : nullptr};
+      there[u] = x[u].there;
+    }
+  }
+};
+
+// A tile's scores made ready for the exponential (settle's work), where rows attend to different limits: left[n], tokens of the tile that this lane's
+// row attends.
+template <int DT, int D, int NR>
+__device__ __forceinline__ void mask_scores(f32x4 (&sc)[NR][2], const int (&left)[NR], bool there0, bool there1) {
+  const int quarter = (threadIdx.x & 48) / 4;
+#pragma unroll
+  for (int n = 0; n < NR; ++n)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float x = (j < 4 ? 0 : 16) + (j & 3) + quarter < left[n] && (j < 4 ? there0 : there1) ? sc[n][j / 4][j & 3] : -INFINITY;
+      keep_here(x);
+      sc[n][j / 4][j & 3] = x;
+    }
+}
+
+// Whether this lane's row attends its eight tokens of a tile, as the second product's operand.
+template <int DT>
+__device__ __forceinline__ uint4 attended(int left, bool there0, bool there1) {
+  const int quarter = (threadIdx.x & 48) / 4;
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int at = (i < 2 ? 0 : 16) + 2 * (i & 1) + quarter;
+    const bool there = i < 2 ? there0 : there1;
+    w[i] = (there && at < left ? kOneBits<DT> : 0u) | (there && at + 1 < left ? kOneBits<DT> << 16 : 0u);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <int DT, int D, bool MX, int NR>
+__device__ __forceinline__ void attend_few(const ChunkArgs& a, int b, int h, const QueryRow (&row)[NR], int first, int step, int end, int whole,
+                                           Result<D, NR>& r) {
+  const int quarter = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    r.m[n] = -INFINITY;
+    r.l[n] = 0.0f;
+#pragma unroll
+    for (int e = 0; e < D / 16; ++e) r.o[n][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  if (first >= end) return;
+  Reference ref[NR];
+  uint4 qf[NR][D / 32];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    ref[n].reset();
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) qf[n][i] = row[n].row >= 0 ? *(const uint4*)(row[n].q + KeyRegs<D, MX>::channel(quarter, i)) : make_uint4(0, 0, 0, 0);
+  }
+  KeyRegs<D, MX> k;
+  ValueRegs<D, MX> v;
+  LaneOffsets<D, MX> at;
+  Halves<D, MX> now, next_;
+  at.set(min(kTile, end - first) - 1);
+  now.find(a.rows, b, h, first >> 4, min(kTile, end - first) - 1);
+  k.load(now.s, at);
+  v.load(now.s, at);
+  load_fence();
+  for (int t = first; t < end; t += step) {
+    const int next = t + step < end ? t + step : t;
+    next_.find(a.rows, b, h, next >> 4, min(kTile, end - next) - 1);
+    f32x4 sc[NR][2];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) sc[n][0] = sc[n][1] = ref[n].negative;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        const uint4 x = k.template operand<DT>(u, i);
+#pragma unroll
+        for (int n = 0; n < NR; ++n) sc[n][u] = Mat<DT>::mma(x, qf[n][i], sc[n][u]);
+      }
+    if (next + kTile > end) at.set(end - next - 1);
+    k.load(next_.s, at);
+    load_fence();
+    const bool there0 = now.there[0], there1 = now.there[1], cut = t + kTile > whole || !there0 || !there1;
+    int left[NR];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) left[n] = row[n].limit - t;
+    if (cut) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v.keep(j, t + (j < 4 ? 0 : 16) + 4 * quarter + (j & 3) < end && (j < 4 ? there0 : there1));
+      mask_scores<DT, D, NR>(sc, left, there0, there1);
+    }
+    settle<DT, D, NR>(sc, kTile, a.scale2, ref, r);
+    uint4 p[NR];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) p[n] = weights<DT, NR>(sc[n], a.scale2, r.l[n]);
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+      uint32_t x[8];
+      v.template widen<DT>(c, x);
+#pragma unroll
+      for (int odd = 0; odd < 2; ++odd) {
+        const uint32_t pick = odd ? 0x07060302u : 0x05040100u;
+        uint4 w = make_uint4(__builtin_amdgcn_perm(x[1], x[0], pick), __builtin_amdgcn_perm(x[3], x[2], pick), __builtin_amdgcn_perm(x[5], x[4], pick),
+                             __builtin_amdgcn_perm(x[7], x[6], pick));
+        if (cut && __any(any_not_finite<DT>(w))) {
+#pragma unroll
+          for (int n = 0; n < NR; ++n)
+            add_not_finite<DT>(w, attended<DT>(left[n], there0, there1), r.o[n][2 * c + odd], [](uint4 m, uint4 q, f32x4 z) { return Mat<DT>::mma(m, q, z); });
+          w = make_uint4(w.x & ~not_finite<DT>(w.x), w.y & ~not_finite<DT>(w.y), w.z & ~not_finite<DT>(w.z), w.w & ~not_finite<DT>(w.w));
+        }
+#pragma unroll
+        for (int n = 0; n < NR; ++n) r.o[n][2 * c + odd] = Mat<DT>::mma(w, p[n], r.o[n][2 * c + odd]);
+      }
+    }
+    v.load(next_.s, at);
+    load_fence();
+    now = next_;
+  }
+  conclude<DT, D, NR>(a.scale2, ref, r);
+}
+
+// The results that the workgroup's waves have for the same rows, each from its own tokens, joined and stored: all write theirs to LDS, then
+// each takes its share of the channels.
+template <int D, int NR>
+__device__ __forceinline__ void finish_few(const ChunkArgs& a, const Result<D, NR>& r, const QueryRow (&row)[NR], int part, int wave, f32x4* lds) {
+  constexpr int FOURS = D / 16;
+  static_assert(FOURS % kWaves == 0, "every wave takes as many channels");
+  const int lane = threadIdx.x & 63, quarter = lane >> 4;
+  float2* const ml = (float2*)(lds + kWaves * NR * FOURS * 64);
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    ml[(wave * NR + n) * 64 + lane] = make_float2(r.m[n], r.l[n]);
+#pragma unroll
+    for (int k = 0; k < FOURS; ++k) {
+      int c;
+      lds[((wave * NR + n) * FOURS + k) * 64 + lane] = four_of<D, false>(r.o[n], k, c);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+    float2 x[kWaves];
+    float top = -INFINITY, total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+      x[i] = ml[(i * NR + n) * 64 + lane];
+      top = fmaxf(top, x[i].x);
+    }
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+      x[i].x = join_factor(x[i].x, x[i].y, top);
+      total += x[i].x * x[i].y;
+    }
+    if (row[n].row < 0) continue;
+    if (row[n].limit == 0) total = 0.0f;
+    if (wave == 0 && quarter == 0) store_sums(a, row[n].row, part, top, total);
+#pragma unroll
+    for (int j = 0; j < FOURS / kWaves; ++j) {
+      const int k = j * kWaves + wave;
+      f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) o += lds[((i * NR + n) * FOURS + k) * 64 + lane] * x[i].x;
+      store_part<D>(a, row[n].row, part, channel_of<D, false>(k), total, o);
+    }
+  }
+}
+
+template <int DT, int D, bool MX, int NR>
+__global__ __launch_bounds__(64 * kWaves, NR == 2 && D == 128 ? 1 : 2) void chunk_few_kernel(ChunkArgs a) {
+  __shared__ f32x4 lds[kWaves * NR * 64 * (D + 8) / 16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int id = blockIdx.x;
+  const int heads = a.n_seqs * a.n_kv, bh = id % heads;
+  id /= heads;
+  const int part = id % a.parts, tile = id / a.parts, b = bh / a.n_kv, h = bh % a.n_kv;
+  const Extent e = extent_of(a, b);
+  QueryRow row[NR];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) row[n] = query_row(a, e, b, h, (tile * NR + n) * 16 + (lane & 15));
+  // Rows that the tile's first token attends, and its last one.
+  const int t0 = tile * NR * 16 / a.g, t1 = min((tile * NR * 16 + NR * 16 - 1) / a.g, e.n - 1);
+  const int whole = max(e.len - e.n + t0 + 1, 0), all = t1 < t0 ? 0 : max(e.len - e.n + t1 + 1, 0);
+  const int begin = part * a.chunk, end = min(begin + a.chunk, all);
+  Result<D, NR> r;
+  attend_few<DT, D, MX, NR>(a, b, h, row, begin + wave * kTile, kWaves * kTile, end, whole, r);
+  finish_few<D, NR>(a, r, row, part, wave, lds);
+}
+
+// ---- many rows: keys and values through LDS --------------------------------------------------------
+// A workgroup stages 64 tokens' keys and values in LDS, in the model dtype (8-bit rows are widened on the way), for four waves of 32 query rows
+// each, on v_mfma_f32_32x32x16: S^T [32 tokens x 32 rows] = K Q^T, O^T [d x 32] += V^T P^T. A lane holds column lane % 32, of tokens
+// 8 (i / 4) + 4 (lane / 32) + i % 4 in register i; the second product's k-th step of 16 tokens takes registers 8 k .. 8 k + 7 as they are. Pieces of 16
+// bytes are swizzled by the row, so that both the keys' 32 rows and the values' transposed reads of four rows spread over all banks.
+template <int DT> struct Wide;
+template <> struct Wide<LKV_BF16> {
+  static __device__ __forceinline__ f32x16 mma(uint4 a, uint4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+};
+template <> struct Wide<LKV_F16> {
+  static __device__ __forceinline__ f32x16 mma(uint4 a, uint4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+};
+
+constexpr int kStage = 64;  // tokens
+template <int D> __device__ __forceinline__ int swizzle(int row) {
+  return D == 128 ? ((row & 3) << 2 | ((row >> 2) & 3)) : ((row & 2) << 1 | ((row >> 2) & 3));
+}
+
+// Where a stage's tokens are: each sixteen of them, and a bit for each that is there.
+template <int D> struct StagePlace {
+  int64_t at0, at1, at2, at3;
+  uint32_t there;
+  __device__ __forceinline__ void find(const PagedRows& p, int b, int h, int t0, int end) {
+    const int last = (end - 1) >> 4, first = t0 >> 4;
+    const Sixteen x0 = sixteen_of<D>(p, b, h, min(first, last)), x1 = sixteen_of<D>(p, b, h, min(first + 1, last)), x2 = sixteen_of<D>(p, b, h, min(first + 2, last)),
+                  x3 = sixteen_of<D>(p, b, h, min(first + 3, last));
+    at0 = x0.at, at1 = x1.at, at2 = x2.at, at3 = x3.at;
+    there = (x0.there ? 1u : 0u) | (x1.there ? 2u : 0u) | (x2.there ? 4u : 0u) | (x3.there ? 8u : 0u);
+  }
+  __device__ __forceinline__ int64_t at(int sixteen) const {
+    const int64_t a = at0, b = at1, c = at2, d = at3;
+    const int64_t lo = sixteen & 1 ? b : a, hi = sixteen & 1 ? d : c;
+    return sixteen & 2 ? hi : lo;
+  }
+};
+
+// What a thread holds of a stage on its way to LDS.
+template <int DT, int D, bool MX> struct StageRegs {
+  static constexpr int PIECES = MX ? D / 16 : D / 8;  // 16-byte pieces of a row
+  static constexpr int LOADS = kStage * PIECES / (64 * kWaves);
+  static constexpr int ROW = MX ? D : 2 * D;
+  static constexpr int BYTES = kStage * 2 * D;  // of keys, and of values, in LDS
+  u32x4 k[LOADS], v[LOADS];
+  uint32_t ks[LOADS], vs[LOADS];
+  // Tokens t0 .. of a sequence; in the place of those behind `end`, the last one.
+  __device__ __forceinline__ void load(const PagedRows& p, const StagePlace<D>& place, int t0, int end) {
+    const int last = (end - 1) >> 4;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int x = i * 64 * kWaves + threadIdx.x, wave_x = i * 64 * kWaves + (threadIdx.x & ~63);
+      const int sixteen = __builtin_amdgcn_readfirstlane(wave_x / PIECES / 16);  // a wave's rows of a load lie in one
+      int row = x / PIECES & 15;
+      const int group = min((t0 >> 4) + sixteen, last);
+      row = min(row, end - 1 - group * 16);
+      const int64_t at = place.at(sixteen);
+      const uint32_t in = (uint32_t)(row * ROW + x % PIECES * 16);
+      k[i] = *(const u32x4*)((const uint8_t*)p.rows.k + (MX ? at : 2 * at) + in);
+      v[i] = *(const u32x4*)((const uint8_t*)p.rows.v + (MX ? at : 2 * at) + in);
+      if constexpr (MX) {
+        ks[i] = p.rows.k_scale[at / kMxGroup + in / kMxGroup];
+        vs[i] = p.rows.v_scale[at / kMxGroup + in / kMxGroup];
+      }
+    }
+  }
+  static __device__ __forceinline__ uint4 widen(uint32_t lo, uint32_t hi, uint32_t scale) {
+    const float f = bits_to_float(scale << 23);
+    return make_uint4(Mat<DT>::template widen<false>(lo, f), Mat<DT>::template widen<true>(lo, f), Mat<DT>::template widen<false>(hi, f),
+                      Mat<DT>::template widen<true>(hi, f));
+  }
+  // Into LDS; values of tokens behind the end and of those that are not there as zeros, which a weight of 0 leaves.
+  __device__ __forceinline__ void store(uint8_t* lds, int live, uint32_t there) const {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int x = i * 64 * kWaves + threadIdx.x, row = x / PIECES, sw = swizzle<D>(row);
+      const uint32_t mask = row < live && (there >> (row >> 4) & 1) ? ~0u : 0u;
+      uint8_t* to = lds + row * (2 * D);
+      if constexpr (!MX) {
+        to += ((x % PIECES) ^ sw) * 16;
+        *(u32x4*)to = k[i];
+        *(u32x4*)(to + BYTES) = v[i] & mask;
+      } else {
+        const int piece = x % PIECES * 2;
+        const u32x4 w = v[i] & mask;  // a code of zero is zero under any scale that is written
+        *(uint4*)(to + (piece ^ sw) * 16) = widen(k[i].x, k[i].y, ks[i]);
+        *(uint4*)(to + ((piece + 1) ^ sw) * 16) = widen(k[i].z, k[i].w, ks[i]);
+        to += BYTES;
+        *(uint4*)(to + (piece ^ sw) * 16) = widen(w.x, w.y, vs[i]);
+        *(uint4*)(to + ((piece + 1) ^ sw) * 16) = widen(w.z, w.w, vs[i]);
+      }
+    }
+  }
+};
+
+// A row's reference (see Reference in lkv_attend.h), here as the exponent's addend.
+struct Level {
+  float less;   // -reference in base 2 (+ the lift); 0 at first
+  float limit;  // raw scores up to here stay; -inf until there is a reference
+};
+
+// 32 staged tokens against the wave's 32 rows. left: tokens that this lane's row attends of them; there: of the two sixteens.
+template <int DT, int D>
+__device__ __forceinline__ void wide_tile(const LdsPointer (&key_at)[D / 16], const LdsPointer (&value_at)[2][D / 32], int at, const uint4 (&qf)[D / 16], bool cut,
+                                          int left, bool there0, bool there1, float scale2, Level& level, float& l, f32x16 (&o)[D / 32]) {
+  constexpr float lift = lift_of(DT, 2), slack = slack_of(DT, 2);
+  const int half = (threadIdx.x & 32) >> 3;  // 4 (lane / 32)
+  f32x16 s;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) s = Wide<DT>::mma(read_piece(key_at[i] + at), qf[i], s);
+  if (cut) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float x = 8 * (i / 4) + i % 4 + half < left && (i < 8 ? there0 : there1) ? s[i] : -INFINITY;
+      keep_here(x);
+      s[i] = x;
+    }
+  }
+  float top = s[0];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+  if (__any(top > level.limit)) {
+    const float up = pair_max<32>(top);
+    const bool move = up > level.limit && up < INFINITY;
+    const float less = lift - up * scale2;
+    const float keep = !move ? 1.0f : level.limit == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(less - level.less);
+    level.less = move ? less : level.less;
+    level.limit = move ? up + slack / scale2 : level.limit;
+    l *= keep;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) o[c] *= keep;
+  }
+  uint4 p[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    float w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * k + i], scale2, level.less));
+    l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+    p[k] = make_uint4(Mat<DT>::pack(w[0], w[1]), Mat<DT>::pack(w[2], w[3]), Mat<DT>::pack(w[4], w[5]), Mat<DT>::pack(w[6], w[7]));
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+      const uint2 lo = read_transposed(value_at[0][c] + at + 16 * k * 2 * D), hi = read_transposed(value_at[1][c] + at + 16 * k * 2 * D);
+      uint4 w = make_uint4(lo.x, lo.y, hi.x, hi.y);
+      if (cut && __any(any_not_finite<DT>(w))) {
+        uint32_t ones[4];
+        const bool there = k == 0 ? there0 : there1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int first = 16 * k + 8 * (i / 2) + 2 * (i & 1) + half;
+          ones[i] = (there && first < left ? kOneBits<DT> : 0u) | (there && first + 1 < left ? kOneBits<DT> << 16 : 0u);
+        }
+        add_not_finite<DT>(w, make_uint4(ones[0], ones[1], ones[2], ones[3]), o[c], [](uint4 m, uint4 q, f32x16 z) { return Wide<DT>::mma(m, q, z); });
+        w = make_uint4(w.x & ~not_finite<DT>(w.x), w.y & ~not_finite<DT>(w.y), w.z & ~not_finite<DT>(w.z), w.w & ~not_finite<DT>(w.w));
+      }
+      o[c] = Wide<DT>::mma(w, p[k], o[c]);
+    }
+}
+
+template <int DT, int D, bool MX>
+__global__ __launch_bounds__(64 * kWaves, 2) void chunk_wide_kernel(ChunkArgs a) {
+  using S = StageRegs<DT, D, MX>;
+  constexpr int ROWS = 32 * kWaves;
+  __shared__ f32x4 lds4[2 * 2 * S::BYTES / 16];
+  uint8_t* const lds = (uint8_t*)lds4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int id = blockIdx.x;
+  const int heads = a.n_seqs * a.n_kv, bh = id % heads;
+  id /= heads;
+  // The longest tiles first: the last ones of a sequence attend the most rows.
+  const int part = id % a.parts, tile = a.tiles - 1 - id / a.parts, b = bh / a.n_kv, h = bh % a.n_kv;
+  const Extent e = extent_of(a, b);
+  const int x0 = tile * ROWS + wave * 32;
+  const QueryRow row = query_row(a, e, b, h, x0 + (lane & 31));
+  const int past = e.len - e.n, begin = part * a.chunk;
+  const int last = min((tile * ROWS + ROWS - 1) / a.g, e.n - 1), wave_first = x0 / a.g, wave_last = min((x0 + 31) / a.g, e.n - 1);
+  const int end = last < tile * ROWS / a.g ? 0 : min(begin + a.chunk, max(past + last + 1, 0));
+  const int wave_end = wave_last < wave_first ? 0 : min(end, max(past + wave_last + 1, 0)), whole = max(past + wave_first + 1, 0);
+  Level level = {0.0f, -INFINITY};
+  float l = 0.0f;
+  f32x16 o[D / 32];
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[c][i] = 0.0f;
+  if (begin < end) {
+    S regs;
+    StagePlace<D> place, next;
+    place.find(a.rows, b, h, begin, end);
+    regs.load(a.rows, place, begin, end);
+    uint4 qf[D / 16];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) qf[i] = row.row >= 0 ? *(const uint4*)(row.q + 16 * i + (lane >> 5) * 8) : make_uint4(0, 0, 0, 0);
+    LdsPointer key_at[D / 16], value_at[2][D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      const int r = lane & 31;
+      key_at[i] = (LdsPointer)lds + r * (2 * D) + ((2 * i + (lane >> 5)) ^ swizzle<D>(r)) * 16;
+      keep_here(key_at[i]);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        const int r = 8 * j + 4 * (lane >> 5) + ((lane & 15) >> 2);
+        value_at[j][c] = (LdsPointer)lds + S::BYTES + r * (2 * D) + ((4 * c + ((lane & 16) >> 3) + ((lane & 2) >> 1)) ^ swizzle<D>(r)) * 16 + (lane & 1) * 8;
+        keep_here(value_at[j][c]);
+      }
+    int buffer = 0;
+    for (int t = begin; t < end; t += kStage) {
+      regs.store(lds + buffer, end - t, place.there);
+      __syncthreads();
+      if (t + kStage < end) {
+        next.find(a.rows, b, h, t + kStage, end);
+        regs.load(a.rows, next, t + kStage, end);
+      }
+      load_fence();
+#pragma unroll
+      for (int sub = 0; sub < 2; ++sub) {
+        const int now = t + 32 * sub;
+        if (now >= wave_end) continue;
+        const bool there0 = place.there >> (2 * sub) & 1, there1 = place.there >> (2 * sub + 1) & 1;
+        const bool cut = now + 32 > whole || !there0 || !there1;
+        wide_tile<DT, D>(key_at, value_at, buffer + sub * 32 * 2 * D, qf, cut, row.limit - now, there0, there1, a.scale2, level, l, o);
+      }
+      buffer ^= 2 * S::BYTES;
+      place = next;
+    }
+  }
+  if (row.row < 0) return;
+  constexpr float down = 1.0f / (float)(1 << (int)lift_of(DT, 2));
+  l = row.limit == 0 ? 0.0f : pair_sum<32>(l) * down;
+  const float m = level.limit == -INFINITY ? -INFINITY : lift_of(DT, 2) - level.less;
+  if (lane < 32) store_sums(a, row.row, part, m, l);
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      store_part<D>(a, row.row, part, 32 * c + 8 * i + 4 * (lane >> 5), l, f32x4{o[c][4 * i], o[c][4 * i + 1], o[c][4 * i + 2], o[c][4 * i + 3]} * down);
+}
+
+// A query row's parts into one, a wave a row: d / 4 lanes take a part's channels, four each, and the others the next part's.
+template <int D>
+__global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs a, int64_t rows) {
+  constexpr int C = D / 4, EACH = 64 / C;
+  const int lane = threadIdx.x & 63, c = lane % C;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const float2* ml = a.part_ml + row * a.parts;
+  const float* from = a.part_o + row * a.parts * D + c * 4;
+  float top = -INFINITY, total = 0.0f;
+  f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int p0 = 0; p0 < a.parts; p0 += 64) {
+    const float2 mine = p0 + lane < a.parts ? ml[p0 + lane] : make_float2(-INFINITY, 0.0f);
+    const float up = fmaxf(top, wave_max_f32(mine.x));
+    const float keep = p0 == 0 ? 0.0f : join_factor(top, total, up), f = join_factor(mine.x, mine.y, up);
+    top = up;
+    total = total * keep + wave_sum_f32(mine.y == 0.0f ? 0.0f : f * mine.y);
+    o *= keep;
+    const int n = min(64, a.parts - p0);
+    for (int p = 0; p < n; p += EACH) {
+      const int mine_p = p + lane / C;
+      const float w = __shfl(f, mine_p), s = __shfl(mine.y, mine_p);
+      if (mine_p < n && s != 0.0f) o += *(const f32x4*)(from + (int64_t)(p0 + mine_p) * D) * w;
+    }
+  }
+  if constexpr (EACH == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = pair_sum<16>(o[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = pair_sum<32>(o[i]);
+  if (lane >= C) return;
+  o = total == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : o * (1.0f / total);
+  if (a.out_dtype == LKV_F32) {
+    store_four<LKV_F32>(a.out, row * D + c * 4, o);
+  } else if (a.out_dtype == LKV_BF16) {
+    store_four<LKV_BF16>(a.out, row * D + c * 4, o);
+  } else {
+    store_four<LKV_F16>(a.out, row * D + c * 4, o);
+  }
+  if (lane == 0) a.lse[row] = total == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(total)) * kLn2;
+}
+
+int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+// How a call is divided: see ChunkArgs. nr: tiles of 16 rows of a wave on its own stream, 0: through LDS.
+struct Plan {
+  int nr, tiles, parts, chunk;
+};
+
+Plan plan_of(const lkv_chunk_desc* d) {
+  Plan p = {};
+  const int64_t rows = (int64_t)d->new_tokens * (d->n_q / d->n_kv), heads = (int64_t)d->n_seqs * d->n_kv;
+  p.nr = rows <= 16 ? 1 : rows <= 32 ? 2 : 0;
+  p.tiles = ceil_div(rows, p.nr ? 16 * p.nr : 32 * kWaves);
+  const int64_t units = heads * p.tiles, room = 512, least = p.nr ? 128 : 256;
+  int64_t parts = units > 0 ? room / units : 1;
+  const int64_t most = ceil_div(d->max_tokens, least);
+  parts = parts < 1 ? 1 : parts > most ? most : parts;
+  parts = parts < 1 ? 1 : parts;
+  const int64_t step = p.nr ? 128 : 64;
+  int64_t chunk = (d->max_tokens + parts - 1) / parts;
+  chunk = (chunk + step - 1) / step * step;
+  p.chunk = (int)(chunk < step ? step : chunk);
+  p.parts = ceil_div(d->max_tokens, p.chunk);
+  p.parts = p.parts < 1 ? 1 : p.parts;
+  return p;
+}
+
+template <int DT, int D, bool MX>
+void launch(const Plan& p, dim3 grid, hipStream_t s, const ChunkArgs& a) {
+  auto kernel = p.nr == 1 ? chunk_few_kernel<DT, D, MX, 1> : p.nr == 2 ? chunk_few_kernel<DT, D, MX, 2> : chunk_wide_kernel<DT, D, MX>;
+  hipLaunchKernelGGL(kernel, grid, dim3(64 * kWaves), 0, s, a);
+}
+
+}  // namespace
+
+int lkv_check_chunk(const lkv_chunk_desc* d) {
+  LKV_CHECK_ARG(d, "NULL pointer");
+  LKV_CHECK_ARG(d->head_dim == 64 || d->head_dim == 128, "head_dim %d unsupported (64 or 128)", d->head_dim);
+  LKV_CHECK_ARG(d->n_seqs >= 0 && d->n_kv > 0 && d->n_q > 0 && d->n_q % d->n_kv == 0 && d->new_tokens >= 0, "bad shape: %d sequences, %d query heads over %d, %d tokens",
+                d->n_seqs, d->n_q, d->n_kv, d->new_tokens);
+  LKV_CHECK_ARG((__int128)d->n_seqs * d->n_q * d->new_tokens <= (1 << 26), "%d x %d x %d query rows in one call", d->n_seqs, d->n_q, d->new_tokens);
+  LKV_CHECK_ARG(d->scale > 0.0f && d->scale * lkv::kLog2e < INFINITY, "scale %g: positive and finite", (double)d->scale);
+  LKV_CHECK_ARG(d->tokens >= 0 && d->max_tokens >= 0 && d->max_tokens <= (1 << 30), "bad extent: %d rows of at most %d", d->tokens, d->max_tokens);
+  LKV_CHECK_ARG(((d->q_stride[0] | d->q_stride[1] | d->q_stride[2]) & 7) == 0, "strides must be multiples of 8 elements");
+  return LKV_OK;
+}
+
+extern "C" size_t lkv_chunk_attend_workspace_bytes(const lkv_chunk_desc* desc) {
+  if (lkv_check_chunk(desc)) return 0;
+  const Plan p = plan_of(desc);
+  const size_t rows = (size_t)desc->n_seqs * desc->n_q * desc->new_tokens;
+  return p.parts < 2 ? 0 : lkv_align_up(rows * p.parts * sizeof(float2), 16) + rows * p.parts * desc->head_dim * sizeof(float);
+}
+
+extern "C" int lkv_chunk_attend(uintptr_t stream, const lkv_chunk_desc* desc, const void* q, int q_dtype, const lkv_kv_rows* rows, const lkv_pages* pages,
+                                const int32_t* lengths, const int32_t* counts, void* out, int out_dtype, float* lse, void* ws, size_t ws_bytes) {
+  if (int rc = lkv_check_chunk(desc)) return rc;
+  LKV_CHECK_ARG(q && out && lse, "NULL pointer");
+  LKV_CHECK_ARG(q_dtype == LKV_F16 || q_dtype == LKV_BF16, "queries are float16 or bfloat16, got dtype %d", q_dtype);
+  LKV_CHECK_ARG(lkv_is_model_dtype(out_dtype), "unsupported output dtype %d", out_dtype);
+  LKV_CHECK_ARG((((uintptr_t)q | (uintptr_t)out) & 15) == 0, "queries and outputs must start on 16 bytes");
+  ChunkArgs a = {};
+  if (int rc = lkv_paged_rows(rows, pages, desc->n_seqs, q_dtype, desc->head_dim, a.rows)) return rc;
+  LKV_CHECK_ARG(desc->max_tokens <= a.rows.capacity, "%d rows of a sequence over %d", desc->max_tokens, a.rows.capacity);
+  const size_t need = lkv_chunk_attend_workspace_bytes(desc);
+  LKV_CHECK_ARG(need == 0 || (ws && ws_bytes >= need), "workspace of %zu bytes: %zu are needed", ws_bytes, need);
+  LKV_CHECK_ARG(need == 0 || ((uintptr_t)ws & 15) == 0, "the workspace must start on 16 bytes");
+  const int64_t n = (int64_t)desc->n_seqs * desc->n_q * desc->new_tokens;
+  if (n == 0) return LKV_OK;
+  const Plan p = plan_of(desc);
+  const int64_t blocks = (int64_t)desc->n_seqs * desc->n_kv * p.tiles * p.parts;
+  LKV_CHECK_ARG(blocks < (1LL << 31), "%lld workgroups in one call", (long long)blocks);
+  a.q = (const uint16_t*)q;
+  a.lengths = lengths;
+  a.counts = counts;
+  a.out = out;
+  a.lse = lse;
+  a.part_ml = (float2*)ws;
+  a.part_o = (float*)((uint8_t*)ws + lkv_align_up(n * p.parts * sizeof(float2), 16));
+  for (int i = 0; i < 3; ++i) a.q_stride[i] = desc->q_stride[i];
+  a.scale2 = desc->scale * kLog2e;
+  a.n_seqs = desc->n_seqs;
+  a.n_q = desc->n_q;
+  a.n_kv = desc->n_kv;
+  a.g = desc->n_q / desc->n_kv;
+  a.new_tokens = desc->new_tokens;
+  a.tokens = desc->tokens;
+  a.max_tokens = desc->max_tokens;
+  a.out_dtype = out_dtype;
+  a.tiles = p.tiles;
+  a.parts = p.parts;
+  a.chunk = p.chunk;
+  const hipStream_t s = (hipStream_t)stream;
+  const bool half = q_dtype == LKV_F16, wide = desc->head_dim == 128, mx = rows->dtype == LKV_MXFP8;
+  const dim3 grid((unsigned)blocks);
+  if (half) {
+    wide ? (mx ? launch<LKV_F16, 128, true>(p, grid, s, a) : launch<LKV_F16, 128, false>(p, grid, s, a))
+         : (mx ? launch<LKV_F16, 64, true>(p, grid, s, a) : launch<LKV_F16, 64, false>(p, grid, s, a));
+  } else {
+    wide ? (mx ? launch<LKV_BF16, 128, true>(p, grid, s, a) : launch<LKV_BF16, 128, false>(p, grid, s, a))
+         : (mx ? launch<LKV_BF16, 64, true>(p, grid, s, a) : launch<LKV_BF16, 64, false>(p, grid, s, a));
+  }
+  LKV_CHECK_LAUNCH("chunk_attend");
+  if (p.parts > 1) {
+    hipLaunchKernelGGL((wide ? chunk_join_kernel<128> : chunk_join_kernel<64>), dim3((unsigned)((n + 3) / 4)), dim3(256), 0, s, a, n);
+    LKV_CHECK_LAUNCH("chunk_attend (join)");
+  }
+  return LKV_OK;
+}

@@ -11,6 +11,11 @@
 
 constexpr int kMxGroup = 32;  // channels that share a scale
 
+// Rows that are written: none of them may share an address with another (lkv_rows.hip). Strides and head_dim in elements of `bytes` bytes; v may be NULL.
+int lkv_distinct_rows(const char* what, const void* k, const void* v, int bytes, int n_seqs, int n_kv, int64_t tokens, int head_dim, int64_t seq_stride,
+                      int64_t head_stride, int64_t token_stride);
+int lkv_distinct_dst(const lkv_kv_rows* dst, int n_kv, int head_dim);
+
 // The arguments every rows call checks the same way. `what` names the rows in the message.
 static inline int lkv_check_rows(const lkv_kv_rows* r, const char* what, int n_seqs, int dtype, int head_dim) {
   LKV_CHECK_ARG(r->k && r->v, "%s: NULL pointer", what);
@@ -49,6 +54,43 @@ __device__ __forceinline__ void mx_widen(uint32_t codes, float scale, float (&ou
   out[1] = a.y * scale;
   out[2] = b.x * scale;
   out[3] = b.y * scale;
+}
+
+// Eight channels of a row to codes; a quad of lanes, which hold a group, shares the scale. Every lane of the quad has to be here.
+template <int DT>
+__device__ __forceinline__ uint2 mx_encode(float (&x)[8], uint32_t& scale) {
+  float most = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float a = fabsf(x[i]);
+    const bool fine = a < INFINITY;
+    most = fmaxf(most, fine ? a : 0.0f);
+    x[i] = fine ? x[i] : NAN;
+  }
+  most = fmaxf(most, dpp<kDppQuadSwap1>(most));
+  most = fmaxf(most, dpp<kDppQuadSwap2>(most));
+  // 448 = 1.75 * 2^8.
+  const float top = fminf(most, mx_largest<DT>());
+  const uint32_t bits = float_to_bits(top);
+  const int e = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  scale = e > 0 ? e : 0;
+  const float up = bits_to_float((254u - scale) << 23);
+  uint32_t code[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float v = x[4 * i + j];
+      // A NaN passes both comparisons' selects.
+      const float lim = v > mx_largest<DT>() ? mx_largest<DT>() : (v < -mx_largest<DT>() ? -mx_largest<DT>() : v);
+      y[j] = lim * up;
+    }
+    int packed = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+    packed = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], packed, true);
+    code[i] = (uint32_t)packed;
+  }
+  return make_uint2(code[0], code[1]);
 }
 
 }  // namespace lkv

@@ -1,0 +1,166 @@
+// New tokens' queries and keys normalised over each head and rotated, keys and values written to their rows (lkv_rotate_append).
+#include "lkv_pages.h"
+
+namespace {
+
+struct RotateArgs {
+  lkv_rotate_desc d;
+  const uint16_t *q, *k, *v;
+  const void *cos, *sin, *q_weight, *k_weight;
+  uint16_t* q_out;
+  lkv::PagedRows rows;
+  const int32_t* starts;
+  const int32_t* counts;
+  int32_t start;
+  uint32_t heads;   // n_q + 2 n_kv
+  uint32_t pieces;  // n_seqs * tokens * heads
+};
+
+// Eight neighbouring values in the model dtype or in float32.
+template <int DT>
+__device__ __forceinline__ void load_eight(const void* p, int64_t at, bool wide, float (&out)[8]) {
+  if (wide) {
+    const float4 a = *(const float4*)((const float*)p + at), b = *(const float4*)((const float*)p + at + 4);
+    out[0] = a.x, out[1] = a.y, out[2] = a.z, out[3] = a.w, out[4] = b.x, out[5] = b.y, out[6] = b.z, out[7] = b.w;
+  } else {
+    const uint4 w = *(const uint4*)((const uint16_t*)p + at);
+    const lkv::RowWords<DT, 8> words = {{w.x, w.y, w.z, w.w}};
+    lkv::widen_row_words<DT, 8>(words, out);
+  }
+}
+
+// Sixteen lanes (head_dim 128) or eight (64) hold a head of a token, 8 channels a lane, the heads of a token next to each other.
+// The channel half a rotation away is loaded again rather than sent by the lane that has it: it is in the cache line or the next, and any
+// rotary width takes the same path.
+template <int DT, int D, bool MX>
+__global__ __launch_bounds__(256) void rotate_append_kernel(RotateArgs a) {
+  constexpr int LPR = D / 8;
+  const uint32_t piece = blockIdx.x * (256u / LPR) + threadIdx.x / LPR;
+  const int c = (threadIdx.x % LPR) * 8;
+  if (piece >= a.pieces) return;  // whole heads leave: the quads of the others stay complete
+  const uint32_t bt = piece / a.heads, head = piece - bt * a.heads;
+  const uint32_t b = bt / (uint32_t)a.d.tokens, t = bt - b * (uint32_t)a.d.tokens;
+  const bool is_q = head < (uint32_t)a.d.n_q, is_v = head >= (uint32_t)(a.d.n_q + a.d.n_kv);
+  const int h = (int)(is_q ? head : is_v ? head - a.d.n_q - a.d.n_kv : head - a.d.n_q);
+  int64_t to = 0;
+  if (!is_q) {
+    if (a.counts && (int)t >= a.counts[b]) return;
+    to = lkv::row_of<D>(a.rows, (int)b, h, (int64_t)a.start + (a.starts ? a.starts[b] : 0) + t);
+    if (to < 0) return;
+  }
+  const int64_t* st = is_q ? a.d.q_stride : is_v ? a.d.v_stride : a.d.k_stride;
+  const uint16_t* x = (is_q ? a.q : is_v ? a.v : a.k) + b * st[0] + h * st[1] + t * st[2];
+  const uint4 raw = *(const uint4*)(x + c);
+  uint4 word = raw;
+  if (!is_v) {
+    const lkv::RowWords<DT, 8> words = {{raw.x, raw.y, raw.z, raw.w}};
+    float y[8];
+    lkv::widen_row_words<DT, 8>(words, y);
+    const int half = a.d.rotary / 2;
+    const bool turns = c < a.d.rotary;
+    const int other = c < half ? c + half : c - half;
+    float z[8], cs[8], sn[8];
+    if (turns) {
+      load_eight<DT>(x, other, false, z);
+      const int64_t at = b * a.d.table_seq_stride + (int64_t)t * a.d.rotary + c;
+      load_eight<DT>(a.cos, at, a.d.table_dtype == LKV_F32, cs);
+      load_eight<DT>(a.sin, at, a.d.table_dtype == LKV_F32, sn);
+    }
+    const void* weight = is_q ? a.q_weight : a.k_weight;
+    if (weight) {
+      float sum = 0.0f, w[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(y[i], y[i], sum);
+      const float inverse = 1.0f / sqrtf(lkv::row_sum<LPR>(sum) * (1.0f / D) + a.d.eps);
+      const bool wide = a.d.weight_dtype == LKV_F32;
+      load_eight<DT>(weight, c, wide, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] *= inverse * w[i];
+      if (turns) {
+        load_eight<DT>(weight, other, wide, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] *= inverse * w[i];
+      }
+    }
+    if (turns) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = y[i] * cs[i] + (c < half ? -z[i] : z[i]) * sn[i];
+    }
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      w[i] = (uint32_t)lkv::Elem<DT>::store(y[2 * i]) | ((uint32_t)lkv::Elem<DT>::store(y[2 * i + 1]) << 16);
+    word = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  if (is_q) {
+    *(uint4*)(a.q_out + b * a.d.out_stride[0] + h * a.d.out_stride[1] + t * a.d.out_stride[2] + c) = word;
+    return;
+  }
+  if constexpr (MX) {
+    // From the rounded values: the cache does not tell by which call a token came.
+    const lkv::RowWords<DT, 8> words = {{word.x, word.y, word.z, word.w}};
+    float y[8];
+    lkv::widen_row_words<DT, 8>(words, y);
+    uint32_t scale;
+    const uint2 codes = lkv::mx_encode<DT>(y, scale);
+    *(uint2*)((uint8_t*)(is_v ? a.rows.rows.v : a.rows.rows.k) + to + c) = codes;
+    if ((threadIdx.x & 3) == 0) ((uint8_t*)(is_v ? a.rows.rows.v_scale : a.rows.rows.k_scale))[(to + c) / kMxGroup] = (uint8_t)scale;
+  } else {
+    *(uint4*)((uint16_t*)(is_v ? a.rows.rows.v : a.rows.rows.k) + to + c) = word;
+  }
+}
+
+}  // namespace
+
+extern "C" int lkv_rotate_append(uintptr_t stream, const lkv_rotate_desc* desc, const void* q, const void* k, const void* v, const void* cos, const void* sin,
+                                 const void* q_weight, const void* k_weight, void* q_out, const lkv_kv_rows* dst, const lkv_pages* pages,
+                                 const int32_t* starts, int start, const int32_t* counts) {
+  LKV_CHECK_ARG(desc && q && k && v && q_out, "NULL pointer");
+  const lkv_rotate_desc& d = *desc;
+  LKV_CHECK_ARG(d.dtype == LKV_F16 || d.dtype == LKV_BF16, "tokens are float16 or bfloat16, got dtype %d", d.dtype);
+  LKV_CHECK_ARG(d.head_dim == 64 || d.head_dim == 128, "head_dim %d unsupported (64 or 128)", d.head_dim);
+  LKV_CHECK_ARG(d.n_seqs >= 0 && d.n_q > 0 && d.n_kv > 0 && d.tokens >= 0, "bad shape: %d sequences, %d and %d heads, %d tokens", d.n_seqs, d.n_q, d.n_kv, d.tokens);
+  LKV_CHECK_ARG(d.rotary >= 0 && d.rotary <= d.head_dim && d.rotary % 16 == 0, "%d channels rotated: a multiple of 16, at most %d", d.rotary, d.head_dim);
+  LKV_CHECK_ARG(d.rotary == 0 || (cos && sin), "a rotation without its tables");
+  LKV_CHECK_ARG(d.rotary == 0 || d.table_dtype == d.dtype || d.table_dtype == LKV_F32, "tables of dtype %d", d.table_dtype);
+  LKV_CHECK_ARG((!q_weight && !k_weight) || d.weight_dtype == d.dtype || d.weight_dtype == LKV_F32, "weights of dtype %d", d.weight_dtype);
+  LKV_CHECK_ARG(d.eps >= 0.0f && d.eps < INFINITY, "eps %g", (double)d.eps);
+  uintptr_t all = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out | (uintptr_t)q_weight | (uintptr_t)k_weight;
+  if (d.rotary) all |= (uintptr_t)cos | (uintptr_t)sin;
+  LKV_CHECK_ARG((all & 15) == 0, "tokens, tables and weights must start on 16 bytes");
+  int64_t strides = d.table_seq_stride;
+  for (int i = 0; i < 3; ++i) strides |= d.q_stride[i] | d.k_stride[i] | d.v_stride[i] | d.out_stride[i];
+  LKV_CHECK_ARG((strides & 7) == 0, "strides must be multiples of 8 elements");
+  RotateArgs a = {};
+  if (int rc = lkv_paged_rows(dst, pages, d.n_seqs, d.dtype, d.head_dim, a.rows)) return rc;
+  if (!starts) LKV_CHECK_ARG(start >= 0 && (int64_t)start + d.tokens <= a.rows.capacity, "rows %d..%lld exceed the %d there are", start,
+                             (long long)start + d.tokens, a.rows.capacity);
+  const int64_t heads = (int64_t)d.n_q + 2 * (int64_t)d.n_kv, n = heads * d.n_seqs * d.tokens;
+  LKV_CHECK_ARG(heads < (1LL << 31) && (int64_t)d.n_seqs * d.tokens < (1LL << 31) && n < (1LL << 31), "%lld heads of tokens in one call", (long long)n);
+  if (n == 0) return LKV_OK;
+  if (int rc = lkv_distinct_dst(dst, d.n_kv, d.head_dim)) return rc;
+  if (int rc = lkv_distinct_rows("q_out", q_out, nullptr, 2, d.n_seqs, d.n_q, d.tokens, d.head_dim, d.out_stride[0], d.out_stride[1], d.out_stride[2])) return rc;
+  a.d = d;
+  a.q = (const uint16_t*)q;
+  a.k = (const uint16_t*)k;
+  a.v = (const uint16_t*)v;
+  a.cos = cos;
+  a.sin = sin;
+  a.q_weight = q_weight;
+  a.k_weight = k_weight;
+  a.q_out = (uint16_t*)q_out;
+  a.starts = starts;
+  a.counts = counts;
+  a.start = start;
+  a.heads = (uint32_t)heads;
+  a.pieces = (uint32_t)n;
+  const bool mx = dst->dtype == LKV_MXFP8, half = d.dtype == LKV_F16, wide = d.head_dim == 128;
+  auto kernel = half ? (wide ? (mx ? rotate_append_kernel<LKV_F16, 128, true> : rotate_append_kernel<LKV_F16, 128, false>)
+                             : (mx ? rotate_append_kernel<LKV_F16, 64, true> : rotate_append_kernel<LKV_F16, 64, false>))
+                     : (wide ? (mx ? rotate_append_kernel<LKV_BF16, 128, true> : rotate_append_kernel<LKV_BF16, 128, false>)
+                             : (mx ? rotate_append_kernel<LKV_BF16, 64, true> : rotate_append_kernel<LKV_BF16, 64, false>));
+  const uint32_t per = 256 / (d.head_dim / 8);
+  hipLaunchKernelGGL(kernel, dim3((a.pieces + per - 1) / per), dim3(256), 0, (hipStream_t)stream, a);
+  LKV_CHECK_LAUNCH("rotate_append");
+  return LKV_OK;
+}

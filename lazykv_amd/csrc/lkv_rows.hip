@@ -43,38 +43,9 @@ __global__ __launch_bounds__(256) void append_rows_kernel(RowPlan p, const uint1
       lkv::RowWords<DT, 8> words = {{w.x, w.y, w.z, w.w}};
       float x[8];
       lkv::widen_row_words<DT, 8>(words, x);
-      float most = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float a = fabsf(x[i]);
-        const bool fine = a < INFINITY;
-        most = fmaxf(most, fine ? a : 0.0f);
-        x[i] = fine ? x[i] : NAN;
-      }
-      most = fmaxf(most, lkv::dpp<lkv::kDppQuadSwap1>(most));
-      most = fmaxf(most, lkv::dpp<lkv::kDppQuadSwap2>(most));
-      // 448 = 1.75 * 2^8.
-      const float top = fminf(most, lkv::mx_largest<DT>());
-      const uint32_t bits = lkv::float_to_bits(top);
-      const int e = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
-      const uint32_t scale = e > 0 ? e : 0;
-      const float up = lkv::bits_to_float((254u - scale) << 23);
-      uint32_t code[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float y[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float v = x[4 * i + j];
-          // A NaN passes both comparisons' selects.
-          const float lim = v > lkv::mx_largest<DT>() ? lkv::mx_largest<DT>() : (v < -lkv::mx_largest<DT>() ? -lkv::mx_largest<DT>() : v);
-          y[j] = lim * up;
-        }
-        int packed = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-        packed = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], packed, true);
-        code[i] = (uint32_t)packed;
-      }
-      *(uint2*)((which ? cv : ck) + dst) = make_uint2(code[0], code[1]);
+      uint32_t scale;
+      const uint2 codes = lkv::mx_encode<DT>(x, scale);
+      *(uint2*)((which ? cv : ck) + dst) = codes;
       if ((threadIdx.x & 3) == 0) (which ? sv : sk)[dst / kMxGroup] = (uint8_t)scale;
     }
   }
@@ -166,16 +137,6 @@ bool rows_apart(Dim (&dims)[4], int64_t length) {
   return true;
 }
 
-// Two rows that are written must not share an address. Strides and head_dim are in elements of `bytes` bytes.
-int distinct_rows(const char* what, const void* k, const void* v, int bytes, int n_seqs, int n_kv, int64_t tokens, int head_dim, int64_t seq_stride,
-                  int64_t head_stride, int64_t token_stride) {
-  const int64_t apart = (int64_t)((uintptr_t)v - (uintptr_t)k);
-  Dim dims[4] = {{2, apart}, {n_seqs, seq_stride * bytes}, {n_kv, head_stride * bytes}, {tokens, token_stride * bytes}};
-  if (token_stride == head_dim) dims[3] = {1, 0};
-  LKV_CHECK_ARG(rows_apart(dims, (token_stride == head_dim ? tokens : 1) * head_dim * bytes), "%s: rows that are written share an address", what);
-  return LKV_OK;
-}
-
 // The checks that both calls share; a plan without rows is a call without work.
 int row_plan(const lkv_kv_rows* rows, const void* k, const void* v, int dtype, int64_t seq_stride, int64_t head_stride,
              int64_t token_stride, int n_seqs, int n_kv, int head_dim, int tokens, RowPlan& p) {
@@ -194,6 +155,24 @@ int row_plan(const lkv_kv_rows* rows, const void* k, const void* v, int dtype, i
 
 }  // namespace
 
+// Two rows that are written must not share an address. Strides and head_dim are in elements of `bytes` bytes.
+int lkv_distinct_rows(const char* what, const void* k, const void* v, int bytes, int n_seqs, int n_kv, int64_t tokens, int head_dim, int64_t seq_stride,
+                  int64_t head_stride, int64_t token_stride) {
+  const int64_t apart = (int64_t)((uintptr_t)v - (uintptr_t)k);
+  Dim dims[4] = {{v ? 2 : 1, apart}, {n_seqs, seq_stride * bytes}, {n_kv, head_stride * bytes}, {tokens, token_stride * bytes}};
+  if (token_stride == head_dim) dims[3] = {1, 0};
+  LKV_CHECK_ARG(rows_apart(dims, (token_stride == head_dim ? tokens : 1) * head_dim * bytes), "%s: rows that are written share an address", what);
+  return LKV_OK;
+}
+
+int lkv_distinct_dst(const lkv_kv_rows* dst, int n_kv, int head_dim) {
+  const int es = dst->dtype == LKV_MXFP8 ? 1 : 2;
+  if (int rc = lkv_distinct_rows("dst", dst->k, dst->v, es, dst->seqs, n_kv, dst->tokens, head_dim, dst->seq_stride, dst->head_stride, head_dim)) return rc;
+  if (es == 2) return LKV_OK;
+  return lkv_distinct_rows("dst's scales", dst->k_scale, dst->v_scale, 1, dst->seqs, n_kv, dst->tokens, head_dim / kMxGroup, dst->seq_stride / kMxGroup,
+                           dst->head_stride / kMxGroup, head_dim / kMxGroup);
+}
+
 extern "C" int lkv_append_rows(uintptr_t stream, const lkv_kv_rows* dst, const void* k, const void* v, int dtype, int64_t seq_stride,
                                int64_t head_stride, int64_t token_stride, int n_seqs, int n_kv, int head_dim, int tokens,
                                const int32_t* starts, int start) {
@@ -202,13 +181,7 @@ extern "C" int lkv_append_rows(uintptr_t stream, const lkv_kv_rows* dst, const v
   if (!starts) LKV_CHECK_ARG(start >= 0 && (int64_t)start + tokens <= dst->tokens, "rows %d..%lld exceed the %lld there are", start,
                              (long long)start + tokens, (long long)dst->tokens);
   if (p.rows == 0) return LKV_OK;
-  const int es = dst->dtype == LKV_MXFP8 ? 1 : 2;
-  if (int rc = distinct_rows("dst", dst->k, dst->v, es, n_seqs, n_kv, dst->tokens, head_dim, dst->seq_stride, dst->head_stride, head_dim)) return rc;
-  if (es == 1) {
-    if (int rc = distinct_rows("dst's scales", dst->k_scale, dst->v_scale, 1, n_seqs, n_kv, dst->tokens, head_dim / kMxGroup, dst->seq_stride / kMxGroup,
-                               dst->head_stride / kMxGroup, head_dim / kMxGroup))
-      return rc;
-  }
+  if (int rc = lkv_distinct_dst(dst, n_kv, head_dim)) return rc;
   p.start = start;
   p.starts = starts;
   const bool mx = dst->dtype == LKV_MXFP8, half = dtype == LKV_F16, wide = head_dim == 128;
@@ -230,7 +203,7 @@ extern "C" int lkv_read_rows(uintptr_t stream, const lkv_kv_rows* src, int n_seq
   LKV_CHECK_ARG(first >= 0 && (int64_t)first + tokens <= src->tokens, "rows %d..%lld exceed the %lld there are", first,
                 (long long)first + tokens, (long long)src->tokens);
   if (p.rows == 0) return LKV_OK;
-  if (int rc = distinct_rows("out", k, v, 2, n_seqs, n_kv, tokens, head_dim, seq_stride, head_stride, token_stride)) return rc;
+  if (int rc = lkv_distinct_rows("out", k, v, 2, n_seqs, n_kv, tokens, head_dim, seq_stride, head_stride, token_stride)) return rc;
   p.start = first;
   const bool half = dtype == LKV_F16, wide = head_dim == 128;
   auto kernel = half ? (wide ? read_rows_kernel<LKV_F16, 128> : read_rows_kernel<LKV_F16, 64>)

@@ -1,0 +1,267 @@
+// The weights that rows get from a chunk's tokens, summed up (lkv_weigh_rows):
+//   sum_i = sum over the KV head's query heads and the tokens that attend row i of exp(scale q . k_i - lse).
+//
+// A wave holds 64 rows' keys as the second operand of v_mfma_f32_16x16x32 and takes the query rows 16 at a time as the first,
+// S [16 queries x 16 rows] = Q K^T, so that a row's scores lie in one lane of each quarter: its sum stays there from the first query to the last.
+// The accumulators start at -lse / scale, and the scores come out relative to it.
+#include "lkv_attend.h"
+#include "lkv_pages.h"
+
+int lkv_check_chunk(const lkv_chunk_desc* d);  // lkv_chunk.hip
+
+namespace {
+
+using namespace lkv;
+
+constexpr int kWaves = 4;
+constexpr int kWaveRows = 64;
+constexpr int kBlockRows = kWaves * kWaveRows;
+
+struct WeighArgs {
+  const uint16_t* q;
+  const float* lse;
+  PagedRows rows;
+  const int32_t *lengths, *counts, *seen;
+  const float* sums;
+  float* out;
+  int32_t* positions;
+  float* part;  // [parts][sequences * KV heads][padded rows]
+  int64_t q_stride[3], sums_stride[2], out_stride[2], positions_stride[2];
+  float scale2, per_scale;  // scale * log2(e), 1 / scale
+  int32_t n_seqs, n_q, n_kv, g, new_tokens, tokens, max_tokens;
+  int32_t blocks, parts, chunk;  // of a KV head's rows; of its query rows, in ranges of `chunk`
+};
+
+struct Extent {
+  int len, n;
+};
+__device__ __forceinline__ Extent extent_of(const WeighArgs& a, int b) {
+  const int64_t len = (int64_t)a.tokens + (a.lengths ? a.lengths[b] : 0);
+  const int n = a.counts ? a.counts[b] : a.new_tokens;
+  return {(int)(len < 0 ? 0 : (len > a.max_tokens ? a.max_tokens : len)), n < 0 ? 0 : (n > a.new_tokens ? a.new_tokens : n)};
+}
+
+// A row's sum of the call, where it belongs.
+__device__ __forceinline__ void store_sum(const WeighArgs& a, const Extent& e, int b, int h, int row, float got) {
+  if (row >= e.len) return;
+  const int past = e.len - e.n;
+  if (row < past && a.sums) got += a.sums[b * a.sums_stride[0] + h * a.sums_stride[1] + row];
+  a.out[b * a.out_stride[0] + h * a.out_stride[1] + row] = got;
+  if (a.positions && row >= past && row >= 0)
+    a.positions[b * a.positions_stride[0] + h * a.positions_stride[1] + row] = (a.seen ? a.seen[b] : max(past, 0)) + row - past;
+}
+
+// Sixteen query rows as the lanes hold them.
+template <int D, bool MX> struct QueryRegs {
+  uint4 w[D / 32];
+  float start;  // -lse / scale; -inf for a row that is not there or attends nothing
+  int limit;
+  __device__ __forceinline__ void load(const WeighArgs& a, const Extent& e, int b, int h, int x) {
+    const int quarter = (threadIdx.x & 63) >> 4;
+    const int t = x / a.g, j = h * a.g + (x - t * a.g);
+    const bool live = t < e.n;
+    start = -INFINITY;
+    limit = live ? e.len - e.n + t + 1 : 0;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) w[i] = make_uint4(0, 0, 0, 0);
+    if (live) {
+      const uint16_t* q = a.q + b * a.q_stride[0] + j * a.q_stride[1] + t * a.q_stride[2];
+      const float lse = a.lse[((int64_t)b * a.n_q + j) * a.new_tokens + t];
+      const bool adds = lse != -INFINITY;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        const uint4 x = *(const uint4*)(q + KeyRegs<D, MX>::channel(quarter, i));
+        w[i] = adds ? x : w[i];
+      }
+      start = adds ? -lse * a.per_scale : -INFINITY;
+    }
+  }
+};
+
+template <int DT, int D, bool MX>
+__global__ __launch_bounds__(64 * kWaves, 2) void weigh_rows_kernel(WeighArgs a) {
+  const int lane = threadIdx.x & 63, quarter = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int id = blockIdx.x;
+  const int heads = a.n_seqs * a.n_kv, bh = id % heads;
+  id /= heads;
+  const int part = id % a.parts, block = id / a.parts, b = bh / a.n_kv, h = bh % a.n_kv;
+  const Extent e = extent_of(a, b);
+  const int row0 = block * kBlockRows + wave * kWaveRows;
+  if (row0 >= e.len) return;
+  KeyRegs<D, MX> k[2];
+  bool there[2][2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int t = min(row0 + 32 * u, (e.len - 1) & ~31), last = min(kTile, e.len - t) - 1;
+    LaneOffsets<D, MX> at;
+    at.set(last);
+    Stream s[2];
+    const Sixteen x0 = sixteen_of<D>(a.rows, b, h, t >> 4), x1 = last >= 16 ? sixteen_of<D>(a.rows, b, h, (t >> 4) + 1) : Sixteen{x0.at + 16 * D, x0.there};
+    const int64_t e0 = x0.at, e1 = x1.at - 16 * D;  // as if the tile lay together
+    s[0] = {(const uint8_t*)a.rows.rows.k + (MX ? e0 : 2 * e0), nullptr, MX ? a.rows.rows.k_scale + e0 / kMxGroup : nullptr, nullptr};
+    s[1] = {(const uint8_t*)a.rows.rows.k + (MX ? e1 : 2 * e1), nullptr, MX ? a.rows.rows.k_scale + e1 / kMxGroup : nullptr, nullptr};
+    there[u][0] = x0.there;
+    there[u][1] = x1.there;
+    k[u].load(s, at);
+  }
+  float sum[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
+  // The first query that attends the wave's first row, and the first one that attends all its rows.
+  const int past = e.len - e.n, x_end = min(e.n * a.g, (part + 1) * a.chunk);
+  const int x_first = max(part * a.chunk, max(row0 - past, 0) * a.g & ~15), x_whole = max(row0 + kWaveRows - 1 - past, 0) * a.g;
+  if (x_first < x_end) {
+    QueryRegs<D, MX> now, next;
+    now.load(a, e, b, h, x_first + (lane & 15));
+    for (int x = x_first; x < x_end; x += 16) {
+      next.load(a, e, b, h, min(x + 16, x_end - 1) + (lane & 15));
+      load_fence();
+      f32x4 start;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) start[i] = __shfl(now.start, (lane & 48) + 4 * quarter + i);
+      f32x4 sc[2][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          sc[u][w] = start;
+#pragma unroll
+          for (int i = 0; i < D / 32; ++i) sc[u][w] = Mat<DT>::mma(now.w[i], k[u].template operand<DT>(w, i), sc[u][w]);
+        }
+      if (x < x_whole) {
+        int limit[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) limit[i] = __shfl(now.limit, (lane & 48) + 4 * quarter + i) - row0 - (lane & 15);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int w = 0; w < 2; ++w)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float y = 32 * u + 16 * w < limit[i] ? sc[u][w][i] : -INFINITY;
+              keep_here(y);
+              sc[u][w][i] = y;
+            }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          float p[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(sc[u][w][i] * a.scale2);
+          sum[u][w] += (p[0] + p[1]) + (p[2] + p[3]);
+        }
+      now = next;
+    }
+  }
+  // Each quarter stores sixteen of the wave's rows.
+  float mine = 0.0f;
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const float total = pair_sum<32>(pair_sum<16>(sum[u][w]));
+      mine = quarter == 2 * u + w ? (there[u][w] ? total : 0.0f) : mine;
+    }
+  if (a.parts > 1) {
+    a.part[((int64_t)part * heads + bh) * a.blocks * kBlockRows + row0 + lane] = mine;
+  } else {
+    store_sum(a, e, b, h, row0 + lane, mine);
+  }
+}
+
+// The parts' sums of a row, in their order.
+__global__ __launch_bounds__(256) void weigh_join_kernel(WeighArgs a) {
+  const int heads = a.n_seqs * a.n_kv, bh = blockIdx.x % heads, row = blockIdx.x / heads * kBlockRows + threadIdx.x, b = bh / a.n_kv, h = bh % a.n_kv;
+  const Extent e = extent_of(a, b);
+  if (row >= e.len) return;
+  float got = 0.0f;
+  for (int p = 0; p < a.parts; ++p) got += a.part[((int64_t)p * heads + bh) * a.blocks * kBlockRows + row];
+  store_sum(a, e, b, h, row, got);
+}
+
+int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+struct Plan {
+  int blocks, parts, chunk;
+};
+Plan plan_of(const lkv_chunk_desc* d) {
+  Plan p = {};
+  const int64_t x = (int64_t)d->new_tokens * (d->n_q / d->n_kv);
+  p.blocks = ceil_div(d->max_tokens, kBlockRows);
+  const int64_t units = (int64_t)d->n_seqs * d->n_kv * p.blocks;
+  int64_t parts = units > 0 ? 1024 / units : 1;
+  const int64_t most = x / 128;
+  parts = parts > most ? most : parts;
+  parts = parts < 1 ? 1 : parts;
+  p.chunk = ceil_div(ceil_div(x, parts), 16) * 16;
+  p.chunk = p.chunk < 16 ? 16 : p.chunk;
+  p.parts = ceil_div(x, p.chunk);
+  p.parts = p.parts < 1 ? 1 : p.parts;
+  return p;
+}
+
+}  // namespace
+
+extern "C" size_t lkv_weigh_rows_workspace_bytes(const lkv_chunk_desc* desc) {
+  if (lkv_check_chunk(desc)) return 0;
+  const Plan p = plan_of(desc);
+  return p.parts < 2 ? 0 : (size_t)p.parts * desc->n_seqs * desc->n_kv * p.blocks * kBlockRows * sizeof(float);
+}
+
+extern "C" int lkv_weigh_rows(uintptr_t stream, const lkv_chunk_desc* desc, const void* q, int q_dtype, const float* lse, const lkv_kv_rows* rows,
+                              const lkv_pages* pages, const int32_t* lengths, const int32_t* counts, const float* sums, const int64_t* sums_stride, float* out,
+                              const int64_t* out_stride, int32_t* positions, const int64_t* positions_stride, const int32_t* seen, void* ws, size_t ws_bytes) {
+  if (int rc = lkv_check_chunk(desc)) return rc;
+  LKV_CHECK_ARG(q && lse && out && out_stride && (!sums || sums_stride) && (!positions || positions_stride), "NULL pointer");
+  LKV_CHECK_ARG(q_dtype == LKV_F16 || q_dtype == LKV_BF16, "queries are float16 or bfloat16, got dtype %d", q_dtype);
+  LKV_CHECK_ARG(((uintptr_t)q & 15) == 0, "queries must start on 16 bytes");
+  WeighArgs a = {};
+  if (int rc = lkv_paged_rows(rows, pages, desc->n_seqs, q_dtype, desc->head_dim, a.rows)) return rc;
+  LKV_CHECK_ARG(desc->max_tokens <= a.rows.capacity, "%d rows of a sequence over %d", desc->max_tokens, a.rows.capacity);
+  const size_t need = lkv_weigh_rows_workspace_bytes(desc);
+  LKV_CHECK_ARG(need == 0 || (ws && ws_bytes >= need && ((uintptr_t)ws & 15) == 0), "workspace of %zu bytes, on 16: %zu are needed", ws_bytes, need);
+  const Plan p = plan_of(desc);
+  const int64_t blocks = (int64_t)desc->n_seqs * desc->n_kv * p.blocks;
+  LKV_CHECK_ARG(blocks * p.parts < (1LL << 31), "%lld workgroups in one call", (long long)blocks * p.parts);
+  if (blocks == 0) return LKV_OK;
+  a.q = (const uint16_t*)q;
+  a.lse = lse;
+  a.lengths = lengths;
+  a.counts = counts;
+  a.seen = seen;
+  a.sums = sums;
+  a.out = out;
+  a.positions = positions;
+  a.part = (float*)ws;
+  for (int i = 0; i < 3; ++i) a.q_stride[i] = desc->q_stride[i];
+  for (int i = 0; i < 2; ++i) {
+    a.sums_stride[i] = sums ? sums_stride[i] : 0;
+    a.out_stride[i] = out_stride[i];
+    a.positions_stride[i] = positions ? positions_stride[i] : 0;
+  }
+  a.scale2 = desc->scale * kLog2e;
+  a.per_scale = 1.0f / desc->scale;
+  a.n_seqs = desc->n_seqs;
+  a.n_q = desc->n_q;
+  a.n_kv = desc->n_kv;
+  a.g = desc->n_q / desc->n_kv;
+  a.new_tokens = desc->new_tokens;
+  a.tokens = desc->tokens;
+  a.max_tokens = desc->max_tokens;
+  a.blocks = p.blocks;
+  a.parts = p.parts;
+  a.chunk = p.chunk;
+  const hipStream_t s = (hipStream_t)stream;
+  const bool half = q_dtype == LKV_F16, wide = desc->head_dim == 128, mx = rows->dtype == LKV_MXFP8;
+  auto kernel = half ? (wide ? (mx ? weigh_rows_kernel<LKV_F16, 128, true> : weigh_rows_kernel<LKV_F16, 128, false>)
+                             : (mx ? weigh_rows_kernel<LKV_F16, 64, true> : weigh_rows_kernel<LKV_F16, 64, false>))
+                     : (wide ? (mx ? weigh_rows_kernel<LKV_BF16, 128, true> : weigh_rows_kernel<LKV_BF16, 128, false>)
+                             : (mx ? weigh_rows_kernel<LKV_BF16, 64, true> : weigh_rows_kernel<LKV_BF16, 64, false>));
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks * p.parts)), dim3(64 * kWaves), 0, s, a);
+  LKV_CHECK_LAUNCH("weigh_rows");
+  if (p.parts > 1) {
+    hipLaunchKernelGGL(weigh_join_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a);
+    LKV_CHECK_LAUNCH("weigh_rows (join)");
+  }
+  return LKV_OK;
+}

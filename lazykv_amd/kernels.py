@@ -921,6 +921,343 @@ def shared_decode(
     return out, lse
 
 
+# -- a layer's forward over a bounded cache in pages -------------------------------------------------------
+
+
+def _paged(rows: Rows, pages: torch.Tensor | None, seqs: int) -> tuple[object, int]:
+    """(the C call's page table or None, rows that a sequence can have): `rows` are `seqs` sequences' own, or a pool of pages that the table
+    `pages` [seqs, n] (int32, on the device) names."""
+    if pages is None:
+        if rows.seqs != seqs:
+            raise ValueError(f"rows of {rows.seqs} sequences, tokens of {seqs}")
+        return None, rows.tokens
+    shape, st = pages.shape, pages.stride()
+    if len(shape) != 2 or shape[0] != seqs or pages.dtype != torch.int32 or pages.get_device() != rows.device_index or (st[1] != 1 and shape[1] > 1) or st[0] < 0:
+        raise ValueError(f"pages must be int32 [{seqs}, n] with contiguous rows on {rows.device}, got {pages.dtype} {tuple(shape)} on {pages.device}")
+    return ctypes.byref(_lib.Pages(pages.data_ptr() or None, st[0], shape[1])), rows.tokens * shape[1]
+
+
+def _reach(x: torch.Tensor) -> tuple[int, int]:
+    """The addresses between which a tensor's elements lie."""
+    at = x.data_ptr()
+    if x.numel() == 0:
+        return at, at
+    return at, at + x.element_size() * (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride())))
+
+
+def _meets(x: torch.Tensor, spans: tuple) -> bool:
+    a, b = _reach(x)
+    return any(a < d and c < b for c, d in spans)
+
+
+def _row_spans(rows: Rows) -> tuple:
+    """Where the rows lie, of a cache in the model dtype."""
+    if rows.span is None:
+        return ()
+    k, v, n = rows.span
+    return (k, k + n), (v, v + n)
+
+
+def rotate_append(
+    dst: Rows,
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    *,
+    cos: torch.Tensor | None = None,
+    sin: torch.Tensor | None = None,
+    q_weight: torch.Tensor | None = None,
+    k_weight: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    start: int = 0,
+    starts: torch.Tensor | None = None,
+    counts: torch.Tensor | None = None,
+    pages: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """New tokens on their way into a cache (lkv_rotate_append): queries q `[seqs, n_q, T, d]` and keys k `[seqs, h, T, d]` normalised over each head
+    (where `q_weight` / `k_weight` `[d]` are given: x / sqrt(mean x^2 + eps) * weight) and their first r channels rotated by `cos` / `sin`
+    `[seqs or 1, T, r]` (a model's rotary tables, halves paired: channel i with i + r / 2), in float32 and rounded once. Keys and values become rows
+    `start + starts[b] + t` of `dst`, as with `append_rows`, with `pages` `[seqs, n]` those of a pool; tokens from `counts[b]` on go to no row.
+    Returns the queries (in `out`, which must not be any of the inputs). No gradient."""
+    shape, kv, dtype, index = q.shape, k.shape, dst.model_dtype, dst.device_index
+    if len(shape) != 4 or len(kv) != 4 or v.shape != kv or kv[0] != shape[0] or kv[2:] != shape[2:] or q.dtype != dtype or k.dtype != dtype or v.dtype != dtype:
+        raise ValueError(f"expected {dtype} queries [seqs, n_q, T, d] and matching keys/values [seqs, h, T, d], got {tuple(shape)} {q.dtype}, {tuple(kv)} {k.dtype}, "
+                         f"{tuple(v.shape)} {v.dtype}")
+    seqs, n_q, n, d = shape
+    if kv[1] != dst.n_kv or d != dst.head_dim:
+        raise ValueError(f"keys/values {tuple(kv)} do not match rows of {dst.n_kv} heads and head_dim {dst.head_dim}")
+    if q.get_device() != index or k.get_device() != index or v.get_device() != index:
+        raise ValueError(f"tokens on {q.device} / {k.device} / {v.device}, the cache on {dst.device}")
+    _int32("start", start)
+    rotary = table_stride = 0
+    table = weight = dst.model_code
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin come together")
+    if cos is not None:
+        cs = cos.shape
+        if len(cs) != 3 or cs[0] not in (1, seqs) or cs[1] != n or sin.shape != cs or cos.dtype != sin.dtype or cos.dtype not in (dtype, torch.float32):
+            raise ValueError(f"cos/sin must be {dtype} or float32 [{seqs} or 1, {n}, r], got {cos.dtype} {tuple(cs)} / {sin.dtype} {tuple(sin.shape)}")
+        if cos.get_device() != index or sin.get_device() != index:
+            raise ValueError(f"cos/sin on {cos.device} / {sin.device}, the cache on {dst.device}")
+        rotary = cs[2]
+        cos, sin = _whole(cos), _whole(sin)
+        table_stride = n * rotary if cs[0] != 1 else 0
+        table = _lib.dtype_code(cos.dtype)
+    for w in (q_weight, k_weight):
+        if w is not None and (w.shape != (d,) or w.dtype not in (dtype, torch.float32) or w.get_device() != index):
+            raise ValueError(f"weights must be {dtype} or float32 [{d}] on {dst.device}, got {w.dtype} {tuple(w.shape)} on {w.device}")
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise ValueError(f"weights of {q_weight.dtype} and {k_weight.dtype}")
+    if q_weight is not None or k_weight is not None:
+        weight = _lib.dtype_code((q_weight if q_weight is not None else k_weight).dtype)
+        q_weight, k_weight = (w if w is None else _whole(w) for w in (q_weight, k_weight))
+    given = tuple(x for x in (cos, sin, q_weight, k_weight, out) if x is not None)
+    _no_gradients("rotate_append", (q, k, v, *dst.owners, *given))
+    at, count = _counts(starts, seqs, index, "starts"), _counts(counts, seqs, index, "counts")
+    table_ref, _ = _paged(dst, pages, seqs)
+    if out is not None:
+        if out.shape != shape or out.dtype != dtype or out.get_device() != index:
+            raise ValueError(f"out must be {dtype} {tuple(shape)} on {dst.device}, got {out.dtype} {tuple(out.shape)} on {out.device}")
+        ot = _meant(shape, out.stride())
+        if ot[3] != 1 or (ot[0] | ot[1] | ot[2]) % 8 or out.data_ptr() % 16:
+            raise ValueError("out's rows must be contiguous and start on 16 bytes")
+        if _meets(out, (*(_reach(x) for x in (q, k, v, *given[:-1])), *_row_spans(dst))):
+            raise ValueError("out must not lie among the inputs or the cache's rows")
+    if 0 in shape:
+        return q.new_empty(shape) if out is None else out
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=q.device)
+    (x, xt), (y, yt), (z, zt) = _placed(q), _placed(k), _placed(v)
+    spans = _row_spans(dst)
+    if spans:  # the cache's own rows: none is written before all are read
+        x, y, z = (w.clone(memory_format=torch.contiguous_format) if _meets(w, spans) else w for w in (x, y, z))
+        xt, yt, zt = (_meant(w.shape, w.stride()) for w in (x, y, z))
+    _WRITTEN((*dst.owners, out))
+    desc = _lib.RotateDesc(seqs, n_q, kv[1], d, n, dst.model_code, rotary, table, weight, eps, _lib.Triple(*xt[:3]), _lib.Triple(*yt[:3]), _lib.Triple(*zt[:3]),
+                           _lib.Triple(*_meant(shape, out.stride())[:3]), table_stride)
+    rc = _launch(index, _lib.lib().lkv_rotate_append, ctypes.byref(desc), x.data_ptr(), y.data_ptr(), z.data_ptr(), cos.data_ptr() if rotary else None,
+                 sin.data_ptr() if rotary else None, q_weight.data_ptr() if q_weight is not None else None, k_weight.data_ptr() if k_weight is not None else None,
+                 out.data_ptr(), dst.ref, table_ref, at, start, count)
+    if rc:
+        _lib.check(rc, "rotate_append")
+    return out
+
+
+def _whole(x: torch.Tensor) -> torch.Tensor:
+    """`x` as the kernels read tables: contiguous, on 16 bytes."""
+    return x if x.is_contiguous() and x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
+
+
+def _chunk(what: str, q: torch.Tensor, rows: Rows, scale: float, tokens: int, lengths: torch.Tensor | None, counts: torch.Tensor | None, max_tokens: int | None,
+           pages: torch.Tensor | None, others: tuple) -> tuple:
+    """What the calls over a chunk of new tokens check alike: (descriptor, queries as the kernels read them, addresses of lengths and counts, page table, the
+    most rows of a sequence)."""
+    shape, index = q.shape, rows.device_index
+    if len(shape) != 4 or q.dtype != rows.model_dtype or shape[3] != rows.head_dim or shape[1] == 0 or shape[1] % rows.n_kv or q.get_device() != index:
+        raise ValueError(f"query {tuple(shape)} {q.dtype} on {q.device} does not match {rows.model_dtype} rows of {rows.n_kv} heads and head_dim {rows.head_dim} on "
+                         f"{rows.device}")
+    seqs, n_q, n, d = shape
+    _no_gradients(what, (q, *rows.owners, *others))
+    table, room = _paged(rows, pages, seqs)
+    if max_tokens is None:
+        max_tokens = tokens if lengths is None else room
+    if (tokens | max_tokens) >> 31:
+        _int32("tokens", tokens)
+        _int32("max_tokens", max_tokens)
+    if lengths is None and tokens > max_tokens:
+        raise ValueError(f"tokens={tokens} exceed max_tokens={max_tokens}")
+    at, count = _counts(lengths, seqs, index, "lengths"), _counts(counts, seqs, index, "counts")
+    q, st = _placed(q)
+    return _lib.ChunkDesc(seqs, n_q, rows.n_kv, d, n, scale, tokens, max_tokens, _lib.Triple(*st[:3])), q, at, count, table, max_tokens
+
+
+def _scratch(need: int, ws: Workspace | None, device: torch.device) -> tuple[int | None, int, object]:
+    """A call's scratch: the workspace's, or torch's own allocation, which no other call on another stream or in a graph can be in."""
+    if ws is not None:
+        return (*ws.get(need), ws)
+    if not need:
+        return None, 0, None
+    buf = torch.empty(need, dtype=torch.uint8, device=device)
+    return buf.data_ptr(), need, buf
+
+
+def chunk_attend(
+    q: torch.Tensor,
+    rows: Rows,
+    *,
+    scale: float,
+    tokens: int = 0,
+    lengths: torch.Tensor | None = None,
+    counts: torch.Tensor | None = None,
+    max_tokens: int | None = None,
+    pages: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+    out_dtype: torch.dtype | None = None,
+    lse: torch.Tensor | None = None,
+    ws: Workspace | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """A chunk of new tokens of each sequence over its rows, q `[seqs, n_q, T, d]` (lkv_chunk_attend): sequence b has
+    `len = tokens + lengths[b]` rows, at most `max_tokens` (default: `tokens` without `lengths`, else all there is room for; a bound near the lengths
+    divides the work better), the last `counts[b]` (default: T) of which are the call's own, written before it. Token t attends rows
+    0 .. len - counts[b] + t. `rows` are the sequences' own or, with `pages` `[seqs, n]`, a pool's pages, in the model dtype or in 8 bits; T = 1 is a
+    decode step. Returns (out [seqs, n_q, T, d], lse [seqs, n_q, T] float32, natural log); tokens from `counts[b]` on and tokens without any row get zeros
+    and -inf. No gradient: inputs that autograd follows are refused. Without `ws` the scratch is torch's, so calls on several streams and in
+    several graphs do not meet."""
+    given = () if out is None and lse is None else tuple(x for x in (out, lse) if x is not None)
+    desc, q, at, count, table, _ = _chunk("chunk_attend", q, rows, scale, tokens, lengths, counts, max_tokens, pages, given)
+    shape, index = q.shape, rows.device_index
+    if out is None:
+        out = torch.empty(shape, dtype=out_dtype or q.dtype, device=q.device)
+    elif not out.is_contiguous() or out.shape != shape or out.get_device() != index or (out_dtype is not None and out.dtype != out_dtype) or out.data_ptr() % 16:
+        raise ValueError(f"out must be contiguous {tuple(shape)} on {rows.device}, on 16 bytes")
+    if lse is None:
+        lse = torch.empty(shape[:3], dtype=torch.float32, device=q.device)
+    elif not lse.is_contiguous() or lse.shape != shape[:3] or lse.dtype != torch.float32 or lse.get_device() != index:
+        raise ValueError(f"lse must be contiguous float32 {tuple(shape[:3])} on {rows.device}")
+    if 0 in shape:
+        return out, lse
+    if given:
+        if any(_meets(x, (_reach(q), *_row_spans(rows))) for x in given) or (len(given) == 2 and _meets(out, (_reach(lse),))):
+            raise ValueError("out and lse must not lie among the inputs or each other")
+        _WRITTEN(given)
+    lib = _lib.lib()
+    ref = ctypes.byref(desc)
+    ws_ptr, ws_n, _held = _scratch(lib.lkv_chunk_attend_workspace_bytes(ref), ws, q.device)
+    rc = _launch(index, lib.lkv_chunk_attend, ref, q.data_ptr(), rows.model_code, rows.ref, table, at, count, out.data_ptr(), _lib.dtype_code(out.dtype),
+                 lse.data_ptr(), ws_ptr, ws_n)
+    if rc:
+        _lib.check(rc, "chunk_attend")
+    return out, lse
+
+
+def _account(name: str, x: torch.Tensor, dtype: torch.dtype, seqs: int, n_kv: int, n: int, device: int) -> object:
+    """The strides of a number for each row, `[seqs, h, n or more]`, of which no two share an address."""
+    shape, st = x.shape, x.stride()
+    if len(shape) != 3 or shape[0] != seqs or shape[1] != n_kv or shape[2] < n or x.dtype != dtype or x.get_device() != device or (st[2] != 1 and shape[2] > 1):
+        raise ValueError(f"{name} must be {dtype} [{seqs}, {n_kv}, {n} or more] with contiguous rows on cuda:{device}, got {x.dtype} {tuple(shape)} on {x.device}")
+    a, b, n = (st[0] if seqs > 1 else 0), (st[1] if n_kv > 1 else 0), shape[2]
+    if (a and b and min(a, b) < n) or (n_kv > 1 and b < n) or (seqs > 1 and a < n) or (a > b > 0 and a < b * (n_kv - 1) + n) or (0 < a <= b and b < a * (seqs - 1) + n):
+        raise ValueError(f"{name}'s rows share addresses")
+    return _lib.Pair(a, b)
+
+
+def _same_or_apart(what: str, out: torch.Tensor, x: torch.Tensor) -> None:
+    if (out.data_ptr() != x.data_ptr() or _meant(out.shape, out.stride()) != _meant(x.shape, x.stride())) and _meets(out, (_reach(x),)):
+        raise ValueError(f"{what} overlap without being the same")
+
+
+def weigh_rows(
+    q: torch.Tensor,
+    lse: torch.Tensor,
+    rows: Rows,
+    *,
+    scale: float,
+    tokens: int = 0,
+    lengths: torch.Tensor | None = None,
+    counts: torch.Tensor | None = None,
+    max_tokens: int | None = None,
+    pages: torch.Tensor | None = None,
+    sums: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+    positions: torch.Tensor | None = None,
+    seen: torch.Tensor | None = None,
+    ws: Workspace | None = None,
+) -> torch.Tensor:
+    """The weights that rows get from a chunk's tokens, summed up (lkv_weigh_rows): with q, rows and extents as `chunk_attend` took them and the `lse` that it
+    gave, each row of a KV head gets the sum of its softmax weights over the head's query heads and the tokens that attend it. That is added to
+    `sums` (float32 `[seqs, h, max_tokens or more]`) for rows from before the chunk and is the sum itself for the chunk's own, in `out` (default: `sums`, or without it
+    a new tensor of zeros); rows from a sequence's end on are left as they are. `positions` (int32, the same layout) of the chunk's rows become
+    `seen[b] + 0, 1, ..` (`seen` int32 `[seqs]`: tokens that the sequence has had before the chunk; default: the rows it has before it). Both are
+    what `evict_rows` goes by. No gradient."""
+    given = tuple(x for x in (lse, sums, out, positions) if x is not None)
+    desc, q, at, count, table, most = _chunk("weigh_rows", q, rows, scale, tokens, lengths, counts, max_tokens, pages, given)
+    seqs, n_q, n, d = q.shape
+    index = rows.device_index
+    if not lse.is_contiguous() or lse.shape != q.shape[:3] or lse.dtype != torch.float32 or lse.get_device() != index:
+        raise ValueError(f"lse must be contiguous float32 {tuple(q.shape[:3])} on {rows.device}")
+    if out is None:
+        out = sums if sums is not None else torch.zeros((seqs, rows.n_kv, most), dtype=torch.float32, device=q.device)
+    sums_st = None if sums is None else _account("sums", sums, torch.float32, seqs, rows.n_kv, most, index)
+    out_st = _account("out", out, torch.float32, seqs, rows.n_kv, most, index)
+    positions_st = None if positions is None else _account("positions", positions, torch.int32, seqs, rows.n_kv, most, index)
+    first = _counts(seen, seqs, index, "seen")
+    if seen is not None and positions is None:
+        raise ValueError("seen says where positions start; there are none")
+    if sums is not None:
+        _same_or_apart("sums and out", out, sums)
+    written = (out,) if positions is None else (out, positions)
+    if any(_meets(x, (_reach(q), _reach(lse), *_row_spans(rows))) for x in written) or (
+            positions is not None and (_meets(positions, (_reach(out),)) or (sums is not None and _meets(positions, (_reach(sums),))))):
+        raise ValueError("out and positions must not lie among the inputs or each other")
+    if seqs == 0 or most == 0:
+        return out
+    _WRITTEN(written)
+    lib = _lib.lib()
+    ref = ctypes.byref(desc)
+    ws_ptr, ws_n, _held = _scratch(lib.lkv_weigh_rows_workspace_bytes(ref), ws, q.device)
+    rc = _launch(index, lib.lkv_weigh_rows, ref, q.data_ptr() or lse.data_ptr() or out.data_ptr(), rows.model_code, lse.data_ptr() or out.data_ptr(), rows.ref, table, at, count,
+                 None if sums is None else sums.data_ptr(), sums_st, out.data_ptr(), out_st, None if positions is None else positions.data_ptr(), positions_st, first,
+                 ws_ptr, ws_n)
+    if rc:
+        _lib.check(rc, "weigh_rows")
+    return out
+
+
+def evict_rows(
+    rows: Rows,
+    sums: torch.Tensor,
+    positions: torch.Tensor,
+    *,
+    keep: int,
+    sinks: int = 0,
+    recent: int = 0,
+    tokens: int = 0,
+    lengths: torch.Tensor | None = None,
+    max_tokens: int | None = None,
+    pages: torch.Tensor | None = None,
+    out: tuple[torch.Tensor, torch.Tensor] | None = None,
+    ws: Workspace | None = None,
+) -> None:
+    """A cache cut to `keep` rows of each sequence and KV head (lkv_evict_rows), of `len = tokens + lengths[b]` that it has: those of the tokens below position
+    `sinks`, those of the `recent` newest positions, and of the rest those with the largest `sums`, ties to the lowest row, NaN after all others. Kept rows behind row
+    `keep - 1` move into the places before it that are not kept, in their order, with their sums and `positions` (as `weigh_rows` leaves them): attention does not go by the
+    order of rows. `out`: (sums, positions) go there instead of back. Afterwards `min(len, keep)` rows are the sequence's; what lies behind them is left as it is.
+    Pages that a call may write to must be in one place of one sequence's table. No gradient."""
+    _lib.require_cuda(sums, positions)
+    seqs, index = sums.shape[0], rows.device_index
+    table, room = _paged(rows, pages, seqs)
+    if max_tokens is None:
+        max_tokens = tokens if lengths is None else room
+    for name, n in (("tokens", tokens), ("max_tokens", max_tokens), ("keep", keep), ("sinks", sinks), ("recent", recent)):
+        _int32(name, n)
+    if lengths is None and tokens > max_tokens:
+        raise ValueError(f"tokens={tokens} exceed max_tokens={max_tokens}")
+    to = (sums, positions) if out is None else out
+    _no_gradients("evict_rows", (*rows.owners, sums, positions, *to))
+    at = _counts(lengths, seqs, index, "lengths")
+    least = max(0, max_tokens)
+    strides = [_account(name, x, t, seqs, rows.n_kv, n, index) for name, x, t, n in (
+        ("sums", sums, torch.float32, least), ("positions", positions, torch.int32, least), ("out's sums", to[0], torch.float32, min(least, max(0, keep))),
+        ("out's positions", to[1], torch.int32, min(least, max(0, keep))))]
+    if out is not None:
+        _same_or_apart("sums", to[0], sums)
+        _same_or_apart("positions", to[1], positions)
+        if _meets(to[0], (_reach(to[1]), _reach(positions))) or _meets(to[1], (_reach(sums),)):
+            raise ValueError("sums and positions share addresses")
+    if _meets(sums, (_reach(positions),)) or any(_meets(x, _row_spans(rows)) for x in (sums, positions, *to)):
+        raise ValueError("sums, positions and rows share addresses")
+    lib = _lib.lib()
+    desc = _lib.EvictDesc(seqs, rows.n_kv, rows.head_dim, rows.model_code, keep, sinks, recent, tokens, max_tokens)
+    ref = ctypes.byref(desc)
+    ws_ptr, ws_n, _held = _scratch(max(16, lib.lkv_evict_rows_workspace_bytes(ref)), ws, sums.device)
+    _WRITTEN((*rows.owners, *to))
+    rc = _launch(index, lib.lkv_evict_rows, ref, rows.ref, table, at, sums.data_ptr(), strides[0], positions.data_ptr(), strides[1], to[0].data_ptr(), strides[2],
+                 to[1].data_ptr(), strides[3], ws_ptr, ws_n)
+    if rc:
+        _lib.check(rc, "evict_rows")
+
+
 def packed_pair_bytes(block_size: int, head_dim: int) -> int:
     return int(_lib.lib().lkv_packed_pair_bytes(block_size, head_dim))
 

@@ -1,0 +1,144 @@
+"""What the calls of a layer's forward over a bounded cache do on the host (CPU): the arithmetic of pages, scratch, and checks that come before any launch."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+
+@pytest.mark.parametrize("sixteens", [1, 2, 3, 5, 7, 8, 12, 60, 63, 64, 65, 341, 1000, 1023, 1024])
+def test_a_rows_page_is_found_by_one_multiplication(sixteens: int) -> None:
+    """The kernels divide a row's group of sixteen by a page's as (group * ceil(2^36 / sixteens)) >> 36: exact for every group below 2^26 (rows below 2^30), within
+    64 bits. The error of the factor is less than sixteens / 2^36, so that of the quotient less than 2^26 * 2^10 / 2^36 = 1 of a step: the borders decide."""
+    magic = ((1 << 36) + sixteens - 1) // sixteens
+    top = 1 << 26
+    assert (top - 1) * magic < 1 << 64
+    quotients = sorted({0, 1, 2, top // sixteens // 2, (top - 1) // sixteens - 1, (top - 1) // sixteens, *range(0, top // sixteens, max(1, top // sixteens // 997))})
+    for quotient in quotients:
+        for group in (quotient * sixteens, quotient * sixteens + sixteens - 1, quotient * sixteens + sixteens // 2):
+            if 0 <= group < top:
+                assert (group * magic) >> 36 == group // sixteens
+
+
+def _chunk(n_seqs: int, n_q: int, n_kv: int, d: int, t: int, most: int):  # noqa: ANN202
+    from lazykv_amd import _lib
+
+    return _lib.ChunkDesc(n_seqs, n_q, n_kv, d, t, 0.1, 0, most, _lib.Triple(n_q * t * d, t * d, d))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize(("n_q", "n_kv"), [(1, 1), (4, 1), (32, 8), (40, 1), (128, 128)])
+def test_scratch_is_bounded(n_q: int, n_kv: int, d: int) -> None:
+    """Partial results of attention are for at most 512 workgroups of 128 query rows (or one part, which needs none); sums by parts for at most 1,024 of 256 rows."""
+    from lazykv_amd import _lib
+
+    lib = _lib.lib()
+    for n_seqs in (1, 3, 16, 257):
+        for t in (0, 1, 2, 7, 9, 33, 203, 2048):
+            for most in (0, 1, 127, 4099, 131072, 1 << 30):
+                if n_seqs * n_q * t > 1 << 26:
+                    continue
+                desc = ctypes.byref(_chunk(n_seqs, n_q, n_kv, d, t, most))
+                assert lib.lkv_chunk_attend_workspace_bytes(desc) <= 512 * 128 * (d + 2) * 4 + 16, (n_seqs, t, most)
+                assert lib.lkv_weigh_rows_workspace_bytes(desc) <= 1024 * 256 * 4, (n_seqs, t, most)
+
+
+CHUNK = {"desc": {"n_seqs": 2, "n_q": 8, "n_kv": 2, "head_dim": 64, "new_tokens": 3, "scale": 0.1, "tokens": 0, "max_tokens": 64}, "strides": (1536, 192, 64), "q": 4096, "dtype": 0,
+         "rows": {"seqs": 9, "tokens": 16, "dtype": 0, "k": 4096, "v": 1 << 20, "seq_stride": 2048, "head_stride": 1024}, "pages": {"table": 4096, "seq_stride": 4, "n_pages": 4},
+         "out": 4096, "lse": 4096, "ws": 4096, "ws_bytes": 1 << 30}
+
+
+def _call(fn: str, change: dict) -> str:
+    """A call with one thing wrong; the refusal's message. Nothing it is given is memory: a refusal comes before any use of it."""
+    from lazykv_amd import _lib
+
+    case = {k: ({**v, **(change.get(k) or {})} if isinstance(v, dict) else change.get(k, v)) for k, v in CHUNK.items()}
+    lib = _lib.lib()
+    r, p = case["rows"], case["pages"]
+    rows = _lib.KVRows(r["k"], r["v"], r.get("k_scale"), r.get("v_scale"), r["seq_stride"], r["head_stride"], r["tokens"], r["seqs"], r["dtype"], 0)
+    pages = _lib.Pages(p["table"], p["seq_stride"], p["n_pages"]) if change.get("pages", 1) is not None else None
+    refs = ctypes.byref(rows), (None if pages is None else ctypes.byref(pages))
+    d = case["desc"]
+    desc = _lib.ChunkDesc(d["n_seqs"], d["n_q"], d["n_kv"], d["head_dim"], d["new_tokens"], d["scale"], d["tokens"], d["max_tokens"], _lib.Triple(*case["strides"]))
+    two = _lib.Pair(128, 64)
+    if fn == "attend":
+        rc = lib.lkv_chunk_attend(0, ctypes.byref(desc), case["q"], case["dtype"], *refs, None, None, case["out"], 0, case["lse"], case["ws"], case["ws_bytes"])
+    elif fn == "weigh":
+        rc = lib.lkv_weigh_rows(0, ctypes.byref(desc), case["q"], case["dtype"], case["lse"], *refs, None, None, None, None, case["out"], two, None, None, None, case["ws"],
+                                case["ws_bytes"])
+    elif fn == "evict":
+        e = {"keep": 8, "sinks": 0, "recent": 0, **change.get("evict", {})}
+        ev = _lib.EvictDesc(d["n_seqs"], d["n_kv"], d["head_dim"], case["dtype"], e["keep"], e["sinks"], e["recent"], d["tokens"], d["max_tokens"])
+        rc = lib.lkv_evict_rows(0, ctypes.byref(ev), *refs, None, case["lse"], two, case["lse"], two, case["out"], two, case["out"], two, case["ws"], case["ws_bytes"])
+    else:
+        x = {"rotary": 64, "table": 0, "weight": 0, "eps": 0.0, "start": 0, "cos": 4096, **change.get("rotate", {})}
+        st = _lib.Triple(*case["strides"])
+        ro = _lib.RotateDesc(d["n_seqs"], d["n_q"], d["n_kv"], d["head_dim"], d["new_tokens"], case["dtype"], x["rotary"], x["table"], x["weight"], x["eps"], st, st, st, st, 0)
+        rc = lib.lkv_rotate_append(0, ctypes.byref(ro), case["q"], case["q"], case["q"], x["cos"], x["cos"], case["q"], case["q"], case["out"], *refs, None, x["start"], None)
+    assert rc == -1, rc
+    return lib.lkv_last_error().decode()
+
+
+EVERY = ("attend", "weigh", "evict", "rotate")
+
+
+@pytest.mark.parametrize(("fns", "change", "says"), [
+    (EVERY, {"desc": {"head_dim": 96}}, "head_dim 96"),
+    (EVERY, {"desc": {"n_seqs": -1}}, "bad shape"),
+    (EVERY, {"desc": {"n_kv": 0}}, "bad shape"),
+    (EVERY, {"dtype": 2}, "dtype"),
+    (EVERY, {"rows": {"k": 0}}, "NULL"),
+    (EVERY, {"rows": {"k": 4104}}, "16 bytes"),
+    (EVERY, {"rows": {"tokens": 24}}, "multiple of 16"),
+    (EVERY, {"rows": {"tokens": 0}}, "multiple of 16"),
+    (EVERY, {"rows": {"tokens": 32768}}, "16384"),
+    (EVERY, {"rows": {"seqs": 0}}, "without pages"),
+    (EVERY, {"rows": {"seq_stride": 2056}}, "multiples of 32"),
+    (EVERY, {"rows": {"dtype": 1}}, "under a call"),
+    (EVERY, {"rows": {"dtype": 4}}, "scales"),
+    (EVERY, {"pages": {"n_pages": -1}}, "page table"),
+    (EVERY, {"pages": {"table": 0}}, "page table"),
+    (EVERY, {"pages": {"n_pages": 1 << 27}}, "at most"),
+    (EVERY, {"pages": None}, "rows of 9 sequences"),
+    (("attend", "weigh", "evict"), {"desc": {"max_tokens": 65}}, "over 64"),
+    (("attend", "weigh", "evict"), {"desc": {"max_tokens": -1}}, "bad extent"),
+    (("attend", "weigh", "evict"), {"desc": {"tokens": -1}}, "bad extent"),
+    (("evict",), {"ws": 0}, "workspace"),
+    (("evict",), {"ws_bytes": 8}, "workspace"),
+    (("evict",), {"ws": 4104}, "workspace"),
+    (("attend", "weigh"), {"desc": {"n_q": 9}}, "bad shape"),
+    (("attend", "weigh"), {"desc": {"new_tokens": -1}}, "bad shape"),
+    (("attend", "weigh"), {"desc": {"new_tokens": 1 << 23}}, "query rows"),
+    (("attend", "weigh"), {"desc": {"scale": 0.0}}, "scale"),
+    (("attend", "weigh"), {"desc": {"scale": float("inf")}}, "scale"),
+    (("attend", "weigh"), {"strides": (1536, 192, 60)}, "multiples of 8"),
+    (("attend", "weigh"), {"q": 4104}, "16 bytes"),
+    (("attend", "weigh"), {"q": 0}, "NULL"),
+    (("evict",), {"evict": {"keep": 0}}, "that are kept"),
+    (("evict",), {"evict": {"sinks": 5, "recent": 4}}, "that are kept"),
+    (("evict",), {"evict": {"recent": -1}}, "that are kept"),
+    (("rotate",), {"rotate": {"rotary": 24}}, "multiple of 16"),
+    (("rotate",), {"rotate": {"rotary": 80}}, "at most 64"),
+    (("rotate",), {"rotate": {"cos": 0}}, "tables"),
+    (("rotate",), {"rotate": {"table": 1}}, "tables of dtype"),
+    (("rotate",), {"rotate": {"weight": 1}}, "weights of dtype"),
+    (("rotate",), {"rotate": {"eps": -1.0}}, "eps"),
+    (("rotate",), {"rotate": {"start": 62}}, "exceed"),
+    (("rotate",), {"strides": (1536, 192, 60)}, "multiples of 8"),
+    (("rotate",), {"strides": (0, 192, 64)}, "share an address"),
+    (("rotate", "evict"), {"rows": {"seq_stride": 1024}}, "share an address"),
+    (("rotate", "evict"), {"rows": {"v": 4096}}, "share an address"),
+])
+def test_calls_are_refused_before_any_launch(fns: tuple, change: dict, says: str) -> None:
+    for fn in fns:
+        assert says in _call(fn, change), (fn, _call(fn, change))
+
+
+def test_tensors_on_the_host_are_refused() -> None:
+    import torch
+
+    from lazykv_amd import kernels
+
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        kernels.evict_rows(None, torch.zeros((1, 1, 8)), torch.zeros((1, 1, 8), dtype=torch.int32), keep=4, tokens=8)

@@ -1,0 +1,304 @@
+"""The weights that rows get, summed up, and rows over a budget evicted by them, on the GPU against the definitions in 64 bits.
+
+A weight exp(s - lse) is off by e = ((d + 8) S + 4 + 2 |lse|) u relative (u = 2^-24, S the largest sum of a score's magnitudes; the lse enters as lse / scale, rounded
+twice), a sum of m weights in float32 by m u, so a row's sum by (e + (m + 4) u) times itself, and 2^-120 for weights below float32's normal range."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from chunk_cases import TYPES, U, Cache, int32, normal
+from oracle import chunk as O
+
+pytestmark = pytest.mark.gpu
+
+
+def weigh_case(seed: int, model: str, d: int, h: int, g: int, t: int, lens: list, counts: list | None = None, *, eight: bool = False, page: int = 0, into: bool = True) -> None:
+    from lazykv_amd import kernels
+
+    gen = torch.Generator().manual_seed(seed)
+    seqs, most, scale = len(lens), max(lens), d**-0.5
+    n = counts or [t] * seqs
+    q = (torch.randn((seqs, t, h * g, d), generator=gen) * 1.5).to(TYPES[model]).cuda().transpose(1, 2)
+    cache = Cache(gen, seqs, h, most, d, model, eight=eight, page=page, room=3)
+    qd = q.double().cpu().numpy()
+    lse = np.full((seqs, h * g, t), -np.inf, np.float32)
+    for b in range(seqs):
+        for j in range(h * g):
+            k, v = (x[b, j // g, : lens[b]] for x in cache.values)
+            lse[b, j] = O.attend(qd[b, j], k, v, n[b], scale)[1]
+    old = torch.rand((seqs, h, most + 5), generator=gen).cuda()
+    sums = old.clone()
+    positions = torch.full((seqs, h, most + 2), -7, dtype=torch.int32, device="cuda")
+    seen = int32([1000 * (b + 1) for b in range(seqs)])
+    out = sums if into else torch.full_like(old, 5.0)
+    got = kernels.weigh_rows(q, torch.from_numpy(lse).cuda(), cache.rows, scale=scale, lengths=int32(lens), counts=None if counts is None else int32(counts), max_tokens=most,
+                             pages=cache.pages, sums=sums, out=None if into else out, positions=positions, seen=seen)
+    assert got is out
+    got, at = got.double().cpu().numpy(), positions.cpu().numpy()
+    if not into:
+        assert torch.equal(sums, old)
+    old = old.double().cpu().numpy()
+    for b in range(seqs):
+        past = lens[b] - n[b]
+        for j in range(h):
+            mine = slice(j * g, (j + 1) * g)
+            k = cache.values[0][b, j, : lens[b]]
+            want = O.weigh(qd[b, mine], k, lse[b, mine].astype(np.float64), n[b], scale)
+            size = max((np.abs(x) @ np.abs(k).T).max(initial=0.0) for x in qd[b, mine]) * scale
+            top = np.abs(lse[b, mine], where=np.isfinite(lse[b, mine]), out=np.zeros((g, t), np.float32)).max(initial=0.0)
+            tol = (((d + 8) * size + 4 + 2 * top) + g * t + 4) * U * want + 2.0**-120
+            first = max(past, 0)
+            want[:first] += old[b, j, :first]
+            tol[:first] += 2 * U * want[:first]
+            bad = ~(np.abs(got[b, j, : lens[b]] - want) <= tol)
+            assert not bad.any(), (b, j, np.argwhere(bad)[:4].ravel(), got[b, j, : lens[b]][bad][:4], want[bad][:4])
+            assert np.all(got[b, j, lens[b] :] == (old[b, j, lens[b] :] if into else 5.0))
+            assert np.all(at[b, j, first : lens[b]] == 1000 * (b + 1) + np.arange(first - past, n[b])) and np.all(at[b, j, :first] == -7) and np.all(at[b, j, lens[b] :] == -7)
+
+
+@pytest.mark.parametrize("model", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize(("eight", "page"), [(False, 0), (False, 16), (True, 0), (True, 48)])
+@pytest.mark.parametrize(("t", "n"), [(1, 1), (1, 63), (1, 64), (1, 300), (3, 17), (20, 20), (33, 290), (70, 129)])
+def test_weights_summed(model: str, d: int, eight: bool, page: int, t: int, n: int) -> None:
+    weigh_case(n, model, d, 2, 4, t, [n, max(t, n // 2)], eight=eight, page=page)
+
+
+@pytest.mark.parametrize("g", [1, 2, 3, 5, 16, 17])
+@pytest.mark.parametrize("t", [1, 9])
+def test_weights_of_groups(g: int, t: int) -> None:
+    weigh_case(g, "bf16", 64, 3, g, t, [t + 50, t], page=16, into=False)
+
+
+@pytest.mark.parametrize(("t", "lens", "counts"), [(1, [0, 5, 200], [0, 1, 1]), (5, [9, 0, 5, 33], [5, 0, 1, 4]), (40, [90, 40, 7, 300], [40, 1, 7, 39]), (4, [2, 1], [4, 3])])
+def test_weights_of_ragged_batches(t: int, lens: list, counts: list) -> None:
+    weigh_case(t, "bf16", 128, 2, 4, t, lens, counts, page=16)
+
+
+@pytest.mark.parametrize(("t", "n"), [(500, 500), (300, 3000)])
+def test_weights_in_parts(t: int, n: int) -> None:
+    weigh_case(t, "f16", 64, 1, 4, t, [n], page=64)
+
+
+def test_weights_of_what_is_not_attended_or_not_there() -> None:
+    from lazykv_amd import kernels
+
+    gen = torch.Generator().manual_seed(3)
+    t, n, d = 20, 90, 64
+    q = normal(gen, (1, 4, t, d), "f16").cuda()
+    cache = Cache(gen, 1, 1, n, d, "f16", page=16)
+    kw = dict(scale=0.125, tokens=n, pages=cache.pages)
+    lse = kernels.chunk_attend(q, cache.rows, **kw)[1]
+    want = kernels.weigh_rows(q, lse, cache.rows, **kw)
+    assert abs(want.double().sum().item() - 4 * t) < 1e-3
+    # A key of the chunk that is not finite: only its own row shows it.
+    where, i = cache.place(0, 80)
+    cache.held[0][0, where, 0, i, 3] = float("nan")
+    got = kernels.weigh_rows(q, lse, cache.rows, **kw)
+    assert got[0, 0, 80].isnan() and torch.equal(got[0, 0, :80], want[0, 0, :80]) and torch.equal(got[0, 0, 81:], want[0, 0, 81:])
+    # Tokens whose lse is -inf add nothing, whatever their queries hold.
+    q2, lse2 = q.clone(), lse.clone()
+    q2[:, :, 7:], lse2[:, :, 7:] = float("nan"), -float("inf")
+    table = cache.pages.clone()
+    table[0, 2] = -1
+    some = kernels.weigh_rows(q2[:, :, :7], lse2[:, :, :7].contiguous(), cache.rows, scale=0.125, lengths=int32([n]), counts=int32([7]), max_tokens=n, pages=table)
+    assert torch.all(some[0, 0, 32:48] == 0) and some[0, 0, :32].isfinite().all()
+    more = kernels.weigh_rows(q2, lse2, cache.rows, scale=0.125, lengths=int32([n]), counts=int32([7]), max_tokens=n, pages=table)
+    assert torch.equal(more[0, 0, :80], some[0, 0, :80])
+    # (The chunk's rows are 70 .. 89 here: its first seven tokens attend up to row 76.)
+    less = kernels.weigh_rows(q2, lse2, cache.rows, scale=0.125, tokens=n, pages=cache.pages)
+    assert less[0, 0, :80].isfinite().all() and torch.all(less[0, 0, 77:80] == 0)
+
+
+def evict_case(seed: int, seqs: int, h: int, n: int, keep: int, sinks: int, recent: int, lens: list | None = None, *, eight: bool = False, page: int = 0, d: int = 64,
+               ties: bool = False, apart: bool = False, special: bool = False) -> None:
+    from lazykv_amd import kernels
+
+    gen = torch.Generator().manual_seed(seed)
+    lens = lens or [n] * seqs
+    cache = Cache(gen, seqs, h, n, d, "f16", eight=eight, page=page)
+    sums = torch.randint(0, 4, (seqs, h, n + 3), generator=gen).float() if ties else torch.randn((seqs, h, n + 3), generator=gen).exp()
+    if special:
+        for i, x in enumerate((float("nan"), float("inf"), -float("inf"), -0.0, 0.0, 1e-42, -1.0, float("nan"))):
+            sums[:, :, i::11] = x
+    positions = torch.stack([torch.randperm(3 * n + 3, generator=gen)[: n + 3] for _ in range(seqs * h)]).view(seqs, h, n + 3).int()
+    args = [sums.cuda(), positions.cuda()]
+    to = [torch.full_like(x, -3) for x in args] if apart else args
+    before = cache.read()
+    kernels.evict_rows(cache.rows, *args, keep=keep, sinks=sinks, recent=recent, lengths=int32(lens), max_tokens=n, pages=cache.pages, out=tuple(to) if apart else None)
+    torch.cuda.synchronize()
+    after = cache.read()
+    got = [x.cpu().numpy() for x in to]
+    for b in range(seqs):
+        for j in range(h):
+            m = lens[b]
+            s, p = sums[b, j].numpy().copy(), positions[b, j].numpy().copy()
+            dst, src = O.evict(s[:m], p[:m], keep, sinks, recent)
+            want = [x[b, j].copy() for x in before]
+            for x in (*want, s, p):
+                x[dst] = x[src]
+            left = min(m, keep)
+            for x, y in zip(want, after):
+                assert np.array_equal(x, y[b, j]), (b, j)
+            assert np.array_equal(got[0][b, j][:left], s[:left], equal_nan=True) and np.array_equal(got[1][b, j][:left], p[:left]), (b, j)
+            if apart:
+                assert np.all(got[0][b, j][left:] == -3) and np.all(got[1][b, j][left:] == -3)
+            else:
+                assert np.array_equal(got[0][b, j][left:], s[left:], equal_nan=True) and np.array_equal(got[1][b, j][left:], p[left:])
+
+
+@pytest.mark.parametrize(("n", "keep"), [(1, 1), (2, 1), (17, 16), (17, 1), (64, 63), (100, 50), (1000, 37), (1000, 999), (5000, 1234), (300, 300), (300, 400)])
+@pytest.mark.parametrize(("eight", "page", "d"), [(False, 0, 64), (True, 16, 128), (False, 48, 128)])
+@pytest.mark.parametrize("ties", [False, True])
+def test_the_rows_that_stay(n: int, keep: int, eight: bool, page: int, d: int, ties: bool) -> None:
+    evict_case(n, 1, 2, n, keep, 0, 0, eight=eight, page=page, d=d, ties=ties)
+
+
+@pytest.mark.parametrize(("keep", "sinks", "recent"), [(40, 4, 16), (40, 40, 0), (40, 0, 40), (40, 20, 20), (100, 1, 60)])
+@pytest.mark.parametrize("apart", [False, True])
+def test_first_and_newest_tokens(keep: int, sinks: int, recent: int, apart: bool) -> None:
+    evict_case(keep, 3, 2, 130, keep, sinks, recent, [130, 0, 77], page=16, apart=apart)
+
+
+@pytest.mark.parametrize("keep", [3, 30, 75])
+def test_sums_that_are_not_finite_or_alike(keep: int) -> None:
+    evict_case(keep, 2, 2, 90, keep, 2, 1, special=True)
+
+
+@pytest.mark.parametrize(("n", "keep"), [(20000, 5000), (40007, 39000), (70001, 128)])
+def test_long_caches(n: int, keep: int) -> None:
+    """Rows by their keys' one channel alone: which rows stay, in which places."""
+    from lazykv_amd import kernels
+
+    gen = torch.Generator().manual_seed(n)
+    store = torch.zeros((2, 1, 2, n, 64), dtype=torch.float16, device="cuda")
+    mark = torch.arange(n, device="cuda")
+    store[0, 0, :, :, 0], store[0, 0, :, :, 1], store[1, 0, :, :, 2] = (mark % 1000).half(), (mark // 1000).half(), (mark % 777).half()
+    was = store.clone()
+    sums = torch.randn((1, 2, n), generator=gen).exp().cuda()
+    sums[0, 1] = (sums[0, 1] * 4).floor()
+    positions = torch.randperm(n, generator=gen).int().expand(1, 2, n).contiguous().cuda()
+    s, p = sums.cpu().numpy().copy(), positions.cpu().numpy().copy()
+    kernels.evict_rows(kernels.dense_rows(store[0], store[1]), sums, positions, keep=keep, sinks=4, recent=100, tokens=n)
+    for j in range(2):
+        to, of = (torch.from_numpy(x).cuda() for x in O.evict(s[0, j], p[0, j], keep, 4, 100))
+        want = was[:, 0, j].clone()
+        want[:, to] = want[:, of]
+        assert torch.equal(store[:, 0, j], want)
+        wanted = torch.from_numpy(p[0, j]).cuda()
+        wanted[to] = wanted[of]
+        assert torch.equal(positions[0, j], wanted)
+
+
+def test_a_captured_eviction_follows_lengths() -> None:
+    from lazykv_amd import kernels
+
+    gen = torch.Generator().manual_seed(4)
+    caches = [Cache(torch.Generator().manual_seed(5), 2, 2, 100, 64, "f16", page=16) for _ in range(2)]
+    sums, positions = torch.rand((2, 2, 100), generator=gen).cuda(), torch.arange(100, dtype=torch.int32).expand(2, 2, 100).contiguous().cuda()
+    lengths = int32([100, 70])
+    to = [[torch.zeros_like(x) for x in (sums, positions)] for _ in range(2)]
+    call = lambda i: kernels.evict_rows(caches[i].rows, sums, positions, keep=40, recent=8, lengths=lengths, max_tokens=100, pages=caches[i].pages, out=tuple(to[i]))  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(0)
+    torch.cuda.current_stream().wait_stream(side)
+    call(1)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(0)
+    for a, b in ((100, 41), (40, 99), (0, 100)):
+        lengths.copy_(int32([a, b]))
+        sums.copy_(torch.rand((2, 2, 100), generator=gen))
+        graph.replay()
+        torch.cuda.synchronize()
+        call(1)
+        for x, y in zip((*caches[0].held, *to[0]), (*caches[1].held, *to[1])):  # to the bit; pages of nobody's hold NaN
+            torch.testing.assert_close(x, y, rtol=0, atol=0, equal_nan=True)
+
+
+def test_what_is_refused() -> None:
+    from lazykv_amd import kernels
+
+    gen = torch.Generator().manual_seed(6)
+    cache = Cache(gen, 2, 2, 64, 64, "f16", page=16)
+    sums, positions = torch.zeros((2, 2, 64), device="cuda"), torch.zeros((2, 2, 64), dtype=torch.int32, device="cuda")
+    kw = dict(tokens=64, pages=cache.pages)
+    for what, args, more in (
+        ("first and", (sums, positions), {"keep": 4, "sinks": 3, "recent": 2}), ("first and", (sums, positions), {"keep": 0}), ("sums must", (sums.half(), positions), {"keep": 4}),
+        ("positions must", (sums, positions.long()), {"keep": 4}), ("sums must", (sums[:, :, :63], positions), {"keep": 4}), ("share addresses", (sums[:, :1].expand(2, 2, 64), positions), {"keep": 4}),
+        ("share addresses", (sums, sums.view(torch.int32)), {"keep": 4}), ("rows of a sequence over", (torch.zeros((2, 2, 99), device="cuda"), positions.new_zeros((2, 2, 99))), {"keep": 4, "tokens": 65}),
+        ("overlap", (sums, positions), {"keep": 4, "out": (torch.zeros((2, 2, 64), device="cuda"), positions[:, :, 1:])}),
+    ):
+        with pytest.raises(ValueError, match=what):
+            kernels.evict_rows(cache.rows, *args, **{**kw, **more})
+    q = normal(gen, (2, 4, 3, 64), "f16").cuda()
+    lse = torch.zeros((2, 4, 3), device="cuda")
+    for what, args, more in (
+        ("lse must", (q, lse[:, :, :2]), {}), ("sums must", (q, lse), {"sums": sums[:1]}), ("seen says", (q, lse), {"seen": int32([1, 2])}), ("positions must", (q, lse), {"positions": sums}),
+        ("must not lie", (q, lse), {"out": sums, "positions": sums.view(torch.int32)}), ("overlap", (q, lse), {"sums": torch.zeros((2, 2, 65), device="cuda")[:, :, 1:], "out": sums[:, :, :0]}),
+    ):
+        if what == "overlap":
+            both = torch.zeros((2, 2, 65), device="cuda")
+            more = {"sums": both[:, :, 1:], "out": both[:, :, :64]}
+        with pytest.raises(ValueError, match=what):
+            kernels.weigh_rows(*args, cache.rows, scale=0.1, **{**kw, **more})
+    with pytest.raises(RuntimeError, match="no gradient"):
+        kernels.evict_rows(cache.rows, sums.clone().requires_grad_(), positions, keep=4, **kw)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_a_layers_decode_over_a_bounded_cache(eight: bool) -> None:
+    """A prompt and forty steps of two sequences through one layer, all four calls: the cache stays at its budget, and at each step the attention is that over the
+    rows that a plain account of the same rules has."""
+    from lazykv_amd import kernels
+
+    gen = torch.Generator().manual_seed(7)
+    seqs, h, g, d, keep, room, page = 2, 2, 2, 64, 48, 64, 16
+    cache = Cache(gen, seqs, h, room, d, "bf16", eight=eight, page=page)
+    sums, positions = torch.zeros((seqs, h, room), device="cuda"), torch.zeros((seqs, h, room), dtype=torch.int32, device="cuda")
+    lengths, seen = int32([0, 0]), int32([0, 0])
+    lens = [0, 0]
+    held = [[{} for _ in range(h)] for _ in range(seqs)]  # position: its sum, as the plain account has it
+    scale, weight = d**-0.5, (torch.rand((d,), generator=gen) + 0.5).bfloat16().cuda()
+    angle = torch.arange(400.0)[:, None] * 10000.0 ** (-torch.arange(0, d, 2) / d)
+    cos, sin = (torch.cat([x, x], -1).bfloat16().cuda() for x in (angle.cos(), angle.sin()))
+    for step in range(41):
+        t = 30 if step == 0 else 16 if step % 7 == 3 else 1
+        q, k, v = (normal(gen, (seqs, n, t, d), "bf16").cuda() for n in (h * g, h, h))
+        at = seen.long()[:, None] + torch.arange(t, device="cuda")
+        q = kernels.rotate_append(cache.rows, q, k, v, cos=cos[at], sin=sin[at], q_weight=weight, k_weight=weight, starts=lengths, pages=cache.pages)
+        lengths += t
+        lens = [n + t for n in lens]
+        kw = dict(scale=scale, lengths=lengths, max_tokens=room, pages=cache.pages)
+        out, lse = kernels.chunk_attend(q, cache.rows, **kw)
+        kernels.weigh_rows(q, lse, cache.rows, sums=sums, positions=positions, seen=seen, **kw)
+        rows, places = cache.read(), positions.cpu().numpy()
+        qd, od, sd = q.double().cpu().numpy(), out.double().cpu().numpy(), sums.double().cpu().numpy()
+        for b in range(seqs):
+            for j in range(h):
+                kk, vv = (x[b, j, : lens[b]] for x in rows)
+                for i in range(j * g, (j + 1) * g):
+                    want, _, a, _ = O.attend(qd[b, i], kk, vv, t, scale)
+                    assert np.all(np.abs(od[b, i] - want) <= 2.0**-7 * a + 2.0**-8 * np.abs(want) + 1e-6)
+                ls = np.stack([O.attend(qd[b, i], kk, vv, t, scale)[1] for i in range(j * g, (j + 1) * g)])
+                got = O.weigh(qd[b, j * g : (j + 1) * g], kk, ls, t, scale)
+                account = held[b][j]
+                for row, p in enumerate(places[b, j, : lens[b]]):
+                    account[int(p)] = account.get(int(p), 0.0) + got[row]
+                assert set(account) == set(places[b, j, : lens[b]].tolist())
+                assert np.allclose(sd[b, j, : lens[b]], [account[int(p)] for p in places[b, j, : lens[b]]], rtol=1e-4, atol=1e-6)
+        kernels.evict_rows(cache.rows, sums, positions, keep=keep, sinks=2, recent=8, lengths=lengths, max_tokens=room, pages=cache.pages)
+        lengths.clamp_(max=keep)
+        seen += t
+        lens = [min(n, keep) for n in lens]
+        places, newest = positions.cpu().numpy(), int(seen[0]) - 1
+        for b in range(seqs):
+            for j in range(h):
+                left = set(places[b, j, : lens[b]].tolist())
+                assert len(left) == lens[b] and all(p in left for p in [0, 1, *range(newest - 7, newest + 1)])
+                held[b][j] = {p: s for p, s in held[b][j].items() if p in left}
