@@ -3,7 +3,9 @@
 //
 // A wave holds 64 rows' keys as the second operand of v_mfma_f32_16x16x32 and takes the query rows 16 at a time as the first,
 // S [16 queries x 16 rows] = Q K^T, so that a row's scores lie in one lane of each quarter: its sum stays there from the first query to the last.
-// The accumulators start at -lse / scale, and the scores come out relative to it.
+// The accumulators start at -lse / scale, and the scores come out relative to it. That form reads the queries from memory, for up to 32 query rows of
+// a KV head. More of them go through LDS, 64 at a time for four waves, on v_mfma_f32_32x32x16; there -lse is the addend of the exponent's one
+// multiply-add.
 #include "lkv_attend.h"
 #include "lkv_pages.h"
 
@@ -60,20 +62,16 @@ template <int D, bool MX> struct QueryRegs {
     const int quarter = (threadIdx.x & 63) >> 4;
     const int t = x / a.g, j = h * a.g + (x - t * a.g);
     const bool live = t < e.n;
-    start = -INFINITY;
+    const int tt = live ? t : 0, jj = live ? j : h * a.g;  // the first row in the place of one that is not there
     limit = live ? e.len - e.n + t + 1 : 0;
+    const uint16_t* q = a.q + b * a.q_stride[0] + jj * a.q_stride[1] + tt * a.q_stride[2];
+    const float lse = a.lse[((int64_t)b * a.n_q + jj) * a.new_tokens + tt];
+    const uint32_t keep = live && lse != -INFINITY ? ~0u : 0u;
+    start = keep ? -lse * a.per_scale : -INFINITY;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) w[i] = make_uint4(0, 0, 0, 0);
-    if (live) {
-      const uint16_t* q = a.q + b * a.q_stride[0] + j * a.q_stride[1] + t * a.q_stride[2];
-      const float lse = a.lse[((int64_t)b * a.n_q + j) * a.new_tokens + t];
-      const bool adds = lse != -INFINITY;
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        const uint4 x = *(const uint4*)(q + KeyRegs<D, MX>::channel(quarter, i));
-        w[i] = adds ? x : w[i];
-      }
-      start = adds ? -lse * a.per_scale : -INFINITY;
+    for (int i = 0; i < D / 32; ++i) {
+      const uint4 y = *(const uint4*)(q + KeyRegs<D, MX>::channel(quarter, i));
+      w[i] = make_uint4(y.x & keep, y.y & keep, y.z & keep, y.w & keep);
     }
   }
 };
@@ -169,6 +167,154 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_rows_kernel(WeighArgs a)
   }
 }
 
+// ---- many query rows: through LDS ------------------------------------------------------------------
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+template <int DT> __device__ __forceinline__ f32x16 wide_mma(uint4 a, uint4 b, f32x16 c) {
+  if constexpr (DT == LKV_BF16) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+}
+
+constexpr int kStage = 64;  // query rows
+template <int D> __device__ __forceinline__ int swizzle(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
+
+// A stage's query rows on their way to LDS, what is added to their exponents, and how many of a sequence's rows they attend.
+template <int D> struct StageQueries {
+  static constexpr int PIECES = D / 8, LOADS = kStage * PIECES / (64 * kWaves);
+  u32x4 w[LOADS];
+  uint32_t keep[LOADS];
+  float less;
+  int limit;
+  __device__ __forceinline__ void load(const WeighArgs& a, const Extent& e, int b, int h, int x0, int x_end) {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int x = min(x0 + (i * 64 * kWaves + (int)threadIdx.x) / PIECES, x_end - 1), t = x / a.g, j = h * a.g + (x - t * a.g);
+      const uint16_t* q = a.q + b * a.q_stride[0] + j * a.q_stride[1] + t * a.q_stride[2];
+      w[i] = *(const u32x4*)(q + threadIdx.x % PIECES * 8);
+      keep[i] = a.lse[((int64_t)b * a.n_q + j) * a.new_tokens + t] != -INFINITY ? ~0u : 0u;
+    }
+    const int x = x0 + (int)(threadIdx.x & (kStage - 1)), y = min(x, x_end - 1), t = y / a.g, j = h * a.g + (y - t * a.g);
+    const float lse = a.lse[((int64_t)b * a.n_q + j) * a.new_tokens + t];
+    less = x < x_end && lse != -INFINITY ? -lse * kLog2e : -INFINITY;
+    limit = e.len - e.n + t + 1;
+  }
+  __device__ __forceinline__ void store(uint8_t* lds, float* less_at, int* limit_at) const {
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int x = i * 64 * kWaves + threadIdx.x, row = x / PIECES;
+      *(u32x4*)(lds + row * (2 * D) + ((x % PIECES) ^ swizzle<D>(row)) * 16) = w[i] & keep[i];
+    }
+    if (threadIdx.x < kStage) {
+      less_at[threadIdx.x] = less;
+      limit_at[threadIdx.x] = limit;
+    }
+  }
+};
+
+template <int DT, int D, bool MX>
+__global__ __launch_bounds__(64 * kWaves, 2) void weigh_wide_kernel(WeighArgs a) {
+  constexpr int BYTES = kStage * 2 * D;
+  __shared__ u32x4 lds4[2 * BYTES / 16];
+  __shared__ __attribute__((aligned(16))) float less_at[2][kStage];
+  __shared__ __attribute__((aligned(16))) int limit_at[2][kStage];
+  uint8_t* const lds = (uint8_t*)lds4;
+  const int lane = threadIdx.x & 63, half = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int id = blockIdx.x;
+  const int heads = a.n_seqs * a.n_kv, bh = id % heads;
+  id /= heads;
+  const int part = id % a.parts, block = id / a.parts, b = bh / a.n_kv, h = bh % a.n_kv;
+  const Extent e = extent_of(a, b);
+  if (block * kBlockRows >= e.len) return;
+  const int row0 = block * kBlockRows + wave * kWaveRows;
+  // A lane's key of each tile of 32, channels 16 i + 8 half .. + 8 for the i-th product; behind the end the last one.
+  uint4 k[2][D / 16];
+  bool there[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int row = min(row0 + 32 * u + (lane & 31), e.len - 1);
+    const Sixteen s = sixteen_of<D, false>(a.rows, b, h, row >> 4);
+    const int64_t at = s.at + (row & 15) * D + 8 * half;
+    there[u] = s.there;
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      if constexpr (MX) {
+        const uint2 c = *(const uint2*)((const uint8_t*)a.rows.rows.k + at + 16 * i);
+        const float f = bits_to_float((uint32_t)a.rows.rows.k_scale[(at + 16 * i) / kMxGroup] << 23);
+        k[u][i] = make_uint4(Mat<DT>::template widen<false>(c.x, f), Mat<DT>::template widen<true>(c.x, f), Mat<DT>::template widen<false>(c.y, f),
+                             Mat<DT>::template widen<true>(c.y, f));
+      } else {
+        k[u][i] = *(const uint4*)((const uint16_t*)a.rows.rows.k + at + 16 * i);
+      }
+    }
+  }
+  // The first query that attends the workgroup's first row, and the first one that attends all the wave's rows.
+  const int past = e.len - e.n, x_end = min(e.n * a.g, (part + 1) * a.chunk);
+  const int x_first = max(part * a.chunk, max(block * kBlockRows - past, 0) * a.g), x_whole = max(row0 + kWaveRows - 1 - past, 0) * a.g;
+  float sum[2] = {0.0f, 0.0f};
+  if (x_first < x_end) {
+    LdsPointer at[D / 16];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      at[i] = (LdsPointer)lds + (lane & 31) * (2 * D) + ((2 * i + half) ^ swizzle<D>(lane & 31)) * 16;
+      keep_here(at[i]);
+    }
+    StageQueries<D> regs;
+    regs.load(a, e, b, h, x_first, x_end);
+    int buffer = 0;
+    for (int x = x_first; x < x_end; x += kStage) {
+      regs.store(lds + buffer * BYTES, less_at[buffer], limit_at[buffer]);
+      __syncthreads();
+      if (x + kStage < x_end) regs.load(a, e, b, h, x + kStage, x_end);
+      load_fence();
+#pragma unroll
+      for (int sub = 0; sub < kStage / 32; ++sub) {
+        if (x + 32 * sub >= x_end) continue;
+        uint4 q[D / 16];
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) q[i] = read_piece(at[i] + buffer * BYTES + sub * 32 * 2 * D);
+        f32x4 less[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) less[i] = *(const f32x4*)&less_at[buffer][32 * sub + 8 * i + 4 * half];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          f32x16 s;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) s = wide_mma<DT>(q[i], k[u][i], s);
+          if (x + 32 * sub < x_whole) {
+            const int mine = row0 + 32 * u + (lane & 31);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float y = mine < limit_at[buffer][32 * sub + 8 * (i / 4) + 4 * half + i % 4] ? s[i] : -INFINITY;
+              keep_here(y);
+              s[i] = y;
+            }
+          }
+          float p[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, less[i / 4][i % 4]));
+#pragma unroll
+          for (int i = 0; i < 8; ++i) p[i] += p[i + 8];
+          sum[u] += ((p[0] + p[4]) + (p[1] + p[5])) + ((p[2] + p[6]) + (p[3] + p[7]));
+        }
+      }
+      buffer ^= 1;
+    }
+  }
+  // Each half stores a tile's rows.
+  const float first = pair_sum<32>(sum[0]), second = pair_sum<32>(sum[1]);
+  const float mine = half ? (there[1] ? second : 0.0f) : (there[0] ? first : 0.0f);
+  if (a.parts > 1) {
+    a.part[((int64_t)part * heads + bh) * a.blocks * kBlockRows + row0 + lane] = mine;
+  } else {
+    store_sum(a, e, b, h, row0 + lane, mine);
+  }
+}
+
 // The parts' sums of a row, in their order.
 __global__ __launch_bounds__(256) void weigh_join_kernel(WeighArgs a) {
   const int heads = a.n_seqs * a.n_kv, bh = blockIdx.x % heads, row = blockIdx.x / heads * kBlockRows + threadIdx.x, b = bh / a.n_kv, h = bh % a.n_kv;
@@ -182,22 +328,29 @@ __global__ __launch_bounds__(256) void weigh_join_kernel(WeighArgs a) {
 int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 struct Plan {
+  bool wide;
   int blocks, parts, chunk;
 };
 Plan plan_of(const lkv_chunk_desc* d) {
   Plan p = {};
   const int64_t x = (int64_t)d->new_tokens * (d->n_q / d->n_kv);
+  p.wide = x > 32;
   p.blocks = ceil_div(d->max_tokens, kBlockRows);
   const int64_t units = (int64_t)d->n_seqs * d->n_kv * p.blocks;
   int64_t parts = units > 0 ? 1024 / units : 1;
-  const int64_t most = x / 128;
+  const int64_t most = x / 256;
   parts = parts > most ? most : parts;
   parts = parts < 1 ? 1 : parts;
-  p.chunk = ceil_div(ceil_div(x, parts), 16) * 16;
-  p.chunk = p.chunk < 16 ? 16 : p.chunk;
+  p.chunk = ceil_div(ceil_div(x, parts), kStage) * kStage;
+  p.chunk = p.chunk < kStage ? kStage : p.chunk;
   p.parts = ceil_div(x, p.chunk);
   p.parts = p.parts < 1 ? 1 : p.parts;
   return p;
+}
+
+template <int DT, int D, bool MX>
+void (*kernel_of(const Plan& p))(WeighArgs) {
+  return p.wide ? weigh_wide_kernel<DT, D, MX> : weigh_rows_kernel<DT, D, MX>;
 }
 
 }  // namespace
@@ -253,10 +406,8 @@ extern "C" int lkv_weigh_rows(uintptr_t stream, const lkv_chunk_desc* desc, cons
   a.chunk = p.chunk;
   const hipStream_t s = (hipStream_t)stream;
   const bool half = q_dtype == LKV_F16, wide = desc->head_dim == 128, mx = rows->dtype == LKV_MXFP8;
-  auto kernel = half ? (wide ? (mx ? weigh_rows_kernel<LKV_F16, 128, true> : weigh_rows_kernel<LKV_F16, 128, false>)
-                             : (mx ? weigh_rows_kernel<LKV_F16, 64, true> : weigh_rows_kernel<LKV_F16, 64, false>))
-                     : (wide ? (mx ? weigh_rows_kernel<LKV_BF16, 128, true> : weigh_rows_kernel<LKV_BF16, 128, false>)
-                             : (mx ? weigh_rows_kernel<LKV_BF16, 64, true> : weigh_rows_kernel<LKV_BF16, 64, false>));
+  auto kernel = half ? (wide ? (mx ? kernel_of<LKV_F16, 128, true>(p) : kernel_of<LKV_F16, 128, false>(p)) : (mx ? kernel_of<LKV_F16, 64, true>(p) : kernel_of<LKV_F16, 64, false>(p)))
+                     : (wide ? (mx ? kernel_of<LKV_BF16, 128, true>(p) : kernel_of<LKV_BF16, 128, false>(p)) : (mx ? kernel_of<LKV_BF16, 64, true>(p) : kernel_of<LKV_BF16, 64, false>(p)));
   hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks * p.parts)), dim3(64 * kWaves), 0, s, a);
   LKV_CHECK_LAUNCH("weigh_rows");
   if (p.parts > 1) {

@@ -107,7 +107,11 @@ def test_weights_of_what_is_not_attended_or_not_there() -> None:
     some = kernels.weigh_rows(q2[:, :, :7], lse2[:, :, :7].contiguous(), cache.rows, scale=0.125, lengths=int32([n]), counts=int32([7]), max_tokens=n, pages=table)
     assert torch.all(some[0, 0, 32:48] == 0) and some[0, 0, :32].isfinite().all()
     more = kernels.weigh_rows(q2, lse2, cache.rows, scale=0.125, lengths=int32([n]), counts=int32([7]), max_tokens=n, pages=table)
-    assert torch.equal(more[0, 0, :80], some[0, 0, :80])
+    # Seven tokens and twenty may take different kernels, each within the bound above of the same sums: they differ by twice that at the most.
+    k = torch.from_numpy(cache.values[0][0, 0]).cuda()
+    size = (q[:, :, :7].double().abs() @ k.abs().T).max().item() * 0.125
+    rel = 2 * ((d + 8) * size + 4 + 2 * lse[:, :, :7].abs().max().item() + 4 * 7 + 4) * U
+    assert torch.all((more[0, 0, :80] - some[0, 0, :80]).abs() <= rel * some[0, 0, :80])
     # (The chunk's rows are 70 .. 89 here: its first seven tokens attend up to row 76.)
     less = kernels.weigh_rows(q2, lse2, cache.rows, scale=0.125, tokens=n, pages=cache.pages)
     assert less[0, 0, :80].isfinite().all() and torch.all(less[0, 0, 77:80] == 0)
