@@ -172,10 +172,18 @@ class RotateDesc(ctypes.Structure):
         ("table_dtype", ctypes.c_int32),
         ("weight_dtype", ctypes.c_int32),
         ("eps", ctypes.c_float),
-        ("q_stride", ctypes.c_int64 * 3),
-        ("k_stride", ctypes.c_int64 * 3),
-        ("v_stride", ctypes.c_int64 * 3),
-        ("out_stride", ctypes.c_int64 * 3),
+        ("q_seq_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("q_token_stride", ctypes.c_int64),
+        ("k_seq_stride", ctypes.c_int64),
+        ("k_head_stride", ctypes.c_int64),
+        ("k_token_stride", ctypes.c_int64),
+        ("v_seq_stride", ctypes.c_int64),
+        ("v_head_stride", ctypes.c_int64),
+        ("v_token_stride", ctypes.c_int64),
+        ("out_seq_stride", ctypes.c_int64),
+        ("out_head_stride", ctypes.c_int64),
+        ("out_token_stride", ctypes.c_int64),
         ("table_seq_stride", ctypes.c_int64),
     ]
 
@@ -192,7 +200,9 @@ class ChunkDesc(ctypes.Structure):
         ("scale", ctypes.c_float),
         ("tokens", ctypes.c_int32),
         ("max_tokens", ctypes.c_int32),
-        ("q_stride", ctypes.c_int64 * 3),
+        ("q_seq_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("q_token_stride", ctypes.c_int64),
     ]
 
 
@@ -213,7 +223,6 @@ class EvictDesc(ctypes.Structure):
 
 
 Pair = ctypes.c_int64 * 2
-Triple = ctypes.c_int64 * 3
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int

@@ -338,50 +338,76 @@ template <int D> __device__ __forceinline__ int swizzle(int row) {
   return D == 128 ? ((row & 3) << 2 | ((row >> 2) & 3)) : ((row & 2) << 1 | ((row >> 2) & 3));
 }
 
-// Where a stage's tokens are: each sixteen of them, and a bit for each that is there.
-template <int D> struct StagePlace {
-  int64_t at0, at1, at2, at3;
-  uint32_t there;
-  __device__ __forceinline__ void find(const PagedRows& p, int b, int h, int t0, int end) {
-    const int last = (end - 1) >> 4, first = t0 >> 4;
-    const Sixteen x0 = sixteen_of<D>(p, b, h, min(first, last)), x1 = sixteen_of<D>(p, b, h, min(first + 1, last)), x2 = sixteen_of<D>(p, b, h, min(first + 2, last)),
-                  x3 = sixteen_of<D>(p, b, h, min(first + 3, last));
-    at0 = x0.at, at1 = x1.at, at2 = x2.at, at3 = x3.at;
-    there = (x0.there ? 1u : 0u) | (x1.there ? 2u : 0u) | (x2.there ? 4u : 0u) | (x3.there ? 8u : 0u);
+// Where tokens are: a lane looks up sixteen of them, a wave 1,024 at once, and a stage's four are read from their lanes.
+template <int D> struct Places {
+  uint32_t lo, hi;  // of the lane's sixteen, in elements
+  uint64_t there;   // a bit a lane
+  // Sixteens first, first + 1, ...; in the place of those behind `last`, that one.
+  __device__ __forceinline__ void find(const PagedRows& p, int b, int h, int first, int last) {
+    const Sixteen x = sixteen_of<D, false>(p, b, h, min(first + (int)(threadIdx.x & 63), last));
+    lo = (uint32_t)x.at;
+    hi = (uint32_t)(x.at >> 32);
+    there = __ballot(x.there);
   }
-  __device__ __forceinline__ int64_t at(int sixteen) const {
-    const int64_t a = at0, b = at1, c = at2, d = at3;
-    const int64_t lo = sixteen & 1 ? b : a, hi = sixteen & 1 ? d : c;
-    return sixteen & 2 ? hi : lo;
+  __device__ __forceinline__ int64_t at(int lane) const {
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane(hi, lane) << 32 | (uint32_t)__builtin_amdgcn_readlane(lo, lane));
   }
 };
 
-// What a thread holds of a stage on its way to LDS.
-template <int DT, int D, bool MX> struct StageRegs {
-  static constexpr int PIECES = MX ? D / 16 : D / 8;  // 16-byte pieces of a row
-  static constexpr int LOADS = kStage * PIECES / (64 * kWaves);
-  static constexpr int ROW = MX ? D : 2 * D;
+// A stage on its way to LDS. Behind the end, and in the place of rows that are not there, some other row lies: no weight goes to them, and what is not finite
+// among their values is taken out where a tile is cut.
+//
+// Model dtype: straight from memory, a wave 1,024 bytes a load to as many of LDS, so that the swizzle is the loads': a lane takes the piece of its row that
+// belongs where it writes.
+template <int DT, int D, bool MX> struct StageLoad {
   static constexpr int BYTES = kStage * 2 * D;  // of keys, and of values, in LDS
+  static constexpr int ROWS = 512 / D;          // of a load
+  static constexpr int LOADS = kStage / ROWS / kWaves;
+  uint32_t in;  // where a lane's piece is, from its sixteen's first row
+  int row;      // its row in a sixteen
+  __device__ __forceinline__ void begin() {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    row = (wave * ROWS + lane / (D / 8)) & 15;
+    in = (uint32_t)(row * 2 * D + ((lane % (D / 8)) ^ swizzle<D>(row)) * 16);
+  }
+  // The stage whose four sixteens lanes first .. of `places` have looked up. CUT: `left` of its tokens are there, 64 or less.
+  template <bool CUT> __device__ __forceinline__ void load(const PagedRows& p, const Places<D>& places, int first, int left, uint8_t* lds) const {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int top = (i * kWaves + wave) * ROWS, sixteen = top / 16;
+      uint32_t from = in;
+      if (CUT) from -= (uint32_t)(max(row - (left - 1 - min(sixteen, (left - 1) / 16) * 16), 0) * 2 * D);
+      const int64_t at = 2 * places.at(first + sixteen);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)((const uint8_t*)p.rows.k + at + from),
+                                       (__attribute__((address_space(3))) uint32_t*)(lds + top * 2 * D), 16, 0, 0);
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)((const uint8_t*)p.rows.v + at + from),
+                                       (__attribute__((address_space(3))) uint32_t*)(lds + BYTES + top * 2 * D), 16, 0, 0);
+    }
+  }
+  __device__ __forceinline__ void store(uint8_t*) const { __builtin_amdgcn_s_waitcnt(0xf70); }  // the loads have arrived: vmcnt(0)
+};
+// 8 bits: through registers, widened on the way.
+template <int DT, int D> struct StageLoad<DT, D, true> {
+  static constexpr int PIECES = D / 16;  // 16-byte pieces of a row
+  static constexpr int LOADS = kStage * PIECES / (64 * kWaves);
+  static constexpr int BYTES = kStage * 2 * D;
   u32x4 k[LOADS], v[LOADS];
   uint32_t ks[LOADS], vs[LOADS];
-  // Tokens t0 .. of a sequence; in the place of those behind `end`, the last one.
-  __device__ __forceinline__ void load(const PagedRows& p, const StagePlace<D>& place, int t0, int end) {
-    const int last = (end - 1) >> 4;
+  __device__ __forceinline__ void begin() {}
+  template <bool CUT> __device__ __forceinline__ void load(const PagedRows& p, const Places<D>& places, int first, int left, uint8_t*) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int x = i * 64 * kWaves + threadIdx.x, wave_x = i * 64 * kWaves + (threadIdx.x & ~63);
       const int sixteen = __builtin_amdgcn_readfirstlane(wave_x / PIECES / 16);  // a wave's rows of a load lie in one
       int row = x / PIECES & 15;
-      const int group = min((t0 >> 4) + sixteen, last);
-      row = min(row, end - 1 - group * 16);
-      const int64_t at = place.at(sixteen);
-      const uint32_t in = (uint32_t)(row * ROW + x % PIECES * 16);
-      k[i] = *(const u32x4*)((const uint8_t*)p.rows.k + (MX ? at : 2 * at) + in);
-      v[i] = *(const u32x4*)((const uint8_t*)p.rows.v + (MX ? at : 2 * at) + in);
-      if constexpr (MX) {
-        ks[i] = p.rows.k_scale[at / kMxGroup + in / kMxGroup];
-        vs[i] = p.rows.v_scale[at / kMxGroup + in / kMxGroup];
-      }
+      if (CUT) row = min(row, left - 1 - min(sixteen, (left - 1) / 16) * 16);
+      const int64_t at = places.at(first + sixteen);
+      const uint32_t in = (uint32_t)(row * D + x % PIECES * 16);
+      k[i] = *(const u32x4*)((const uint8_t*)p.rows.k + at + in);
+      v[i] = *(const u32x4*)((const uint8_t*)p.rows.v + at + in);
+      ks[i] = (p.rows.k_scale + at / kMxGroup)[in / kMxGroup];
+      vs[i] = (p.rows.v_scale + at / kMxGroup)[in / kMxGroup];
     }
   }
   static __device__ __forceinline__ uint4 widen(uint32_t lo, uint32_t hi, uint32_t scale) {
@@ -389,26 +415,16 @@ template <int DT, int D, bool MX> struct StageRegs {
     return make_uint4(Mat<DT>::template widen<false>(lo, f), Mat<DT>::template widen<true>(lo, f), Mat<DT>::template widen<false>(hi, f),
                       Mat<DT>::template widen<true>(hi, f));
   }
-  // Into LDS; values of tokens behind the end and of those that are not there as zeros, which a weight of 0 leaves.
-  __device__ __forceinline__ void store(uint8_t* lds, int live, uint32_t there) const {
+  __device__ __forceinline__ void store(uint8_t* lds) const {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int x = i * 64 * kWaves + threadIdx.x, row = x / PIECES, sw = swizzle<D>(row);
-      const uint32_t mask = row < live && (there >> (row >> 4) & 1) ? ~0u : 0u;
+      const int x = i * 64 * kWaves + threadIdx.x, row = x / PIECES, piece = x % PIECES * 2, sw = swizzle<D>(row);
       uint8_t* to = lds + row * (2 * D);
-      if constexpr (!MX) {
-        to += ((x % PIECES) ^ sw) * 16;
-        *(u32x4*)to = k[i];
-        *(u32x4*)(to + BYTES) = v[i] & mask;
-      } else {
-        const int piece = x % PIECES * 2;
-        const u32x4 w = v[i] & mask;  // a code of zero is zero under any scale that is written
-        *(uint4*)(to + (piece ^ sw) * 16) = widen(k[i].x, k[i].y, ks[i]);
-        *(uint4*)(to + ((piece + 1) ^ sw) * 16) = widen(k[i].z, k[i].w, ks[i]);
-        to += BYTES;
-        *(uint4*)(to + (piece ^ sw) * 16) = widen(w.x, w.y, vs[i]);
-        *(uint4*)(to + ((piece + 1) ^ sw) * 16) = widen(w.z, w.w, vs[i]);
-      }
+      *(uint4*)(to + (piece ^ sw) * 16) = widen(k[i].x, k[i].y, ks[i]);
+      *(uint4*)(to + ((piece + 1) ^ sw) * 16) = widen(k[i].z, k[i].w, ks[i]);
+      to += BYTES;
+      *(uint4*)(to + (piece ^ sw) * 16) = widen(v[i].x, v[i].y, vs[i]);
+      *(uint4*)(to + ((piece + 1) ^ sw) * 16) = widen(v[i].z, v[i].w, vs[i]);
     }
   }
 };
@@ -419,72 +435,120 @@ struct Level {
   float limit;  // raw scores up to here stay; -inf until there is a reference
 };
 
-// 32 staged tokens against the wave's 32 rows. left: tokens that this lane's row attends of them; there: of the two sixteens.
+// The levels of rows whose largest score of some tokens is `top`; their sums follow.
 template <int DT, int D>
-__device__ __forceinline__ void wide_tile(const LdsPointer (&key_at)[D / 16], const LdsPointer (&value_at)[2][D / 32], int at, const uint4 (&qf)[D / 16], bool cut,
-                                          int left, bool there0, bool there1, float scale2, Level& level, float& l, f32x16 (&o)[D / 32]) {
+__device__ __forceinline__ void settle_level(float top, float scale2, Level& level, float& l, f32x16 (&o)[D / 32]) {
   constexpr float lift = lift_of(DT, 2), slack = slack_of(DT, 2);
+  if (!__any(top > level.limit)) return;
+  const float up = pair_max<32>(top);
+  const bool move = up > level.limit && up < INFINITY;
+  const float less = lift - up * scale2;
+  const float keep = !move ? 1.0f : level.limit == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(less - level.less);
+  level.less = move ? less : level.less;
+  level.limit = move ? up + slack / scale2 : level.limit;
+  l *= keep;
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) o[c] *= keep;
+}
+__device__ __forceinline__ float largest(const f32x16& s) {
+  float top = s[0];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+  return top;
+}
+// Scores to weights: the second product's two operands.
+template <int DT>
+__device__ __forceinline__ void wide_weights(const f32x16& s, float scale2, float less, float& l, uint4 (&p)[2]) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    float w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * k + i], scale2, less));
+    l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+    p[k] = make_uint4(Mat<DT>::pack(w[0], w[1]), Mat<DT>::pack(w[2], w[3]), Mat<DT>::pack(w[4], w[5]), Mat<DT>::pack(w[6], w[7]));
+  }
+}
+template <int D>
+__device__ __forceinline__ uint4 wide_value(const LdsPointer (&value_at)[2][D / 32], int c, int at) {
+  const uint2 lo = read_transposed(value_at[0][c] + at), hi = read_transposed(value_at[1][c] + at);
+  return make_uint4(lo.x, lo.y, hi.x, hi.y);
+}
+
+// A stage that all the wave's rows attend: no branch but the level's, so that reads, products and exponentials of its two tiles mix.
+template <int DT, int D>
+__device__ __forceinline__ void whole_stage(const LdsPointer (&key_at)[D / 16], const LdsPointer (&value_at)[2][D / 32], int at, const uint4 (&qf)[D / 16], float scale2,
+                                            Level& level, float& l, f32x16 (&o)[D / 32]) {
+  f32x16 s[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[u][i] = 0.0f;
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) s[u] = Wide<DT>::mma(read_piece(key_at[i] + at + u * 32 * 2 * D), qf[i], s[u]);
+  settle_level<DT, D>(fmaxf(largest(s[0]), largest(s[1])), scale2, level, l, o);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    uint4 p[2];
+    wide_weights<DT>(s[u], scale2, level.less, l, p);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) o[c] = Wide<DT>::mma(wide_value<D>(value_at, c, at + (32 * u + 16 * k) * 2 * D), p[k], o[c]);
+  }
+}
+
+// 32 staged tokens that not all rows attend. left: those that this lane's row attends; there: of the two sixteens.
+template <int DT, int D>
+__device__ __forceinline__ void cut_tile(const LdsPointer (&key_at)[D / 16], const LdsPointer (&value_at)[2][D / 32], int at, const uint4 (&qf)[D / 16], int left, bool there0,
+                                         bool there1, float scale2, Level& level, float& l, f32x16 (&o)[D / 32]) {
   const int half = (threadIdx.x & 32) >> 3;  // 4 (lane / 32)
   f32x16 s;
 #pragma unroll
   for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
   for (int i = 0; i < D / 16; ++i) s = Wide<DT>::mma(read_piece(key_at[i] + at), qf[i], s);
-  if (cut) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      float x = 8 * (i / 4) + i % 4 + half < left && (i < 8 ? there0 : there1) ? s[i] : -INFINITY;
-      keep_here(x);
-      s[i] = x;
-    }
+  for (int i = 0; i < 16; ++i) {
+    float x = 8 * (i / 4) + i % 4 + half < left && (i < 8 ? there0 : there1) ? s[i] : -INFINITY;
+    keep_here(x);
+    s[i] = x;
   }
-  float top = s[0];
-#pragma unroll
-  for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-  if (__any(top > level.limit)) {
-    const float up = pair_max<32>(top);
-    const bool move = up > level.limit && up < INFINITY;
-    const float less = lift - up * scale2;
-    const float keep = !move ? 1.0f : level.limit == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(less - level.less);
-    level.less = move ? less : level.less;
-    level.limit = move ? up + slack / scale2 : level.limit;
-    l *= keep;
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) o[c] *= keep;
-  }
+  settle_level<DT, D>(largest(s), scale2, level, l, o);
   uint4 p[2];
+  wide_weights<DT>(s, scale2, level.less, l, p);
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    float w[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * k + i], scale2, level.less));
-    l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-    p[k] = make_uint4(Mat<DT>::pack(w[0], w[1]), Mat<DT>::pack(w[2], w[3]), Mat<DT>::pack(w[4], w[5]), Mat<DT>::pack(w[6], w[7]));
-  }
-#pragma unroll
-  for (int k = 0; k < 2; ++k)
+    uint4 w[D / 32];
+    bool odd = false;
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
-      const uint2 lo = read_transposed(value_at[0][c] + at + 16 * k * 2 * D), hi = read_transposed(value_at[1][c] + at + 16 * k * 2 * D);
-      uint4 w = make_uint4(lo.x, lo.y, hi.x, hi.y);
-      if (cut && __any(any_not_finite<DT>(w))) {
-        uint32_t ones[4];
-        const bool there = k == 0 ? there0 : there1;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int first = 16 * k + 8 * (i / 2) + 2 * (i & 1) + half;
-          ones[i] = (there && first < left ? kOneBits<DT> : 0u) | (there && first + 1 < left ? kOneBits<DT> << 16 : 0u);
-        }
-        add_not_finite<DT>(w, make_uint4(ones[0], ones[1], ones[2], ones[3]), o[c], [](uint4 m, uint4 q, f32x16 z) { return Wide<DT>::mma(m, q, z); });
-        w = make_uint4(w.x & ~not_finite<DT>(w.x), w.y & ~not_finite<DT>(w.y), w.z & ~not_finite<DT>(w.z), w.w & ~not_finite<DT>(w.w));
-      }
-      o[c] = Wide<DT>::mma(w, p[k], o[c]);
+      w[c] = wide_value<D>(value_at, c, at + 16 * k * 2 * D);
+      odd |= any_not_finite<DT>(w[c]);
     }
+    if (__any(odd)) {
+      uint32_t ones[4];
+      const bool there = k == 0 ? there0 : there1;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int first = 16 * k + 8 * (i / 2) + 2 * (i & 1) + half;
+        ones[i] = (there && first < left ? kOneBits<DT> : 0u) | (there && first + 1 < left ? kOneBits<DT> << 16 : 0u);
+      }
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        add_not_finite<DT>(w[c], make_uint4(ones[0], ones[1], ones[2], ones[3]), o[c], [](uint4 m, uint4 q, f32x16 z) { return Wide<DT>::mma(m, q, z); });
+        w[c] = make_uint4(w[c].x & ~not_finite<DT>(w[c].x), w[c].y & ~not_finite<DT>(w[c].y), w[c].z & ~not_finite<DT>(w[c].z), w[c].w & ~not_finite<DT>(w[c].w));
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) o[c] = Wide<DT>::mma(w[c], p[k], o[c]);
+  }
 }
 
 template <int DT, int D, bool MX>
 __global__ __launch_bounds__(64 * kWaves, 2) void chunk_wide_kernel(ChunkArgs a) {
-  using S = StageRegs<DT, D, MX>;
+  using S = StageLoad<DT, D, MX>;
   constexpr int ROWS = 32 * kWaves;
   __shared__ f32x4 lds4[2 * 2 * S::BYTES / 16];
   uint8_t* const lds = (uint8_t*)lds4;
@@ -500,7 +564,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void chunk_wide_kernel(ChunkArgs a)
   const int past = e.len - e.n, begin = part * a.chunk;
   const int last = min((tile * ROWS + ROWS - 1) / a.g, e.n - 1), wave_first = x0 / a.g, wave_last = min((x0 + 31) / a.g, e.n - 1);
   const int end = last < tile * ROWS / a.g ? 0 : min(begin + a.chunk, max(past + last + 1, 0));
-  const int wave_end = wave_last < wave_first ? 0 : min(end, max(past + wave_last + 1, 0)), whole = max(past + wave_first + 1, 0);
+  const int wave_end = wave_last < wave_first ? 0 : min(end, max(past + wave_last + 1, 0));
   Level level = {0.0f, -INFINITY};
   float l = 0.0f;
   f32x16 o[D / 32];
@@ -509,10 +573,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void chunk_wide_kernel(ChunkArgs a)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[c][i] = 0.0f;
   if (begin < end) {
-    S regs;
-    StagePlace<D> place, next;
-    place.find(a.rows, b, h, begin, end);
-    regs.load(a.rows, place, begin, end);
+    S stage;
+    Places<D> places;
+    const int last16 = (end - 1) >> 4;
+    places.find(a.rows, b, h, begin >> 4, last16);
+    stage.begin();
+    stage.template load<true>(a.rows, places, 0, min(kStage, end - begin), lds);
     uint4 qf[D / 16];
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) qf[i] = row.row >= 0 ? *(const uint4*)(row.q + 16 * i + (lane >> 5) * 8) : make_uint4(0, 0, 0, 0);
@@ -531,25 +597,53 @@ __global__ __launch_bounds__(64 * kWaves, 2) void chunk_wide_kernel(ChunkArgs a)
         value_at[j][c] = (LdsPointer)lds + S::BYTES + r * (2 * D) + ((4 * c + ((lane & 16) >> 3) + ((lane & 2) >> 1)) ^ swizzle<D>(r)) * 16 + (lane & 1) * 8;
         keep_here(value_at[j][c]);
       }
-    int buffer = 0;
-    for (int t = begin; t < end; t += kStage) {
-      regs.store(lds + buffer, end - t, place.there);
+    // Stages that all the workgroup's rows attend; then those that some do not, or that have rows which are not there.
+    const int full = min(end, max(past + tile * ROWS / a.g + 1, 0));
+    int t = begin, buffer = 0;
+    uint64_t there = places.there;
+    for (; t + kStage <= full && (there & 15) == 15; t += kStage) {
+      stage.store(lds + buffer);
       __syncthreads();
-      if (t + kStage < end) {
-        next.find(a.rows, b, h, t + kStage, end);
-        regs.load(a.rows, next, t + kStage, end);
+      // The other buffer's readers came to this barrier after their last read of it.
+      const int next = t + kStage;
+      if (next < end) {
+        const int at = (next - begin) >> 4 & 63;
+        there >>= 4;
+        if (at == 0) {
+          places.find(a.rows, b, h, next >> 4, last16);
+          there = places.there;
+        }
+        if (next + kStage <= end) {
+          stage.template load<false>(a.rows, places, at, kStage, lds + (buffer ^ 2 * S::BYTES));
+        } else {
+          stage.template load<true>(a.rows, places, at, end - next, lds + (buffer ^ 2 * S::BYTES));
+        }
       }
       load_fence();
-#pragma unroll
+      whole_stage<DT, D>(key_at, value_at, buffer, qf, a.scale2, level, l, o);
+      buffer ^= 2 * S::BYTES;
+    }
+    for (; t < end; t += kStage) {
+      stage.store(lds + buffer);
+      __syncthreads();
+      const int next = t + kStage;
+      const uint32_t here = (uint32_t)there;
+      if (next < end) {
+        const int at = (next - begin) >> 4 & 63;
+        there >>= 4;
+        if (at == 0) {
+          places.find(a.rows, b, h, next >> 4, last16);
+          there = places.there;
+        }
+        stage.template load<true>(a.rows, places, at, min(kStage, end - next), lds + (buffer ^ 2 * S::BYTES));
+      }
+      load_fence();
       for (int sub = 0; sub < 2; ++sub) {
         const int now = t + 32 * sub;
-        if (now >= wave_end) continue;
-        const bool there0 = place.there >> (2 * sub) & 1, there1 = place.there >> (2 * sub + 1) & 1;
-        const bool cut = now + 32 > whole || !there0 || !there1;
-        wide_tile<DT, D>(key_at, value_at, buffer + sub * 32 * 2 * D, qf, cut, row.limit - now, there0, there1, a.scale2, level, l, o);
+        if (now >= wave_end) break;
+        cut_tile<DT, D>(key_at, value_at, buffer + sub * 32 * 2 * D, qf, row.limit - now, here >> (2 * sub) & 1, here >> (2 * sub + 1) & 1, a.scale2, level, l, o);
       }
       buffer ^= 2 * S::BYTES;
-      place = next;
     }
   }
   if (row.row < 0) return;

@@ -934,20 +934,27 @@ def _paged(rows: Rows, pages: torch.Tensor | None, seqs: int) -> tuple[object, i
     shape, st = pages.shape, pages.stride()
     if len(shape) != 2 or shape[0] != seqs or pages.dtype != torch.int32 or pages.get_device() != rows.device_index or (st[1] != 1 and shape[1] > 1) or st[0] < 0:
         raise ValueError(f"pages must be int32 [{seqs}, n] with contiguous rows on {rows.device}, got {pages.dtype} {tuple(shape)} on {pages.device}")
-    return ctypes.byref(_lib.Pages(pages.data_ptr() or None, st[0], shape[1])), rows.tokens * shape[1]
+    return _lib.Pages(pages.data_ptr(), st[0], shape[1]), rows.tokens * shape[1]
 
 
 def _reach(x: torch.Tensor) -> tuple[int, int]:
     """The addresses between which a tensor's elements lie."""
     at = x.data_ptr()
-    if x.numel() == 0:
-        return at, at
-    return at, at + x.element_size() * (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride())))
+    if x.is_contiguous():
+        return at, at + x.nbytes
+    n = 1
+    for m, s in zip(x.shape, x.stride()):
+        n += (m - 1) * s
+    return at, at + x.element_size() * n
 
 
-def _meets(x: torch.Tensor, spans: tuple) -> bool:
-    a, b = _reach(x)
-    return any(a < d and c < b for c, d in spans)
+def _meet(some: tuple, others: tuple) -> bool:
+    """Whether any of some spans of addresses meets any of the others."""
+    for a, b in some:
+        for c, d in others:
+            if a < d and c < b:
+                return True
+    return False
 
 
 def _row_spans(rows: Rows) -> tuple:
@@ -981,39 +988,56 @@ def rotate_append(
     `start + starts[b] + t` of `dst`, as with `append_rows`, with `pages` `[seqs, n]` those of a pool; tokens from `counts[b]` on go to no row.
     Returns the queries (in `out`, which must not be any of the inputs). No gradient."""
     shape, kv, dtype, index = q.shape, k.shape, dst.model_dtype, dst.device_index
-    if len(shape) != 4 or len(kv) != 4 or v.shape != kv or kv[0] != shape[0] or kv[2:] != shape[2:] or q.dtype != dtype or k.dtype != dtype or v.dtype != dtype:
+    if len(shape) != 4 or len(kv) != 4 or v.shape != kv or kv[0] != shape[0] or kv[2] != shape[2] or kv[3] != shape[3] or q.dtype != dtype or k.dtype != dtype or v.dtype != dtype:
         raise ValueError(f"expected {dtype} queries [seqs, n_q, T, d] and matching keys/values [seqs, h, T, d], got {tuple(shape)} {q.dtype}, {tuple(kv)} {k.dtype}, "
                          f"{tuple(v.shape)} {v.dtype}")
     seqs, n_q, n, d = shape
-    if kv[1] != dst.n_kv or d != dst.head_dim:
+    h = kv[1]
+    if h != dst.n_kv or d != dst.head_dim:
         raise ValueError(f"keys/values {tuple(kv)} do not match rows of {dst.n_kv} heads and head_dim {dst.head_dim}")
     if q.get_device() != index or k.get_device() != index or v.get_device() != index:
         raise ValueError(f"tokens on {q.device} / {k.device} / {v.device}, the cache on {dst.device}")
     _int32("start", start)
     rotary = table_stride = 0
     table = weight = dst.model_code
-    if (cos is None) != (sin is None):
-        raise ValueError("cos and sin come together")
-    if cos is not None:
+    read = [q, k, v]  # what the call reads
+    cos_at = sin_at = q_at = k_at = None
+    if cos is not None and sin is not None:
         cs = cos.shape
-        if len(cs) != 3 or cs[0] not in (1, seqs) or cs[1] != n or sin.shape != cs or cos.dtype != sin.dtype or cos.dtype not in (dtype, torch.float32):
+        if len(cs) != 3 or cs[0] not in (1, seqs) or cs[1] != n or sin.shape != cs or cos.dtype != sin.dtype or (cos.dtype != dtype and cos.dtype != torch.float32):
             raise ValueError(f"cos/sin must be {dtype} or float32 [{seqs} or 1, {n}, r], got {cos.dtype} {tuple(cs)} / {sin.dtype} {tuple(sin.shape)}")
         if cos.get_device() != index or sin.get_device() != index:
             raise ValueError(f"cos/sin on {cos.device} / {sin.device}, the cache on {dst.device}")
         rotary = cs[2]
         cos, sin = _whole(cos), _whole(sin)
-        table_stride = n * rotary if cs[0] != 1 else 0
-        table = _lib.dtype_code(cos.dtype)
-    for w in (q_weight, k_weight):
-        if w is not None and (w.shape != (d,) or w.dtype not in (dtype, torch.float32) or w.get_device() != index):
-            raise ValueError(f"weights must be {dtype} or float32 [{d}] on {dst.device}, got {w.dtype} {tuple(w.shape)} on {w.device}")
-    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
-        raise ValueError(f"weights of {q_weight.dtype} and {k_weight.dtype}")
+        cos_at, sin_at = cos.data_ptr(), sin.data_ptr()
+        read += (cos, sin)
+        if cs[0] != 1:
+            table_stride = n * rotary
+        if cos.dtype != dtype:
+            table = _lib.F32
+    elif cos is not None or sin is not None:
+        raise ValueError("cos and sin come together")
     if q_weight is not None or k_weight is not None:
-        weight = _lib.dtype_code((q_weight if q_weight is not None else k_weight).dtype)
-        q_weight, k_weight = (w if w is None else _whole(w) for w in (q_weight, k_weight))
-    given = tuple(x for x in (cos, sin, q_weight, k_weight, out) if x is not None)
-    _no_gradients("rotate_append", (q, k, v, *dst.owners, *given))
+        kinds = set()
+        for w in (q_weight, k_weight):
+            if w is not None:
+                kinds.add(w.dtype)
+                if w.shape != (d,) or (w.dtype != dtype and w.dtype != torch.float32) or w.get_device() != index:
+                    raise ValueError(f"weights must be {dtype} or float32 [{d}] on {dst.device}, got {w.dtype} {tuple(w.shape)} on {w.device}")
+        if len(kinds) != 1:
+            raise ValueError(f"weights of {q_weight.dtype} and {k_weight.dtype}")
+        if dtype not in kinds:
+            weight = _lib.F32
+        if q_weight is not None:
+            q_weight = _whole(q_weight)
+            q_at = q_weight.data_ptr()
+            read.append(q_weight)
+        if k_weight is not None:
+            k_weight = _whole(k_weight)
+            k_at = k_weight.data_ptr()
+            read.append(k_weight)
+    _no_gradients("rotate_append", (*read, *dst.owners) if out is None else (*read, *dst.owners, out))
     at, count = _counts(starts, seqs, index, "starts"), _counts(counts, seqs, index, "counts")
     table_ref, _ = _paged(dst, pages, seqs)
     if out is not None:
@@ -1022,23 +1046,31 @@ def rotate_append(
         ot = _meant(shape, out.stride())
         if ot[3] != 1 or (ot[0] | ot[1] | ot[2]) % 8 or out.data_ptr() % 16:
             raise ValueError("out's rows must be contiguous and start on 16 bytes")
-        if _meets(out, (*(_reach(x) for x in (q, k, v, *given[:-1])), *_row_spans(dst))):
+        if _meet((_reach(out),), (*map(_reach, read), *_row_spans(dst))):
             raise ValueError("out must not lie among the inputs or the cache's rows")
+    elif 0 in shape:
+        return q.new_empty(shape)
+    else:
+        out = torch.empty_like(q)
+        ot = out.stride()
     if 0 in shape:
-        return q.new_empty(shape) if out is None else out
-    if out is None:
-        out = torch.empty(shape, dtype=dtype, device=q.device)
-    (x, xt), (y, yt), (z, zt) = _placed(q), _placed(k), _placed(v)
-    spans = _row_spans(dst)
-    if spans:  # the cache's own rows: none is written before all are read
-        x, y, z = (w.clone(memory_format=torch.contiguous_format) if _meets(w, spans) else w for w in (x, y, z))
-        xt, yt, zt = (_meant(w.shape, w.stride()) for w in (x, y, z))
+        return out
+    qt, kt, vt = q.stride(), k.stride(), v.stride()
+    x, y, z = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if (qt[0] | qt[1] | qt[2] | kt[0] | kt[1] | kt[2] | vt[0] | vt[1] | vt[2]) & 7 or (x | y | z) & 15 or qt[3] != 1 or kt[3] != 1 or vt[3] != 1:
+        (q, qt), (k, kt), (v, vt) = _placed(q), _placed(k), _placed(v)
+        x, y, z = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if dst.span is not None:
+        mine = ((x, x + 2 * ((seqs - 1) * qt[0] + (n_q - 1) * qt[1] + (n - 1) * qt[2] + d)), (y, y + 2 * ((seqs - 1) * kt[0] + (h - 1) * kt[1] + (n - 1) * kt[2] + d)),
+                (z, z + 2 * ((seqs - 1) * vt[0] + (h - 1) * vt[1] + (n - 1) * vt[2] + d)))
+        if _meet(mine, _row_spans(dst)):  # the cache's own rows: none is written before all are read
+            q, k, v = (w.clone(memory_format=torch.contiguous_format) for w in (q, k, v))
+            qt, kt, vt = q.stride(), k.stride(), v.stride()
+            x, y, z = q.data_ptr(), k.data_ptr(), v.data_ptr()
     _WRITTEN((*dst.owners, out))
-    desc = _lib.RotateDesc(seqs, n_q, kv[1], d, n, dst.model_code, rotary, table, weight, eps, _lib.Triple(*xt[:3]), _lib.Triple(*yt[:3]), _lib.Triple(*zt[:3]),
-                           _lib.Triple(*_meant(shape, out.stride())[:3]), table_stride)
-    rc = _launch(index, _lib.lib().lkv_rotate_append, ctypes.byref(desc), x.data_ptr(), y.data_ptr(), z.data_ptr(), cos.data_ptr() if rotary else None,
-                 sin.data_ptr() if rotary else None, q_weight.data_ptr() if q_weight is not None else None, k_weight.data_ptr() if k_weight is not None else None,
-                 out.data_ptr(), dst.ref, table_ref, at, start, count)
+    desc = _lib.RotateDesc(seqs, n_q, h, d, n, dst.model_code, rotary, table, weight, eps, qt[0], qt[1], qt[2], kt[0], kt[1], kt[2], vt[0], vt[1], vt[2], ot[0], ot[1], ot[2],
+                           table_stride)
+    rc = _launch(index, _lib.lib().lkv_rotate_append, desc, x, y, z, cos_at, sin_at, q_at, k_at, out.data_ptr(), dst.struct, table_ref, at, start, count)
     if rc:
         _lib.check(rc, "rotate_append")
     return out
@@ -1068,8 +1100,10 @@ def _chunk(what: str, q: torch.Tensor, rows: Rows, scale: float, tokens: int, le
     if lengths is None and tokens > max_tokens:
         raise ValueError(f"tokens={tokens} exceed max_tokens={max_tokens}")
     at, count = _counts(lengths, seqs, index, "lengths"), _counts(counts, seqs, index, "counts")
-    q, st = _placed(q)
-    return _lib.ChunkDesc(seqs, n_q, rows.n_kv, d, n, scale, tokens, max_tokens, _lib.Triple(*st[:3])), q, at, count, table, max_tokens
+    st = q.stride()
+    if (st[0] | st[1] | st[2]) & 7 or st[3] != 1 or q.data_ptr() & 15:
+        q, st = _placed(q)
+    return _lib.ChunkDesc(seqs, n_q, rows.n_kv, d, n, scale, tokens, max_tokens, st[0], st[1], st[2]), q, at, count, table, max_tokens
 
 
 def _scratch(need: int, ws: Workspace | None, device: torch.device) -> tuple[int | None, int, object]:
@@ -1118,7 +1152,8 @@ def chunk_attend(
     if 0 in shape:
         return out, lse
     if given:
-        if any(_meets(x, (_reach(q), *_row_spans(rows))) for x in given) or (len(given) == 2 and _meets(out, (_reach(lse),))):
+        mine = tuple(map(_reach, given))
+        if _meet(mine, (_reach(q), *_row_spans(rows))) or (len(mine) == 2 and _meet(mine[:1], mine[1:])):
             raise ValueError("out and lse must not lie among the inputs or each other")
         _WRITTEN(given)
     lib = _lib.lib()
@@ -1142,8 +1177,9 @@ def _account(name: str, x: torch.Tensor, dtype: torch.dtype, seqs: int, n_kv: in
     return _lib.Pair(a, b)
 
 
-def _same_or_apart(what: str, out: torch.Tensor, x: torch.Tensor) -> None:
-    if (out.data_ptr() != x.data_ptr() or _meant(out.shape, out.stride()) != _meant(x.shape, x.stride())) and _meets(out, (_reach(x),)):
+def _same_or_apart(what: str, out: torch.Tensor, x: torch.Tensor, at: tuple[int, int], x_at: tuple[int, int]) -> None:
+    """Refuses an output that overlaps its input without being it. at, x_at: where they lie."""
+    if at[0] < x_at[1] and x_at[0] < at[1] and (at[0] != x_at[0] or _meant(out.shape, out.stride()) != _meant(x.shape, x.stride())):
         raise ValueError(f"{what} overlap without being the same")
 
 
@@ -1184,11 +1220,18 @@ def weigh_rows(
     first = _counts(seen, seqs, index, "seen")
     if seen is not None and positions is None:
         raise ValueError("seen says where positions start; there are none")
-    if sums is not None:
-        _same_or_apart("sums and out", out, sums)
-    written = (out,) if positions is None else (out, positions)
-    if any(_meets(x, (_reach(q), _reach(lse), *_row_spans(rows))) for x in written) or (
-            positions is not None and (_meets(positions, (_reach(out),)) or (sums is not None and _meets(positions, (_reach(sums),))))):
+    out_at = _reach(out)
+    inputs = (_reach(q), _reach(lse), *_row_spans(rows))
+    if sums is not None and sums is not out:
+        sums_at = _reach(sums)
+        _same_or_apart("sums and out", out, sums, out_at, sums_at)
+    else:
+        sums_at = out_at
+    if positions is None:
+        written, mine = (out,), (out_at,)
+    else:
+        written, mine = (out, positions), (out_at, _reach(positions))
+    if _meet(mine, inputs) or (positions is not None and _meet(mine[1:], (out_at, sums_at))):
         raise ValueError("out and positions must not lie among the inputs or each other")
     if seqs == 0 or most == 0:
         return out
@@ -1240,12 +1283,16 @@ def evict_rows(
     strides = [_account(name, x, t, seqs, rows.n_kv, n, index) for name, x, t, n in (
         ("sums", sums, torch.float32, least), ("positions", positions, torch.int32, least), ("out's sums", to[0], torch.float32, min(least, max(0, keep))),
         ("out's positions", to[1], torch.int32, min(least, max(0, keep))))]
+    spots = _reach(sums), _reach(positions)
     if out is not None:
-        _same_or_apart("sums", to[0], sums)
-        _same_or_apart("positions", to[1], positions)
-        if _meets(to[0], (_reach(to[1]), _reach(positions))) or _meets(to[1], (_reach(sums),)):
+        ends = _reach(to[0]), _reach(to[1])
+        _same_or_apart("sums", to[0], sums, ends[0], spots[0])
+        _same_or_apart("positions", to[1], positions, ends[1], spots[1])
+        if _meet(ends[:1], (ends[1], spots[1])) or _meet(ends[1:], spots[:1]):
             raise ValueError("sums and positions share addresses")
-    if _meets(sums, (_reach(positions),)) or any(_meets(x, _row_spans(rows)) for x in (sums, positions, *to)):
+    else:
+        ends = spots
+    if _meet(spots[:1], spots[1:]) or _meet((*spots, *ends), _row_spans(rows)):
         raise ValueError("sums, positions and rows share addresses")
     lib = _lib.lib()
     desc = _lib.EvictDesc(seqs, rows.n_kv, rows.head_dim, rows.model_code, keep, sinks, recent, tokens, max_tokens)

@@ -24,7 +24,7 @@ def test_a_rows_page_is_found_by_one_multiplication(sixteens: int) -> None:
 def _chunk(n_seqs: int, n_q: int, n_kv: int, d: int, t: int, most: int):  # noqa: ANN202
     from lazykv_amd import _lib
 
-    return _lib.ChunkDesc(n_seqs, n_q, n_kv, d, t, 0.1, 0, most, _lib.Triple(n_q * t * d, t * d, d))
+    return _lib.ChunkDesc(n_seqs, n_q, n_kv, d, t, 0.1, 0, most, n_q * t * d, t * d, d)
 
 
 @pytest.mark.parametrize("d", [64, 128])
@@ -60,7 +60,7 @@ def _call(fn: str, change: dict) -> str:
     pages = _lib.Pages(p["table"], p["seq_stride"], p["n_pages"]) if change.get("pages", 1) is not None else None
     refs = ctypes.byref(rows), (None if pages is None else ctypes.byref(pages))
     d = case["desc"]
-    desc = _lib.ChunkDesc(d["n_seqs"], d["n_q"], d["n_kv"], d["head_dim"], d["new_tokens"], d["scale"], d["tokens"], d["max_tokens"], _lib.Triple(*case["strides"]))
+    desc = _lib.ChunkDesc(d["n_seqs"], d["n_q"], d["n_kv"], d["head_dim"], d["new_tokens"], d["scale"], d["tokens"], d["max_tokens"], *case["strides"])
     two = _lib.Pair(128, 64)
     if fn == "attend":
         rc = lib.lkv_chunk_attend(0, ctypes.byref(desc), case["q"], case["dtype"], *refs, None, None, case["out"], 0, case["lse"], case["ws"], case["ws_bytes"])
@@ -73,8 +73,8 @@ def _call(fn: str, change: dict) -> str:
         rc = lib.lkv_evict_rows(0, ctypes.byref(ev), *refs, None, case["lse"], two, case["lse"], two, case["out"], two, case["out"], two, case["ws"], case["ws_bytes"])
     else:
         x = {"rotary": 64, "table": 0, "weight": 0, "eps": 0.0, "start": 0, "cos": 4096, **change.get("rotate", {})}
-        st = _lib.Triple(*case["strides"])
-        ro = _lib.RotateDesc(d["n_seqs"], d["n_q"], d["n_kv"], d["head_dim"], d["new_tokens"], case["dtype"], x["rotary"], x["table"], x["weight"], x["eps"], st, st, st, st, 0)
+        st = case["strides"]
+        ro = _lib.RotateDesc(d["n_seqs"], d["n_q"], d["n_kv"], d["head_dim"], d["new_tokens"], case["dtype"], x["rotary"], x["table"], x["weight"], x["eps"], *st, *st, *st, *st, 0)
         rc = lib.lkv_rotate_append(0, ctypes.byref(ro), case["q"], case["q"], case["q"], x["cos"], x["cos"], case["q"], case["q"], case["out"], *refs, None, x["start"], None)
     assert rc == -1, rc
     return lib.lkv_last_error().decode()
