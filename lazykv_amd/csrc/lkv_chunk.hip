@@ -60,7 +60,7 @@ __device__ __forceinline__ QueryRow query_row(const ChunkArgs& a, const Extent& 
 template <int D>
 __device__ __forceinline__ void store_part(const ChunkArgs& a, int64_t row, int part, int channel, float l, f32x4 x) {
   if (a.parts > 1) {
-    *(f32x4*)(a.part_o + (row * a.parts + part) * D + channel) = x;
+    if (l != 0.0f) *(f32x4*)(a.part_o + (row * a.parts + part) * D + channel) = x;  // a part without weight is not read
     return;
   }
   x = l == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : x * (1.0f / l);
@@ -547,7 +547,7 @@ __device__ __forceinline__ void cut_tile(const LdsPointer (&key_at)[D / 16], con
 }
 
 template <int DT, int D, bool MX>
-__global__ __launch_bounds__(64 * kWaves, 2) void chunk_wide_kernel(ChunkArgs a) {
+__global__ __launch_bounds__(64 * kWaves, D == 64 && !MX ? 3 : 2) void chunk_wide_kernel(ChunkArgs a) {
   using S = StageLoad<DT, D, MX>;
   constexpr int ROWS = 32 * kWaves;
   __shared__ f32x4 lds4[2 * 2 * S::BYTES / 16];
@@ -646,16 +646,41 @@ __global__ __launch_bounds__(64 * kWaves, 2) void chunk_wide_kernel(ChunkArgs a)
       buffer ^= 2 * S::BYTES;
     }
   }
-  if (row.row < 0) return;
   constexpr float down = 1.0f / (float)(1 << (int)lift_of(DT, 2));
   l = row.limit == 0 ? 0.0f : pair_sum<32>(l) * down;
-  const float m = level.limit == -INFINITY ? -INFINITY : lift_of(DT, 2) - level.less;
-  if (lane < 32) store_sums(a, row.row, part, m, l);
+  if (row.row >= 0 && lane < 32) store_sums(a, row.row, part, level.limit == -INFINITY ? -INFINITY : lift_of(DT, 2) - level.less, l);
+  // Through LDS to rows that lie together: a wave's own 32 rows, 16-byte pieces swizzled by the row. (Stored from where they are, 16 bytes a lane, a row's neighbours in
+  // the other half of the lanes: 2,048 workgroups' parts took 45 us more than 512's.)
+  constexpr int PIECES = D / 4;
+  f32x4* const mine = lds4 + wave * 32 * PIECES;
+  __syncthreads();  // what LDS held before is read no more
+  const float f = a.parts > 1 ? down : l == 0.0f ? 0.0f : down / l;
 #pragma unroll
   for (int c = 0; c < D / 32; ++c)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      store_part<D>(a, row.row, part, 32 * c + 8 * i + 4 * (lane >> 5), l, f32x4{o[c][4 * i], o[c][4 * i + 1], o[c][4 * i + 2], o[c][4 * i + 3]} * down);
+    for (int i = 0; i < 4; ++i) {
+      const f32x4 x = f32x4{o[c][4 * i], o[c][4 * i + 1], o[c][4 * i + 2], o[c][4 * i + 3]} * f;
+      mine[(lane & 31) * PIECES + ((8 * c + 2 * i + (lane >> 5)) ^ (lane & (PIECES - 1) & 31))] = l == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : x;
+    }
+  const int lo = (int)(uint32_t)row.row, hi = (int)(row.row >> 32);
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll 4
+  for (int i = 0; i < 32 * PIECES / 64; ++i) {
+    const int r = (i * 64 + lane) / PIECES, piece = lane % PIECES;
+    const int64_t to = (int64_t)((uint64_t)(uint32_t)__shfl(hi, r) << 32 | (uint32_t)__shfl(lo, r));
+    const float sum = __shfl(l, r);
+    const f32x4 x = mine[r * PIECES + (piece ^ (r & (PIECES - 1)))];
+    if (to < 0) continue;
+    if (a.parts > 1) {
+      if (sum != 0.0f) *(f32x4*)(a.part_o + (to * a.parts + part) * D + piece * 4) = x;  // a part without weight is not read
+    } else if (a.out_dtype == LKV_F32) {
+      store_four<LKV_F32>(a.out, to * D + piece * 4, x);
+    } else if (a.out_dtype == LKV_BF16) {
+      store_four<LKV_BF16>(a.out, to * D + piece * 4, x);
+    } else {
+      store_four<LKV_F16>(a.out, to * D + piece * 4, x);
+    }
+  }
 }
 
 // A query row's parts into one, a wave a row: d / 4 lanes take a part's channels, four each, and the others the next part's.

@@ -6,6 +6,8 @@
 // The accumulators start at -lse / scale, and the scores come out relative to it. That form reads the queries from memory, for up to 32 query rows of
 // a KV head. More of them go through LDS, 64 at a time for four waves, on v_mfma_f32_32x32x16; there -lse is the addend of the exponent's one
 // multiply-add.
+#include <type_traits>
+
 #include "lkv_attend.h"
 #include "lkv_pages.h"
 
@@ -32,6 +34,8 @@ struct WeighArgs {
   float scale2, per_scale;  // scale * log2(e), 1 / scale
   int32_t n_seqs, n_q, n_kv, g, new_tokens, tokens, max_tokens;
   int32_t blocks, parts, chunk;  // of a KV head's rows; of its query rows, in ranges of `chunk`
+  int32_t step_t, step_j;        // a stage of query rows further: tokens, heads of the group; and in elements
+  int64_t step_at, wrap_at;      // , and from the last head of a token to the first of the next beyond a head's step
 };
 
 struct Extent {
@@ -181,31 +185,63 @@ template <int DT> __device__ __forceinline__ f32x16 wide_mma(uint4 a, uint4 b, f
 constexpr int kStage = 64;  // query rows
 template <int D> __device__ __forceinline__ int swizzle(int row) { return D == 128 ? row & 15 : (row >> 1) & 7; }
 
-// A stage's query rows on their way to LDS, what is added to their exponents, and how many of a sequence's rows they attend.
+// A query row that goes on by a stage at a time: its token, its head in the group and where it is, without a division for each.
+struct Walk {
+  int t, j;
+  int64_t at;
+  __device__ __forceinline__ void begin(const WeighArgs& a, int b, int h, int x) {
+    t = x / a.g;
+    j = x - t * a.g;
+    at = b * a.q_stride[0] + (h * a.g + j) * a.q_stride[1] + t * a.q_stride[2];
+  }
+  __device__ __forceinline__ void next(const WeighArgs& a) {
+    t += a.step_t;
+    j += a.step_j;
+    at += a.step_at;
+    if (j >= a.g) {
+      j -= a.g;
+      t += 1;
+      at += a.wrap_at;
+    }
+  }
+};
+
+// A stage's query rows on their way to LDS, what is added to their exponents, and how many of a sequence's rows they attend. Rows from x_end on are the first
+// one of the range again, without weight.
 template <int D> struct StageQueries {
   static constexpr int PIECES = D / 8, LOADS = kStage * PIECES / (64 * kWaves);
   u32x4 w[LOADS];
-  uint32_t keep[LOADS];
-  float less;
+  float lse[LOADS], less;
   int limit;
-  __device__ __forceinline__ void load(const WeighArgs& a, const Extent& e, int b, int h, int x0, int x_end) {
+  Walk row[LOADS], mine;
+  int x;  // the stage's first row
+  __device__ __forceinline__ void begin(const WeighArgs& a, int b, int h, int x0) {
+    x = x0;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) row[i].begin(a, b, h, x0 + (i * 64 * kWaves + (int)threadIdx.x) / PIECES);
+    mine.begin(a, b, h, x0 + (int)(threadIdx.x & (kStage - 1)));
+  }
+  __device__ __forceinline__ void load(const WeighArgs& a, const Extent& e, int b, int h, const Walk& first, int x_end) {
+    const float* lses = a.lse + ((int64_t)b * a.n_q + h * a.g) * a.new_tokens;
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int x = min(x0 + (i * 64 * kWaves + (int)threadIdx.x) / PIECES, x_end - 1), t = x / a.g, j = h * a.g + (x - t * a.g);
-      const uint16_t* q = a.q + b * a.q_stride[0] + j * a.q_stride[1] + t * a.q_stride[2];
-      w[i] = *(const u32x4*)(q + threadIdx.x % PIECES * 8);
-      keep[i] = a.lse[((int64_t)b * a.n_q + j) * a.new_tokens + t] != -INFINITY ? ~0u : 0u;
+      const bool live = x + (i * 64 * kWaves + (int)threadIdx.x) / PIECES < x_end;
+      w[i] = *(const u32x4*)(a.q + (live ? row[i].at : first.at) + threadIdx.x % PIECES * 8);
+      lse[i] = lses[(int64_t)(live ? row[i].j : first.j) * a.new_tokens + (live ? row[i].t : first.t)];
+      row[i].next(a);
     }
-    const int x = x0 + (int)(threadIdx.x & (kStage - 1)), y = min(x, x_end - 1), t = y / a.g, j = h * a.g + (y - t * a.g);
-    const float lse = a.lse[((int64_t)b * a.n_q + j) * a.new_tokens + t];
-    less = x < x_end && lse != -INFINITY ? -lse * kLog2e : -INFINITY;
-    limit = e.len - e.n + t + 1;
+    const bool live = x + (int)(threadIdx.x & (kStage - 1)) < x_end;
+    const float l = lses[(int64_t)(live ? mine.j : first.j) * a.new_tokens + (live ? mine.t : first.t)];
+    less = live && l != -INFINITY ? -l * kLog2e : -INFINITY;
+    limit = e.len - e.n + mine.t + 1;
+    mine.next(a);
+    x += kStage;
   }
   __device__ __forceinline__ void store(uint8_t* lds, float* less_at, int* limit_at) const {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const int x = i * 64 * kWaves + threadIdx.x, row = x / PIECES;
-      *(u32x4*)(lds + row * (2 * D) + ((x % PIECES) ^ swizzle<D>(row)) * 16) = w[i] & keep[i];
+      const int y = i * 64 * kWaves + threadIdx.x, r = y / PIECES;
+      *(u32x4*)(lds + r * (2 * D) + ((y % PIECES) ^ swizzle<D>(r)) * 16) = w[i] & (lse[i] != -INFINITY ? ~0u : 0u);
     }
     if (threadIdx.x < kStage) {
       less_at[threadIdx.x] = less;
@@ -213,6 +249,29 @@ template <int D> struct StageQueries {
     }
   }
 };
+
+// The weights of 32 staged queries for a tile of 32 keys, summed. CUT: not all of them attend all keys; `row` is the lane's.
+template <int DT, int D, bool CUT>
+__device__ __forceinline__ float tile_sum(const uint4 (&q)[D / 16], const uint4 (&k)[D / 16], const f32x4 (&less)[4], const int* limits, int row, float scale2) {
+  f32x16 s;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s[i] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i) s = wide_mma<DT>(q[i], k[i], s);
+  float p[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    float y = __builtin_fmaf(s[i], scale2, less[i / 4][i % 4]);
+    if constexpr (CUT) {
+      y = row < limits[8 * (i / 4) + i % 4] ? y : -INFINITY;
+      keep_here(y);
+    }
+    p[i] = __builtin_amdgcn_exp2f(y);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) p[i] += p[i + 8];
+  return ((p[0] + p[4]) + (p[1] + p[5])) + ((p[2] + p[6]) + (p[3] + p[7]));
+}
 
 template <int DT, int D, bool MX>
 __global__ __launch_bounds__(64 * kWaves, 2) void weigh_wide_kernel(WeighArgs a) {
@@ -250,9 +309,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_wide_kernel(WeighArgs a)
       }
     }
   }
-  // The first query that attends the workgroup's first row, and the first one that attends all the wave's rows.
+  // The first query that attends the workgroup's first row, and the first one that attends all its rows.
   const int past = e.len - e.n, x_end = min(e.n * a.g, (part + 1) * a.chunk);
-  const int x_first = max(part * a.chunk, max(block * kBlockRows - past, 0) * a.g), x_whole = max(row0 + kWaveRows - 1 - past, 0) * a.g;
+  const int x_first = max(part * a.chunk, max(block * kBlockRows - past, 0) * a.g), x_whole = max(min(block * kBlockRows + kBlockRows, e.len) - 1 - past, 0) * a.g;
   float sum[2] = {0.0f, 0.0f};
   if (x_first < x_end) {
     LdsPointer at[D / 16];
@@ -261,17 +320,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_wide_kernel(WeighArgs a)
       at[i] = (LdsPointer)lds + (lane & 31) * (2 * D) + ((2 * i + half) ^ swizzle<D>(lane & 31)) * 16;
       keep_here(at[i]);
     }
-    StageQueries<D> regs;
-    regs.load(a, e, b, h, x_first, x_end);
+    Walk first;
+    first.begin(a, b, h, x_first);
+    StageQueries<D> stage;
+    stage.begin(a, b, h, x_first);
+    stage.load(a, e, b, h, first, x_end);
     int buffer = 0;
-    for (int x = x_first; x < x_end; x += kStage) {
-      regs.store(lds + buffer * BYTES, less_at[buffer], limit_at[buffer]);
+    const auto round = [&](int x, auto cut) __attribute__((always_inline)) {
+      stage.store(lds + buffer * BYTES, less_at[buffer], limit_at[buffer]);
       __syncthreads();
-      if (x + kStage < x_end) regs.load(a, e, b, h, x + kStage, x_end);
+      if (x + kStage < x_end) stage.load(a, e, b, h, first, x_end);
       load_fence();
 #pragma unroll
       for (int sub = 0; sub < kStage / 32; ++sub) {
-        if (x + 32 * sub >= x_end) continue;
         uint4 q[D / 16];
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) q[i] = read_piece(at[i] + buffer * BYTES + sub * 32 * 2 * D);
@@ -279,31 +340,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_wide_kernel(WeighArgs a)
 #pragma unroll
         for (int i = 0; i < 4; ++i) less[i] = *(const f32x4*)&less_at[buffer][32 * sub + 8 * i + 4 * half];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          f32x16 s;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[i] = 0.0f;
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) s = wide_mma<DT>(q[i], k[u][i], s);
-          if (x + 32 * sub < x_whole) {
-            const int mine = row0 + 32 * u + (lane & 31);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              float y = mine < limit_at[buffer][32 * sub + 8 * (i / 4) + 4 * half + i % 4] ? s[i] : -INFINITY;
-              keep_here(y);
-              s[i] = y;
-            }
-          }
-          float p[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, less[i / 4][i % 4]));
-#pragma unroll
-          for (int i = 0; i < 8; ++i) p[i] += p[i + 8];
-          sum[u] += ((p[0] + p[4]) + (p[1] + p[5])) + ((p[2] + p[6]) + (p[3] + p[7]));
-        }
+        for (int u = 0; u < 2; ++u)
+          sum[u] += tile_sum<DT, D, decltype(cut)::value>(q, k[u], less, &limit_at[buffer][32 * sub + 4 * half], row0 + 32 * u + (lane & 31), a.scale2);
       }
       buffer ^= 1;
-    }
+    };
+    int x = x_first;
+    for (; x < min(x_whole, x_end); x += kStage) round(x, std::true_type());
+    for (; x < x_end; x += kStage) round(x, std::false_type());
   }
   // Each half stores a tile's rows.
   const float first = pair_sum<32>(sum[0]), second = pair_sum<32>(sum[1]);
@@ -404,6 +448,10 @@ extern "C" int lkv_weigh_rows(uintptr_t stream, const lkv_chunk_desc* desc, cons
   a.blocks = p.blocks;
   a.parts = p.parts;
   a.chunk = p.chunk;
+  a.step_t = kStage / a.g;
+  a.step_j = kStage % a.g;
+  a.step_at = a.step_t * a.q_stride[2] + a.step_j * a.q_stride[1];
+  a.wrap_at = a.q_stride[2] - a.g * a.q_stride[1];
   const hipStream_t s = (hipStream_t)stream;
   const bool half = q_dtype == LKV_F16, wide = desc->head_dim == 128, mx = rows->dtype == LKV_MXFP8;
   auto kernel = half ? (wide ? (mx ? kernel_of<LKV_F16, 128, true>(p) : kernel_of<LKV_F16, 128, false>(p)) : (mx ? kernel_of<LKV_F16, 64, true>(p) : kernel_of<LKV_F16, 64, false>(p)))
