@@ -24,12 +24,14 @@ struct ChunkArgs {
   const int32_t* counts;
   void* out;
   float* lse;
-  float2* part_ml;  // [query rows][parts]: a part's maximum (base 2) and sum
-  float* part_o;    // [query rows][parts][d]
+  float2* part_ml;  // [parts][query rows of a sequence]: a part's maximum (base 2) and sum
+  float* part_o;    // [parts][query rows of a sequence][d]
   int64_t q_stride[3];
   float scale2;  // scale * log2(e)
   int32_t n_seqs, n_q, n_kv, g, new_tokens, tokens, max_tokens, out_dtype;
-  int32_t tiles, parts, chunk;  // row tiles of a KV head; its rows in `parts` ranges of `chunk`
+  int32_t tiles;   // of a KV head's query rows
+  int32_t unit;    // log2 of the rows that they are divided by
+  int32_t share;   // parts that the sequences' rows are divided into at most; 0: each sequence in one, which writes the output
 };
 
 // What a sequence has: rows in all, and the call's own among them.
@@ -56,11 +58,67 @@ __device__ __forceinline__ QueryRow query_row(const ChunkArgs& a, const Extent& 
   return {row, limit, a.q + b * a.q_stride[0] + j * a.q_stride[1] + t * a.q_stride[2]};
 }
 
+// The division of the sequences' rows: by what there is of them on the device, so that all parts are about as long, however the sequences' lengths differ. Rows are counted in
+// units; a part has as many as make `share` parts of all at the most, and each sequence at least one part. (Each sequence in
+// as many parts as the next, four sequences of 1,643 to 16,475 rows under 64 tokens each took 82 us and now 66, a step of sixteen of up to 8,192 71 and now 57.)
+__device__ __forceinline__ uint32_t units_of(const ChunkArgs& a, int b) { return b < a.n_seqs ? (uint32_t)(extent_of(a, b).len + (1 << a.unit) - 1) >> a.unit : 0; }
+__device__ __forceinline__ uint32_t wave_total(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)wave_inclusive_sum(x), 63); }
+__device__ __forceinline__ uint32_t parts_of(const ChunkArgs& a, int b, uint32_t units) { return b < a.n_seqs ? max((units_of(a, b) + units - 1) / units, 1u) : 0; }
+// Units of a part: at least those that make `share` parts of all, and so many that the sequences' parts, whose last ones are not whole, are no more than `share`.
+// That ends: n_seqs is less, and parts as long as the longest sequence are as many. The sum stays below 2^32 (plan_of).
+__device__ __forceinline__ uint32_t part_units(const ChunkArgs& a) {
+  uint32_t all = 0;
+  for (int i = threadIdx.x & 63; i < a.n_seqs; i += 64) all += units_of(a, i);
+  uint32_t units = max((wave_total(all) + a.share - 1) / a.share, 1u);
+  for (;;) {
+    uint32_t parts = 0;
+    for (int i = 0; i < a.n_seqs; i += 64) parts += parts_of(a, i + (int)(threadIdx.x & 63), units);
+    if (wave_total(parts) <= (uint32_t)a.share) return units;
+    units += max(units >> 4, 1u);
+  }
+}
+
+// What a workgroup does: rows begin .. begin + chunk of sequence b for a tile of KV head h's query rows.
+struct Item {
+  int b, h, tile, slot, begin, chunk;  // slot: which part of all; -1: the only one of its sequence. b < 0: nothing
+};
+__device__ __forceinline__ Item item_of(const ChunkArgs& a) {
+  int id = blockIdx.x;
+  if (a.share == 0) {
+    const int heads = a.n_seqs * a.n_kv, bh = id % heads;
+    // The longest tiles first: the last ones of a sequence attend the most rows.
+    return {bh / a.n_kv, bh % a.n_kv, a.tiles - 1 - id / heads, -1, 0, 1 << 30};
+  }
+  const int h = id % a.n_kv;
+  id /= a.n_kv;
+  const int tile = a.tiles - 1 - id % a.tiles;
+  const uint32_t slot = (uint32_t)(id / a.tiles), units = part_units(a);
+  uint32_t before = 0;
+  for (int i = 0; i < a.n_seqs; i += 64) {
+    const uint32_t mine = parts_of(a, i + (int)(threadIdx.x & 63), units), up_to = before + wave_inclusive_sum(mine);
+    const uint64_t behind = __ballot(up_to > slot);
+    if (behind) {
+      const int lane = __builtin_ctzll(behind);
+      const uint32_t part = slot - (uint32_t)__builtin_amdgcn_readlane((int)(up_to - mine), lane);
+      const int chunk = (int)min((uint64_t)units << a.unit, (uint64_t)(1 << 30));
+      return {i + lane, h, tile, (int)slot, (int)min((uint64_t)part * units << a.unit, (uint64_t)(1 << 30)), chunk};
+    }
+    before = (uint32_t)__builtin_amdgcn_readlane((int)up_to, 63);
+  }
+  return {-1, h, tile, (int)slot, 0, 0};
+}
+
+// Where a query row's partial result is.
+__device__ __forceinline__ int64_t part_row(const ChunkArgs& a, int slot, int b, int64_t row) {
+  const int64_t rows = (int64_t)a.n_q * a.new_tokens;
+  return slot * rows + row - b * rows;
+}
+
 // Four channels of a row: a part's, or, where it is the only part, the output's.
 template <int D>
-__device__ __forceinline__ void store_part(const ChunkArgs& a, int64_t row, int part, int channel, float l, f32x4 x) {
-  if (a.parts > 1) {
-    if (l != 0.0f) *(f32x4*)(a.part_o + (row * a.parts + part) * D + channel) = x;  // a part without weight is not read
+__device__ __forceinline__ void store_part(const ChunkArgs& a, const Item& item, int64_t row, int channel, float l, f32x4 x) {
+  if (item.slot >= 0) {
+    if (l != 0.0f) *(f32x4*)(a.part_o + part_row(a, item.slot, item.b, row) * D + channel) = x;  // a part without weight is not read
     return;
   }
   x = l == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : x * (1.0f / l);
@@ -72,9 +130,9 @@ __device__ __forceinline__ void store_part(const ChunkArgs& a, int64_t row, int 
     store_four<LKV_F16>(a.out, row * D + channel, x);
   }
 }
-__device__ __forceinline__ void store_sums(const ChunkArgs& a, int64_t row, int part, float m, float l) {
-  if (a.parts > 1) {
-    a.part_ml[row * a.parts + part] = make_float2(m, l);
+__device__ __forceinline__ void store_sums(const ChunkArgs& a, const Item& item, int64_t row, float m, float l) {
+  if (item.slot >= 0) {
+    a.part_ml[part_row(a, item.slot, item.b, row)] = make_float2(m, l);
   } else {
     a.lse[row] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
   }
@@ -252,7 +310,7 @@ __device__ __forceinline__ void attend_few(const ChunkArgs& a, int b, int h, con
 // The results that the workgroup's waves have for the same rows, each from its own tokens, joined and stored: all write theirs to LDS, then
 // each takes its share of the channels.
 template <int D, int NR>
-__device__ __forceinline__ void finish_few(const ChunkArgs& a, const Result<D, NR>& r, const QueryRow (&row)[NR], int part, int wave, f32x4* lds) {
+__device__ __forceinline__ void finish_few(const ChunkArgs& a, const Result<D, NR>& r, const QueryRow (&row)[NR], const Item& item, int wave, f32x4* lds) {
   constexpr int FOURS = D / 16;
   static_assert(FOURS % kWaves == 0, "every wave takes as many channels");
   const int lane = threadIdx.x & 63, quarter = lane >> 4;
@@ -283,14 +341,14 @@ __device__ __forceinline__ void finish_few(const ChunkArgs& a, const Result<D, N
     }
     if (row[n].row < 0) continue;
     if (row[n].limit == 0) total = 0.0f;
-    if (wave == 0 && quarter == 0) store_sums(a, row[n].row, part, top, total);
+    if (wave == 0 && quarter == 0) store_sums(a, item, row[n].row, top, total);
 #pragma unroll
     for (int j = 0; j < FOURS / kWaves; ++j) {
       const int k = j * kWaves + wave;
       f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int i = 0; i < kWaves; ++i) o += lds[((i * NR + n) * FOURS + k) * 64 + lane] * x[i].x;
-      store_part<D>(a, row[n].row, part, channel_of<D, false>(k), total, o);
+      store_part<D>(a, item, row[n].row, channel_of<D, false>(k), total, o);
     }
   }
 }
@@ -299,10 +357,9 @@ template <int DT, int D, bool MX, int NR>
 __global__ __launch_bounds__(64 * kWaves, NR == 2 && D == 128 ? 1 : 2) void chunk_few_kernel(ChunkArgs a) {
   __shared__ f32x4 lds[kWaves * NR * 64 * (D + 8) / 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int id = blockIdx.x;
-  const int heads = a.n_seqs * a.n_kv, bh = id % heads;
-  id /= heads;
-  const int part = id % a.parts, tile = id / a.parts, b = bh / a.n_kv, h = bh % a.n_kv;
+  const Item item = item_of(a);
+  const int b = item.b, h = item.h, tile = item.tile;
+  if (b < 0) return;
   const Extent e = extent_of(a, b);
   QueryRow row[NR];
 #pragma unroll
@@ -310,10 +367,10 @@ __global__ __launch_bounds__(64 * kWaves, NR == 2 && D == 128 ? 1 : 2) void chun
   // Rows that the tile's first token attends, and its last one.
   const int t0 = tile * NR * 16 / a.g, t1 = min((tile * NR * 16 + NR * 16 - 1) / a.g, e.n - 1);
   const int whole = max(e.len - e.n + t0 + 1, 0), all = t1 < t0 ? 0 : max(e.len - e.n + t1 + 1, 0);
-  const int begin = part * a.chunk, end = min(begin + a.chunk, all);
+  const int begin = item.begin, end = (int)min((int64_t)begin + item.chunk, (int64_t)all);
   Result<D, NR> r;
   attend_few<DT, D, MX, NR>(a, b, h, row, begin + wave * kTile, kWaves * kTile, end, whole, r);
-  finish_few<D, NR>(a, r, row, part, wave, lds);
+  finish_few<D, NR>(a, r, row, item, wave, lds);
 }
 
 // ---- many rows: keys and values through LDS --------------------------------------------------------
@@ -553,17 +610,16 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 && !MX ? 3 : 2) void chunk_wid
   __shared__ f32x4 lds4[2 * 2 * S::BYTES / 16];
   uint8_t* const lds = (uint8_t*)lds4;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int id = blockIdx.x;
-  const int heads = a.n_seqs * a.n_kv, bh = id % heads;
-  id /= heads;
-  // The longest tiles first: the last ones of a sequence attend the most rows.
-  const int part = id % a.parts, tile = a.tiles - 1 - id / a.parts, b = bh / a.n_kv, h = bh % a.n_kv;
+  const Item item = item_of(a);
+  const int b = item.b, h = item.h, tile = item.tile;
+  if (b < 0) return;
   const Extent e = extent_of(a, b);
   const int x0 = tile * ROWS + wave * 32;
-  const QueryRow row = query_row(a, e, b, h, x0 + (lane & 31));
-  const int past = e.len - e.n, begin = part * a.chunk;
+  const QueryRow query = query_row(a, e, b, h, x0 + (lane & 31));
+  const int limit = query.limit;
+  const int past = e.len - e.n, begin = item.begin;
   const int last = min((tile * ROWS + ROWS - 1) / a.g, e.n - 1), wave_first = x0 / a.g, wave_last = min((x0 + 31) / a.g, e.n - 1);
-  const int end = last < tile * ROWS / a.g ? 0 : min(begin + a.chunk, max(past + last + 1, 0));
+  const int end = last < tile * ROWS / a.g ? 0 : (int)min((int64_t)begin + item.chunk, (int64_t)max(past + last + 1, 0));
   const int wave_end = wave_last < wave_first ? 0 : min(end, max(past + wave_last + 1, 0));
   Level level = {0.0f, -INFINITY};
   float l = 0.0f;
@@ -581,7 +637,7 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 && !MX ? 3 : 2) void chunk_wid
     stage.template load<true>(a.rows, places, 0, min(kStage, end - begin), lds);
     uint4 qf[D / 16];
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) qf[i] = row.row >= 0 ? *(const uint4*)(row.q + 16 * i + (lane >> 5) * 8) : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < D / 16; ++i) qf[i] = query.row >= 0 ? *(const uint4*)(query.q + 16 * i + (lane >> 5) * 8) : make_uint4(0, 0, 0, 0);
     LdsPointer key_at[D / 16], value_at[2][D / 32];
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) {
@@ -641,20 +697,23 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 && !MX ? 3 : 2) void chunk_wid
       for (int sub = 0; sub < 2; ++sub) {
         const int now = t + 32 * sub;
         if (now >= wave_end) break;
-        cut_tile<DT, D>(key_at, value_at, buffer + sub * 32 * 2 * D, qf, row.limit - now, here >> (2 * sub) & 1, here >> (2 * sub + 1) & 1, a.scale2, level, l, o);
+        cut_tile<DT, D>(key_at, value_at, buffer + sub * 32 * 2 * D, qf, limit - now, here >> (2 * sub) & 1, here >> (2 * sub + 1) & 1, a.scale2, level, l, o);
       }
       buffer ^= 2 * S::BYTES;
     }
   }
+  int x = x0 + (lane & 31);
+  keep_here(x);  // worked out anew: held from the start it would cost registers
+  const QueryRow row = query_row(a, e, b, h, x);
   constexpr float down = 1.0f / (float)(1 << (int)lift_of(DT, 2));
   l = row.limit == 0 ? 0.0f : pair_sum<32>(l) * down;
-  if (row.row >= 0 && lane < 32) store_sums(a, row.row, part, level.limit == -INFINITY ? -INFINITY : lift_of(DT, 2) - level.less, l);
+  if (row.row >= 0 && lane < 32) store_sums(a, item, row.row, level.limit == -INFINITY ? -INFINITY : lift_of(DT, 2) - level.less, l);
   // Through LDS to rows that lie together: a wave's own 32 rows, 16-byte pieces swizzled by the row. (Stored from where they are, 16 bytes a lane, a row's neighbours in
   // the other half of the lanes: 2,048 workgroups' parts took 45 us more than 512's.)
   constexpr int PIECES = D / 4;
   f32x4* const mine = lds4 + wave * 32 * PIECES;
   __syncthreads();  // what LDS held before is read no more
-  const float f = a.parts > 1 ? down : l == 0.0f ? 0.0f : down / l;
+  const float f = item.slot >= 0 ? down : l == 0.0f ? 0.0f : down / l;
 #pragma unroll
   for (int c = 0; c < D / 32; ++c)
 #pragma unroll
@@ -671,8 +730,8 @@ __global__ __launch_bounds__(64 * kWaves, D == 64 && !MX ? 3 : 2) void chunk_wid
     const float sum = __shfl(l, r);
     const f32x4 x = mine[r * PIECES + (piece ^ (r & (PIECES - 1)))];
     if (to < 0) continue;
-    if (a.parts > 1) {
-      if (sum != 0.0f) *(f32x4*)(a.part_o + (to * a.parts + part) * D + piece * 4) = x;  // a part without weight is not read
+    if (item.slot >= 0) {
+      if (sum != 0.0f) *(f32x4*)(a.part_o + part_row(a, item.slot, b, to) * D + piece * 4) = x;  // a part without weight is not read
     } else if (a.out_dtype == LKV_F32) {
       store_four<LKV_F32>(a.out, to * D + piece * 4, x);
     } else if (a.out_dtype == LKV_BF16) {
@@ -690,22 +749,38 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs a, int64_t ro
   const int lane = threadIdx.x & 63, c = lane % C;
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= rows) return;
-  const float2* ml = a.part_ml + row * a.parts;
-  const float* from = a.part_o + row * a.parts * D + c * 4;
+  // The sequence's parts, as the workgroups above divided its rows.
+  const int64_t seq_rows = (int64_t)a.n_q * a.new_tokens;
+  const int b = (int)(row / seq_rows);
+  const uint32_t units = part_units(a);
+  uint32_t first = 0, parts = 0;
+  for (int i = 0; i <= b; i += 64) {
+    const uint32_t mine = parts_of(a, i + lane, units), before = wave_inclusive_sum(mine) - mine;
+    if (b - i < 64) {
+      first += (uint32_t)__builtin_amdgcn_readlane((int)before, b - i);
+      parts = (uint32_t)__builtin_amdgcn_readlane((int)mine, b - i);
+    } else {
+      first += (uint32_t)__builtin_amdgcn_readlane((int)(before + mine), 63);
+    }
+  }
+  const int n_parts = (int)parts;
+  const int64_t at = first * seq_rows + (row - b * seq_rows);
+  const float2* ml = a.part_ml + at;
+  const float* from = a.part_o + at * D + c * 4;
   float top = -INFINITY, total = 0.0f;
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int p0 = 0; p0 < a.parts; p0 += 64) {
-    const float2 mine = p0 + lane < a.parts ? ml[p0 + lane] : make_float2(-INFINITY, 0.0f);
+  for (int p0 = 0; p0 < n_parts; p0 += 64) {
+    const float2 mine = p0 + lane < n_parts ? ml[(p0 + lane) * seq_rows] : make_float2(-INFINITY, 0.0f);
     const float up = fmaxf(top, wave_max_f32(mine.x));
     const float keep = p0 == 0 ? 0.0f : join_factor(top, total, up), f = join_factor(mine.x, mine.y, up);
     top = up;
     total = total * keep + wave_sum_f32(mine.y == 0.0f ? 0.0f : f * mine.y);
     o *= keep;
-    const int n = min(64, a.parts - p0);
+    const int n = min(64, n_parts - p0);
     for (int p = 0; p < n; p += EACH) {
       const int mine_p = p + lane / C;
       const float w = __shfl(f, mine_p), s = __shfl(mine.y, mine_p);
-      if (mine_p < n && s != 0.0f) o += *(const f32x4*)(from + (int64_t)(p0 + mine_p) * D) * w;
+      if (mine_p < n && s != 0.0f) o += *(const f32x4*)(from + (p0 + mine_p) * seq_rows * D) * w;
     }
   }
   if constexpr (EACH == 4) {
@@ -730,26 +805,32 @@ int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 // How a call is divided: see ChunkArgs. nr: tiles of 16 rows of a wave on its own stream, 0: through LDS.
 struct Plan {
-  int nr, tiles, parts, chunk;
+  int nr, tiles, unit, share;
+  int64_t blocks;
 };
 
 Plan plan_of(const lkv_chunk_desc* d) {
   Plan p = {};
-  const int64_t rows = (int64_t)d->new_tokens * (d->n_q / d->n_kv), heads = (int64_t)d->n_seqs * d->n_kv;
+  const int64_t rows = (int64_t)d->new_tokens * (d->n_q / d->n_kv);
   p.nr = rows <= 16 ? 1 : rows <= 32 ? 2 : 0;
   p.tiles = ceil_div(rows, p.nr ? 16 * p.nr : 32 * kWaves);
-  const int64_t units = heads * p.tiles, room = 512, least = p.nr ? 128 : 256;
-  int64_t parts = units > 0 ? room / units : 1;
-  const int64_t most = ceil_div(d->max_tokens, least);
-  parts = parts < 1 ? 1 : parts > most ? most : parts;
-  parts = parts < 1 ? 1 : parts;
-  const int64_t step = p.nr ? 128 : 64;
-  int64_t chunk = (d->max_tokens + parts - 1) / parts;
-  chunk = (chunk + step - 1) / step * step;
-  p.chunk = (int)(chunk < step ? step : chunk);
-  p.parts = ceil_div(d->max_tokens, p.chunk);
-  p.parts = p.parts < 1 ? 1 : p.parts;
+  // Workgroups for about as many parts as run at once, two a CU, one where its registers or an even division allow no more; none shorter than 256 rows on average.
+  // One token over 131,072 rows (d 128): 104 us by 256, 116 by 512; 8 tokens (two tiles of 16 rows a wave, one workgroup a CU) over 16,419 26 and 33;
+  // sixteen sequences of up to 8,192 71 and 57; 203 tokens over 32,971 199 and 152, by 768 164.
+  const int64_t units = (int64_t)d->n_kv * p.tiles, room = p.nr && (d->n_seqs == 1 || (p.nr == 2 && d->head_dim == 128)) ? 256 : 512;
+  int64_t share = units > 0 ? room / units : 1;
+  const int64_t most = d->n_seqs * (int64_t)ceil_div(d->max_tokens, 256);
+  share = share > most ? most : share;
+  p.unit = p.nr ? 7 : 6;  // a round of the workgroup
+  if (share * (((int64_t)d->max_tokens >> p.unit) + 1) >= 1LL << 32) p.unit = 9;
+  p.share = share > d->n_seqs ? (int)share : 0;
+  p.blocks = units * (p.share ? p.share : d->n_seqs);
   return p;
+}
+
+size_t scratch_of(const lkv_chunk_desc* d, const Plan& p) {
+  const size_t rows = (size_t)p.share * d->n_q * d->new_tokens;
+  return lkv_align_up(rows * sizeof(float2), 16) + rows * d->head_dim * sizeof(float);
 }
 
 template <int DT, int D, bool MX>
@@ -774,9 +855,7 @@ int lkv_check_chunk(const lkv_chunk_desc* d) {
 
 extern "C" size_t lkv_chunk_attend_workspace_bytes(const lkv_chunk_desc* desc) {
   if (lkv_check_chunk(desc)) return 0;
-  const Plan p = plan_of(desc);
-  const size_t rows = (size_t)desc->n_seqs * desc->n_q * desc->new_tokens;
-  return p.parts < 2 ? 0 : lkv_align_up(rows * p.parts * sizeof(float2), 16) + rows * p.parts * desc->head_dim * sizeof(float);
+  return scratch_of(desc, plan_of(desc));
 }
 
 extern "C" int lkv_chunk_attend(uintptr_t stream, const lkv_chunk_desc* desc, const void* q, int q_dtype, const lkv_kv_rows* rows, const lkv_pages* pages,
@@ -795,15 +874,14 @@ extern "C" int lkv_chunk_attend(uintptr_t stream, const lkv_chunk_desc* desc, co
   const int64_t n = (int64_t)desc->n_seqs * desc->n_q * desc->new_tokens;
   if (n == 0) return LKV_OK;
   const Plan p = plan_of(desc);
-  const int64_t blocks = (int64_t)desc->n_seqs * desc->n_kv * p.tiles * p.parts;
-  LKV_CHECK_ARG(blocks < (1LL << 31), "%lld workgroups in one call", (long long)blocks);
+  LKV_CHECK_ARG(p.blocks < (1LL << 31), "%lld workgroups in one call", (long long)p.blocks);
   a.q = (const uint16_t*)q;
   a.lengths = lengths;
   a.counts = counts;
   a.out = out;
   a.lse = lse;
   a.part_ml = (float2*)ws;
-  a.part_o = (float*)((uint8_t*)ws + lkv_align_up(n * p.parts * sizeof(float2), 16));
+  a.part_o = (float*)((uint8_t*)ws + lkv_align_up((size_t)p.share * desc->n_q * desc->new_tokens * sizeof(float2), 16));
   for (int i = 0; i < 3; ++i) a.q_stride[i] = desc->q_stride[i];
   a.scale2 = desc->scale * kLog2e;
   a.n_seqs = desc->n_seqs;
@@ -815,11 +893,11 @@ extern "C" int lkv_chunk_attend(uintptr_t stream, const lkv_chunk_desc* desc, co
   a.max_tokens = desc->max_tokens;
   a.out_dtype = out_dtype;
   a.tiles = p.tiles;
-  a.parts = p.parts;
-  a.chunk = p.chunk;
+  a.unit = p.unit;
+  a.share = p.share;
   const hipStream_t s = (hipStream_t)stream;
   const bool half = q_dtype == LKV_F16, wide = desc->head_dim == 128, mx = rows->dtype == LKV_MXFP8;
-  const dim3 grid((unsigned)blocks);
+  const dim3 grid((unsigned)p.blocks);
   if (half) {
     wide ? (mx ? launch<LKV_F16, 128, true>(p, grid, s, a) : launch<LKV_F16, 128, false>(p, grid, s, a))
          : (mx ? launch<LKV_F16, 64, true>(p, grid, s, a) : launch<LKV_F16, 64, false>(p, grid, s, a));
@@ -828,7 +906,7 @@ extern "C" int lkv_chunk_attend(uintptr_t stream, const lkv_chunk_desc* desc, co
          : (mx ? launch<LKV_BF16, 64, true>(p, grid, s, a) : launch<LKV_BF16, 64, false>(p, grid, s, a));
   }
   LKV_CHECK_LAUNCH("chunk_attend");
-  if (p.parts > 1) {
+  if (p.share) {
     hipLaunchKernelGGL((wide ? chunk_join_kernel<128> : chunk_join_kernel<64>), dim3((unsigned)((n + 3) / 4)), dim3(256), 0, s, a, n);
     LKV_CHECK_LAUNCH("chunk_attend (join)");
   }

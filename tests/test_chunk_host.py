@@ -30,7 +30,8 @@ def _chunk(n_seqs: int, n_q: int, n_kv: int, d: int, t: int, most: int):  # noqa
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize(("n_q", "n_kv"), [(1, 1), (4, 1), (32, 8), (40, 1), (128, 128)])
 def test_scratch_is_bounded(n_q: int, n_kv: int, d: int) -> None:
-    """Partial results of attention are for at most 512 workgroups of 128 query rows (or one part, which needs none); sums by parts for at most 1,024 of 256 rows."""
+    """Partial results of attention are for at most 512 workgroups of 128 query rows (or for none: a sequence's one part writes the output); sums by parts for at most 1,024
+    workgroups of 256 rows."""
     from lazykv_amd import _lib
 
     lib = _lib.lib()
