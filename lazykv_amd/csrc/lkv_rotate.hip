@@ -1,4 +1,5 @@
 // New tokens' queries and keys normalised over each head and rotated, keys and values written to their rows (lkv_rotate_append).
+#include "lkv_attend.h"
 #include "lkv_pages.h"
 
 namespace {
@@ -13,7 +14,8 @@ struct RotateArgs {
   const int32_t* counts;
   int32_t start;
   uint32_t heads;   // n_q + 2 n_kv
-  uint32_t pieces;  // n_seqs * tokens * heads
+  uint32_t splits;  // workgroups of a token
+  uint32_t share;   // heads of each
 };
 
 // Eight neighbouring values in the model dtype or in float32.
@@ -29,84 +31,97 @@ __device__ __forceinline__ void load_eight(const void* p, int64_t at, bool wide,
   }
 }
 
-// Sixteen lanes (head_dim 128) or eight (64) hold a head of a token, 8 channels a lane, the heads of a token next to each other.
-// The channel half a rotation away is loaded again rather than sent by the lane that has it: it is in the cache line or the next, and any
+// A workgroup takes a token, or some of its heads where there are few tokens: sixteen lanes (head_dim 128) or eight (64) hold a head, 8 channels a lane, and go on to
+// the head 16 further with the same tables and weights. Those are folded once: a channel becomes
+//   (x a + z b) / rms,  a = weight cos, b = -+ weight' sin,
+// z the channel half a rotation away. It is loaded again rather than sent by the lane that has it: it is in the cache line or the next, and any
 // rotary width takes the same path.
+constexpr int kHeads = 16;  // that a workgroup holds at a time
 template <int DT, int D, bool MX>
-__global__ __launch_bounds__(256) void rotate_append_kernel(RotateArgs a) {
+__global__ __launch_bounds__(kHeads * D / 8) void rotate_append_kernel(RotateArgs a) {
   constexpr int LPR = D / 8;
-  const uint32_t piece = blockIdx.x * (256u / LPR) + threadIdx.x / LPR;
-  const int c = (threadIdx.x % LPR) * 8;
-  if (piece >= a.pieces) return;  // whole heads leave: the quads of the others stay complete
-  const uint32_t bt = piece / a.heads, head = piece - bt * a.heads;
+  const uint32_t bt = blockIdx.x / a.splits, split = blockIdx.x - bt * a.splits;
   const uint32_t b = bt / (uint32_t)a.d.tokens, t = bt - b * (uint32_t)a.d.tokens;
-  const bool is_q = head < (uint32_t)a.d.n_q, is_v = head >= (uint32_t)(a.d.n_q + a.d.n_kv);
-  const int h = (int)(is_q ? head : is_v ? head - a.d.n_q - a.d.n_kv : head - a.d.n_q);
-  int64_t to = 0;
-  if (!is_q) {
-    if (a.counts && (int)t >= a.counts[b]) return;
-    to = lkv::row_of<D>(a.rows, (int)b, h, (int64_t)a.start + (a.starts ? a.starts[b] : 0) + t);
-    if (to < 0) return;
-  }
-  const int64_t* st = is_q ? a.d.q_stride : is_v ? a.d.v_stride : a.d.k_stride;
-  const uint16_t* x = (is_q ? a.q : is_v ? a.v : a.k) + b * st[0] + h * st[1] + t * st[2];
-  const uint4 raw = *(const uint4*)(x + c);
-  uint4 word = raw;
-  if (!is_v) {
-    const lkv::RowWords<DT, 8> words = {{raw.x, raw.y, raw.z, raw.w}};
-    float y[8];
-    lkv::widen_row_words<DT, 8>(words, y);
-    const int half = a.d.rotary / 2;
-    const bool turns = c < a.d.rotary;
-    const int other = c < half ? c + half : c - half;
-    float z[8], cs[8], sn[8];
-    if (turns) {
-      load_eight<DT>(x, other, false, z);
-      const int64_t at = b * a.d.table_seq_stride + (int64_t)t * a.d.rotary + c;
-      load_eight<DT>(a.cos, at, a.d.table_dtype == LKV_F32, cs);
-      load_eight<DT>(a.sin, at, a.d.table_dtype == LKV_F32, sn);
+  const int c = (threadIdx.x % LPR) * 8, half = a.d.rotary / 2, other = c < half ? c + half : c - half;
+  const bool turns = c < a.d.rotary;
+  // The token's row: the same in every head.
+  const int64_t row = (int64_t)a.start + (a.starts ? a.starts[b] : 0) + t;
+  const bool kept = (!a.counts || (int)t < a.counts[b]) && row >= 0 && row < a.rows.capacity;
+  const lkv::Sixteen place = kept ? lkv::sixteen_of<D>(a.rows, (int)b, 0, (int)(row >> 4)) : lkv::Sixteen{0, false};
+  const int64_t to = place.at + (row & 15) * D + c;
+  float qa[8], qb[8], ka[8], kb[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) qa[i] = ka[i] = 1.0f, qb[i] = kb[i] = 0.0f;
+  if (turns) {
+    const int64_t at = b * a.d.table_seq_stride + (int64_t)t * a.d.rotary + c;
+    load_eight<DT>(a.cos, at, a.d.table_dtype == LKV_F32, qa);
+    load_eight<DT>(a.sin, at, a.d.table_dtype == LKV_F32, qb);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      qb[i] = c < half ? -qb[i] : qb[i];
+      ka[i] = qa[i];
+      kb[i] = qb[i];
     }
-    const void* weight = is_q ? a.q_weight : a.k_weight;
-    if (weight) {
-      float sum = 0.0f, w[8];
+  }
+  const auto weigh = [&](const void* weight, float(&wa)[8], float(&wb)[8]) {
+    if (!weight) return;
+    const bool wide = a.d.weight_dtype == LKV_F32;
+    float w[8];
+    load_eight<DT>(weight, c, wide, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(y[i], y[i], sum);
-      const float inverse = 1.0f / sqrtf(lkv::row_sum<LPR>(sum) * (1.0f / D) + a.d.eps);
-      const bool wide = a.d.weight_dtype == LKV_F32;
-      load_eight<DT>(weight, c, wide, w);
+    for (int i = 0; i < 8; ++i) wa[i] *= w[i];
+    if (!turns) return;
+    load_eight<DT>(weight, other, wide, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] *= inverse * w[i];
-      if (turns) {
-        load_eight<DT>(weight, other, wide, w);
+    for (int i = 0; i < 8; ++i) wb[i] *= w[i];
+  };
+  weigh(a.q_weight, qa, qb);
+  weigh(a.k_weight, ka, kb);
+  const uint32_t end = min((split + 1) * a.share, a.heads);
+  for (uint32_t head = split * a.share + threadIdx.x / LPR; head < end; head += kHeads) {  // whole heads leave: the quads of the others stay complete
+    const bool is_q = head < (uint32_t)a.d.n_q, is_v = head >= (uint32_t)(a.d.n_q + a.d.n_kv);
+    const int h = (int)(is_q ? head : is_v ? head - a.d.n_q - a.d.n_kv : head - a.d.n_q);
+    if (!is_q && !place.there) continue;
+    const uint16_t* x = is_q   ? a.q + b * a.d.q_stride[0] + h * a.d.q_stride[1] + t * a.d.q_stride[2]
+                        : is_v ? a.v + b * a.d.v_stride[0] + h * a.d.v_stride[1] + t * a.d.v_stride[2]
+                               : a.k + b * a.d.k_stride[0] + h * a.d.k_stride[1] + t * a.d.k_stride[2];
+    uint4 word = *(const uint4*)(x + c);
+    if (!is_v) {
+      const lkv::RowWords<DT, 8> words = {{word.x, word.y, word.z, word.w}};
+      float y[8], z[8];
+      lkv::widen_row_words<DT, 8>(words, y);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) z[i] *= inverse * w[i];
+      for (int i = 0; i < 8; ++i) z[i] = 0.0f;
+      if (turns) load_eight<DT>(x, other, false, z);
+      float inverse = 1.0f;
+      if (is_q ? a.q_weight != nullptr : a.k_weight != nullptr) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(y[i], y[i], sum);
+        inverse = __builtin_amdgcn_rsqf(lkv::row_sum<LPR>(sum) * (1.0f / D) + a.d.eps);
       }
-    }
-    if (turns) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = y[i] * cs[i] + (c < half ? -z[i] : z[i]) * sn[i];
+      for (int i = 0; i < 8; ++i) y[i] = __builtin_fmaf(y[i], is_q ? qa[i] : ka[i], z[i] * (is_q ? qb[i] : kb[i])) * inverse;
+      using M = lkv::Mat<DT>;
+      word = make_uint4(M::pack(y[0], y[1]), M::pack(y[2], y[3]), M::pack(y[4], y[5]), M::pack(y[6], y[7]));
     }
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      w[i] = (uint32_t)lkv::Elem<DT>::store(y[2 * i]) | ((uint32_t)lkv::Elem<DT>::store(y[2 * i + 1]) << 16);
-    word = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-  if (is_q) {
-    *(uint4*)(a.q_out + b * a.d.out_stride[0] + h * a.d.out_stride[1] + t * a.d.out_stride[2] + c) = word;
-    return;
-  }
-  if constexpr (MX) {
-    // From the rounded values: the cache does not tell by which call a token came.
-    const lkv::RowWords<DT, 8> words = {{word.x, word.y, word.z, word.w}};
-    float y[8];
-    lkv::widen_row_words<DT, 8>(words, y);
-    uint32_t scale;
-    const uint2 codes = lkv::mx_encode<DT>(y, scale);
-    *(uint2*)((uint8_t*)(is_v ? a.rows.rows.v : a.rows.rows.k) + to + c) = codes;
-    if ((threadIdx.x & 3) == 0) ((uint8_t*)(is_v ? a.rows.rows.v_scale : a.rows.rows.k_scale))[(to + c) / kMxGroup] = (uint8_t)scale;
-  } else {
-    *(uint4*)((uint16_t*)(is_v ? a.rows.rows.v : a.rows.rows.k) + to + c) = word;
+    if (is_q) {
+      *(uint4*)(a.q_out + b * a.d.out_stride[0] + h * a.d.out_stride[1] + t * a.d.out_stride[2] + c) = word;
+      continue;
+    }
+    const int64_t at = to + h * a.rows.rows.head_stride;
+    if constexpr (MX) {
+      // From the rounded values: the cache does not tell by which call a token came.
+      const lkv::RowWords<DT, 8> words = {{word.x, word.y, word.z, word.w}};
+      float y[8];
+      lkv::widen_row_words<DT, 8>(words, y);
+      uint32_t scale;
+      const uint2 codes = lkv::mx_encode<DT>(y, scale);
+      *(uint2*)((uint8_t*)(is_v ? a.rows.rows.v : a.rows.rows.k) + at) = codes;
+      if ((threadIdx.x & 3) == 0) ((uint8_t*)(is_v ? a.rows.rows.v_scale : a.rows.rows.k_scale))[at / kMxGroup] = (uint8_t)scale;
+    } else {
+      *(uint4*)((uint16_t*)(is_v ? a.rows.rows.v : a.rows.rows.k) + at) = word;
+    }
   }
 }
 
@@ -153,14 +168,16 @@ extern "C" int lkv_rotate_append(uintptr_t stream, const lkv_rotate_desc* desc, 
   a.counts = counts;
   a.start = start;
   a.heads = (uint32_t)heads;
-  a.pieces = (uint32_t)n;
+  // All heads of a token by one workgroup, or, of few tokens, as many at a time as it has lanes for.
+  const int64_t tokens = (int64_t)d.n_seqs * d.tokens;
+  a.splits = tokens >= 1024 ? 1 : (a.heads + kHeads - 1) / kHeads;
+  a.share = a.splits == 1 ? a.heads : kHeads;
   const bool mx = dst->dtype == LKV_MXFP8, half = d.dtype == LKV_F16, wide = d.head_dim == 128;
   auto kernel = half ? (wide ? (mx ? rotate_append_kernel<LKV_F16, 128, true> : rotate_append_kernel<LKV_F16, 128, false>)
                              : (mx ? rotate_append_kernel<LKV_F16, 64, true> : rotate_append_kernel<LKV_F16, 64, false>))
                      : (wide ? (mx ? rotate_append_kernel<LKV_BF16, 128, true> : rotate_append_kernel<LKV_BF16, 128, false>)
                              : (mx ? rotate_append_kernel<LKV_BF16, 64, true> : rotate_append_kernel<LKV_BF16, 64, false>));
-  const uint32_t per = 256 / (d.head_dim / 8);
-  hipLaunchKernelGGL(kernel, dim3((a.pieces + per - 1) / per), dim3(256), 0, (hipStream_t)stream, a);
+  hipLaunchKernelGGL(kernel, dim3((uint32_t)(tokens * a.splits)), dim3(kHeads * d.head_dim / 8), 0, (hipStream_t)stream, a);
   LKV_CHECK_LAUNCH("rotate_append");
   return LKV_OK;
 }
