@@ -206,32 +206,31 @@ struct Walk {
   }
 };
 
-// A stage's query rows on their way to LDS, what is added to their exponents, and how many of a sequence's rows they attend. Rows from x_end on are the first
-// one of the range again, without weight.
+// A stage's query rows on their way to LDS, what is added to their exponents, and how many of a sequence's rows they attend. Every wave's lane l knows row l; a
+// row's 16-byte pieces are loaded by other lanes, which ask it where it is. Rows from x_end on are the first one of the range again, without weight.
 template <int D> struct StageQueries {
+  static_assert(kStage == 64, "a row of the stage for each lane");
   static constexpr int PIECES = D / 8, LOADS = kStage * PIECES / (64 * kWaves);
   u32x4 w[LOADS];
-  float lse[LOADS], less;
+  float less;
   int limit;
-  Walk row[LOADS], mine;
+  Walk mine;
   int x;  // the stage's first row
   __device__ __forceinline__ void begin(const WeighArgs& a, int b, int h, int x0) {
     x = x0;
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) row[i].begin(a, b, h, x0 + (i * 64 * kWaves + (int)threadIdx.x) / PIECES);
-    mine.begin(a, b, h, x0 + (int)(threadIdx.x & (kStage - 1)));
+    mine.begin(a, b, h, x0 + (int)(threadIdx.x & 63));
   }
   __device__ __forceinline__ void load(const WeighArgs& a, const Extent& e, int b, int h, const Walk& first, int x_end) {
-    const float* lses = a.lse + ((int64_t)b * a.n_q + h * a.g) * a.new_tokens;
+    const bool live = x + (int)(threadIdx.x & 63) < x_end;
+    const int64_t at = live ? mine.at : first.at;
+    const int lo = (int)(uint32_t)at, hi = (int)(at >> 32);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-      const bool live = x + (i * 64 * kWaves + (int)threadIdx.x) / PIECES < x_end;
-      w[i] = *(const u32x4*)(a.q + (live ? row[i].at : first.at) + threadIdx.x % PIECES * 8);
-      lse[i] = lses[(int64_t)(live ? row[i].j : first.j) * a.new_tokens + (live ? row[i].t : first.t)];
-      row[i].next(a);
+      const int r = (i * 64 * kWaves + (int)threadIdx.x) / PIECES;
+      const int64_t from = (int64_t)((uint64_t)(uint32_t)__shfl(hi, r) << 32 | (uint32_t)__shfl(lo, r));
+      w[i] = *(const u32x4*)(a.q + from + threadIdx.x % PIECES * 8);
     }
-    const bool live = x + (int)(threadIdx.x & (kStage - 1)) < x_end;
-    const float l = lses[(int64_t)(live ? mine.j : first.j) * a.new_tokens + (live ? mine.t : first.t)];
+    const float l = a.lse[((int64_t)b * a.n_q + h * a.g + (live ? mine.j : first.j)) * a.new_tokens + (live ? mine.t : first.t)];
     less = live && l != -INFINITY ? -l * kLog2e : -INFINITY;
     limit = e.len - e.n + mine.t + 1;
     mine.next(a);
@@ -241,7 +240,7 @@ template <int D> struct StageQueries {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int y = i * 64 * kWaves + threadIdx.x, r = y / PIECES;
-      *(u32x4*)(lds + r * (2 * D) + ((y % PIECES) ^ swizzle<D>(r)) * 16) = w[i] & (lse[i] != -INFINITY ? ~0u : 0u);
+      *(u32x4*)(lds + r * (2 * D) + ((y % PIECES) ^ swizzle<D>(r)) * 16) = w[i] & (__shfl(less, r) != -INFINITY ? ~0u : 0u);
     }
     if (threadIdx.x < kStage) {
       less_at[threadIdx.x] = less;
