@@ -532,9 +532,14 @@ __device__ __forceinline__ uint4 wide_value(const LdsPointer (&value_at)[2][D / 
 }
 
 // A stage that all the wave's rows attend: no branch but the level's, so that reads, products and exponentials of its two tiles mix.
+// 64 channels: as long in exponentials as in products, and three waves a SIMD. A wave that has come to its exponentials goes before the others' products,
+// which the matrix unit holds anyway: 4,099 tokens, 32 query heads on 8, 105.2 -> 98.9 us. 128 channels: twice the products, two waves; there the
+// same costs 1130 -> 1140 us (2,048 tokens behind 32,768, 32 heads on 8), and products first gain 0.4%: left to the hardware.
 template <int DT, int D>
 __device__ __forceinline__ void whole_stage(const LdsPointer (&key_at)[D / 16], const LdsPointer (&value_at)[2][D / 32], int at, const uint4 (&qf)[D / 16], float scale2,
                                             Level& level, float& l, f32x16 (&o)[D / 32]) {
+  constexpr bool FIRST = D == 64;
+  if constexpr (FIRST) __builtin_amdgcn_s_setprio(0);
   f32x16 s[2];
 #pragma unroll
   for (int u = 0; u < 2; ++u)
@@ -544,15 +549,18 @@ __device__ __forceinline__ void whole_stage(const LdsPointer (&key_at)[D / 16], 
   for (int u = 0; u < 2; ++u)
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) s[u] = Wide<DT>::mma(read_piece(key_at[i] + at + u * 32 * 2 * D), qf[i], s[u]);
+  if constexpr (FIRST) __builtin_amdgcn_s_setprio(1);
   settle_level<DT, D>(fmaxf(largest(s[0]), largest(s[1])), scale2, level, l, o);
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     uint4 p[2];
     wide_weights<DT>(s[u], scale2, level.less, l, p);
+    if constexpr (FIRST) __builtin_amdgcn_s_setprio(0);
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) o[c] = Wide<DT>::mma(wide_value<D>(value_at, c, at + (32 * u + 16 * k) * 2 * D), p[k], o[c]);
+    if constexpr (FIRST) __builtin_amdgcn_s_setprio(1);
   }
 }
 
