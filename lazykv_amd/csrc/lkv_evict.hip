@@ -10,6 +10,11 @@ namespace {
 
 using namespace lkv;
 
+// Of the rows whose ranks begin with these digits, how many are wanted.
+struct Wanted {
+  uint32_t prefix, left;
+};
+
 struct EvictArgs {
   PagedRows rows;
   const int32_t* lengths;
@@ -22,6 +27,7 @@ struct EvictArgs {
   int32_t* list;       // [sequences * KV heads][2][moves]: where to, and from where
   int32_t* newest;     // [sequences * KV heads][spans]: largest positions
   uint32_t* digits;    // [sequences * KV heads][3][kDigits]: how many rows have each digit
+  Wanted* wanted;      // [sequences * KV heads][3]: after each of them
   uint32_t* split;     // [sequences * KV heads][spans][4]: see Split
   int32_t n_seqs, n_kv, keep, sinks, recent, tokens, max_tokens, moves;
   int32_t spans;       // of a head's rows, kSpan each
@@ -65,10 +71,7 @@ __device__ __forceinline__ uint32_t block_before(uint32_t x, uint32_t* lds, uint
   return before + up_to - x;
 }
 
-// Of rows with these digits, the one that the wanted-th largest has, and how many of its own are wanted. `digits`: LDS or memory.
-struct Wanted {
-  uint32_t prefix, left;
-};
+// `digits`: LDS or memory.
 __device__ __forceinline__ Wanted next_digit(const uint32_t* digits, int place, Wanted w, uint32_t* lds, Wanted* found) {
   // Two digits a thread, the largest first.
   const int d = place == 2 ? 1023 - (int)threadIdx.x : kDigits - 1 - 2 * (int)threadIdx.x;
@@ -251,8 +254,9 @@ __global__ __launch_bounds__(kThreads) void evict_short_kernel(EvictArgs a) {
 }
 
 // ---- long caches: a head's rows in spans of a workgroup each, a launch for each step ---------------------
-// The steps' counts are whole numbers added in memory: their order changes nothing.
-constexpr int kEach = 8, kSpan = kThreads * kEach;
+// The steps' counts are whole numbers added in memory: their order changes nothing. Four rows a thread: 131,072 rows of eight heads are 256 workgroups, one a
+// CU, 86.1 us with the move; eight rows 94.0, two (twice the counters to add) 88.4.
+constexpr int kEach = 4, kSpan = kThreads * kEach;
 
 __global__ __launch_bounds__(kThreads) void evict_newest_kernel(EvictArgs a) {
   __shared__ uint32_t lds[kWaves];
@@ -273,10 +277,12 @@ __device__ __forceinline__ void load_ranks(const EvictArgs& a, Span<EACH>& x, in
   x.order(a, (int)(wave_max_u32((uint32_t)newest ^ 0x80000000u) ^ 0x80000000u));
 }
 
-// The rank's first `places` digits.
-__device__ __forceinline__ Wanted found_digits(const EvictArgs& a, int bh, int places, uint32_t* lds, Wanted* found) {
-  Wanted w = {0, (uint32_t)a.keep};
-  for (int place = 0; place < places; ++place) w = next_digit(a.digits + ((int64_t)bh * 3 + place) * kDigits, place, w, lds, found);
+// The rank's first `places` digits, of which the steps before left all but the last; the first span leaves them for the next step.
+__device__ __forceinline__ Wanted found_digits(const EvictArgs& a, int bh, int span, int places, uint32_t* lds, Wanted* found) {
+  if (places == 0) return {0, (uint32_t)a.keep};
+  Wanted* steps = a.wanted + (int64_t)bh * 3;
+  const Wanted w = next_digit(a.digits + ((int64_t)bh * 3 + places - 1) * kDigits, places - 1, places == 1 ? Wanted{0, (uint32_t)a.keep} : steps[places - 2], lds, found);
+  if (span == 0 && threadIdx.x == 0) steps[places - 1] = w;
   return w;
 }
 
@@ -288,7 +294,7 @@ __global__ __launch_bounds__(kThreads) void evict_digit_kernel(EvictArgs a, int 
   if (n <= a.keep || (int64_t)span * kSpan >= n) return;
   Span<kEach> x;
   load_ranks(a, x, bh, span, n);
-  const Wanted w = found_digits(a, bh, place, lds, &found);
+  const Wanted w = found_digits(a, bh, span, place, lds, &found);
   clear_digits(digits);
   x.count_digits(digits, place, w.prefix);
   __syncthreads();
@@ -314,7 +320,7 @@ __global__ __launch_bounds__(kThreads) void evict_split_kernel(EvictArgs a) {
   Span<kEach> x;
   load_ranks(a, x, bh, span, n);
   if (threadIdx.x < 4) counts[threadIdx.x] = 0;
-  const Wanted last = found_digits(a, bh, 3, lds, &found);
+  const Wanted last = found_digits(a, bh, span, 3, lds, &found);
   uint32_t c[4] = {0, 0, 0, 0};
 #pragma unroll
   for (int j = 0; j < kEach; ++j) {
@@ -334,7 +340,6 @@ __global__ __launch_bounds__(kThreads) void evict_split_kernel(EvictArgs a) {
 
 __global__ __launch_bounds__(kThreads) void evict_list_kernel(EvictArgs a) {
   __shared__ uint32_t lds[kWaves];
-  __shared__ Wanted found;
   const int heads = a.n_seqs * a.n_kv, bh = blockIdx.x % heads, span = blockIdx.x / heads, b = bh / a.n_kv, n = length_of(a, b);
   if (span == 0 && threadIdx.x == 0 && n <= a.keep) a.count[bh] = 0;
   if ((int64_t)span * kSpan >= n) return;
@@ -343,7 +348,7 @@ __global__ __launch_bounds__(kThreads) void evict_list_kernel(EvictArgs a) {
   Wanted last = {0, (uint32_t)a.keep};
   uint32_t c[4] = {0, 0, 0, 0}, all_front_equal = 0;
   if (n > a.keep) {
-    last = found_digits(a, bh, 3, lds, &found);
+    last = a.wanted[(int64_t)bh * 3 + 2];
     const int spans = (n + kSpan - 1) / kSpan;
     for (int i = threadIdx.x & 63; i < spans; i += 64) {
       const uint4 y = *(const uint4*)(a.split + ((int64_t)bh * a.spans + i) * 4);
@@ -395,7 +400,7 @@ int moves_of(const lkv_evict_desc* d) {
 // The scratch: offsets of its parts.
 struct Layout {
   int spans;  // 0: a head's rows fit one workgroup
-  size_t list, newest, digits, split, bytes;
+  size_t list, newest, digits, wanted, split, bytes;
 };
 Layout layout_of(const lkv_evict_desc* d) {
   Layout l = {};
@@ -405,7 +410,8 @@ Layout layout_of(const lkv_evict_desc* d) {
   if (d->max_tokens <= kThreads * 16) return l;
   l.spans = (int)(((int64_t)d->max_tokens + kSpan - 1) / kSpan);
   l.digits = l.newest + lkv_align_up(heads * l.spans * sizeof(int32_t), 16);
-  l.split = l.digits + heads * 3 * kDigits * sizeof(uint32_t);
+  l.wanted = l.digits + heads * 3 * kDigits * sizeof(uint32_t);
+  l.split = l.wanted + lkv_align_up(heads * 3 * sizeof(Wanted), 16);
   l.bytes = l.split + heads * l.spans * sizeof(Split);
   return l;
 }
@@ -477,6 +483,7 @@ extern "C" int lkv_evict_rows(uintptr_t stream, const lkv_evict_desc* desc, cons
   a.list = (int32_t*)(at + l.list);
   a.newest = (int32_t*)(at + l.newest);
   a.digits = (uint32_t*)(at + l.digits);
+  a.wanted = (Wanted*)(at + l.wanted);
   a.split = (uint32_t*)(at + l.split);
   a.n_seqs = desc->n_seqs;
   a.n_kv = desc->n_kv;
