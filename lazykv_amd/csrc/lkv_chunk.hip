@@ -31,7 +31,8 @@ struct ChunkArgs {
   int32_t n_seqs, n_q, n_kv, g, new_tokens, tokens, max_tokens, out_dtype;
   int32_t tiles;   // of a KV head's query rows
   int32_t unit;    // log2 of the rows that they are divided by
-  int32_t share;   // parts that the sequences' rows are divided into at most; 0: each sequence in one, which writes the output
+  int32_t share;   // parts that the sequences' rows would make, were they one sequence's; 0: each sequence in one, which writes the output
+  int32_t most;    // parts that they make at most
 };
 
 // What a sequence has: rows in all, and the call's own among them.
@@ -59,28 +60,32 @@ __device__ __forceinline__ QueryRow query_row(const ChunkArgs& a, const Extent& 
 }
 
 // The division of the sequences' rows: by what there is of them on the device, so that all parts are about as long, however the sequences' lengths differ. Rows are counted in
-// units; a part has as many as make `share` parts of all at the most, and each sequence at least one part. (Each sequence in
-// as many parts as the next, four sequences of 1,643 to 16,475 rows under 64 tokens each took 82 us and now 66, a step of sixteen of up to 8,192 71 and now 57.)
+// units; a part has as many as make `share` parts of all at the most, and each sequence at least one part, which writes the output where it is the only one.
+// (Each sequence in as many parts as the next, four sequences of 1,643 to 16,475 rows under 64 tokens each took 82 us and now 66, a step of sixteen of up to
+// 8,192 71 and now 57.)
 __device__ __forceinline__ uint32_t units_of(const ChunkArgs& a, int b) { return b < a.n_seqs ? (uint32_t)(extent_of(a, b).len + (1 << a.unit) - 1) >> a.unit : 0; }
 __device__ __forceinline__ uint32_t wave_total(uint32_t x) { return (uint32_t)__builtin_amdgcn_readlane((int)wave_inclusive_sum(x), 63); }
 __device__ __forceinline__ uint32_t parts_of(const ChunkArgs& a, int b, uint32_t units) { return b < a.n_seqs ? max((units_of(a, b) + units - 1) / units, 1u) : 0; }
-// Units of a part: at least those that make `share` parts of all, and so many that the sequences' parts, whose last ones are not whole, are no more than `share`.
-// That ends: n_seqs is less, and parts as long as the longest sequence are as many. The sum stays below 2^32 (plan_of).
+// Units of a part: at least those that make `share` parts of all, and so many that the sequences' parts, whose last ones are not whole, are no more than `most`.
+// That ends: n_seqs is no more, and parts as long as the longest sequence are as many. The sum stays below 2^32 (plan_of).
 __device__ __forceinline__ uint32_t part_units(const ChunkArgs& a) {
   uint32_t all = 0;
   for (int i = threadIdx.x & 63; i < a.n_seqs; i += 64) all += units_of(a, i);
   uint32_t units = max((wave_total(all) + a.share - 1) / a.share, 1u);
+  if (a.most >= a.n_seqs + a.share - 1) return units;  // only the sequences' last parts are not whole
   for (;;) {
     uint32_t parts = 0;
     for (int i = 0; i < a.n_seqs; i += 64) parts += parts_of(a, i + (int)(threadIdx.x & 63), units);
-    if (wave_total(parts) <= (uint32_t)a.share) return units;
+    if (wave_total(parts) <= (uint32_t)a.most) return units;
     units += max(units >> 4, 1u);
   }
 }
+// Parts have places for their partial results where a sequence has several.
+__device__ __forceinline__ uint32_t several(uint32_t parts) { return parts > 1 ? parts : 0; }
 
 // What a workgroup does: rows begin .. begin + chunk of sequence b for a tile of KV head h's query rows.
 struct Item {
-  int b, h, tile, slot, begin, chunk;  // slot: which part of all; -1: the only one of its sequence. b < 0: nothing
+  int b, h, tile, slot, begin, chunk;  // slot: the place of its partial results; -1: the only part of its sequence. b < 0: nothing
 };
 __device__ __forceinline__ Item item_of(const ChunkArgs& a) {
   int id = blockIdx.x;
@@ -92,20 +97,22 @@ __device__ __forceinline__ Item item_of(const ChunkArgs& a) {
   const int h = id % a.n_kv;
   id /= a.n_kv;
   const int tile = a.tiles - 1 - id % a.tiles;
-  const uint32_t slot = (uint32_t)(id / a.tiles), units = part_units(a);
-  uint32_t before = 0;
+  const uint32_t number = (uint32_t)(id / a.tiles), units = part_units(a);
+  uint32_t before = 0, slots = 0;
   for (int i = 0; i < a.n_seqs; i += 64) {
-    const uint32_t mine = parts_of(a, i + (int)(threadIdx.x & 63), units), up_to = before + wave_inclusive_sum(mine);
-    const uint64_t behind = __ballot(up_to > slot);
+    const uint32_t mine = parts_of(a, i + (int)(threadIdx.x & 63), units), up_to = before + wave_inclusive_sum(mine), slot = slots + wave_inclusive_sum(several(mine));
+    const uint64_t behind = __ballot(up_to > number);
     if (behind) {
       const int lane = __builtin_ctzll(behind);
-      const uint32_t part = slot - (uint32_t)__builtin_amdgcn_readlane((int)(up_to - mine), lane);
+      const uint32_t parts = (uint32_t)__builtin_amdgcn_readlane((int)mine, lane), part = number + parts - (uint32_t)__builtin_amdgcn_readlane((int)up_to, lane);
+      const int at = parts > 1 ? (int)((uint32_t)__builtin_amdgcn_readlane((int)slot, lane) - parts + part) : -1;
       const int chunk = (int)min((uint64_t)units << a.unit, (uint64_t)(1 << 30));
-      return {i + lane, h, tile, (int)slot, (int)min((uint64_t)part * units << a.unit, (uint64_t)(1 << 30)), chunk};
+      return {i + lane, h, tile, at, (int)min((uint64_t)part * units << a.unit, (uint64_t)(1 << 30)), chunk};
     }
     before = (uint32_t)__builtin_amdgcn_readlane((int)up_to, 63);
+    slots = (uint32_t)__builtin_amdgcn_readlane((int)slot, 63);
   }
-  return {-1, h, tile, (int)slot, 0, 0};
+  return {-1, h, tile, -1, 0, 0};
 }
 
 // Where a query row's partial result is.
@@ -763,7 +770,7 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs a, int64_t ro
   const uint32_t units = part_units(a);
   uint32_t first = 0, parts = 0;
   for (int i = 0; i <= b; i += 64) {
-    const uint32_t mine = parts_of(a, i + lane, units), before = wave_inclusive_sum(mine) - mine;
+    const uint32_t mine = several(parts_of(a, i + lane, units)), before = wave_inclusive_sum(mine) - mine;
     if (b - i < 64) {
       first += (uint32_t)__builtin_amdgcn_readlane((int)before, b - i);
       parts = (uint32_t)__builtin_amdgcn_readlane((int)mine, b - i);
@@ -772,6 +779,7 @@ __global__ __launch_bounds__(256) void chunk_join_kernel(ChunkArgs a, int64_t ro
     }
   }
   const int n_parts = (int)parts;
+  if (n_parts == 0) return;  // one part, which wrote the output
   const int64_t at = first * seq_rows + (row - b * seq_rows);
   const float2* ml = a.part_ml + at;
   const float* from = a.part_o + at * D + c * 4;
@@ -813,7 +821,8 @@ int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 // How a call is divided: see ChunkArgs. nr: tiles of 16 rows of a wave on its own stream, 0: through LDS.
 struct Plan {
-  int nr, tiles, unit, share;
+  int nr, tiles, unit, share, most;
+  int slots;  // for partial results: a sequence of several parts has fewer than twice as many as its rows make whole ones
   int64_t blocks;
 };
 
@@ -825,19 +834,28 @@ Plan plan_of(const lkv_chunk_desc* d) {
   // Workgroups for about as many parts as run at once, two a CU, one where its registers or an even division allow no more; none shorter than 256 rows on average.
   // One token over 131,072 rows (d 128): 104 us by 256, 116 by 512; 8 tokens (two tiles of 16 rows a wave, one workgroup a CU) over 16,419 26 and 33;
   // sixteen sequences of up to 8,192 71 and 57; 203 tokens over 32,971 199 and 152, by 768 164.
+  // Of many parts a sequence, no more than that; of few, those that are not whole come on top. On top, sixteen sequences' steps cost 60.8 us for 57.3 and four questions
+  // of 64 tokens 75.2 for 61.6; not on top, sixteen of 64 tokens (two parts each) 135.4 for 121.8. Undivided, a step of 64 sequences of 1,024 rows and one of
+  // 65,536 among them cost 1,029 us for 105, 32 chunks of 128 tokens of the same kind 1,916 for 275; 64 and 100 of equal lengths 184.4 for 186.9 and 308.7 for 312.1.
+  // More than 256 sequences fill the device, and the division would be looked for too long.
   const int64_t units = (int64_t)d->n_kv * p.tiles, room = p.nr && (d->n_seqs == 1 || (p.nr == 2 && d->head_dim == 128)) ? 256 : 512;
   int64_t share = units > 0 ? room / units : 1;
-  const int64_t most = d->n_seqs * (int64_t)ceil_div(d->max_tokens, 256);
-  share = share > most ? most : share;
+  const int64_t longest = d->n_seqs * (int64_t)ceil_div(d->max_tokens, 256);
+  share = share > longest ? longest : share;
+  int64_t most = share >= (p.nr ? 2 : 4) * (int64_t)d->n_seqs ? share : d->n_seqs + share - 1;
+  most = most > longest ? longest : most;
+  const bool divided = share > 1 && most > d->n_seqs && d->n_seqs <= 256;
   p.unit = p.nr ? 7 : 6;  // a round of the workgroup
-  if (share * (((int64_t)d->max_tokens >> p.unit) + 1) >= 1LL << 32) p.unit = 9;
-  p.share = share > d->n_seqs ? (int)share : 0;
-  p.blocks = units * (p.share ? p.share : d->n_seqs);
+  if (d->n_seqs * (((int64_t)d->max_tokens >> p.unit) + 1) >= 1LL << 31) p.unit = 12;
+  p.share = divided ? (int)share : 0;
+  p.most = divided ? (int)most : 0;
+  p.slots = divided ? (int)(most < 2 * share ? most : 2 * share) : 0;
+  p.blocks = units * (divided ? most : d->n_seqs);
   return p;
 }
 
 size_t scratch_of(const lkv_chunk_desc* d, const Plan& p) {
-  const size_t rows = (size_t)p.share * d->n_q * d->new_tokens;
+  const size_t rows = (size_t)p.slots * d->n_q * d->new_tokens;
   return lkv_align_up(rows * sizeof(float2), 16) + rows * d->head_dim * sizeof(float);
 }
 
@@ -889,7 +907,7 @@ extern "C" int lkv_chunk_attend(uintptr_t stream, const lkv_chunk_desc* desc, co
   a.out = out;
   a.lse = lse;
   a.part_ml = (float2*)ws;
-  a.part_o = (float*)((uint8_t*)ws + lkv_align_up((size_t)p.share * desc->n_q * desc->new_tokens * sizeof(float2), 16));
+  a.part_o = (float*)((uint8_t*)ws + lkv_align_up((size_t)p.slots * desc->n_q * desc->new_tokens * sizeof(float2), 16));
   for (int i = 0; i < 3; ++i) a.q_stride[i] = desc->q_stride[i];
   a.scale2 = desc->scale * kLog2e;
   a.n_seqs = desc->n_seqs;
@@ -903,6 +921,7 @@ extern "C" int lkv_chunk_attend(uintptr_t stream, const lkv_chunk_desc* desc, co
   a.tiles = p.tiles;
   a.unit = p.unit;
   a.share = p.share;
+  a.most = p.most;
   const hipStream_t s = (hipStream_t)stream;
   const bool half = q_dtype == LKV_F16, wide = desc->head_dim == 128, mx = rows->dtype == LKV_MXFP8;
   const dim3 grid((unsigned)p.blocks);

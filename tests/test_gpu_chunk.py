@@ -100,6 +100,44 @@ def test_long_caches_in_many_parts(model: str, d: int, t: int, past: int) -> Non
     case(t, model, d, 1, 4, t, [past + t], page=16)
 
 
+@pytest.mark.parametrize(("seqs", "h", "g", "t", "long", "short"), [
+    (70, 1, 4, 1, 900, 300), (100, 3, 4, 1, 700, 400), (64, 8, 2, 1, 500, 40), (300, 1, 2, 1, 300, 80), (33, 1, 8, 3, 900, 200), (5, 4, 4, 70, 1500, 200), (8, 8, 4, 70, 900, 200),
+    (3, 2, 16, 130, 700, 150), (2, 8, 4, 200, 900, 250),
+])
+@pytest.mark.parametrize("kind", ["alike", "any", "one long"])
+def test_batches_of_lengths_alike_and_far_apart(seqs: int, h: int, g: int, t: int, long: int, short: int, kind: str) -> None:
+    """However the rows are divided among parts, sequences of one part and of several."""
+    gen = torch.Generator().manual_seed(seqs + t)
+    lens = [long // 2] * seqs if kind == "alike" else torch.randint(0, long + 1, (seqs,), generator=gen).tolist() if kind == "any" else [short] * seqs
+    lens[seqs // 2] = long if kind == "one long" else lens[seqs // 2]
+    lens[-1] = long if kind == "any" else lens[-1]
+    case(seqs, "bf16", 64, h, g, t, lens, [min(n, t) for n in lens])
+
+
+def test_a_captured_batch_follows_lengths_from_alike_to_far_apart() -> None:
+    from lazykv_amd import kernels
+
+    gen = torch.Generator().manual_seed(13)
+    q = normal(gen, (40, 8, 1, 64), "f16").cuda()
+    cache = Cache(gen, 40, 4, 600, 64, "f16")
+    lengths = int32([600] * 40)
+    kw = dict(scale=0.1, lengths=lengths, max_tokens=600)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        kernels.chunk_attend(q, cache.rows, **kw)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = kernels.chunk_attend(q, cache.rows, **kw)
+    for lens in ([600] + [1] * 39, [0] * 40, [300] * 40, list(range(40)), [600] * 40):
+        lengths.copy_(int32(lens))
+        out.fill_(9.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        check((out, lse), q, cache, lens, [1] * 40, 0.1)
+
+
 @pytest.mark.parametrize("q_scale", [0.0, 40.0])
 @pytest.mark.parametrize("t", [1, 40])
 def test_scores_that_are_alike_and_far_apart(q_scale: float, t: int) -> None:
