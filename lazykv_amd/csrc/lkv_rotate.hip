@@ -1,4 +1,6 @@
 // New tokens' queries and keys normalised over each head and rotated, keys and values written to their rows (lkv_rotate_append).
+#include <cfloat>
+
 #include "lkv_attend.h"
 #include "lkv_pages.h"
 
@@ -139,7 +141,8 @@ extern "C" int lkv_rotate_append(uintptr_t stream, const lkv_rotate_desc* desc, 
   LKV_CHECK_ARG(d.rotary == 0 || (cos && sin), "a rotation without its tables");
   LKV_CHECK_ARG(d.rotary == 0 || d.table_dtype == d.dtype || d.table_dtype == LKV_F32, "tables of dtype %d", d.table_dtype);
   LKV_CHECK_ARG((!q_weight && !k_weight) || d.weight_dtype == d.dtype || d.weight_dtype == LKV_F32, "weights of dtype %d", d.weight_dtype);
-  LKV_CHECK_ARG(d.eps >= 0.0f && d.eps < INFINITY, "eps %g", (double)d.eps);
+  // The reciprocal root takes a subnormal number for 0.
+  LKV_CHECK_ARG((d.eps == 0.0f || d.eps >= FLT_MIN) && d.eps < INFINITY, "eps %g: 0 or a normal number", (double)d.eps);
   uintptr_t all = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out | (uintptr_t)q_weight | (uintptr_t)k_weight;
   if (d.rotary) all |= (uintptr_t)cos | (uintptr_t)sin;
   LKV_CHECK_ARG((all & 15) == 0, "tokens, tables and weights must start on 16 bytes");

@@ -30,8 +30,8 @@ def _chunk(n_seqs: int, n_q: int, n_kv: int, d: int, t: int, most: int):  # noqa
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize(("n_q", "n_kv"), [(1, 1), (4, 1), (32, 8), (40, 1), (128, 128)])
 def test_scratch_is_bounded(n_q: int, n_kv: int, d: int) -> None:
-    """Partial results of attention are for at most 512 workgroups of 128 query rows (or for none: a sequence's one part writes the output); sums by parts for at most 1,024
-    workgroups of 256 rows."""
+    """Partial results of attention are for at most 1,024 workgroups of 128 query rows: rows are divided as 512 workgroups would share them, a sequence of several parts has
+    fewer than twice as many as its rows make whole ones, and one of a single part writes the output. Sums by parts are for at most 1,024 workgroups of 256 rows."""
     from lazykv_amd import _lib
 
     lib = _lib.lib()
@@ -41,7 +41,7 @@ def test_scratch_is_bounded(n_q: int, n_kv: int, d: int) -> None:
                 if n_seqs * n_q * t > 1 << 26:
                     continue
                 desc = ctypes.byref(_chunk(n_seqs, n_q, n_kv, d, t, most))
-                assert lib.lkv_chunk_attend_workspace_bytes(desc) <= 512 * 128 * (d + 2) * 4 + 16, (n_seqs, t, most)
+                assert lib.lkv_chunk_attend_workspace_bytes(desc) <= 1024 * 128 * (d + 2) * 4 + 16, (n_seqs, t, most)
                 assert lib.lkv_weigh_rows_workspace_bytes(desc) <= 1024 * 256 * 4, (n_seqs, t, most)
 
 
@@ -125,6 +125,8 @@ EVERY = ("attend", "weigh", "evict", "rotate")
     (("rotate",), {"rotate": {"table": 1}}, "tables of dtype"),
     (("rotate",), {"rotate": {"weight": 1}}, "weights of dtype"),
     (("rotate",), {"rotate": {"eps": -1.0}}, "eps"),
+    (("rotate",), {"rotate": {"eps": 1e-40}}, "eps"),
+    (("weigh",), {"desc": {"scale": 1e-39}}, "reciprocal"),
     (("rotate",), {"rotate": {"start": 62}}, "exceed"),
     (("rotate",), {"strides": (1536, 192, 60)}, "multiples of 8"),
     (("rotate",), {"strides": (0, 192, 64)}, "share an address"),

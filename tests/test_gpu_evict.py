@@ -117,6 +117,82 @@ def test_weights_of_what_is_not_attended_or_not_there() -> None:
     assert less[0, 0, :80].isfinite().all() and torch.all(less[0, 0, 77:80] == 0)
 
 
+@pytest.mark.parametrize(("t", "d"), [(20, 64), (20, 128), (6, 128)])
+@pytest.mark.parametrize("what", [float("nan"), float("inf")])
+def test_a_query_reaches_only_the_rows_that_it_attends(t: int, d: int, what: float) -> None:
+    """One token's query, or its lse, is not finite: the rows behind those that it attends are as without it, to the bit."""
+    from lazykv_amd import kernels
+
+    gen = torch.Generator().manual_seed(t)
+    past, at = 300, t // 2
+    n = past + t
+    q = normal(gen, (1, 8, t, d), "bf16").cuda()
+    cache = Cache(gen, 1, 2, n, d, "bf16", page=16)
+    kw = dict(scale=0.1, tokens=n, pages=cache.pages)
+    lse = kernels.chunk_attend(q, cache.rows, **kw)[1]
+    want = kernels.weigh_rows(q, lse, cache.rows, **kw)
+    q2, lse2 = q.clone(), lse.clone()
+    q2[0, 1, at], lse2[0, 5, at] = what, float("nan")
+    for x, y, head in ((q2, lse, 0), (q, lse2, 1)):
+        got = kernels.weigh_rows(x, y, cache.rows, **kw)
+        assert torch.equal(got[0, 1 - head], want[0, 1 - head]) and torch.equal(got[0, head, past + at + 1 :], want[0, head, past + at + 1 :])
+    got = kernels.weigh_rows(q, lse2, cache.rows, **kw)
+    assert got[0, 1, : past + at + 1].isnan().all()
+
+
+def test_a_captured_account_follows_lengths_and_pages() -> None:
+    from lazykv_amd import kernels
+
+    gen = torch.Generator().manual_seed(9)
+    for t in (2, 40, 200):
+        q = normal(gen, (2, 8, t, 64), "f16").cuda()
+        cache = Cache(gen, 2, 2, 700, 64, "f16", page=16)
+        lengths, counts, seen, pages = int32([700, 213]), int32([t, t]), int32([0, 5]), cache.pages.clone()
+        lse = torch.randn((2, 8, t), generator=gen).cuda() + 4
+        old = torch.rand((2, 2, 700), generator=gen).cuda()
+        kw = dict(scale=0.09, lengths=lengths, counts=counts, max_tokens=700, pages=pages, seen=seen)
+        held = [[old.clone(), torch.zeros((2, 2, 700), dtype=torch.int32, device="cuda")] for _ in range(2)]
+        call = lambda i: kernels.weigh_rows(q, lse, cache.rows, sums=held[i][0], positions=held[i][1], **kw)  # noqa: E731, B023
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            call(0)
+        torch.cuda.current_stream().wait_stream(side)
+        call(1)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call(0)
+        for i, (a, b, c, d) in enumerate([(700, 213, t, 1), (5, 699, min(5, t), t), (0, 1, 0, 1), (350, 351, t, t)]):
+            lengths.copy_(int32([a, b]))
+            counts.copy_(int32([c, d]))
+            pages.copy_(cache.pages.flip(0) if i == 3 else cache.pages)
+            lse.add_(0.25)
+            graph.replay()
+            torch.cuda.synchronize()
+            call(1)
+            for x, y in zip(*held):  # to the bit; swapped pages bring rows of nobody's, which hold NaN, before the end
+                torch.testing.assert_close(x, y, rtol=0, atol=0, equal_nan=True)
+
+
+def test_weights_past_32_bits_of_bytes() -> None:
+    """One head of 17 million rows: the last ones get what they would at a cache's start, in the few rows' form and in the other."""
+    from lazykv_amd import kernels
+
+    gen = torch.Generator().manual_seed(10)
+    n = (1 << 24) + 4096
+    keys = torch.zeros((1, 1, n, 128), dtype=torch.bfloat16, device="cuda")
+    tail = normal(gen, (1, 1, 4096, 128), "bf16").cuda()
+    keys[:, :, -4096:] = tail
+    for t in (1, 40):
+        q, lse = normal(gen, (1, 2, t, 128), "bf16").cuda(), torch.full((1, 2, t), 20.0, device="cuda")
+        got = kernels.weigh_rows(q, lse, kernels.dense_rows(keys, keys), scale=0.09, tokens=n)
+        want = kernels.weigh_rows(q, lse, kernels.dense_rows(tail, tail), scale=0.09, tokens=4096)
+        assert torch.equal(got[..., -4096:], want) or t > 1  # parts may differ with the length: their order of sums too
+        # g t weights, each the same number, summed in float32 in two orders.
+        assert torch.all((got[..., -4096:] - want).abs() <= 2 * 2 * t * U * want)
+        assert torch.all((got[..., :-4096] - 2 * t * np.exp(-20.0)).abs() <= (2 * t + 60) * U * 2 * t * np.exp(-20.0))
+
+
 def evict_case(seed: int, seqs: int, h: int, n: int, keep: int, sinks: int, recent: int, lens: list | None = None, *, eight: bool = False, page: int = 0, d: int = 64,
                ties: bool = False, apart: bool = False, special: bool = False) -> None:
     from lazykv_amd import kernels
@@ -223,6 +299,84 @@ def test_a_captured_eviction_follows_lengths() -> None:
         call(1)
         for x, y in zip((*caches[0].held, *to[0]), (*caches[1].held, *to[1])):  # to the bit; pages of nobody's hold NaN
             torch.testing.assert_close(x, y, rtol=0, atol=0, equal_nan=True)
+
+
+def test_a_captured_long_eviction_follows_lengths_and_sums() -> None:
+    """Twice the long form in one graph, on caches and scratch of their own."""
+    from lazykv_amd import kernels
+
+    gen = torch.Generator().manual_seed(14)
+    n, keep = 20011, 5000
+    stores = [torch.zeros((2, 2, 1, n, 64), dtype=torch.float16, device="cuda") for _ in range(3)]
+    sums, positions = torch.rand((2, 1, n), generator=gen).cuda(), torch.arange(n, dtype=torch.int32, device="cuda").expand(2, 1, n).contiguous()
+    lengths = int32([n, n])
+    to = [[torch.zeros_like(x) for x in (sums, positions)] for _ in range(3)]
+    call = lambda i: kernels.evict_rows(kernels.dense_rows(*stores[i]), sums, positions, keep=keep, sinks=4, recent=100, lengths=lengths, max_tokens=n, out=tuple(to[i]))  # noqa: E731
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(0)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(0)
+        call(1)
+    fresh = normal(gen, (2, 2, 1, n, 64), "f16").cuda()
+    for a, b in ((n, 16000), (5001, 0), (4999, n - 1)):
+        lengths.copy_(int32([a, b]))
+        sums.copy_(torch.rand((2, 1, n), generator=gen).mul_(8).floor() if b == 0 else torch.rand((2, 1, n), generator=gen))
+        for x in stores:
+            x.copy_(fresh)
+        graph.replay()
+        torch.cuda.synchronize()
+        call(2)
+        for i in range(2):
+            assert torch.equal(stores[i], stores[2]) and all(torch.equal(x, y) for x, y in zip(to[i], to[2]))
+
+
+def test_pages_that_a_pool_lacks_are_not_moved() -> None:
+    """A row whose page is not there keeps its rank: its sums and positions move, and no keys or values."""
+    from lazykv_amd import kernels
+
+    gen = torch.Generator().manual_seed(15)
+    cache = Cache(gen, 1, 1, 64, 64, "f16", page=16)
+    before = cache.read()
+    sums, positions = torch.arange(64.0, device="cuda").expand(1, 1, 64).contiguous(), torch.arange(64, dtype=torch.int32, device="cuda").expand(1, 1, 64).contiguous()
+    pages = cache.pages.clone()
+    pages[0, 0], pages[0, 3] = -5, cache.rows.seqs
+    kernels.evict_rows(cache.rows, sums, positions, keep=32, tokens=64, pages=pages)  # rows 32 .. 63 stay, in places 0 .. 31
+    assert torch.equal(sums[0, 0, :32], torch.arange(32.0, 64.0, device="cuda")) and torch.equal(positions[0, 0, :32].cpu(), torch.arange(32, 64, dtype=torch.int32))
+    for x, y in zip(cache.read(), before):
+        assert np.array_equal(x, y)  # rows 32 .. 47 to a page that is not there, rows 48 .. 63 from one
+
+
+def test_two_streams_evict_and_account_at_once() -> None:
+    from lazykv_amd import kernels
+
+    gen = torch.Generator().manual_seed(16)
+    n, keep = 18000, 6000
+    first = normal(gen, (2, 1, 2, n, 64), "f16").cuda()
+    q, lse = normal(gen, (1, 8, 100, 64), "f16").cuda(), torch.full((1, 8, 100), 9.0, device="cuda")
+    results = []
+
+    def both() -> tuple:
+        store = first.clone()
+        rows = kernels.dense_rows(store[0], store[1])
+        positions = torch.zeros((1, 2, n), dtype=torch.int32, device="cuda")
+        sums = kernels.weigh_rows(q, lse, rows, scale=0.1, tokens=n, positions=positions)
+        positions[..., : n - 100] = torch.arange(n - 100, device="cuda")
+        kernels.evict_rows(rows, sums, positions, keep=keep, sinks=2, recent=500, tokens=n)
+        return store, sums, positions
+
+    want = both()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                results.append(both())
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for got in results for x, y in zip(got, want))
 
 
 def test_what_is_refused() -> None:
