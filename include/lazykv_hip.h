@@ -372,14 +372,14 @@ typedef struct lkv_pages {
  * y_i cos_i - y_(i + rotary / 2) sin_i, i + rotary / 2 to y_(i + rotary / 2) cos_(i + rotary / 2) + y_i sin_(i + rotary / 2); cos and sin
  * [n_seqs or 1, tokens, rotary] at b * table_seq_stride + t * rotary), in float32 and rounded to the model dtype once. Queries go to
  * q_out (strides of its own), keys and values to rows start + starts[b] + t of `dst` as in lkv_append_rows; tokens from counts[b] on
- * go to no row (counts NULL: all go). Of two tokens that go to one row (a page in two tables) either may be what it holds. */
+ * go to no row (counts NULL: all go). What a row holds that two tokens of a call go to (a page in two tables) is not defined. */
 typedef struct lkv_rotate_desc {
   int32_t n_seqs, n_q, n_kv, head_dim, tokens;
   int32_t dtype;        /* of q, k, v, q_out */
   int32_t rotary;       /* 0, or a multiple of 16 up to head_dim */
   int32_t table_dtype;  /* of cos and sin: dtype or LKV_F32 */
   int32_t weight_dtype; /* of the weights: dtype or LKV_F32 */
-  float eps;
+  float eps;            /* 0 or a normal number */
   int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3]; /* sequence, head, token */
   int64_t table_seq_stride;                                     /* 0: one table for all */
 } lkv_rotate_desc;
@@ -404,7 +404,7 @@ int lkv_chunk_attend(uintptr_t stream, const lkv_chunk_desc* desc, const void* q
 
 /* The weights that rows get from a chunk's tokens, summed up: with lse [n_seqs, n_q, new_tokens] as lkv_chunk_attend gives it, row i of KV
  * head h of sequence b gets  sum over the head's query heads and the tokens that attend i of  exp(scale q . k_i - lse), added
- * to sums for rows from before the chunk and by itself for the chunk's own, into out; a token whose lse is -inf adds nothing. sums (NULL: 0) and
+ * to sums for rows from before the chunk and by itself for the chunk's own, into out; a token whose lse is -inf adds nothing. 1 / scale must be finite. sums (NULL: 0) and
  * out are float32, element (b, h, i) at b * sums_stride[0] + h * sums_stride[1] + i; they may be the same; rows from len on are left as they are.
  * positions (int32, laid out the same; may be NULL) of the chunk's own rows are set to seen[b] + their place in it (seen NULL:
  * len - n, the rows before). */

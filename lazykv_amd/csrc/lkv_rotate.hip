@@ -171,9 +171,10 @@ extern "C" int lkv_rotate_append(uintptr_t stream, const lkv_rotate_desc* desc, 
   a.counts = counts;
   a.start = start;
   a.heads = (uint32_t)heads;
-  // All heads of a token by one workgroup, or, of few tokens, as many at a time as it has lanes for.
+  // All heads of a token by one workgroup, or, of few tokens, as many as it has lanes for (48 heads, d 128): 64 tokens 5.6 and 4.4 us, 256 5.9 and 5.1,
+  // 512 6.6 and 6.9, 1,024 8.5 and 10.4, 4,096 21.8 and 33.
   const int64_t tokens = (int64_t)d.n_seqs * d.tokens;
-  a.splits = tokens >= 1024 ? 1 : (a.heads + kHeads - 1) / kHeads;
+  a.splits = tokens >= 512 ? 1 : (a.heads + kHeads - 1) / kHeads;
   a.share = a.splits == 1 ? a.heads : kHeads;
   const bool mx = dst->dtype == LKV_MXFP8, half = d.dtype == LKV_F16, wide = d.head_dim == 128;
   auto kernel = half ? (wide ? (mx ? rotate_append_kernel<LKV_F16, 128, true> : rotate_append_kernel<LKV_F16, 128, false>)

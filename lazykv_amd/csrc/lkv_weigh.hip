@@ -377,11 +377,15 @@ struct Plan {
 Plan plan_of(const lkv_chunk_desc* d) {
   Plan p = {};
   const int64_t x = (int64_t)d->new_tokens * (d->n_q / d->n_kv);
+  // Few query rows from memory, many through LDS (8 heads, d 128): 32 over 4,096 rows 6.2 us and by the other form 6.5, over 65,536 29.5 and 33.3; 36 over 4,096
+  // 6.6 and 6.5; 64 over 65,536 38.3 and 33.8; 4,096 over 16,384 258 and 187.
   p.wide = x > 32;
   p.blocks = ceil_div(d->max_tokens, kBlockRows);
   const int64_t units = (int64_t)d->n_seqs * d->n_kv * p.blocks;
-  int64_t parts = units > 0 ? 1024 / units : 1;
-  const int64_t most = x / 256;
+  // Query rows in parts for 2,048 workgroups, a stage each at the least: 8,192 of them over 4,096 rows 97 us, by 1,024 workgroups 108, by 4,096 100; 800 over 700
+  // 12.2, by four stages each 20.4.
+  int64_t parts = units > 0 ? 2048 / units : 1;
+  const int64_t most = x / kStage;
   parts = parts > most ? most : parts;
   parts = parts < 1 ? 1 : parts;
   p.chunk = ceil_div(ceil_div(x, parts), kStage) * kStage;
