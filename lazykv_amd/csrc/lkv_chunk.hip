@@ -872,7 +872,7 @@ int lkv_check_chunk(const lkv_chunk_desc* d) {
   LKV_CHECK_ARG(d->head_dim == 64 || d->head_dim == 128, "head_dim %d unsupported (64 or 128)", d->head_dim);
   LKV_CHECK_ARG(d->n_seqs >= 0 && d->n_kv > 0 && d->n_q > 0 && d->n_q % d->n_kv == 0 && d->new_tokens >= 0, "bad shape: %d sequences, %d query heads over %d, %d tokens",
                 d->n_seqs, d->n_q, d->n_kv, d->new_tokens);
-  LKV_CHECK_ARG((__int128)d->n_seqs * d->n_q * d->new_tokens <= (1 << 26), "%d x %d x %d query rows in one call", d->n_seqs, d->n_q, d->new_tokens);
+  LKV_CHECK_ARG((__int128)d->n_seqs * d->n_q * (d->new_tokens > 0 ? d->new_tokens : 1) <= (1 << 26), "%d x %d x %d query rows in one call", d->n_seqs, d->n_q, d->new_tokens);
   LKV_CHECK_ARG(d->scale > 0.0f && d->scale * lkv::kLog2e < INFINITY, "scale %g: positive and finite", (double)d->scale);
   LKV_CHECK_ARG(d->tokens >= 0 && d->max_tokens >= 0 && d->max_tokens <= (1 << 30), "bad extent: %d rows of at most %d", d->tokens, d->max_tokens);
   LKV_CHECK_ARG(((d->q_stride[0] | d->q_stride[1] | d->q_stride[2]) & 7) == 0, "strides must be multiples of 8 elements");
@@ -900,7 +900,7 @@ extern "C" int lkv_chunk_attend(uintptr_t stream, const lkv_chunk_desc* desc, co
   const int64_t n = (int64_t)desc->n_seqs * desc->n_q * desc->new_tokens;
   if (n == 0) return LKV_OK;
   const Plan p = plan_of(desc);
-  LKV_CHECK_ARG(p.blocks < (1LL << 31), "%lld workgroups in one call", (long long)p.blocks);
+  LKV_CHECK_ARG(p.blocks < (1 << 24), "%lld workgroups in one call", (long long)p.blocks);
   a.q = (const uint16_t*)q;
   a.lengths = lengths;
   a.counts = counts;

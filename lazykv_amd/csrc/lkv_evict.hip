@@ -385,6 +385,7 @@ int check_evict(const lkv_evict_desc* d) {
   LKV_CHECK_ARG(d->head_dim == 64 || d->head_dim == 128, "head_dim %d unsupported (64 or 128)", d->head_dim);
   LKV_CHECK_ARG(d->dtype == LKV_F16 || d->dtype == LKV_BF16, "rows are float16 or bfloat16, got dtype %d", d->dtype);
   LKV_CHECK_ARG(d->n_seqs >= 0 && d->n_kv > 0, "bad shape: %d sequences, %d heads", d->n_seqs, d->n_kv);
+  LKV_CHECK_ARG((int64_t)d->n_seqs * d->n_kv < (1 << 22), "%d x %d heads in one call", d->n_seqs, d->n_kv);
   LKV_CHECK_ARG(d->tokens >= 0 && d->max_tokens >= 0 && d->max_tokens <= (1 << 30), "bad extent: %d rows of at most %d", d->tokens, d->max_tokens);
   LKV_CHECK_ARG(d->keep > 0 && d->sinks >= 0 && d->recent >= 0 && (int64_t)d->sinks + d->recent <= d->keep, "%d first and %d newest of %d rows that are kept", d->sinks,
                 d->recent, d->keep);
@@ -466,8 +467,8 @@ extern "C" int lkv_evict_rows(uintptr_t stream, const lkv_evict_desc* desc, cons
   const Layout l = layout_of(desc);
   a.moves = moves_of(desc);
   a.spans = l.spans;
-  const int64_t per = 256 / (desc->head_dim / 8), moving = (a.moves + per - 1) / per, blocks = heads * (moving > l.spans ? moving : l.spans);
-  LKV_CHECK_ARG(heads < (1LL << 31) && blocks < (1LL << 31), "%lld workgroups in one call", (long long)blocks);
+  const int64_t per = 256 / (desc->head_dim / 8), moving = (a.moves + per - 1) / per, planning = heads * (l.spans ? l.spans : 1);
+  LKV_CHECK_ARG(planning < (1 << 22) && heads * moving < (1 << 24), "%lld and %lld workgroups in one call", (long long)planning, (long long)(heads * moving));
   if (heads == 0 || desc->max_tokens == 0) return LKV_OK;
   if (int rc = lkv_distinct_dst(rows, desc->n_kv, desc->head_dim)) return rc;
   a.lengths = lengths;

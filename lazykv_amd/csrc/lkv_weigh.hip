@@ -423,7 +423,7 @@ extern "C" int lkv_weigh_rows(uintptr_t stream, const lkv_chunk_desc* desc, cons
   LKV_CHECK_ARG(need == 0 || (ws && ws_bytes >= need && ((uintptr_t)ws & 15) == 0), "workspace of %zu bytes, on 16: %zu are needed", ws_bytes, need);
   const Plan p = plan_of(desc);
   const int64_t blocks = (int64_t)desc->n_seqs * desc->n_kv * p.blocks;
-  LKV_CHECK_ARG(blocks * p.parts < (1LL << 31), "%lld workgroups in one call", (long long)blocks * p.parts);
+  LKV_CHECK_ARG(blocks * p.parts < (1 << 24), "%lld workgroups in one call", (long long)blocks * p.parts);
   if (blocks == 0) return LKV_OK;
   a.q = (const uint16_t*)q;
   a.lse = lse;

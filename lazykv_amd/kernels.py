@@ -1097,6 +1097,7 @@ def _chunk(what: str, q: torch.Tensor, rows: Rows, scale: float, tokens: int, le
     if (tokens | max_tokens) >> 31:
         _int32("tokens", tokens)
         _int32("max_tokens", max_tokens)
+        raise ValueError(f"bad extent: {tokens} rows of at most {max_tokens}")
     if lengths is None and tokens > max_tokens:
         raise ValueError(f"tokens={tokens} exceed max_tokens={max_tokens}")
     at, count = _counts(lengths, seqs, index, "lengths"), _counts(counts, seqs, index, "counts")
@@ -1294,6 +1295,8 @@ def evict_rows(
         ends = spots
     if _meet(spots[:1], spots[1:]) or _meet((*spots, *ends), _row_spans(rows)):
         raise ValueError("sums, positions and rows share addresses")
+    if seqs == 0 or max_tokens == 0:
+        return
     lib = _lib.lib()
     desc = _lib.EvictDesc(seqs, rows.n_kv, rows.head_dim, rows.model_code, keep, sinks, recent, tokens, max_tokens)
     ref = ctypes.byref(desc)

@@ -128,6 +128,13 @@ EVERY = ("attend", "weigh", "evict", "rotate")
     (("rotate",), {"rotate": {"eps": 1e-40}}, "eps"),
     (("weigh",), {"desc": {"scale": 1e-39}}, "reciprocal"),
     (("rotate",), {"rotate": {"start": 62}}, "exceed"),
+    (("rotate",), {"desc": {"n_q": 1 << 20, "new_tokens": 1 << 11}, "rows": {"tokens": 16384}}, "in one call"),
+    (("rotate",), {"desc": {"n_q": 1, "n_kv": 1, "n_seqs": 1 << 14, "new_tokens": 1 << 10}, "rows": {"tokens": 16384}}, "in one call"),
+    (("attend", "weigh"), {"desc": {"n_seqs": 1 << 30, "new_tokens": 0}}, "query rows"),
+    (("evict",), {"desc": {"n_seqs": 1 << 30, "n_kv": 1 << 30}}, "in one call"),
+    (("attend",), {"desc": {"n_seqs": 1 << 25, "n_q": 2, "new_tokens": 1}}, "in one call"),
+    (("weigh",), {"desc": {"n_seqs": 1 << 25, "n_q": 2, "new_tokens": 1}}, "in one call"),
+    (("evict",), {"desc": {"n_seqs": 1 << 10, "n_kv": 8, "max_tokens": 1 << 24}, "rows": {"tokens": 16384}, "pages": {"n_pages": 1024}, "ws_bytes": 1 << 60}, "in one call"),
     (("rotate",), {"strides": (1536, 192, 60)}, "multiples of 8"),
     (("rotate",), {"strides": (0, 192, 64)}, "share an address"),
     (("rotate", "evict"), {"rows": {"seq_stride": 1024}}, "share an address"),

@@ -350,6 +350,26 @@ def test_pages_that_a_pool_lacks_are_not_moved() -> None:
         assert np.array_equal(x, y)  # rows 32 .. 47 to a page that is not there, rows 48 .. 63 from one
 
 
+def test_calls_without_tokens_or_rows() -> None:
+    from lazykv_amd import kernels
+
+    gen = torch.Generator().manual_seed(17)
+    cache = Cache(gen, 2, 2, 64, 64, "f16", page=16)
+    sums, out = torch.rand((2, 2, 64), generator=gen).cuda(), torch.full((2, 2, 64), 5.0, device="cuda")
+    q, lse = torch.zeros((2, 4, 0, 64), dtype=torch.float16, device="cuda"), torch.zeros((2, 4, 0), device="cuda")
+    got = kernels.weigh_rows(q, lse, cache.rows, scale=0.1, lengths=int32([50, 0]), pages=cache.pages, sums=sums, out=out)
+    assert torch.equal(got[0, :, :50], sums[0, :, :50]) and torch.all(got[0, :, 50:] == 5) and torch.all(got[1] == 5)
+    before = cache.read()
+    none, nowhere = torch.zeros((2, 2, 0), device="cuda"), torch.zeros((2, 2, 0), dtype=torch.int32, device="cuda")
+    kernels.evict_rows(cache.rows, none, nowhere, keep=4, tokens=0, pages=cache.pages)
+    kernels.evict_rows(cache.rows, sums[:0], torch.zeros((0, 2, 64), dtype=torch.int32, device="cuda"), keep=4, tokens=9, pages=cache.pages[:0])
+    assert all(np.array_equal(x, y) for x, y in zip(cache.read(), before))
+    for tokens, most in ((-1, 4), (4, -1)):
+        with pytest.raises(ValueError, match="bad extent"):
+            kernels.weigh_rows(torch.zeros((2, 4, 1, 64), dtype=torch.float16, device="cuda"), torch.zeros((2, 4, 1), device="cuda"), cache.rows, scale=0.1, tokens=tokens,
+                               max_tokens=most, lengths=int32([1, 1]), pages=cache.pages)
+
+
 def test_two_streams_evict_and_account_at_once() -> None:
     from lazykv_amd import kernels
 
