@@ -1009,9 +1009,8 @@ def rotate_append(
         if cos.get_device() != index or sin.get_device() != index:
             raise ValueError(f"cos/sin on {cos.device} / {sin.device}, the cache on {dst.device}")
         rotary = cs[2]
-        cos, sin = _whole(cos), _whole(sin)
-        cos_at, sin_at = cos.data_ptr(), sin.data_ptr()
         read += (cos, sin)
+        (cos, cos_at), (sin, sin_at) = _whole(cos), _whole(sin)
         if cs[0] != 1:
             table_stride = n * rotary
         if cos.dtype != dtype:
@@ -1019,24 +1018,22 @@ def rotate_append(
     elif cos is not None or sin is not None:
         raise ValueError("cos and sin come together")
     if q_weight is not None or k_weight is not None:
-        kinds = set()
+        kind = None
         for w in (q_weight, k_weight):
             if w is not None:
-                kinds.add(w.dtype)
-                if w.shape != (d,) or (w.dtype != dtype and w.dtype != torch.float32) or w.get_device() != index:
-                    raise ValueError(f"weights must be {dtype} or float32 [{d}] on {dst.device}, got {w.dtype} {tuple(w.shape)} on {w.device}")
-        if len(kinds) != 1:
-            raise ValueError(f"weights of {q_weight.dtype} and {k_weight.dtype}")
-        if dtype not in kinds:
+                mine = w.dtype
+                if w.shape != (d,) or (mine != dtype and mine != torch.float32) or w.get_device() != index:
+                    raise ValueError(f"weights must be {dtype} or float32 [{d}] on {dst.device}, got {mine} {tuple(w.shape)} on {w.device}")
+                if kind is not None and mine != kind:
+                    raise ValueError(f"weights of {kind} and {mine}")
+                kind = mine
+                read.append(w)
+        if kind != dtype:
             weight = _lib.F32
         if q_weight is not None:
-            q_weight = _whole(q_weight)
-            q_at = q_weight.data_ptr()
-            read.append(q_weight)
+            q_weight, q_at = _whole(q_weight)
         if k_weight is not None:
-            k_weight = _whole(k_weight)
-            k_at = k_weight.data_ptr()
-            read.append(k_weight)
+            k_weight, k_at = _whole(k_weight)
     _no_gradients("rotate_append", (*read, *dst.owners) if out is None else (*read, *dst.owners, out))
     at, count = _counts(starts, seqs, index, "starts"), _counts(counts, seqs, index, "counts")
     table_ref, _ = _paged(dst, pages, seqs)
@@ -1076,9 +1073,13 @@ def rotate_append(
     return out
 
 
-def _whole(x: torch.Tensor) -> torch.Tensor:
-    """`x` as the kernels read tables: contiguous, on 16 bytes."""
-    return x if x.is_contiguous() and x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
+def _whole(x: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """`x` as the kernels read tables, contiguous and on 16 bytes, and where it is."""
+    at = x.data_ptr()
+    if at % 16 or not x.is_contiguous():
+        x = x.clone(memory_format=torch.contiguous_format)
+        at = x.data_ptr()
+    return x, at
 
 
 def _chunk(what: str, q: torch.Tensor, rows: Rows, scale: float, tokens: int, lengths: torch.Tensor | None, counts: torch.Tensor | None, max_tokens: int | None,
@@ -1107,13 +1108,13 @@ def _chunk(what: str, q: torch.Tensor, rows: Rows, scale: float, tokens: int, le
     return _lib.ChunkDesc(seqs, n_q, rows.n_kv, d, n, scale, tokens, max_tokens, st[0], st[1], st[2]), q, at, count, table, max_tokens
 
 
-def _scratch(need: int, ws: Workspace | None, device: torch.device) -> tuple[int | None, int, object]:
-    """A call's scratch: the workspace's, or torch's own allocation, which no other call on another stream or in a graph can be in."""
+def _scratch(need: int, ws: Workspace | None, beside: torch.Tensor) -> tuple[int | None, int, object]:
+    """A call's scratch: the workspace's, or torch's own allocation on a tensor's device, which no other call on another stream or in a graph can be in."""
     if ws is not None:
         return (*ws.get(need), ws)
     if not need:
         return None, 0, None
-    buf = torch.empty(need, dtype=torch.uint8, device=device)
+    buf = beside.new_empty(need, dtype=torch.uint8)
     return buf.data_ptr(), need, buf
 
 
@@ -1143,11 +1144,11 @@ def chunk_attend(
     desc, q, at, count, table, _ = _chunk("chunk_attend", q, rows, scale, tokens, lengths, counts, max_tokens, pages, given)
     shape, index = q.shape, rows.device_index
     if out is None:
-        out = torch.empty(shape, dtype=out_dtype or q.dtype, device=q.device)
+        out = q.new_empty(shape, dtype=out_dtype)
     elif not out.is_contiguous() or out.shape != shape or out.get_device() != index or (out_dtype is not None and out.dtype != out_dtype) or out.data_ptr() % 16:
         raise ValueError(f"out must be contiguous {tuple(shape)} on {rows.device}, on 16 bytes")
     if lse is None:
-        lse = torch.empty(shape[:3], dtype=torch.float32, device=q.device)
+        lse = q.new_empty(shape[:3], dtype=torch.float32)
     elif not lse.is_contiguous() or lse.shape != shape[:3] or lse.dtype != torch.float32 or lse.get_device() != index:
         raise ValueError(f"lse must be contiguous float32 {tuple(shape[:3])} on {rows.device}")
     if 0 in shape:
@@ -1159,7 +1160,7 @@ def chunk_attend(
         _WRITTEN(given)
     lib = _lib.lib()
     ref = ctypes.byref(desc)
-    ws_ptr, ws_n, _held = _scratch(lib.lkv_chunk_attend_workspace_bytes(ref), ws, q.device)
+    ws_ptr, ws_n, _held = _scratch(lib.lkv_chunk_attend_workspace_bytes(ref), ws, q)
     rc = _launch(index, lib.lkv_chunk_attend, ref, q.data_ptr(), rows.model_code, rows.ref, table, at, count, out.data_ptr(), _lib.dtype_code(out.dtype),
                  lse.data_ptr(), ws_ptr, ws_n)
     if rc:
@@ -1172,6 +1173,8 @@ def _account(name: str, x: torch.Tensor, dtype: torch.dtype, seqs: int, n_kv: in
     shape, st = x.shape, x.stride()
     if len(shape) != 3 or shape[0] != seqs or shape[1] != n_kv or shape[2] < n or x.dtype != dtype or x.get_device() != device or (st[2] != 1 and shape[2] > 1):
         raise ValueError(f"{name} must be {dtype} [{seqs}, {n_kv}, {n} or more] with contiguous rows on cuda:{device}, got {x.dtype} {tuple(shape)} on {x.device}")
+    if x.is_contiguous():
+        return _lib.Pair(st[0], st[1])
     a, b, n = (st[0] if seqs > 1 else 0), (st[1] if n_kv > 1 else 0), shape[2]
     if (a and b and min(a, b) < n) or (n_kv > 1 and b < n) or (seqs > 1 and a < n) or (a > b > 0 and a < b * (n_kv - 1) + n) or (0 < a <= b and b < a * (seqs - 1) + n):
         raise ValueError(f"{name}'s rows share addresses")
@@ -1239,7 +1242,7 @@ def weigh_rows(
     _WRITTEN(written)
     lib = _lib.lib()
     ref = ctypes.byref(desc)
-    ws_ptr, ws_n, _held = _scratch(lib.lkv_weigh_rows_workspace_bytes(ref), ws, q.device)
+    ws_ptr, ws_n, _held = _scratch(lib.lkv_weigh_rows_workspace_bytes(ref), ws, q)
     rc = _launch(index, lib.lkv_weigh_rows, ref, q.data_ptr() or lse.data_ptr() or out.data_ptr(), rows.model_code, lse.data_ptr() or out.data_ptr(), rows.ref, table, at, count,
                  None if sums is None else sums.data_ptr(), sums_st, out.data_ptr(), out_st, None if positions is None else positions.data_ptr(), positions_st, first,
                  ws_ptr, ws_n)
@@ -1273,37 +1276,39 @@ def evict_rows(
     table, room = _paged(rows, pages, seqs)
     if max_tokens is None:
         max_tokens = tokens if lengths is None else room
-    for name, n in (("tokens", tokens), ("max_tokens", max_tokens), ("keep", keep), ("sinks", sinks), ("recent", recent)):
-        _int32(name, n)
+    if (tokens | max_tokens | keep | sinks | recent) >> 31:
+        for name, n in (("tokens", tokens), ("max_tokens", max_tokens), ("keep", keep), ("sinks", sinks), ("recent", recent)):
+            _int32(name, n)
     if lengths is None and tokens > max_tokens:
         raise ValueError(f"tokens={tokens} exceed max_tokens={max_tokens}")
-    to = (sums, positions) if out is None else out
-    _no_gradients("evict_rows", (*rows.owners, sums, positions, *to))
     at = _counts(lengths, seqs, index, "lengths")
-    least = max(0, max_tokens)
-    strides = [_account(name, x, t, seqs, rows.n_kv, n, index) for name, x, t, n in (
-        ("sums", sums, torch.float32, least), ("positions", positions, torch.int32, least), ("out's sums", to[0], torch.float32, min(least, max(0, keep))),
-        ("out's positions", to[1], torch.int32, min(least, max(0, keep))))]
+    h, least = rows.n_kv, max(0, max_tokens)
+    sums_st, positions_st = _account("sums", sums, torch.float32, seqs, h, least, index), _account("positions", positions, torch.int32, seqs, h, least, index)
     spots = _reach(sums), _reach(positions)
-    if out is not None:
-        ends = _reach(to[0]), _reach(to[1])
-        _same_or_apart("sums", to[0], sums, ends[0], spots[0])
-        _same_or_apart("positions", to[1], positions, ends[1], spots[1])
+    if out is None:
+        to_sums, to_positions, to_sums_st, to_positions_st, ends = sums, positions, sums_st, positions_st, ()
+    else:
+        to_sums, to_positions = out
+        left = min(least, max(0, keep))
+        to_sums_st = _account("out's sums", to_sums, torch.float32, seqs, h, left, index)
+        to_positions_st = _account("out's positions", to_positions, torch.int32, seqs, h, left, index)
+        ends = _reach(to_sums), _reach(to_positions)
+        _same_or_apart("sums", to_sums, sums, ends[0], spots[0])
+        _same_or_apart("positions", to_positions, positions, ends[1], spots[1])
         if _meet(ends[:1], (ends[1], spots[1])) or _meet(ends[1:], spots[:1]):
             raise ValueError("sums and positions share addresses")
-    else:
-        ends = spots
-    if _meet(spots[:1], spots[1:]) or _meet((*spots, *ends), _row_spans(rows)):
+    _no_gradients("evict_rows", (*rows.owners, sums, positions) if out is None else (*rows.owners, sums, positions, to_sums, to_positions))
+    if _meet(spots[:1], spots[1:]) or (rows.span is not None and _meet((*spots, *ends), _row_spans(rows))):
         raise ValueError("sums, positions and rows share addresses")
     if seqs == 0 or max_tokens == 0:
         return
     lib = _lib.lib()
     desc = _lib.EvictDesc(seqs, rows.n_kv, rows.head_dim, rows.model_code, keep, sinks, recent, tokens, max_tokens)
     ref = ctypes.byref(desc)
-    ws_ptr, ws_n, _held = _scratch(max(16, lib.lkv_evict_rows_workspace_bytes(ref)), ws, sums.device)
-    _WRITTEN((*rows.owners, *to))
-    rc = _launch(index, lib.lkv_evict_rows, ref, rows.ref, table, at, sums.data_ptr(), strides[0], positions.data_ptr(), strides[1], to[0].data_ptr(), strides[2],
-                 to[1].data_ptr(), strides[3], ws_ptr, ws_n)
+    ws_ptr, ws_n, _held = _scratch(max(16, lib.lkv_evict_rows_workspace_bytes(ref)), ws, sums)
+    _WRITTEN((*rows.owners, to_sums, to_positions))
+    rc = _launch(index, lib.lkv_evict_rows, ref, rows.ref, table, at, sums.data_ptr(), sums_st, positions.data_ptr(), positions_st, to_sums.data_ptr(), to_sums_st,
+                 to_positions.data_ptr(), to_positions_st, ws_ptr, ws_n)
     if rc:
         _lib.check(rc, "evict_rows")
 
