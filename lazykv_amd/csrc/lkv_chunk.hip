@@ -180,6 +180,8 @@ __device__ __forceinline__ void add_not_finite(uint4 v, uint4 attended, ACC& o, 
 }
 
 // ---- few rows: every wave on its own stream of tokens, straight from memory to registers -----------------
+// Bound by memory, where there are enough rows: a token of each of sixteen sequences of up to 8,192 rows (8 heads, d 128, 268 MB) takes 41 us, 6.5 TB/s, and 6 more to join
+// the parts; one token over 131,072 rows 104 us.
 
 // The two halves of a wave's tile of 32 rows, each in one page; a half that is not there reads the other's rows, or the pool's first.
 template <int D, bool MX> struct Halves {
@@ -385,6 +387,9 @@ __global__ __launch_bounds__(64 * kWaves, NR == 2 && D == 128 ? 1 : 2) void chun
 // each, on v_mfma_f32_32x32x16: S^T [32 tokens x 32 rows] = K Q^T, O^T [d x 32] += V^T P^T. A lane holds column lane % 32, of tokens
 // 8 (i / 4) + 4 (lane / 32) + i % 4 in register i; the second product's k-th step of 16 tokens takes registers 8 k .. 8 k + 7 as they are. Pieces of 16
 // bytes are swizzled by the row, so that both the keys' 32 rows and the values' transposed reads of four rows spread over all banks.
+// Bound by issue: a product of 32 x 32 x 16 holds the matrix unit for 32 cycles, and the scores behind it cost, at 128 channels, some five vector operations and an exponential,
+// 35 cycles, which two waves of a SIMD hide for two thirds (44.5 for both). 2,048 tokens behind 32,768 (32 heads on 8, d 128) take 1,110 to 1,170 us,
+// 1.0 PFLOP/s, the matrix units busy for 47% of the cycles; at 64 channels the vector operations are as long as the products twice over: 4,099 tokens 100 us, 0.69 PFLOP/s.
 template <int DT> struct Wide;
 template <> struct Wide<LKV_BF16> {
   static __device__ __forceinline__ f32x16 mma(uint4 a, uint4 b, f32x16 c) {
@@ -619,6 +624,7 @@ __device__ __forceinline__ void cut_tile(const LdsPointer (&key_at)[D / 16], con
 }
 
 template <int DT, int D, bool MX>
+// Three waves a SIMD where the registers allow it without spills: 4,099 tokens, 32 query heads on 8, d 64, 118 us a launch and by two 131; 512 behind 8,192 78 and 76.
 __global__ __launch_bounds__(64 * kWaves, D == 64 && !MX ? 3 : 2) void chunk_wide_kernel(ChunkArgs a) {
   using S = StageLoad<DT, D, MX>;
   constexpr int ROWS = 32 * kWaves;
@@ -829,9 +835,13 @@ struct Plan {
 Plan plan_of(const lkv_chunk_desc* d) {
   Plan p = {};
   const int64_t rows = (int64_t)d->new_tokens * (d->n_q / d->n_kv);
+  // Few rows from memory, more through LDS (8 heads, d 128): 16 over 32,768 rows 34.4 us, as a wave's two tiles 36.2, through LDS 44.2; 32 over 32,768 36.4 and
+  // 44.8, over 4,096 18.2 and 20.4.
   p.nr = rows <= 16 ? 1 : rows <= 32 ? 2 : 0;
   p.tiles = ceil_div(rows, p.nr ? 16 * p.nr : 32 * kWaves);
-  // Workgroups for about as many parts as run at once, two a CU, one where its registers or an even division allow no more; none shorter than 256 rows on average.
+  // Workgroups for about as many parts as run at once, two a CU, one where its registers or an even division allow no more; none shorter than 128 rows on average (one token over
+  // 1,000: 11.4 us, by 256 12.5) or 256 through LDS (40 over 2,040: 22.5, by 128 23.7), and 512 rows are not divided (one token over 300: 9.4 and 11.0, sixteen sequences of 500 12.3 and
+  // 15.5; over 700 divided 11.3 and 13.8).
   // One token over 131,072 rows (d 128): 104 us by 256, 116 by 512; 8 tokens (two tiles of 16 rows a wave, one workgroup a CU) over 16,419 26 and 33;
   // sixteen sequences of up to 8,192 71 and 57; 203 tokens over 32,971 199 and 152, by 768 164.
   // Of many parts a sequence, no more than that; of few, those that are not whole come on top. On top, sixteen sequences' steps cost 60.8 us for 57.3 and four questions
@@ -840,11 +850,11 @@ Plan plan_of(const lkv_chunk_desc* d) {
   // More than 256 sequences fill the device, and the division would be looked for too long.
   const int64_t units = (int64_t)d->n_kv * p.tiles, room = p.nr && (d->n_seqs == 1 || (p.nr == 2 && d->head_dim == 128)) ? 256 : 512;
   int64_t share = units > 0 ? room / units : 1;
-  const int64_t longest = d->n_seqs * (int64_t)ceil_div(d->max_tokens, 256);
+  const int64_t longest = d->n_seqs * (int64_t)ceil_div(d->max_tokens, p.nr ? 128 : 256);
   share = share > longest ? longest : share;
   int64_t most = share >= (p.nr ? 2 : 4) * (int64_t)d->n_seqs ? share : d->n_seqs + share - 1;
   most = most > longest ? longest : most;
-  const bool divided = share > 1 && most > d->n_seqs && d->n_seqs <= 256;
+  const bool divided = share > 1 && d->max_tokens > 512 && most > d->n_seqs && d->n_seqs <= 256;
   p.unit = p.nr ? 7 : 6;  // a round of the workgroup
   if (d->n_seqs * (((int64_t)d->max_tokens >> p.unit) + 1) >= 1LL << 31) p.unit = 12;
   p.share = divided ? (int)share : 0;
