@@ -214,6 +214,48 @@ def test_pages_that_sequences_share_and_repeat(t: int) -> None:
     check(got, q, cache, lens, [t, t], 0.125)
 
 
+@pytest.mark.parametrize(("t", "n"), [(4, 40), (4, 3000), (60, 200), (60, 3000)])
+def test_tokens_behind_a_count_show_nothing_of_their_queries(t: int, n: int) -> None:
+    """Few rows and many, in one part and in several; under inference mode too."""
+    from lazykv_amd import kernels
+
+    gen = torch.Generator().manual_seed(t + n)
+    q = normal(gen, (2, 8, t, 64), "f16").cuda()
+    cache = Cache(gen, 2, 2, n, 64, "f16", page=16)
+    kw = dict(scale=0.1, lengths=int32([n, n]), counts=int32([t // 2, 0]), max_tokens=n, pages=cache.pages)
+    want = kernels.chunk_attend(q, cache.rows, **kw)
+    q[0, :, t // 2 :], q[1] = float("nan"), float("inf")
+    with torch.inference_mode():
+        out, lse = kernels.chunk_attend(q, cache.rows, **kw)
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+        assert torch.all(out[0, :, t // 2 :] == 0) and torch.all(out[1] == 0) and torch.all(lse[0, :, t // 2 :] == -math.inf) and torch.all(lse[1] == -math.inf)
+        sums = kernels.weigh_rows(q, lse, cache.rows, **kw)
+        assert sums.isfinite().all() and torch.all(sums[1] == 0)
+        turned = kernels.rotate_append(cache.rows, q, *(normal(gen, (2, 2, t, 64), "f16").cuda() for _ in range(2)), starts=int32([0, n - t]), pages=cache.pages)
+        assert turned.is_inference() and torch.equal(turned[0, :, : t // 2], q[0, :, : t // 2])
+
+
+def test_queries_that_lie_past_32_bits() -> None:
+    from lazykv_amd import kernels
+
+    gen = torch.Generator().manual_seed(18)
+    far = (1 << 31) + 64
+    base, other = (torch.empty(far + 4096 * 8, dtype=torch.float16, device="cuda") for _ in range(2))
+    cache = Cache(gen, 2, 2, 200, 64, "f16", page=16)
+    for t in (2, 40):
+        near = normal(gen, (2, 4, t, 64), "f16").cuda()
+        q = base.as_strided((2, 4, t, 64), (far, 64 * t, 64, 1))
+        q.copy_(near)
+        kw = dict(scale=0.1, tokens=200, pages=cache.pages)
+        got, want = (kernels.chunk_attend(x, cache.rows, **kw) for x in (q, near))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        sums = [kernels.weigh_rows(x, want[1], cache.rows, **kw) for x in (q, near)]
+        assert torch.equal(*sums)
+        k = normal(gen, (2, 2, t, 64), "f16").cuda()
+        out = other.as_strided((2, 4, t, 64), (far, 64 * t, 64, 1))
+        assert torch.equal(kernels.rotate_append(cache.rows, q, k, k, start=0, pages=cache.pages, out=out), near)
+
+
 def test_results_repeat_to_the_bit() -> None:
     from lazykv_amd import kernels
 
