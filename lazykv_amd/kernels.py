@@ -715,12 +715,8 @@ def _launch(index: int, fn, *args: object) -> int:  # noqa: ANN001
 _CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
-def _raw_stream(index: int) -> int:
-    """The current stream of a device as an integer, without an object for it where torch offers that."""
-    return _GET_RAW_STREAM(index) if _GET_RAW_STREAM is not None else torch.cuda.current_stream(index).cuda_stream
-
-
-_GET_RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+# The current stream of a device as an integer, without an object for it where torch offers that.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _meant(shape: tuple, strides: tuple) -> tuple:
@@ -1000,41 +996,44 @@ def rotate_append(
     _int32("start", start)
     rotary = table_stride = 0
     table = weight = dst.model_code
-    read = [q, k, v]  # what the call reads
+    read = (q, k, v)  # what the call reads
     cos_at = sin_at = q_at = k_at = None
     if cos is not None and sin is not None:
         cs = cos.shape
-        if len(cs) != 3 or cs[0] not in (1, seqs) or cs[1] != n or sin.shape != cs or cos.dtype != sin.dtype or (cos.dtype != dtype and cos.dtype != torch.float32):
+        kind = cos.dtype
+        if len(cs) != 3 or (cs[0] != 1 and cs[0] != seqs) or cs[1] != n or sin.shape != cs or sin.dtype != kind or (kind != dtype and kind != torch.float32):
             raise ValueError(f"cos/sin must be {dtype} or float32 [{seqs} or 1, {n}, r], got {cos.dtype} {tuple(cs)} / {sin.dtype} {tuple(sin.shape)}")
         if cos.get_device() != index or sin.get_device() != index:
             raise ValueError(f"cos/sin on {cos.device} / {sin.device}, the cache on {dst.device}")
         rotary = cs[2]
-        read += (cos, sin)
-        (cos, cos_at), (sin, sin_at) = _whole(cos), _whole(sin)
+        read = (q, k, v, cos, sin)
+        cos_at, sin_at = cos.data_ptr(), sin.data_ptr()
+        if (cos_at | sin_at) & 15 or not (cos.is_contiguous() and sin.is_contiguous()):
+            cos, sin = _whole(cos), _whole(sin)
+            cos_at, sin_at = cos.data_ptr(), sin.data_ptr()
         if cs[0] != 1:
             table_stride = n * rotary
-        if cos.dtype != dtype:
+        if kind != dtype:
             table = _lib.F32
     elif cos is not None or sin is not None:
         raise ValueError("cos and sin come together")
     if q_weight is not None or k_weight is not None:
-        kind = None
+        kind = (k_weight if q_weight is None else q_weight).dtype
         for w in (q_weight, k_weight):
             if w is not None:
-                mine = w.dtype
-                if w.shape != (d,) or (mine != dtype and mine != torch.float32) or w.get_device() != index:
-                    raise ValueError(f"weights must be {dtype} or float32 [{d}] on {dst.device}, got {mine} {tuple(w.shape)} on {w.device}")
-                if kind is not None and mine != kind:
-                    raise ValueError(f"weights of {kind} and {mine}")
-                kind = mine
-                read.append(w)
+                if w.shape != (d,) or w.dtype != kind or (kind != dtype and kind != torch.float32) or w.get_device() != index:
+                    raise ValueError(f"weights must be {dtype} or float32, both the same, [{d}] on {dst.device}, got {w.dtype} {tuple(w.shape)} on {w.device}")
+                read += (w,)
         if kind != dtype:
             weight = _lib.F32
         if q_weight is not None:
-            q_weight, q_at = _whole(q_weight)
+            q_weight = _whole(q_weight)
+            q_at = q_weight.data_ptr()
         if k_weight is not None:
-            k_weight, k_at = _whole(k_weight)
-    _no_gradients("rotate_append", (*read, *dst.owners) if out is None else (*read, *dst.owners, out))
+            k_weight = _whole(k_weight)
+            k_at = k_weight.data_ptr()
+    if _GRAD_ENABLED() or _forward_level() >= 0:
+        _no_gradients("rotate_append", (*read, *dst.owners) if out is None else (*read, *dst.owners, out))
     at, count = _counts(starts, seqs, index, "starts"), _counts(counts, seqs, index, "counts")
     table_ref, _ = _paged(dst, pages, seqs)
     if out is not None:
@@ -1073,13 +1072,9 @@ def rotate_append(
     return out
 
 
-def _whole(x: torch.Tensor) -> tuple[torch.Tensor, int]:
-    """`x` as the kernels read tables, contiguous and on 16 bytes, and where it is."""
-    at = x.data_ptr()
-    if at % 16 or not x.is_contiguous():
-        x = x.clone(memory_format=torch.contiguous_format)
-        at = x.data_ptr()
-    return x, at
+def _whole(x: torch.Tensor) -> torch.Tensor:
+    """`x` as the kernels read tables: contiguous, on 16 bytes."""
+    return x if x.is_contiguous() and x.data_ptr() % 16 == 0 else x.clone(memory_format=torch.contiguous_format)
 
 
 def _chunk(what: str, q: torch.Tensor, rows: Rows, scale: float, tokens: int, lengths: torch.Tensor | None, counts: torch.Tensor | None, max_tokens: int | None,
@@ -1091,7 +1086,8 @@ def _chunk(what: str, q: torch.Tensor, rows: Rows, scale: float, tokens: int, le
         raise ValueError(f"query {tuple(shape)} {q.dtype} on {q.device} does not match {rows.model_dtype} rows of {rows.n_kv} heads and head_dim {rows.head_dim} on "
                          f"{rows.device}")
     seqs, n_q, n, d = shape
-    _no_gradients(what, (q, *rows.owners, *others))
+    if _GRAD_ENABLED() or _forward_level() >= 0:
+        _no_gradients(what, (q, *rows.owners, *others))
     table, room = _paged(rows, pages, seqs)
     if max_tokens is None:
         max_tokens = tokens if lengths is None else room
@@ -1168,17 +1164,18 @@ def chunk_attend(
     return out, lse
 
 
-def _account(name: str, x: torch.Tensor, dtype: torch.dtype, seqs: int, n_kv: int, n: int, device: int) -> object:
-    """The strides of a number for each row, `[seqs, h, n or more]`, of which no two share an address."""
+def _account(name: str, x: torch.Tensor, dtype: torch.dtype, seqs: int, n_kv: int, n: int, device: int) -> tuple[object, tuple[int, int]]:
+    """(strides, the addresses between which it lies) of a number for each row, `[seqs, h, n or more]`, of which no two share an address."""
     shape, st = x.shape, x.stride()
     if len(shape) != 3 or shape[0] != seqs or shape[1] != n_kv or shape[2] < n or x.dtype != dtype or x.get_device() != device or (st[2] != 1 and shape[2] > 1):
         raise ValueError(f"{name} must be {dtype} [{seqs}, {n_kv}, {n} or more] with contiguous rows on cuda:{device}, got {x.dtype} {tuple(shape)} on {x.device}")
     if x.is_contiguous():
-        return _lib.Pair(st[0], st[1])
+        at = x.data_ptr()
+        return _lib.Pair(st[0], st[1]), (at, at + x.nbytes)
     a, b, n = (st[0] if seqs > 1 else 0), (st[1] if n_kv > 1 else 0), shape[2]
     if (a and b and min(a, b) < n) or (n_kv > 1 and b < n) or (seqs > 1 and a < n) or (a > b > 0 and a < b * (n_kv - 1) + n) or (0 < a <= b and b < a * (seqs - 1) + n):
         raise ValueError(f"{name}'s rows share addresses")
-    return _lib.Pair(a, b)
+    return _lib.Pair(a, b), _reach(x)
 
 
 def _same_or_apart(what: str, out: torch.Tensor, x: torch.Tensor, at: tuple[int, int], x_at: tuple[int, int]) -> None:
@@ -1218,23 +1215,21 @@ def weigh_rows(
         raise ValueError(f"lse must be contiguous float32 {tuple(q.shape[:3])} on {rows.device}")
     if out is None:
         out = sums if sums is not None else torch.zeros((seqs, rows.n_kv, most), dtype=torch.float32, device=q.device)
-    sums_st = None if sums is None else _account("sums", sums, torch.float32, seqs, rows.n_kv, most, index)
-    out_st = _account("out", out, torch.float32, seqs, rows.n_kv, most, index)
-    positions_st = None if positions is None else _account("positions", positions, torch.int32, seqs, rows.n_kv, most, index)
-    first = _counts(seen, seqs, index, "seen")
-    if seen is not None and positions is None:
-        raise ValueError("seen says where positions start; there are none")
-    out_at = _reach(out)
-    inputs = (_reach(q), _reach(lse), *_row_spans(rows))
-    if sums is not None and sums is not out:
-        sums_at = _reach(sums)
+    h, of = rows.n_kv, torch.float32
+    out_st, out_at = _account("sums" if out is sums else "out", out, of, seqs, h, most, index)
+    if sums is None or sums is out:
+        sums_st, sums_at = (None if sums is None else out_st), out_at
+    else:
+        sums_st, sums_at = _account("sums", sums, of, seqs, h, most, index)
         _same_or_apart("sums and out", out, sums, out_at, sums_at)
-    else:
-        sums_at = out_at
     if positions is None:
-        written, mine = (out,), (out_at,)
+        if seen is not None:
+            raise ValueError("seen says where positions start; there are none")
+        positions_st, written, mine, first = None, (out,), (out_at,), None
     else:
-        written, mine = (out, positions), (out_at, _reach(positions))
+        positions_st, positions_at = _account("positions", positions, torch.int32, seqs, h, most, index)
+        written, mine, first = (out, positions), (out_at, positions_at), _counts(seen, seqs, index, "seen")
+    inputs = (_reach(q), _reach(lse), *_row_spans(rows))
     if _meet(mine, inputs) or (positions is not None and _meet(mine[1:], (out_at, sums_at))):
         raise ValueError("out and positions must not lie among the inputs or each other")
     if seqs == 0 or most == 0:
@@ -1244,8 +1239,7 @@ def weigh_rows(
     ref = ctypes.byref(desc)
     ws_ptr, ws_n, _held = _scratch(lib.lkv_weigh_rows_workspace_bytes(ref), ws, q)
     rc = _launch(index, lib.lkv_weigh_rows, ref, q.data_ptr() or lse.data_ptr() or out.data_ptr(), rows.model_code, lse.data_ptr() or out.data_ptr(), rows.ref, table, at, count,
-                 None if sums is None else sums.data_ptr(), sums_st, out.data_ptr(), out_st, None if positions is None else positions.data_ptr(), positions_st, first,
-                 ws_ptr, ws_n)
+                 None if sums is None else sums_at[0], sums_st, out_at[0], out_st, None if positions is None else positions_at[0], positions_st, first, ws_ptr, ws_n)
     if rc:
         _lib.check(rc, "weigh_rows")
     return out
@@ -1283,22 +1277,21 @@ def evict_rows(
         raise ValueError(f"tokens={tokens} exceed max_tokens={max_tokens}")
     at = _counts(lengths, seqs, index, "lengths")
     h, least = rows.n_kv, max(0, max_tokens)
-    sums_st, positions_st = _account("sums", sums, torch.float32, seqs, h, least, index), _account("positions", positions, torch.int32, seqs, h, least, index)
-    spots = _reach(sums), _reach(positions)
+    sums_st, sums_at = _account("sums", sums, torch.float32, seqs, h, least, index)
+    positions_st, positions_at = _account("positions", positions, torch.int32, seqs, h, least, index)
     if out is None:
-        to_sums, to_positions, to_sums_st, to_positions_st, ends = sums, positions, sums_st, positions_st, ()
+        to_sums, to_positions, to_sums_st, to_positions_st, to_sums_at, to_positions_at = sums, positions, sums_st, positions_st, sums_at, positions_at
     else:
         to_sums, to_positions = out
         left = min(least, max(0, keep))
-        to_sums_st = _account("out's sums", to_sums, torch.float32, seqs, h, left, index)
-        to_positions_st = _account("out's positions", to_positions, torch.int32, seqs, h, left, index)
-        ends = _reach(to_sums), _reach(to_positions)
-        _same_or_apart("sums", to_sums, sums, ends[0], spots[0])
-        _same_or_apart("positions", to_positions, positions, ends[1], spots[1])
-        if _meet(ends[:1], (ends[1], spots[1])) or _meet(ends[1:], spots[:1]):
-            raise ValueError("sums and positions share addresses")
-    _no_gradients("evict_rows", (*rows.owners, sums, positions) if out is None else (*rows.owners, sums, positions, to_sums, to_positions))
-    if _meet(spots[:1], spots[1:]) or (rows.span is not None and _meet((*spots, *ends), _row_spans(rows))):
+        to_sums_st, to_sums_at = _account("out's sums", to_sums, torch.float32, seqs, h, left, index)
+        to_positions_st, to_positions_at = _account("out's positions", to_positions, torch.int32, seqs, h, left, index)
+        _same_or_apart("sums", to_sums, sums, to_sums_at, sums_at)
+        _same_or_apart("positions", to_positions, positions, to_positions_at, positions_at)
+    if _GRAD_ENABLED() or _forward_level() >= 0:
+        _no_gradients("evict_rows", (*rows.owners, sums, positions, to_sums, to_positions))
+    both = (sums_at, to_sums_at)
+    if _meet(both, (positions_at, to_positions_at)) or (rows.span is not None and _meet((*both, positions_at, to_positions_at), _row_spans(rows))):
         raise ValueError("sums, positions and rows share addresses")
     if seqs == 0 or max_tokens == 0:
         return
@@ -1307,8 +1300,8 @@ def evict_rows(
     ref = ctypes.byref(desc)
     ws_ptr, ws_n, _held = _scratch(max(16, lib.lkv_evict_rows_workspace_bytes(ref)), ws, sums)
     _WRITTEN((*rows.owners, to_sums, to_positions))
-    rc = _launch(index, lib.lkv_evict_rows, ref, rows.ref, table, at, sums.data_ptr(), sums_st, positions.data_ptr(), positions_st, to_sums.data_ptr(), to_sums_st,
-                 to_positions.data_ptr(), to_positions_st, ws_ptr, ws_n)
+    rc = _launch(index, lib.lkv_evict_rows, ref, rows.ref, table, at, sums_at[0], sums_st, positions_at[0], positions_st, to_sums_at[0], to_sums_st, to_positions_at[0],
+                 to_positions_st, ws_ptr, ws_n)
     if rc:
         _lib.check(rc, "evict_rows")
 
