@@ -391,7 +391,8 @@ int lkv_rotate_append(uintptr_t stream, const lkv_rotate_desc* desc, const void*
  * 0 .. max_tokens), the last n = counts[b] (counts NULL: new_tokens; limited to 0 .. new_tokens) of them the call's own. Its token t
  * attends rows 0 .. len - n + t. q [n_seqs, n_q, new_tokens, head_dim] with strides; out [n_seqs, n_q, new_tokens, head_dim] (out_dtype) and
  * lse [n_seqs, n_q, new_tokens] (float32, natural log) contiguous. Tokens from n on and tokens without any row get zeros and -inf. What rows hold that a token
- * does not attend does not reach it, NaN or not. The launch depends on max_tokens and new_tokens, not on what is on the device. */
+ * does not attend does not reach it, NaN or not. Softmax weights are rounded to q_dtype for the product with the values and nothing else is before
+ * out: with out in float32 an output is off by about half a step of q_dtype. The launch depends on max_tokens and new_tokens, not on what is on the device. */
 typedef struct lkv_chunk_desc {
   int32_t n_seqs, n_q, n_kv, head_dim, new_tokens;
   float scale; /* positive */

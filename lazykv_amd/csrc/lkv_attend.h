@@ -335,7 +335,10 @@ __device__ __forceinline__ void settle(f32x4 (&sc)[NR][2], int left, float scale
   }
 }
 
-// Settled scores to weights, the second product's operand.
+// Settled scores to weights, the second product's operand: in the model dtype, as the matrix units take them at the full rate. Each is then off by half a
+// step of it at the most, and independently of the others, so that an output of many rows is off by about as much again as its own rounding makes it: relative to
+// 64 bits (root mean square, normal scores and values) 0.0017 by that rounding and 0.0022 by both in bfloat16, 0.00021 and 0.00027 in float16. Their sum is of the weights
+// before they are rounded, in float32; of the rounded ones it would change no digit of these.
 template <int DT, int NR>
 __device__ __forceinline__ uint4 weights(const f32x4 (&sc)[2], float scale2, float& l) {
   float w[8];

@@ -2,7 +2,9 @@
 //
 // Token t of a sequence's n new ones, of len rows in all, attends rows 0 .. len - n + t:
 //   s_i = scale * q . k_i,  m = max s_i,  out = sum exp(s_i - m) v_i / sum exp(s_i - m),  lse = m + ln sum exp(s_i - m),
-// in one pass over the rows, base 2, as in the batch decode (lkv_shared.hip), whose rounding of weights and lift in float16 it has too.
+// in one pass over the rows, base 2, as in the batch decode (lkv_shared.hip), whose rounding of weights and lift in float16 it has too. Scores, exponents, sums and partial
+// results are float32; the weights' rounding to the model dtype shows beside the output's own: against 64 bits 0.0022 for 0.0017 where many rows have weight (bfloat16,
+// 2,048 tokens behind 32,768), 0.00024 for 0.00021 (float16, 4,099 from nothing).
 //
 // The query rows of a KV head are its g heads of every token, x = t * g + j, so that a tile of them spans few tokens: the rows
 // that some of them attend and others do not are few.
@@ -525,7 +527,7 @@ __device__ __forceinline__ float largest(const f32x16& s) {
   for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
   return top;
 }
-// Scores to weights: the second product's two operands.
+// Scores to weights: the second product's two operands, rounded as `weights` does it.
 template <int DT>
 __device__ __forceinline__ void wide_weights(const f32x16& s, float scale2, float less, float& l, uint4 (&p)[2]) {
 #pragma unroll

@@ -1135,7 +1135,7 @@ def chunk_attend(
     0 .. len - counts[b] + t. `rows` are the sequences' own or, with `pages` `[seqs, n]`, a pool's pages, in the model dtype or in 8 bits; T = 1 is a
     decode step. Returns (out [seqs, n_q, T, d], lse [seqs, n_q, T] float32, natural log); tokens from `counts[b]` on and tokens without any row get zeros
     and -inf. No gradient: inputs that autograd follows are refused. Without `ws` the scratch is torch's, so calls on several streams and in
-    several graphs do not meet."""
+    several graphs do not meet. Weights are rounded to the model dtype for the product with the values, as the batch decode's are; all else is float32 up to `out`."""
     given = () if out is None and lse is None else tuple(x for x in (out, lse) if x is not None)
     desc, q, at, count, table, _ = _chunk("chunk_attend", q, rows, scale, tokens, lengths, counts, max_tokens, pages, given)
     shape, index = q.shape, rows.device_index
