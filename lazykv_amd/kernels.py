@@ -1049,6 +1049,9 @@ def rotate_append(
     else:
         out = torch.empty_like(q)
         ot = out.stride()
+        if ot[3] != 1 or (ot[0] | ot[1] | ot[2]) & 7:  # laid out as queries that the kernel does not read where they are
+            out = q.new_empty(shape)
+            ot = out.stride()
     if 0 in shape:
         return out
     qt, kt, vt = q.stride(), k.stride(), v.stride()

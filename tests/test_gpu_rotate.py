@@ -204,3 +204,24 @@ def test_what_is_refused() -> None:
     with pytest.raises(RuntimeError, match="no gradient"):
         kernels.rotate_append(cache.rows, q.clone().requires_grad_(), k, k, **kw)
     assert kernels.rotate_append(cache.rows, q[:, :, :0], k[:, :, :0], k[:, :, :0], **kw).shape == (2, 4, 0, 64)
+
+
+@pytest.mark.parametrize("out_of", ["channels", "heads", "tokens of one"])
+def test_queries_however_they_lie(out_of: str) -> None:
+    """Queries whose channels are not innermost, or whose single token's stride is no multiple of 8: as contiguous ones, to the bit."""
+    from lazykv_amd import kernels
+
+    gen = torch.Generator().manual_seed(11)
+    t = 1 if out_of == "tokens of one" else 8
+    q, k = normal(gen, (2, 4, t, 64), "bf16").cuda(), normal(gen, (2, 2, t, 64), "bf16").cuda()
+    if out_of == "channels":
+        x = q.transpose(2, 3).contiguous().transpose(2, 3)
+    elif out_of == "heads":
+        x = q.contiguous(memory_format=torch.channels_last)
+    else:
+        x = q.as_strided(q.shape, (256, 64, 3, 1))
+    assert torch.equal(x, q) and (x.stride(3) != 1 or x.stride(2) == 3)
+    cos, sin = (y.cuda() for y in tables(torch.arange(t)[None], 64, torch.bfloat16))
+    stores = [torch.zeros((2, 2, 2, t, 64), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    got, want = (kernels.rotate_append(kernels.dense_rows(s[0], s[1]), y, k, k, cos=cos, sin=sin) for s, y in zip(stores, (x, q)))
+    assert torch.equal(got, want) and torch.equal(*stores)
