@@ -989,6 +989,8 @@ def rotate_append(
                          f"{tuple(v.shape)} {v.dtype}")
     seqs, n_q, n, d = shape
     h = kv[1]
+    if n_q == 0:
+        raise ValueError(f"queries without heads: {tuple(shape)}")
     if h != dst.n_kv or d != dst.head_dim:
         raise ValueError(f"keys/values {tuple(kv)} do not match rows of {dst.n_kv} heads and head_dim {dst.head_dim}")
     if q.get_device() != index or k.get_device() != index or v.get_device() != index:

@@ -152,3 +152,25 @@ def test_tensors_on_the_host_are_refused() -> None:
 
     with pytest.raises(RuntimeError, match="no CPU path"):
         kernels.evict_rows(None, torch.zeros((1, 1, 8)), torch.zeros((1, 1, 8), dtype=torch.int32), keep=4, tokens=8)
+
+
+@pytest.fixture
+def kernels(monkeypatch: pytest.MonkeyPatch):  # noqa: ANN201
+    """The calls' checks over tensors on the host. Nothing is launched: a call that comes so far fails the test."""
+    from lazykv_amd import _lib, kernels
+
+    monkeypatch.setattr(_lib, "require_cuda", lambda *_: None)
+    monkeypatch.setattr(kernels, "_launch", lambda _, fn, *args: pytest.fail(f"{fn} was launched"))
+    return kernels
+
+
+def test_queries_without_heads_are_refused(kernels) -> None:  # noqa: ANN001
+    """Their keys and values would be new rows: returning without them would lose them."""
+    import torch
+
+    rows = kernels.dense_rows(*torch.zeros((2, 2, 2, 16, 64), dtype=torch.bfloat16))
+    q, k = torch.zeros((2, 0, 3, 64), dtype=torch.bfloat16), torch.zeros((2, 2, 3, 64), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="without heads"):
+        kernels.rotate_append(rows, q, k, k)
+    with pytest.raises(ValueError, match="does not match"):
+        kernels.chunk_attend(q, rows, scale=0.1, tokens=9)
