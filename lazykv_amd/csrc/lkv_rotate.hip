@@ -102,7 +102,11 @@ __global__ __launch_bounds__(kHeads * D / 8) void rotate_append_kernel(RotateArg
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(y[i], y[i], sum);
-        inverse = __builtin_amdgcn_rsqf(lkv::row_sum<LPR>(sum) * (1.0f / D) + a.d.eps);
+        // The reciprocal root takes a subnormal number for 0: such a mean square (without eps, of bfloat16 values below 2^-63) is taken times 2^48.
+        const float mean = lkv::row_sum<LPR>(sum) * (1.0f / D) + a.d.eps;
+        const bool tiny = mean < FLT_MIN;
+        inverse = __builtin_amdgcn_rsqf(tiny ? mean * 0x1p48f : mean);
+        inverse = tiny ? inverse * 0x1p24f : inverse;
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] = __builtin_fmaf(y[i], is_q ? qa[i] : ka[i], z[i] * (is_q ? qb[i] : kb[i])) * inverse;
@@ -143,7 +147,7 @@ extern "C" int lkv_rotate_append(uintptr_t stream, const lkv_rotate_desc* desc, 
   LKV_CHECK_ARG(d.rotary == 0 || (cos && sin), "a rotation without its tables");
   LKV_CHECK_ARG(d.rotary == 0 || d.table_dtype == d.dtype || d.table_dtype == LKV_F32, "tables of dtype %d", d.table_dtype);
   LKV_CHECK_ARG((!q_weight && !k_weight) || d.weight_dtype == d.dtype || d.weight_dtype == LKV_F32, "weights of dtype %d", d.weight_dtype);
-  // The reciprocal root takes a subnormal number for 0.
+  // Few bits would be left of a subnormal eps.
   LKV_CHECK_ARG((d.eps == 0.0f || d.eps >= FLT_MIN) && d.eps < INFINITY, "eps %g: 0 or a normal number", (double)d.eps);
   uintptr_t all = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out | (uintptr_t)q_weight | (uintptr_t)k_weight;
   if (d.rotary) all |= (uintptr_t)cos | (uintptr_t)sin;

@@ -225,3 +225,18 @@ def test_queries_however_they_lie(out_of: str) -> None:
     stores = [torch.zeros((2, 2, 2, t, 64), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
     got, want = (kernels.rotate_append(kernels.dense_rows(s[0], s[1]), y, k, k, cos=cos, sin=sin) for s, y in zip(stores, (x, q)))
     assert torch.equal(got, want) and torch.equal(*stores)
+
+
+def test_norms_without_eps_of_values_whose_squares_are_subnormal() -> None:
+    """Squares of 1e-19 and less lie below float32's normal range, down to 2^-149: with a square of m steps of that, in float32, a mean is off by one step in m (half a step a
+    square, half of the division), its root by half of that: 2^-7 at 3e-22 (m = 64), and bfloat16 rounds by 2^-8. Heads of zeros give 0 / 0."""
+    from lazykv_amd import kernels
+
+    sizes = (2.0**-62, 2.0**-63, 1e-19, 1e-20, 1e-21, 3e-22)
+    x = torch.stack([torch.where(torch.arange(64) % 3 == 0, -s, s) for s in sizes] + [torch.zeros(64)]).bfloat16().cuda().expand(1, 2, 7, 64).contiguous()
+    w = torch.full((64,), 1.5, device="cuda")
+    store = torch.empty((2, 1, 2, 7, 64), dtype=torch.bfloat16, device="cuda")
+    q = kernels.rotate_append(kernels.dense_rows(store[0], store[1]), x, x, x, q_weight=w, k_weight=w, eps=0.0)
+    want = 1.5 * x[:, :, :6].sign().float()
+    assert torch.all((q[:, :, :6].float() - want).abs() <= 1.5 * (2.0**-8 + 2.0**-7)) and q[:, :, 6].isnan().all()
+    assert torch.equal(store[0][:, :, :6], q[:, :, :6])
