@@ -405,7 +405,7 @@ int lkv_chunk_attend(uintptr_t stream, const lkv_chunk_desc* desc, const void* q
 
 /* The weights that rows get from a chunk's tokens, summed up: with lse [n_seqs, n_q, new_tokens] as lkv_chunk_attend gives it, row i of KV
  * head h of sequence b gets  sum over the head's query heads and the tokens that attend i of  exp(scale q . k_i - lse), added
- * to sums for rows from before the chunk and by itself for the chunk's own, into out; a token whose lse is -inf adds nothing. 1 / scale must be finite. sums (NULL: 0) and
+ * to sums for rows from before the chunk and by itself for the chunk's own, into out; a token whose lse is -inf adds nothing. scale must be 2^-120 or more. sums (NULL: 0) and
  * out are float32, element (b, h, i) at b * sums_stride[0] + h * sums_stride[1] + i; they may be the same; rows from len on are left as they are.
  * positions (int32, laid out the same; may be NULL) of the chunk's own rows are set to seen[b] + their place in it (seen NULL:
  * len - n, the rows before). */

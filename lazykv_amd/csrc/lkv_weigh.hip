@@ -415,7 +415,9 @@ extern "C" int lkv_weigh_rows(uintptr_t stream, const lkv_chunk_desc* desc, cons
                               const lkv_pages* pages, const int32_t* lengths, const int32_t* counts, const float* sums, const int64_t* sums_stride, float* out,
                               const int64_t* out_stride, int32_t* positions, const int64_t* positions_stride, const int32_t* seen, void* ws, size_t ws_bytes) {
   if (int rc = lkv_check_chunk(desc)) return rc;
-  LKV_CHECK_ARG(1.0f / desc->scale < INFINITY, "scale %g: its reciprocal is not finite", (double)desc->scale);
+  // Of few query rows the scores start from -lse / scale. A weight that float32 holds, or one above, has an lse of -89 to 104 beside a score of about 0 at such scales: 104 * 2^120 is
+  // finite, and an lse beyond that gives 0 or infinity as it should.
+  LKV_CHECK_ARG(desc->scale >= 0x1p-120f, "scale %g: at least 2^-120, its reciprocal times an lse would not be finite", (double)desc->scale);
   LKV_CHECK_ARG(q && lse && out && out_stride && (!sums || sums_stride) && (!positions || positions_stride), "NULL pointer");
   LKV_CHECK_ARG(q_dtype == LKV_F16 || q_dtype == LKV_BF16, "queries are float16 or bfloat16, got dtype %d", q_dtype);
   LKV_CHECK_ARG(((uintptr_t)q & 15) == 0, "queries must start on 16 bytes");

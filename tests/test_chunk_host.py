@@ -174,3 +174,9 @@ def test_queries_without_heads_are_refused(kernels) -> None:  # noqa: ANN001
         kernels.rotate_append(rows, q, k, k)
     with pytest.raises(ValueError, match="does not match"):
         kernels.chunk_attend(q, rows, scale=0.1, tokens=9)
+
+
+@pytest.mark.parametrize("scale", [1e-39, 1e-38, 2.0**-121])
+def test_accounts_of_scales_whose_reciprocal_times_an_lse_is_not_finite_are_refused(scale: float) -> None:
+    """Few query rows' scores start from -lse / scale: at 1e-38 an lse of 4.2 (64 rows alike) is past float32's range there, and every weight would be 0."""
+    assert "reciprocal" in _call("weigh", {"desc": {"scale": scale}})

@@ -480,3 +480,23 @@ def test_a_layers_decode_over_a_bounded_cache(eight: bool) -> None:
                 left = set(places[b, j, : lens[b]].tolist())
                 assert len(left) == lens[b] and all(p in left for p in [0, 1, *range(newest - 7, newest + 1)])
                 held[b][j] = {p: s for p, s in held[b][j].items() if p in left}
+
+
+@pytest.mark.parametrize("t", [1, 40])
+def test_accounts_of_the_smallest_scale(t: int) -> None:
+    """Every row as good as the next: 1 / n of a weight from each token and head, in the few rows' form and in the other."""
+    from lazykv_amd import kernels
+
+    gen = torch.Generator().manual_seed(19)
+    n, scale = 4096, 2.0**-120
+    q = normal(gen, (1, 8, t, 64), "bf16").cuda()
+    cache = Cache(gen, 1, 2, n, 64, "bf16", page=16)
+    kw = dict(scale=scale, tokens=n, pages=cache.pages)
+    lse = kernels.chunk_attend(q, cache.rows, **kw)[1]
+    # Token t attends n - T + t + 1 rows. n u for the sum behind an lse of ln n (off by 16 u of 1 + ln n besides), 2 |lse| u of a weight, and the account's sum of 4 t of them.
+    rows = torch.arange(n - t + 1, n + 1, device="cuda").double()
+    assert torch.all((lse.double() - rows.log()).abs() <= (n + 16 * (1 + np.log(n))) * U)
+    got = kernels.weigh_rows(q, lse, cache.rows, **kw).double()
+    i = torch.arange(n, device="cuda")
+    want = torch.where(i[:, None] <= n - t + torch.arange(t, device="cuda"), 1 / rows, 0.0).sum(-1) * 4
+    assert torch.all((got - want).abs() <= (n + 18 * (1 + np.log(n)) + 4 * t + 8) * U * want)
