@@ -60,26 +60,26 @@ __device__ __forceinline__ void store_sum(const WeighArgs& a, const Extent& e, i
     a.positions[b * a.positions_stride[0] + h * a.positions_stride[1] + row] = (a.seen ? a.seen[b] : max(past, 0)) + row - past;
 }
 
+// A query row without weight, one that is not there or whose lse is -inf, attends nothing: its limit is 0. Its scores may be NaN, whatever its query is taken for, where a key
+// is not finite, so that sixteen or a stage with such a row takes the form that looks at the limits.
+
 // Sixteen query rows as the lanes hold them.
 template <int D, bool MX> struct QueryRegs {
   uint4 w[D / 32];
-  float start;  // -lse / scale; -inf for a row that is not there or attends nothing
+  float start;  // -lse / scale; -inf for a row without weight
   int limit;
   __device__ __forceinline__ void load(const WeighArgs& a, const Extent& e, int b, int h, int x) {
     const int quarter = (threadIdx.x & 63) >> 4;
     const int t = x / a.g, j = h * a.g + (x - t * a.g);
     const bool live = t < e.n;
     const int tt = live ? t : 0, jj = live ? j : h * a.g;  // the first row in the place of one that is not there
-    limit = live ? e.len - e.n + t + 1 : 0;
     const uint16_t* q = a.q + b * a.q_stride[0] + jj * a.q_stride[1] + tt * a.q_stride[2];
     const float lse = a.lse[((int64_t)b * a.n_q + jj) * a.new_tokens + tt];
-    const uint32_t keep = live && lse != -INFINITY ? ~0u : 0u;
-    start = keep ? -lse * a.per_scale : -INFINITY;
+    const bool weighs = live && lse != -INFINITY;
+    limit = weighs ? e.len - e.n + t + 1 : 0;
+    start = weighs ? -lse * a.per_scale : -INFINITY;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) {
-      const uint4 y = *(const uint4*)(q + KeyRegs<D, MX>::channel(quarter, i));
-      w[i] = make_uint4(y.x & keep, y.y & keep, y.z & keep, y.w & keep);
-    }
+    for (int i = 0; i < D / 32; ++i) w[i] = *(const uint4*)(q + KeyRegs<D, MX>::channel(quarter, i));
   }
 };
 
@@ -131,7 +131,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_rows_kernel(WeighArgs a)
 #pragma unroll
           for (int i = 0; i < D / 32; ++i) sc[u][w] = Mat<DT>::mma(now.w[i], k[u].template operand<DT>(w, i), sc[u][w]);
         }
-      if (x < x_whole) {
+      if (x < x_whole || __any(now.start == -INFINITY)) {
         int limit[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) limit[i] = __shfl(now.limit, (lane & 48) + 4 * quarter + i) - row0 - (lane & 15);
@@ -210,7 +210,7 @@ struct Walk {
 };
 
 // A stage's query rows on their way to LDS, what is added to their exponents, and how many of a sequence's rows they attend. Every wave's lane l knows row l; a
-// row's 16-byte pieces are loaded by other lanes, which ask it where it is. Rows from x_end on are the first one of the range again, without weight.
+// row's 16-byte pieces are loaded by other lanes, which ask it where it is. In the place of rows from x_end on the first one of the range lies, without weight.
 template <int D> struct StageQueries {
   static_assert(kStage == 64, "a row of the stage for each lane");
   static constexpr int PIECES = D / 8, LOADS = kStage * PIECES / (64 * kWaves);
@@ -235,7 +235,7 @@ template <int D> struct StageQueries {
     }
     const float l = a.lse[((int64_t)b * a.n_q + h * a.g + (live ? mine.j : first.j)) * a.new_tokens + (live ? mine.t : first.t)];
     less = live && l != -INFINITY ? -l * kLog2e : -INFINITY;
-    limit = e.len - e.n + mine.t + 1;
+    limit = less != -INFINITY ? e.len - e.n + mine.t + 1 : 0;
     mine.next(a);
     x += kStage;
   }
@@ -243,7 +243,7 @@ template <int D> struct StageQueries {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int y = i * 64 * kWaves + threadIdx.x, r = y / PIECES;
-      *(u32x4*)(lds + r * (2 * D) + ((y % PIECES) ^ swizzle<D>(r)) * 16) = w[i] & (__shfl(less, r) != -INFINITY ? ~0u : 0u);
+      *(u32x4*)(lds + r * (2 * D) + ((y % PIECES) ^ swizzle<D>(r)) * 16) = w[i];
     }
     if (threadIdx.x < kStage) {
       less_at[threadIdx.x] = less;
@@ -252,7 +252,7 @@ template <int D> struct StageQueries {
   }
 };
 
-// The weights of 32 staged queries for a tile of 32 keys, summed. CUT: not all of them attend all keys; `row` is the lane's.
+// The weights of 32 staged queries for a tile of 32 keys, summed. CUT: not all of them attend all keys, or have weight; `row` is the lane's.
 template <int DT, int D, bool CUT>
 __device__ __forceinline__ float tile_sum(const uint4 (&q)[D / 16], const uint4 (&k)[D / 16], const f32x4 (&less)[4], const int* limits, int row, float scale2) {
   f32x16 s;
@@ -328,11 +328,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_wide_kernel(WeighArgs a)
     stage.begin(a, b, h, x_first);
     stage.load(a, e, b, h, first, x_end);
     int buffer = 0;
-    const auto round = [&](int x, auto cut) __attribute__((always_inline)) {
-      stage.store(lds + buffer * BYTES, less_at[buffer], limit_at[buffer]);
-      __syncthreads();
-      if (x + kStage < x_end) stage.load(a, e, b, h, first, x_end);
-      load_fence();
+    const auto tiles = [&](auto cut) __attribute__((always_inline)) {
 #pragma unroll
       for (int sub = 0; sub < kStage / 32; ++sub) {
         uint4 q[D / 16];
@@ -345,11 +341,20 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_wide_kernel(WeighArgs a)
         for (int u = 0; u < 2; ++u)
           sum[u] += tile_sum<DT, D, decltype(cut)::value>(q, k[u], less, &limit_at[buffer][32 * sub + 4 * half], row0 + 32 * u + (lane & 31), a.scale2);
       }
-      buffer ^= 1;
     };
-    int x = x_first;
-    for (; x < min(x_whole, x_end); x += kStage) round(x, std::true_type());
-    for (; x < x_end; x += kStage) round(x, std::false_type());
+    for (int x = x_first; x < x_end; x += kStage) {
+      const bool cut = x < x_whole || __any(stage.less == -INFINITY);
+      stage.store(lds + buffer * BYTES, less_at[buffer], limit_at[buffer]);
+      __syncthreads();
+      if (x + kStage < x_end) stage.load(a, e, b, h, first, x_end);
+      load_fence();
+      if (cut) {
+        tiles(std::true_type());
+      } else {
+        tiles(std::false_type());
+      }
+      buffer ^= 1;
+    }
   }
   // Each half stores a tile's rows.
   const float first = pair_sum<32>(sum[0]), second = pair_sum<32>(sum[1]);

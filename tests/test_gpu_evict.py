@@ -500,3 +500,32 @@ def test_accounts_of_the_smallest_scale(t: int) -> None:
     i = torch.arange(n, device="cuda")
     want = torch.where(i[:, None] <= n - t + torch.arange(t, device="cuda"), 1 / rows, 0.0).sum(-1) * 4
     assert torch.all((got - want).abs() <= (n + 18 * (1 + np.log(n)) + 4 * t + 8) * U * want)
+
+
+@pytest.mark.parametrize(("t", "counts"), [(1, 1), (3, 3), (3, 2), (20, 20), (20, 17), (70, 70)])
+@pytest.mark.parametrize(("model", "d", "eight"), [("bf16", 128, False), ("f16", 64, False), ("f16", 64, True)])
+def test_tokens_that_add_nothing_and_lanes_without_one_show_no_key(t: int, counts: int, model: str, d: int, eight: bool) -> None:
+    """A token whose lse is -inf adds nothing to a row whose key is not finite, nor does a lane that has no token; a score of -inf is a weight of 0."""
+    from lazykv_amd import kernels
+
+    gen = torch.Generator().manual_seed(t)
+    past = 300
+    n = past + counts
+    q = normal(gen, (1, 8, t, d), model).cuda()
+    q[..., 0] = 1.0
+    cache = Cache(gen, 1, 2, n, d, model, eight=eight, page=16)
+    kw = dict(scale=0.1, lengths=int32([n]), counts=int32([counts]), max_tokens=n, pages=cache.pages)
+    lse = kernels.chunk_attend(q, cache.rows, **kw)[1]
+    lse[:, :, counts - 1] = -float("inf")
+    want = kernels.weigh_rows(q, lse, cache.rows, **kw)
+    assert want.isfinite().all() and torch.all(want[0, :, n - 1] == 0)
+    where, i = cache.place(0, n - 1)
+    if eight:  # NaN is the code 0x7f; there is no infinity
+        cache.held[0][0, where, :, i, 3] = 0x7F
+    else:
+        cache.held[0][0, where, :, i, 3] = float("nan")
+        where, i = cache.place(0, 5)
+        cache.held[0][0, where, :, i, 0] = -float("inf")
+        want[0, :, 5] = 0
+    got = kernels.weigh_rows(q, lse, cache.rows, **kw)
+    assert torch.equal(got, want), (got != want).nonzero()[:4]
