@@ -637,15 +637,19 @@ class Rows:
     """A `lkv_kv_rows`: the keys' and values' rows of `seqs` sequences, one per token, in the model dtype or in 8 bits
     (`dense_rows`, `mx_rows`). It describes the tensors it was made of and keeps them; a program may keep it."""
 
-    __slots__ = ("seqs", "n_kv", "tokens", "head_dim", "dtype", "model_dtype", "model_code", "device_index", "owners", "span", "struct", "ref")
+    __slots__ = ("seqs", "n_kv", "tokens", "head_dim", "dtype", "model_dtype", "model_code", "device_index", "owners", "spans", "struct", "ref")
 
     def __init__(self, k: int, v: int, k_scale: int | None, v_scale: int | None, strides: tuple, seqs: int, n_kv: int, tokens: int, head_dim: int,
                  dtype: int, model_dtype: torch.dtype, model_code: int, device_index: int, owners: tuple) -> None:
         self.seqs, self.n_kv, self.tokens, self.head_dim = seqs, n_kv, tokens, head_dim
         self.dtype = dtype  # _lib.F16, _lib.BF16 or _lib.MXFP8
         self.model_dtype, self.model_code, self.device_index, self.owners = model_dtype, model_code, device_index, owners
-        # Where model-dtype rows lie: the first addresses, and the bytes that they reach.
-        self.span = (k, v, 2 * ((seqs - 1) * strides[0] + (n_kv - 1) * strides[1] + tokens * head_dim)) if k_scale is None else None
+        # The addresses between which keys, values and their scales lie.
+        n = (seqs - 1) * strides[0] + (n_kv - 1) * strides[1] + tokens * head_dim
+        if k_scale is None:
+            self.spans = (k, k + 2 * n), (v, v + 2 * n)
+        else:
+            self.spans = (k, k + n), (v, v + n), (k_scale, k_scale + n // MX_GROUP), (v_scale, v_scale + n // MX_GROUP)
         self.struct = _lib.KVRows(k, v, k_scale, v_scale, *strides, tokens, seqs, dtype, model_code)
         self.ref = ctypes.byref(self.struct)
 
@@ -790,13 +794,10 @@ def append_rows(dst: Rows, keys: torch.Tensor, values: torch.Tensor, *, start: i
             x, y = torch.stack([x, y]).unbind(0)
             st = x.stride()
         at_x, at_y = x.data_ptr(), y.data_ptr()
-    if dst.span is not None:
-        k, v, span = dst.span
-        n_bytes = 2 * ((seqs - 1) * st[0] + (n_kv - 1) * st[1] + (n - 1) * st[2] + d)
-        if min(at_x, at_y) < max(k, v) + span and max(at_x, at_y) + n_bytes > min(k, v) and any(
-                a < b + span and b < a + n_bytes for a in (at_x, at_y) for b in (k, v)):
-            x, y = torch.stack([x, y]).unbind(0)  # the cache's own rows, moved: none is written before all are read
-            st, at_x, at_y = x.stride(), x.data_ptr(), y.data_ptr()
+    n_bytes = 2 * ((seqs - 1) * st[0] + (n_kv - 1) * st[1] + (n - 1) * st[2] + d)
+    if _meet(((at_x, at_x + n_bytes), (at_y, at_y + n_bytes)), dst.spans):
+        x, y = torch.stack([x, y]).unbind(0)  # the cache's own rows, moved: none is written before all are read
+        st, at_x, at_y = x.stride(), x.data_ptr(), y.data_ptr()
     _WRITTEN(dst.owners)
     rc = _launch(index, _lib.lib().lkv_append_rows, dst.ref, at_x, at_y, dst.model_code, st[0], st[1], st[2], seqs, n_kv, d, n, at, start)
     if rc:
@@ -953,14 +954,6 @@ def _meet(some: tuple, others: tuple) -> bool:
     return False
 
 
-def _row_spans(rows: Rows) -> tuple:
-    """Where the rows lie, of a cache in the model dtype."""
-    if rows.span is None:
-        return ()
-    k, v, n = rows.span
-    return (k, k + n), (v, v + n)
-
-
 def rotate_append(
     dst: Rows,
     q: torch.Tensor,
@@ -1044,7 +1037,7 @@ def rotate_append(
         ot = _meant(shape, out.stride())
         if ot[3] != 1 or (ot[0] | ot[1] | ot[2]) % 8 or out.data_ptr() % 16:
             raise ValueError("out's rows must be contiguous and start on 16 bytes")
-        if _meet((_reach(out),), (*map(_reach, read), *_row_spans(dst))):
+        if _meet((_reach(out),), (*map(_reach, read), *dst.spans)):
             raise ValueError("out must not lie among the inputs or the cache's rows")
     elif 0 in shape:
         return q.new_empty(shape)
@@ -1061,13 +1054,12 @@ def rotate_append(
     if (qt[0] | qt[1] | qt[2] | kt[0] | kt[1] | kt[2] | vt[0] | vt[1] | vt[2]) & 7 or (x | y | z) & 15 or qt[3] != 1 or kt[3] != 1 or vt[3] != 1:
         (q, qt), (k, kt), (v, vt) = _placed(q), _placed(k), _placed(v)
         x, y, z = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    if dst.span is not None:
-        mine = ((x, x + 2 * ((seqs - 1) * qt[0] + (n_q - 1) * qt[1] + (n - 1) * qt[2] + d)), (y, y + 2 * ((seqs - 1) * kt[0] + (h - 1) * kt[1] + (n - 1) * kt[2] + d)),
-                (z, z + 2 * ((seqs - 1) * vt[0] + (h - 1) * vt[1] + (n - 1) * vt[2] + d)))
-        if _meet(mine, _row_spans(dst)):  # the cache's own rows: none is written before all are read
-            q, k, v = (w.clone(memory_format=torch.contiguous_format) for w in (q, k, v))
-            qt, kt, vt = q.stride(), k.stride(), v.stride()
-            x, y, z = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    mine = ((x, x + 2 * ((seqs - 1) * qt[0] + (n_q - 1) * qt[1] + (n - 1) * qt[2] + d)), (y, y + 2 * ((seqs - 1) * kt[0] + (h - 1) * kt[1] + (n - 1) * kt[2] + d)),
+            (z, z + 2 * ((seqs - 1) * vt[0] + (h - 1) * vt[1] + (n - 1) * vt[2] + d)))
+    if _meet(mine, dst.spans):  # the cache's own rows: none is written before all are read
+        q, k, v = (w.clone(memory_format=torch.contiguous_format) for w in (q, k, v))
+        qt, kt, vt = q.stride(), k.stride(), v.stride()
+        x, y, z = q.data_ptr(), k.data_ptr(), v.data_ptr()
     _WRITTEN((*dst.owners, out))
     desc = _lib.RotateDesc(seqs, n_q, h, d, n, dst.model_code, rotary, table, weight, eps, qt[0], qt[1], qt[2], kt[0], kt[1], kt[2], vt[0], vt[1], vt[2], ot[0], ot[1], ot[2],
                            table_stride)
@@ -1156,7 +1148,7 @@ def chunk_attend(
         return out, lse
     if given:
         mine = tuple(map(_reach, given))
-        if _meet(mine, (_reach(q), *_row_spans(rows))) or (len(mine) == 2 and _meet(mine[:1], mine[1:])):
+        if _meet(mine, (_reach(q), *rows.spans)) or (len(mine) == 2 and _meet(mine[:1], mine[1:])):
             raise ValueError("out and lse must not lie among the inputs or each other")
         _WRITTEN(given)
     lib = _lib.lib()
@@ -1234,7 +1226,7 @@ def weigh_rows(
     else:
         positions_st, positions_at = _account("positions", positions, torch.int32, seqs, h, most, index)
         written, mine, first = (out, positions), (out_at, positions_at), _counts(seen, seqs, index, "seen")
-    inputs = (_reach(q), _reach(lse), *_row_spans(rows))
+    inputs = (_reach(q), _reach(lse), *rows.spans)
     if _meet(mine, inputs) or (positions is not None and _meet(mine[1:], (out_at, sums_at))):
         raise ValueError("out and positions must not lie among the inputs or each other")
     if seqs == 0 or most == 0:
@@ -1296,7 +1288,7 @@ def evict_rows(
     if _GRAD_ENABLED() or _forward_level() >= 0:
         _no_gradients("evict_rows", (*rows.owners, sums, positions, to_sums, to_positions))
     both = (sums_at, to_sums_at)
-    if _meet(both, (positions_at, to_positions_at)) or (rows.span is not None and _meet((*both, positions_at, to_positions_at), _row_spans(rows))):
+    if _meet(both, (positions_at, to_positions_at)) or _meet((*both, positions_at, to_positions_at), rows.spans):
         raise ValueError("sums, positions and rows share addresses")
     if seqs == 0 or max_tokens == 0:
         return

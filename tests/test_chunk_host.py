@@ -180,3 +180,80 @@ def test_queries_without_heads_are_refused(kernels) -> None:  # noqa: ANN001
 def test_accounts_of_scales_whose_reciprocal_times_an_lse_is_not_finite_are_refused(scale: float) -> None:
     """Few query rows' scores start from -lse / scale: at 1e-38 an lse of 4.2 (64 rows alike) is past float32's range there, and every weight would be 0."""
     assert "reciprocal" in _call("weigh", {"desc": {"scale": scale}})
+
+
+def _pool(eight: bool, n_bytes: int):  # noqa: ANN202
+    """(a buffer of bytes, (sequences, h, tokens, d), rows at its start): two sequences of two heads, 16 rows of 64 channels."""
+    import torch
+
+    from lazykv_amd import kernels
+
+    pool = torch.zeros(n_bytes, dtype=torch.uint8)
+    if eight:
+        return pool, kernels.mx_rows(pool[:8192].view(2, 2, 2, 16, 64), pool[8192:8448].view(2, 2, 2, 16, 2), torch.bfloat16)
+    return pool, kernels.dense_rows(*pool[:16384].view(torch.bfloat16).view(2, 2, 2, 16, 64))
+
+
+@pytest.mark.parametrize(("eight", "at"), [(False, 0), (False, 8192), (False, 16128), (True, 0), (True, 4096), (True, 8064), (True, 8192), (True, 8320)])
+def test_what_lies_among_a_caches_rows_is_refused(kernels, eight: bool, at: int) -> None:  # noqa: ANN001
+    """A pool of bytes cut into a cache and what calls write: what is cut from keys, values, their codes or their scales, or reaches into them, is refused."""
+    import torch
+
+    pool, rows = _pool(eight, 1 << 16)
+    cut = lambda dtype, *shape: pool[at:].view(dtype)[: torch.Size(shape).numel()].view(shape)  # noqa: E731
+    q, k = torch.zeros((2, 4, 3, 64), dtype=torch.bfloat16), torch.zeros((2, 2, 3, 64), dtype=torch.bfloat16)
+    lse, sums, positions = torch.zeros((2, 4, 3)), torch.zeros((2, 2, 16)), torch.zeros((2, 2, 16), dtype=torch.int32)
+    with pytest.raises(ValueError, match="must not lie among"):
+        kernels.rotate_append(rows, q, k, k, out=cut(torch.bfloat16, 2, 4, 3, 64))
+    kw = dict(scale=0.1, tokens=16)
+    for out in ({"out": cut(torch.bfloat16, 2, 4, 3, 64)}, {"lse": cut(torch.float32, 2, 4, 3)}):
+        with pytest.raises(ValueError, match="must not lie among"):
+            kernels.chunk_attend(q, rows, **kw, **out)
+    for out in ({"out": cut(torch.float32, 2, 2, 16)}, {"sums": cut(torch.float32, 2, 2, 16)}, {"positions": cut(torch.int32, 2, 2, 16)}):
+        with pytest.raises(ValueError, match="must not lie among"):
+            kernels.weigh_rows(q, lse, rows, **kw, **out)
+    for args, out in (((cut(torch.float32, 2, 2, 16), positions), None), ((sums, cut(torch.int32, 2, 2, 16)), None), ((sums, positions), (cut(torch.float32, 2, 2, 8), positions)),
+                      ((sums, positions), (sums, cut(torch.int32, 2, 2, 8)))):
+        with pytest.raises(ValueError, match="share addresses"):
+            kernels.evict_rows(rows, *args, keep=8, tokens=16, out=out)
+
+
+@pytest.mark.parametrize("eight", [False, True])
+def test_what_lies_beside_a_caches_rows_is_launched(monkeypatch: pytest.MonkeyPatch, kernels, eight: bool) -> None:  # noqa: ANN001
+    import torch
+
+    launched = []
+    monkeypatch.setattr(kernels, "_launch", lambda _, fn, *args: launched.append(args) or 0)
+    pool, rows = _pool(eight, 1 << 16)
+    at = 8448 if eight else 16384
+    cut = lambda dtype, *shape: pool[at:].view(dtype)[: torch.Size(shape).numel()].view(shape)  # noqa: E731
+    q, k = torch.zeros((2, 4, 3, 64), dtype=torch.bfloat16), torch.zeros((2, 2, 3, 64), dtype=torch.bfloat16)
+    lse, sums, positions = torch.zeros((2, 4, 3)), torch.zeros((2, 2, 16)), torch.zeros((2, 2, 16), dtype=torch.int32)
+    kernels.rotate_append(rows, q, k, k, out=cut(torch.bfloat16, 2, 4, 3, 64))
+    kernels.chunk_attend(q, rows, scale=0.1, tokens=16, out=cut(torch.bfloat16, 2, 4, 3, 64))
+    kernels.weigh_rows(q, lse, rows, scale=0.1, tokens=16, sums=cut(torch.float32, 2, 2, 16), positions=positions)
+    kernels.evict_rows(rows, sums, cut(torch.int32, 2, 2, 16), keep=8, tokens=16)
+    assert len(launched) == 4
+
+
+@pytest.mark.parametrize(("eight", "at"), [(False, 0), (False, 8192), (True, 0), (True, 4096), (True, 8192), (True, 8320)])
+def test_new_tokens_that_lie_among_a_caches_rows_are_copied_first(monkeypatch: pytest.MonkeyPatch, kernels, eight: bool, at: int) -> None:  # noqa: ANN001
+    """Their bytes are the cache's, in its dtype or not: the launch gets others."""
+    import torch
+
+    launched = []
+    monkeypatch.setattr(kernels, "_launch", lambda _, fn, *args: launched.append(args) or 0)
+    pool, rows = _pool(eight, 1 << 16)
+    lo = pool.data_ptr()
+    hi = lo + (8448 if eight else 16384)
+    mine = pool[at:].view(torch.bfloat16)[: 2 * 2 * 3 * 64].view(2, 2, 3, 64)
+    other = torch.zeros((2, 2, 3, 64), dtype=torch.bfloat16)
+    kernels.append_rows(rows, mine, other)
+    kernels.append_rows(rows, other, mine)
+    kernels.rotate_append(rows, mine, other, other)
+    kernels.rotate_append(rows, other, mine, other)
+    kernels.rotate_append(rows, other, other, mine)
+    assert len(launched) == 5
+    for args in launched:
+        addresses = [x for x in args[1:4] if isinstance(x, int) and x > 1 << 20]
+        assert len(addresses) >= 2 and not any(lo <= x < hi for x in addresses), (lo, hi, addresses)
