@@ -934,6 +934,27 @@ def _paged(rows: Rows, pages: torch.Tensor | None, seqs: int) -> tuple[object, i
     return _lib.Pages(pages.data_ptr(), st[0], shape[1]), rows.tokens * shape[1]
 
 
+def _among(written: tuple, seqs: int, pages: torch.Tensor | None, *at: int | None) -> bool:
+    """Whether a call's page table, or numbers at these addresses, one for each sequence, lie among spans of addresses that it writes."""
+    n = 4 * seqs
+    for a, b in written:
+        for x in at:
+            if x is not None and x < b and a < x + n:
+                return True
+    if pages is not None:
+        x = pages.data_ptr()
+        end = x + 4 * ((seqs - 1) * pages.stride(0) + pages.shape[1])
+        for a, b in written:
+            if x < b and a < end:
+                return True
+    return False
+
+
+def _copies(*tensors: torch.Tensor | None) -> tuple:
+    """Copies of numbers that lie among what a call writes: all are read before any is written."""
+    return tuple(None if x is None else x.clone() for x in tensors)
+
+
 def _reach(x: torch.Tensor) -> tuple[int, int]:
     """The addresses between which a tensor's elements lie."""
     at = x.data_ptr()
@@ -1039,6 +1060,9 @@ def rotate_append(
             raise ValueError("out's rows must be contiguous and start on 16 bytes")
         if _meet((_reach(out),), (*map(_reach, read), *dst.spans)):
             raise ValueError("out must not lie among the inputs or the cache's rows")
+        if _among((_reach(out),), seqs, pages, at, count):
+            starts, counts, pages = _copies(starts, counts, pages)
+            at, count, table_ref = _counts(starts, seqs, index, "starts"), _counts(counts, seqs, index, "counts"), _paged(dst, pages, seqs)[0]
     elif 0 in shape:
         return q.new_empty(shape)
     else:
@@ -1150,6 +1174,9 @@ def chunk_attend(
         mine = tuple(map(_reach, given))
         if _meet(mine, (_reach(q), *rows.spans)) or (len(mine) == 2 and _meet(mine[:1], mine[1:])):
             raise ValueError("out and lse must not lie among the inputs or each other")
+        if _among(mine, len(q), pages, at, count):
+            lengths, counts, pages = _copies(lengths, counts, pages)
+            desc, q, at, count, table, _ = _chunk("chunk_attend", q, rows, scale, tokens, lengths, counts, max_tokens, pages, given)
         _WRITTEN(given)
     lib = _lib.lib()
     ref = ctypes.byref(desc)
@@ -1231,6 +1258,10 @@ def weigh_rows(
         raise ValueError("out and positions must not lie among the inputs or each other")
     if seqs == 0 or most == 0:
         return out
+    if _among(mine, seqs, pages, at, count, first):
+        lengths, counts, pages, seen = _copies(lengths, counts, pages, seen)
+        desc, q, at, count, table, _ = _chunk("weigh_rows", q, rows, scale, tokens, lengths, counts, max_tokens, pages, given)
+        first = _counts(seen, seqs, index, "seen")
     _WRITTEN(written)
     lib = _lib.lib()
     ref = ctypes.byref(desc)
@@ -1287,11 +1318,17 @@ def evict_rows(
         _same_or_apart("positions", to_positions, positions, to_positions_at, positions_at)
     if _GRAD_ENABLED() or _forward_level() >= 0:
         _no_gradients("evict_rows", (*rows.owners, sums, positions, to_sums, to_positions))
-    both = (sums_at, to_sums_at)
-    if _meet(both, (positions_at, to_positions_at)) or _meet((*both, positions_at, to_positions_at), rows.spans):
+    if out is None:
+        accounts, others = (sums_at,), (positions_at,)
+    else:
+        accounts, others = (sums_at, to_sums_at), (positions_at, to_positions_at)
+    if _meet(accounts, others) or _meet((*accounts, *others), rows.spans):
         raise ValueError("sums, positions and rows share addresses")
     if seqs == 0 or max_tokens == 0:
         return
+    if _among((to_sums_at, to_positions_at, *rows.spans), seqs, pages, at):
+        lengths, pages = _copies(lengths, pages)
+        at, table = _counts(lengths, seqs, index, "lengths"), _paged(rows, pages, seqs)[0]
     lib = _lib.lib()
     desc = _lib.EvictDesc(seqs, rows.n_kv, rows.head_dim, rows.model_code, keep, sinks, recent, tokens, max_tokens)
     ref = ctypes.byref(desc)

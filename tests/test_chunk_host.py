@@ -257,3 +257,58 @@ def test_new_tokens_that_lie_among_a_caches_rows_are_copied_first(monkeypatch: p
     for args in launched:
         addresses = [x for x in args[1:4] if isinstance(x, int) and x > 1 << 20]
         assert len(addresses) >= 2 and not any(lo <= x < hi for x in addresses), (lo, hi, addresses)
+
+
+def test_numbers_that_lie_among_what_a_call_writes_are_copied_first(monkeypatch: pytest.MonkeyPatch, kernels) -> None:  # noqa: ANN001
+    """Lengths, counts, page tables and the tokens seen are read by workgroups that others are ahead of: where one buffer holds them and a call's outputs, the launch
+    gets copies, with their values, and elsewhere the tensors themselves."""
+    import torch
+
+    launched = []
+
+    def launch(_: int, fn, *args) -> int:  # noqa: ANN001, ANN002
+        flat = [y for x in args for y in ((x.table,) if isinstance(x, _lib.Pages) else (x,)) if isinstance(y, int) and y > 1 << 20]
+        launched.append({y: ctypes.c_int32.from_address(y).value for y in flat})
+        return 0
+
+    from lazykv_amd import _lib
+
+    monkeypatch.setattr(kernels, "_launch", launch)
+    rows = kernels.dense_rows(*torch.zeros((2, 4, 2, 16, 64), dtype=torch.bfloat16))
+    q, k = torch.zeros((2, 4, 3, 64), dtype=torch.bfloat16), torch.zeros((2, 2, 3, 64), dtype=torch.bfloat16)
+    lse, sums = torch.zeros((2, 4, 3)), torch.zeros((2, 2, 16))
+    state = torch.zeros(4096, dtype=torch.int32)
+    far = torch.zeros(16, dtype=torch.int32)
+    for one, (name, n) in enumerate((("counts", 2), ("pages", 2), ("lengths", 2), ("seen", 2))):
+        for among in (True, False):
+            mine = (state[6:8] if among else far[:n]).copy_(torch.tensor([one + 1, 2]))
+            lo = state.data_ptr()
+            kw = {"lengths": torch.tensor([9, 9], dtype=torch.int32), "pages": torch.tensor([[0], [1]], dtype=torch.int32), name: mine.view(2, 1) if name == "pages" else mine}
+            calls = [lambda: kernels.weigh_rows(q, lse, rows, scale=0.1, sums=sums, positions=state[:64].view(2, 2, 16), **kw)]  # noqa: B023
+            chunk = {x: y for x, y in kw.items() if x != "seen"}
+            if name != "seen":
+                calls.append(lambda: kernels.chunk_attend(q, rows, scale=0.1, out=state[:768].view(torch.bfloat16).view(2, 4, 3, 64), **chunk))  # noqa: B023
+                calls.append(lambda: kernels.chunk_attend(q, rows, scale=0.1, lse=state[:24].view(torch.float32).view(2, 4, 3), **chunk))  # noqa: B023
+                moved = {"starts" if x == "lengths" else x: y for x, y in chunk.items()}
+                calls.append(lambda: kernels.rotate_append(rows, q, k, k, out=state[:768].view(torch.bfloat16).view(2, 4, 3, 64), **moved))  # noqa: B023
+            if name in ("pages", "lengths"):
+                calls.append(lambda: kernels.evict_rows(rows, sums, state[:64].view(2, 2, 16), keep=4, **{x: kw[x] for x in ("pages", "lengths")}))  # noqa: B023
+            for call in calls:
+                launched.clear()
+                call()
+                (got,) = launched
+                there = [x for x in got if lo + 24 <= x < lo + 32]
+                assert not there and (one + 1 in got.values()), (name, among)
+                assert among or mine.data_ptr() in got, name
+
+
+def test_a_page_table_among_rows_that_an_eviction_moves_is_copied_first(monkeypatch: pytest.MonkeyPatch, kernels) -> None:  # noqa: ANN001
+    import torch
+
+    tables = []
+    monkeypatch.setattr(kernels, "_launch", lambda _, fn, *args: tables.extend(x.table for x in args if hasattr(x, "table")) or 0)
+    pool = torch.zeros((2, 4, 2, 16, 64), dtype=torch.bfloat16)
+    rows = kernels.dense_rows(pool[0], pool[1])
+    table = pool.view(torch.int32).flatten()[32:34].view(2, 1)
+    kernels.evict_rows(rows, torch.zeros((2, 2, 16)), torch.zeros((2, 2, 16), dtype=torch.int32), keep=4, tokens=16, pages=table)
+    assert len(tables) == 1 and tables[0] != table.data_ptr()
