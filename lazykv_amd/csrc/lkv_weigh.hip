@@ -86,10 +86,7 @@ template <int D, bool MX> struct QueryRegs {
 template <int DT, int D, bool MX>
 __global__ __launch_bounds__(64 * kWaves, 2) void weigh_rows_kernel(WeighArgs a) {
   const int lane = threadIdx.x & 63, quarter = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  int id = blockIdx.x;
-  const int heads = a.n_seqs * a.n_kv, bh = id % heads;
-  id /= heads;
-  const int part = id % a.parts, block = id / a.parts, b = bh / a.n_kv, h = bh % a.n_kv;
+  const int heads = a.n_seqs * a.n_kv, bh = blockIdx.x % heads, block = blockIdx.x / heads, b = bh / a.n_kv, h = bh % a.n_kv;
   const Extent e = extent_of(a, b);
   const int row0 = block * kBlockRows + wave * kWaveRows;
   if (row0 >= e.len) return;
@@ -111,8 +108,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_rows_kernel(WeighArgs a)
   }
   float sum[2][2] = {{0.0f, 0.0f}, {0.0f, 0.0f}};
   // The first query that attends the wave's first row, and the first one that attends all its rows.
-  const int past = e.len - e.n, x_end = min(e.n * a.g, (part + 1) * a.chunk);
-  const int x_first = max(part * a.chunk, max(row0 - past, 0) * a.g & ~15), x_whole = max(row0 + kWaveRows - 1 - past, 0) * a.g;
+  const int past = e.len - e.n, x_end = e.n * a.g;
+  const int x_first = max(row0 - past, 0) * a.g & ~15, x_whole = max(row0 + kWaveRows - 1 - past, 0) * a.g;
   if (x_first < x_end) {
     QueryRegs<D, MX> now, next;
     now.load(a, e, b, h, x_first + (lane & 15));
@@ -167,11 +164,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_rows_kernel(WeighArgs a)
       const float total = pair_sum<32>(pair_sum<16>(sum[u][w]));
       mine = quarter == 2 * u + w ? (there[u][w] ? total : 0.0f) : mine;
     }
-  if (a.parts > 1) {
-    a.part[((int64_t)part * heads + bh) * a.blocks * kBlockRows + row0 + lane] = mine;
-  } else {
-    store_sum(a, e, b, h, row0 + lane, mine);
-  }
+  store_sum(a, e, b, h, row0 + lane, mine);
 }
 
 // ---- many query rows: through LDS ------------------------------------------------------------------
@@ -390,7 +383,7 @@ Plan plan_of(const lkv_chunk_desc* d) {
   p.wide = x > 32;
   p.blocks = ceil_div(d->max_tokens, kBlockRows);
   const int64_t units = (int64_t)d->n_seqs * d->n_kv * p.blocks;
-  // Query rows in parts for 2,048 workgroups, a stage each at the least: 8,192 of them over 4,096 rows 97 us, by 1,024 workgroups 108, by 4,096 100; 800 over 700
+  // Query rows in parts for 2,048 workgroups, a stage each at the least, which few rows are not: 8,192 of them over 4,096 rows 97 us, by 1,024 workgroups 108, by 4,096 100; 800 over 700
   // 12.2, by four stages each 20.4.
   int64_t parts = units > 0 ? 2048 / units : 1;
   const int64_t most = x / kStage;
