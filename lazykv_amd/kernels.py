@@ -1253,7 +1253,8 @@ def weigh_rows(
     else:
         positions_st, positions_at = _account("positions", positions, torch.int32, seqs, h, most, index)
         written, mine, first = (out, positions), (out_at, positions_at), _counts(seen, seqs, index, "seen")
-    inputs = (_reach(q), _reach(lse), *rows.spans)
+    st, x, y = q.stride(), q.data_ptr(), lse.data_ptr()
+    inputs = ((x, x + 2 * ((seqs - 1) * st[0] + (n_q - 1) * st[1] + (n - 1) * st[2] + d)), (y, y + 4 * seqs * n_q * n), *rows.spans)
     if _meet(mine, inputs) or (positions is not None and _meet(mine[1:], (out_at, sums_at))):
         raise ValueError("out and positions must not lie among the inputs or each other")
     if seqs == 0 or most == 0:
@@ -1266,7 +1267,7 @@ def weigh_rows(
     lib = _lib.lib()
     ref = ctypes.byref(desc)
     ws_ptr, ws_n, _held = _scratch(lib.lkv_weigh_rows_workspace_bytes(ref), ws, q)
-    rc = _launch(index, lib.lkv_weigh_rows, ref, q.data_ptr() or lse.data_ptr() or out.data_ptr(), rows.model_code, lse.data_ptr() or out.data_ptr(), rows.ref, table, at, count,
+    rc = _launch(index, lib.lkv_weigh_rows, ref, x or y or out_at[0], rows.model_code, y or out_at[0], rows.ref, table, at, count,
                  None if sums is None else sums_at[0], sums_st, out_at[0], out_st, None if positions is None else positions_at[0], positions_st, first, ws_ptr, ws_n)
     if rc:
         _lib.check(rc, "weigh_rows")
