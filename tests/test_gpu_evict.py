@@ -529,3 +529,116 @@ def test_tokens_that_add_nothing_and_lanes_without_one_show_no_key(t: int, count
         want[0, :, 5] = 0
     got = kernels.weigh_rows(q, lse, cache.rows, **kw)
     assert torch.equal(got, want), (got != want).nonzero()[:4]
+
+
+def marked(n: int, d: int, *, seqs: int, h: int, eight: bool, page: int, gen: torch.Generator) -> tuple:
+    """(rows, page table, what the rows hold as a function, their number): a cache in which sequence b's row i of head j is told by its first channels, b, j and i in small numbers, built
+    without a step a row."""
+    from lazykv_amd import kernels
+
+    each = -(-n // page) if page else 1
+    store = (seqs * each + 2, h, page, d) if page else (seqs, h, n, d)
+    table = torch.randperm(store[0], generator=gen)[: seqs * each].view(seqs, each) if page else None
+    at = torch.full((*store[:1], 1, store[2], 2), -1)
+    place = torch.arange(n)
+    for b in range(seqs):
+        where, i = (table[b, place // page], place % page) if page else (torch.full_like(place, b), place)
+        at[where, 0, i] = torch.stack([torch.full_like(place, b), place], -1)
+    b, i = at.expand(-1, h, -1, -1).unbind(-1)
+    j = torch.arange(h)[None, :, None].expand_as(b)
+    marks = torch.stack([b + 1, j + 1, i % 128 + 1, i // 128 + 1], -1)  # 8-bit codes take them as bytes
+    both = torch.zeros((2, *store), dtype=torch.uint8 if eight else torch.float16)
+    both[..., :4], both[1, ..., 4] = marks.to(both.dtype), 9
+    both = both.cuda()
+    if eight:
+        scales = torch.where(torch.arange(d // 32) == 0, 100, 7).to(torch.uint8).expand(2, *store[:3], d // 32).clone()
+        scales[..., 0] += (i % 32).to(torch.uint8)
+        held = [both, scales.cuda()]
+        rows = kernels.mx_rows(*held, torch.float16)
+    else:
+        held, rows = [both], kernels.dense_rows(both[0], both[1])
+    pages = None if table is None else table.int().cuda()
+
+    def read(b: int, j: int) -> list:
+        if table is None:
+            return [x[:, b, j] for x in held]
+        where, i = table[b, place // page].cuda(), (place % page).cuda()
+        return [x[:, where, j, i] for x in held]
+
+    return rows, pages, read, held
+
+
+SPECIAL = (float("nan"), float("inf"), -float("inf"), -0.0, 0.0, 1e-42, -1.0, float("nan"))
+
+
+def border_case(n: int, keep: int, *, sums_of: str, eight: bool = False, page: int = 0, d: int = 64, lens: list | None = None, apart: bool = False) -> None:
+    from lazykv_amd import kernels
+
+    gen = torch.Generator().manual_seed(n + keep)
+    seqs, h = len(lens or [n]), 2
+    lens = lens or [n]
+    rows, pages, read, held = marked(n, d, seqs=seqs, h=h, eight=eight, page=page, gen=gen)
+    sums = torch.randn((seqs, h, n), generator=gen).exp()
+    if sums_of == "ties":
+        sums = torch.randint(0, 3, (seqs, h, n), generator=gen).float()
+    elif sums_of == "special":
+        for i, x in enumerate(SPECIAL):
+            sums[:, :, i::11] = x
+    elif sums_of == "nan":
+        sums = torch.where(torch.rand((seqs, h, n), generator=gen) < 0.9, float("nan"), sums)
+    positions = torch.stack([torch.randperm(n, generator=gen) for _ in range(seqs * h)]).view(seqs, h, n).int()
+    args = [sums.cuda(), positions.cuda()]
+    to = [torch.full_like(x, -3) for x in args] if apart else args
+    before = [[[x.clone() for x in read(b, j)] for j in range(h)] for b in range(seqs)]
+    kernels.evict_rows(rows, *args, keep=keep, sinks=min(2, keep), recent=min(5, max(0, keep - 2)), lengths=int32(lens), max_tokens=n, pages=pages, out=tuple(to) if apart else None)
+    torch.cuda.synchronize()
+    for b in range(seqs):
+        for j in range(h):
+            m = lens[b]
+            s, p = sums[b, j].numpy().copy(), positions[b, j].numpy().copy()
+            dst, src = O.evict(s[:m], p[:m], keep, min(2, keep), min(5, max(0, keep - 2))) if m else (np.zeros(0, np.int64),) * 2
+            s[dst], p[dst] = s[src], p[src]
+            to_rows, of_rows = torch.from_numpy(dst).cuda(), torch.from_numpy(src).cuda()
+            for want, got in zip(before[b][j], read(b, j)):
+                want[:, to_rows] = want[:, of_rows]
+                assert torch.equal(got, want), (b, j)
+            end = min(m, keep)
+            left = slice(0, end if apart else n)
+            assert np.array_equal(to[0][b, j].cpu().numpy()[left], s[left], equal_nan=True) and np.array_equal(to[1][b, j].cpu().numpy()[left], p[left]), (b, j)
+            if apart:
+                assert torch.all(to[0][b, j, end:] == -3) and torch.all(to[1][b, j, end:] == -3)
+
+
+# Two, four, eight and sixteen rows a thread, and the first size by spans.
+BORDERS = [2047, 2048, 2049, 4095, 4096, 4097, 8191, 8192, 8193, 16383, 16384, 16385]
+
+
+@pytest.mark.parametrize("n", BORDERS)
+@pytest.mark.parametrize("over", [1, 256, 257, 1500])
+@pytest.mark.parametrize("sums_of", ["exp", "ties", "special"])
+def test_both_sides_of_each_size(n: int, over: int, sums_of: str) -> None:
+    """Rows over the budget: as many as the planning workgroup moves by itself, one more, and many."""
+    border_case(n, n - over, sums_of=sums_of)
+
+
+@pytest.mark.parametrize("n", [2049, 4097, 16384, 16385, 20001])
+@pytest.mark.parametrize("keep", [1, 7, 200, 1024])
+@pytest.mark.parametrize(("eight", "page", "d"), [(False, 16, 128), (True, 0, 64), (True, 48, 128)])
+def test_few_rows_of_many_stay_in_pages_and_in_8_bits(n: int, keep: int, eight: bool, page: int, d: int) -> None:
+    border_case(n, keep, sums_of="ties", eight=eight, page=page, d=d)
+
+
+@pytest.mark.parametrize("n", [4096, 16384, 16385, 33000])
+@pytest.mark.parametrize("sums_of", ["special", "nan", "ties"])
+@pytest.mark.parametrize("share", [0.02, 0.3, 0.6, 0.97])
+@pytest.mark.parametrize(("eight", "page"), [(False, 0), (True, 64)])
+def test_special_sums_by_spans(n: int, sums_of: str, share: float, eight: bool, page: int) -> None:
+    """NaN, which has the lowest rank of all, infinities, zeros of both signs and ties on both sides of row `keep`, in one workgroup and across spans."""
+    border_case(n, max(1, int(n * share)), sums_of=sums_of, eight=eight, page=page)
+
+
+@pytest.mark.parametrize(("n", "keep"), [(4097, 3000), (16384, 12000), (20001, 4096), (20001, 4095)])
+@pytest.mark.parametrize("apart", [False, True])
+def test_ragged_lengths_of_every_size(n: int, keep: int, apart: bool) -> None:
+    """Sequences without rows, within the budget, one over it, at the last row of a span and one behind, and full."""
+    border_case(n, keep, sums_of="ties", page=16, apart=apart, lens=[0, 1, keep - 1, keep, keep + 1, min(n, 4096 * (n // 4096)), min(n, 4096 * (n // 4096) + 1), n])
