@@ -160,7 +160,12 @@ extern "C" int lkv_rotate_append(uintptr_t stream, const lkv_rotate_desc* desc, 
   if (!starts) LKV_CHECK_ARG(start >= 0 && (int64_t)start + d.tokens <= a.rows.capacity, "rows %d..%lld exceed the %d there are", start,
                              (long long)start + d.tokens, a.rows.capacity);
   const int64_t heads = (int64_t)d.n_q + 2 * (int64_t)d.n_kv, tokens = (int64_t)d.n_seqs * d.tokens;
-  LKV_CHECK_ARG(heads < (1LL << 31) && (__int128)heads * tokens < (1LL << 31) && tokens < (1 << 24), "%lld heads of %lld tokens in one call", (long long)heads, (long long)tokens);
+  // All heads of a token by one workgroup, or, of few tokens, as many as it has lanes for (48 heads, d 128): 64 tokens 5.6 and 4.4 us, 256 5.9 and 5.1,
+  // 512 6.6 and 6.9, 1,024 8.5 and 10.4, 4,096 21.8 and 33.
+  const int64_t splits = tokens >= 512 ? 1 : (heads + kHeads - 1) / kHeads;
+  // (2^24 workgroups of 256 threads are more than a launch has.)
+  LKV_CHECK_ARG(heads < (1LL << 31) && (__int128)heads * tokens < (1LL << 31) && (__int128)tokens * splits < (1 << 24), "%lld heads of %lld tokens in one call", (long long)heads,
+                (long long)tokens);
   if (tokens == 0) return LKV_OK;
   if (int rc = lkv_distinct_dst(dst, d.n_kv, d.head_dim)) return rc;
   if (int rc = lkv_distinct_rows("q_out", q_out, nullptr, 2, d.n_seqs, d.n_q, d.tokens, d.head_dim, d.out_stride[0], d.out_stride[1], d.out_stride[2])) return rc;
@@ -177,10 +182,8 @@ extern "C" int lkv_rotate_append(uintptr_t stream, const lkv_rotate_desc* desc, 
   a.counts = counts;
   a.start = start;
   a.heads = (uint32_t)heads;
-  // All heads of a token by one workgroup, or, of few tokens, as many as it has lanes for (48 heads, d 128): 64 tokens 5.6 and 4.4 us, 256 5.9 and 5.1,
-  // 512 6.6 and 6.9, 1,024 8.5 and 10.4, 4,096 21.8 and 33.
-  a.splits = tokens >= 512 ? 1 : (a.heads + kHeads - 1) / kHeads;
-  a.share = a.splits == 1 ? a.heads : kHeads;
+  a.splits = (uint32_t)splits;
+  a.share = splits == 1 ? a.heads : kHeads;
   const bool mx = dst->dtype == LKV_MXFP8, half = d.dtype == LKV_F16, wide = d.head_dim == 128;
   auto kernel = half ? (wide ? (mx ? rotate_append_kernel<LKV_F16, 128, true> : rotate_append_kernel<LKV_F16, 128, false>)
                              : (mx ? rotate_append_kernel<LKV_F16, 64, true> : rotate_append_kernel<LKV_F16, 64, false>))

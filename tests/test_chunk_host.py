@@ -312,3 +312,11 @@ def test_a_page_table_among_rows_that_an_eviction_moves_is_copied_first(monkeypa
     table = pool.view(torch.int32).flatten()[32:34].view(2, 1)
     kernels.evict_rows(rows, torch.zeros((2, 2, 16)), torch.zeros((2, 2, 16), dtype=torch.int32), keep=4, tokens=16, pages=table)
     assert len(tables) == 1 and tables[0] != table.data_ptr()
+
+
+@pytest.mark.parametrize(("n_q", "tokens"), [(1 << 29, 1), ((1 << 28) + 16, 1), (1 << 22, 511)])
+def test_rotations_of_more_threads_than_a_launch_has_are_refused(n_q: int, tokens: int) -> None:
+    """Few tokens of many heads: sixteen heads a workgroup of up to 256 threads, 2^24 of which are 2^32 threads."""
+    change = {"desc": {"n_seqs": 1, "n_q": n_q, "n_kv": 1, "new_tokens": tokens}, "strides": (n_q * 64 * tokens, 64 * tokens, 64),
+              "rows": {"tokens": 1024, "v": 1 << 40, "seq_stride": 1 << 16, "head_stride": 1 << 16}}
+    assert "in one call" in _call("rotate", change)
