@@ -372,7 +372,8 @@ typedef struct lkv_pages {
  * y_i cos_i - y_(i + rotary / 2) sin_i, i + rotary / 2 to y_(i + rotary / 2) cos_(i + rotary / 2) + y_i sin_(i + rotary / 2); cos and sin
  * [n_seqs or 1, tokens, rotary] at b * table_seq_stride + t * rotary), in float32 and rounded to the model dtype once. Queries go to
  * q_out (strides of its own), keys and values to rows start + starts[b] + t of `dst` as in lkv_append_rows; tokens from counts[b] on
- * go to no row (counts NULL: all go). What a row holds that two tokens of a call go to (a page in two tables) is not defined. */
+ * go to no row (counts NULL: all go). What a row holds that two tokens of a call go to (a page in two tables) is not defined.
+ * Here and in the calls below nothing that a call reads may lie among what it writes, but for what a call says. */
 typedef struct lkv_rotate_desc {
   int32_t n_seqs, n_q, n_kv, head_dim, tokens;
   int32_t dtype;        /* of q, k, v, q_out */

@@ -182,8 +182,8 @@ __device__ __forceinline__ void add_not_finite(uint4 v, uint4 attended, ACC& o, 
 }
 
 // ---- few rows: every wave on its own stream of tokens, straight from memory to registers -----------------
-// Bound by memory, where there are enough rows: a token of each of sixteen sequences of up to 8,192 rows (8 heads, d 128, 268 MB) takes 41 us, 6.5 TB/s, and 6 more to join
-// the parts; one token over 131,072 rows 104 us.
+// Bound by memory, where there are enough rows: a token of each of sixteen sequences, 54,810 rows in all (8 heads, d 128, 224 MB), takes 40 us, 5.6 TB/s, and 6 more to join
+// the parts, 76,414 61 with the join; one token over 131,072 rows 104 us, in 8 bits 75.
 
 // The two halves of a wave's tile of 32 rows, each in one page; a half that is not there reads the other's rows, or the pool's first.
 template <int D, bool MX> struct Halves {
@@ -849,7 +849,9 @@ Plan plan_of(const lkv_chunk_desc* d) {
   // Of many parts a sequence, no more than that; of few, those that are not whole come on top. On top, sixteen sequences' steps cost 60.8 us for 57.3 and four questions
   // of 64 tokens 75.2 for 61.6; not on top, sixteen of 64 tokens (two parts each) 135.4 for 121.8. Undivided, a step of 64 sequences of 1,024 rows and one of
   // 65,536 among them cost 1,029 us for 105, 32 chunks of 128 tokens of the same kind 1,916 for 275; 64 and 100 of equal lengths 184.4 for 186.9 and 308.7 for 312.1.
-  // More than 256 sequences fill the device, and the division would be looked for too long.
+  // More than 256 sequences are not divided: every workgroup goes through their lengths for its part, and a part more than a sequence each is looked for again. 257 and 300 of 1,024 rows a token
+  // each 219 and 253 us, divided 227 and 259; 300 under 32 tokens each 300, divided 410. What that leaves: with one of 65,536 rows among them, a workgroup a head has it, 1,140 and
+  // 1,157 us for 272 and 307, under 32 tokens 1,727 for 457.
   const int64_t units = (int64_t)d->n_kv * p.tiles, room = p.nr && (d->n_seqs == 1 || (p.nr == 2 && d->head_dim == 128)) ? 256 : 512;
   int64_t share = units > 0 ? room / units : 1;
   const int64_t longest = d->n_seqs * (int64_t)ceil_div(d->max_tokens, p.nr ? 128 : 256);

@@ -6,7 +6,7 @@
 // than must. What a row holds is told by its position, not by its place.
 //
 // The moves are bound by memory: 131,072 rows of 8 heads (d 128) cut to 32,768 take 43 us, 4.6 TB/s of rows that are read one by one, and the planning before it another
-// 43, six launches whose ends are most of that. A decode step's one row over 2,048, of sixteen sequences: 8.8 us, one launch's latency from length to move.
+// 43, six launches whose ends are most of that. A decode step's one row over 2,048, of sixteen sequences: 9.5 us, one launch's latency from length to move.
 #include "lkv_pages.h"
 
 namespace {
@@ -411,7 +411,7 @@ Layout layout_of(const lkv_evict_desc* d) {
   const size_t heads = (size_t)d->n_seqs * d->n_kv;
   l.list = lkv_align_up(heads * sizeof(int32_t), 16);
   l.bytes = l.newest = l.list + lkv_align_up(heads * 2 * moves_of(d) * sizeof(int32_t), 16);
-  // One workgroup's registers hold 16,384 rows: that many take 25.1 us (8,000 of one sequence stay), by spans 36.4; 6,000 14.3 and 31.1.
+  // One workgroup's registers hold 16,384 rows: that many take 26.0 us (8,000 of one sequence stay), by spans 36.8; 6,000 15.0 and 31.9, 2,049 of sixteen sequences 9.5 and 30.3.
   if (d->max_tokens <= kThreads * 16) return l;
   l.spans = (int)(((int64_t)d->max_tokens + kSpan - 1) / kSpan);
   l.digits = l.newest + lkv_align_up(heads * l.spans * sizeof(int32_t), 16);
@@ -426,7 +426,8 @@ int launch(const EvictArgs& a, hipStream_t s, int64_t heads) {
   const dim3 block(kThreads);
   const bool few = a.spans == 0 && a.moves <= kFew;
   if (a.spans == 0) {
-    // Rows a thread, no more than needed: 2,049 rows 8.8 us by two and 15.3 by sixteen, 6,000 14.3 by eight and 18.9.
+    // Rows a thread, no more than needed (sixteen sequences over their budget by one): 2,048 rows 8.6 us by two and 16.0 by sixteen, 2,049 9.5 by four; 6,000 of one, cut to 2,000, 15.0 by
+    // eight and 19.7.
     const int each = a.max_tokens <= 2 * kThreads ? 2 : a.max_tokens <= 4 * kThreads ? 4 : a.max_tokens <= 8 * kThreads ? 8 : 16;
     auto kernel = each == 2   ? (few ? evict_short_kernel<2, D, MX, true> : evict_short_kernel<2, D, MX, false>)
                   : each == 4 ? (few ? evict_short_kernel<4, D, MX, true> : evict_short_kernel<4, D, MX, false>)

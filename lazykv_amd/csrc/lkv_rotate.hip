@@ -39,7 +39,8 @@ __device__ __forceinline__ void load_eight(const void* p, int64_t at, bool wide,
 // z the channel half a rotation away. It is loaded again rather than sent by the lane that has it: it is in the cache line or the next, and any
 // rotary width takes the same path.
 //
-// Bound by memory: 4,099 tokens of 48 heads (d 128), 103 MB, 22.5 us, 4.6 TB/s of the 5.1 that a large copy reaches; one token 4 us, a launch.
+// Bound by memory: 4,099 tokens of 48 heads (d 128), 103 MB, 22.6 us, 4.6 TB/s of the 5.1 that a large copy reaches; one token 4 us, a launch. With few tokens by their rounds of heads, of
+// which each loads, reduces and stores before the next: 2,600 tokens of 48 heads (d 64) into 8-bit rows, 49 MB, 13.9 us, 3.5 TB/s.
 constexpr int kHeads = 16;  // that a workgroup holds at a time
 template <int DT, int D, bool MX>
 __global__ __launch_bounds__(kHeads * D / 8) void rotate_append_kernel(RotateArgs a) {

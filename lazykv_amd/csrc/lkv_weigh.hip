@@ -7,8 +7,9 @@
 // a KV head. More of them go through LDS, 64 at a time for four waves, on v_mfma_f32_32x32x16; there -lse is the addend of the exponent's one
 // multiply-add.
 //
-// Bound by issue: behind each 32 x 32 x 16 product of 32 cycles, at 128 channels, stand ten vector operations, two of them exponentials, that hide for a part. 1,024 tokens over
-// 16,384 rows (32 heads on 8, d 128): 178 us, 0.75 PFLOP/s, the matrix units busy for 38%. One token over 4,099 (d 64): 4.7 us on the device, launch and latency.
+// Bound by issue, and by products and vector operations that hardly overlap: behind each 32 x 32 x 16 product of 32 cycles, at 128 channels, the stage's loop has six vector operations, two of
+// them exponentials, and some two and a half more bring a stage's queries to LDS. 1,024 tokens over 16,384 rows (32 heads on 8, d 128): 178 us, 0.75 PFLOP/s, the matrix
+// units busy for 39% of the cycles, the vector units for 57%. One token over 4,099 (d 64): 4.9 us on the device, launch and latency.
 #include <type_traits>
 
 #include "lkv_attend.h"

@@ -996,7 +996,8 @@ def rotate_append(
     (where `q_weight` / `k_weight` `[d]` are given: x / sqrt(mean x^2 + eps) * weight) and their first r channels rotated by `cos` / `sin`
     `[seqs or 1, T, r]` (a model's rotary tables, halves paired: channel i with i + r / 2), in float32 and rounded once. Keys and values become rows
     `start + starts[b] + t` of `dst`, as with `append_rows`, with `pages` `[seqs, n]` those of a pool; tokens from `counts[b]` on go to no row.
-    Returns the queries (in `out`, which must not be any of the inputs). No gradient."""
+    Tokens may be rows of `dst` itself; tables, weights, `starts`, `counts` and `pages` may not lie among the rows that are written. Returns the queries (in `out`, which must not
+    be any of the inputs). No gradient."""
     shape, kv, dtype, index = q.shape, k.shape, dst.model_dtype, dst.device_index
     if len(shape) != 4 or len(kv) != 4 or v.shape != kv or kv[0] != shape[0] or kv[2] != shape[2] or kv[3] != shape[3] or q.dtype != dtype or k.dtype != dtype or v.dtype != dtype:
         raise ValueError(f"expected {dtype} queries [seqs, n_q, T, d] and matching keys/values [seqs, h, T, d], got {tuple(shape)} {q.dtype}, {tuple(kv)} {k.dtype}, "
